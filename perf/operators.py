@@ -1,0 +1,636 @@
+"""The paged KV cache's operators as measurable cases.
+
+Three kinds of case, all through the public entry points of ``ops``:
+
+- ``attention``: a batch of new tokens (one per sequence, a few, or a prefill
+  chunk) attends its sequences' cached rows (``ops.paged_attention``), causal,
+  with or without a sliding window and first tokens that stay visible;
+- ``qk``: the norm of each query and key head and the position rotation
+  (``ops.qk_norm_rope``), keys and values stored in the cache's pages, or keys
+  returned;
+- ``pages``: what a serving loop does to its page tables between steps:
+  sequences forked and freed, then pages taken for new tokens
+  (``ops.fork_pages``, ``ops.extend_pages``), or live pages moved to the lowest
+  ids (``ops.compact_pages``).
+
+``run`` is the plain form (elementary torch operations, 32-bit arithmetic)
+unless ``own`` is set.
+"""
+import math
+
+import torch
+
+own = False
+
+DEV = "cuda:0"
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
+EPS = 1e-6
+THETA = 500000.0
+
+
+def listed():
+    return [
+        # One new token of one 128k sequence, the dense layer beside the
+        # retrieval layers (8 KV heads, 32 query heads): streaming K and V.
+        _attention("attn_decode_128k", [131072], [1]),
+        # A decode batch of sequences at very different lengths, eight query
+        # heads per KV head, rows of a token together (token-major pages).
+        _attention("attn_decode_batch", _spread(40, 300, 40000), [1] * 40, kv_heads=4, groups=8, layout="tokens"),
+        # The smallest call: a short sequence's next token; launches count.
+        _attention("attn_decode_small", [519], [1], page=8),
+        # Five drafted tokens of each sequence verified in a windowed layer
+        # with 64-wide heads, in half precision.
+        _attention("attn_verify_window", _spread(24, 600, 20000), [5] * 24, kv_heads=8, groups=4, dim=64, page=32,
+                   dtype="fp16", window=4096, sinks=32),
+        # Chunked prefill: the last 8192 tokens of a 32k prompt.
+        _attention("attn_chunk_32k", [32768], [8192]),
+        # A serving step that mixes decode tokens with two prompts' odd chunks,
+        # seven query heads per KV head.
+        _attention("attn_mixed", [4001, 130, 9000, 77, 20011, 2500, 1, 6143, 12000], [1, 1, 1111, 77, 1, 5, 1, 777, 1],
+                   kv_heads=4, groups=7, page=16, pad=19),
+        # Prefill of a windowed layer straight from the projections (no pages):
+        # 32 first tokens stay visible.
+        _attention("attn_prefill_window", [16384], [16384], page=0, layout="tokens", window=4096, sinks=32),
+        # One token of each of 24 sequences normed, rotated, stored.
+        _qk("qk_decode", _spread(24, 200, 100000), [1] * 24),
+        # A prefill chunk's, ragged, with rows behind the last sequence.
+        _qk("qk_chunk", [32768, 1000, 5003], [8192, 1000, 1337], pad=23),
+        # A short prompt, interleaved pairs over half of a 64-wide head, half
+        # precision, keys returned.
+        _qk("qk_positions", [777], [777], dim=64, dtype="fp16", rotary=32, interleaved=True, page=0, kv_heads=2,
+            groups=6),
+        # Beam search: four prompts of eight beams each re-parented, then one
+        # more token: shared last pages are copied.
+        _pages("pages_beam", [2001] * 8 + [777] * 8 + [4096] * 8 + [1203] * 8, fork="beam", width=8, new="1"),
+        # A long-running server frees finished sequences and moves what is
+        # left to the lowest pages.
+        _pages("pages_compact", _spread(96, 200, 4000), fork="free", new="", compact=True, layers=4),
+    ]
+
+
+def _attention(name, lens, news, kv_heads=8, groups=4, dim=128, page=16, layout="heads", window=0, sinks=0,
+               dtype="bf16", pad=0):
+    return dict(name=name, kind="attention", lens=_text(lens), news=_text(news), kv_heads=kv_heads, groups=groups,
+                dim=dim, page=page, layout=layout, window=window, sinks=sinks, dtype=dtype, pad=pad)
+
+
+def _qk(name, lens, news, kv_heads=8, groups=4, dim=128, page=16, dtype="bf16", rotary=0, interleaved=False, pad=0,
+        norm=True):
+    return dict(name=name, kind="qk", lens=_text(lens), news=_text(news), kv_heads=kv_heads, groups=groups, dim=dim,
+                page=page, layout="heads", dtype=dtype, rotary=rotary or dim, interleaved=interleaved, pad=pad,
+                norm=norm)
+
+
+def _pages(name, lens, fork, new, width=1, compact=False, layers=2, page=16, kv_heads=8, dim=128):
+    return dict(name=name, kind="pages", lens=_text(lens), fork=fork, width=width, new=new, compact=compact,
+                layers=layers, page=page, kv_heads=kv_heads, dim=dim)
+
+
+def _text(values):
+    return ",".join(str(int(v)) for v in values)
+
+
+def _ints(text):
+    return [int(v) for v in text.split(",")] if text else []
+
+
+def _spread(n, lo, hi):
+    """n lengths spread evenly over the logarithm of lo..hi, odd ones among
+    them, in an order that mixes long and short."""
+    vals = [int(round(math.exp(math.log(lo) + (math.log(hi) - math.log(lo)) * i / max(n - 1, 1)))) for i in range(n)]
+    return [vals[(i * 7) % n] if math.gcd(7, n) == 1 else vals[i] for i in range(n)]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["attention"] * 5 + ["qk"] * 2 + ["pages"] * 2)
+    if kind == "qk":
+        dim = rng.choice([64, 128, 128])
+        page = rng.choice([0, 8, 16, 64])
+        n = 1 if page == 0 else rng.choice([1, 3, 17])
+        if rng.random() < 0.4:
+            n = rng.randint(1, 64)
+            lens = [_log(rng, 1, 100000) for _ in range(n)]
+            news = [1] * n
+            if page == 0:
+                lens, news = lens[:1], news[:1]
+        else:
+            lens = [_log(rng, 100, 20000) for _ in range(n)]
+            news = [_log(rng, 1, max(1, min(v, 8000 // n))) for v in lens]
+        c = _qk("", lens, news, rng.choice([1, 2, 4, 8]), rng.choice([1, 4, 5, 8]), dim, page,
+                rng.choice(["bf16", "bf16", "fp16"]), rng.choice([0, 0, dim // 2]), rng.random() < 0.3,
+                rng.choice([0, 0, 9]), rng.random() < 0.8)
+        return _strip(c)
+    if kind == "pages":
+        page = rng.choice([8, 16, 32])
+        if rng.random() < 0.6:
+            width = rng.choice([2, 4, 6])
+            prompts = rng.randint(1, 8)
+            lens = [v for v in (_log(rng, 1, 8000) for _ in range(prompts)) for _ in range(width)]
+            c = _pages("", lens, "beam", rng.choice(["1", "3", "mixed"]), width, False, rng.choice([1, 2]), page,
+                       rng.choice([2, 8]))
+        else:
+            lens = [_log(rng, 1, 4000) for _ in range(rng.randint(5, 90))]
+            c = _pages("", lens, "free", rng.choice(["", "mixed"]), 1, True, rng.choice([1, 2, 3]), page,
+                       rng.choice([2, 8]))
+        return _strip(c)
+    dim = rng.choice([64, 128, 128])
+    groups = rng.choice([1, 2, 4, 5, 7, 8, 16])
+    kv_heads = rng.choice([1, 2, 4, 8])
+    page = rng.choice([0, 8, 16, 16, 32, 128])
+    window, sinks = rng.choice([(0, 0), (0, 0), (128, 4), (1000, 0), (4096, 32)])
+    form = rng.choice(["decode", "batch", "few", "chunk", "mixed"])
+    if form == "decode":
+        lens = [_log(rng, 1, 131072)]
+        news = [1]
+    elif form == "batch":
+        lens = [_log(rng, 1, 30000) for _ in range(rng.randint(2, 48))]
+        news = [1] * len(lens)
+    elif form == "few":
+        lens = [_log(rng, 50, 20000) for _ in range(rng.randint(1, 24))]
+        news = [min(v, rng.randint(2, 9)) for v in lens]
+    elif form == "chunk":
+        lens = [_log(rng, 100, 24000)]
+        news = [_log(rng, 16, min(lens[0], 8192))]
+    else:
+        lens = [_log(rng, 1, 12000) for _ in range(rng.randint(3, 12))]
+        news = [rng.choice([1, 1, 1, _log(rng, 1, min(v, 1500))]) for v in lens]
+    if page == 0:   # contiguous rows: every sequence padded to the longest
+        top = max(lens)
+        keep = max(1, 400000 // top)
+        lens, news = lens[:keep], news[:keep]
+    return _strip(_attention("", lens, news, kv_heads, groups, dim, page, rng.choice(["heads", "tokens"]), window,
+                             sinks, rng.choice(["bf16", "bf16", "fp16"]), rng.choice([0, 0, 7])))
+
+
+def _strip(case):
+    return {k: v for k, v in case.items() if k != "name"}
+
+
+# ------------------------------------------------------------------ inputs --
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _table(lens, page, gen, slack=1.2, width=0):
+    """Random distinct pages of a pool for each sequence: (table [S, width]
+    int32 with -1 past a sequence's pages, pages in the pool)."""
+    held = [-(-n // page) for n in lens]
+    pool = max(int(sum(held) * slack), sum(held) + 2, 4)
+    ids = torch.randperm(pool, generator=gen, device=DEV).to(torch.int32)
+    width = width or max(max(held), 1)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV)
+    at = 0
+    for s, n in enumerate(held):
+        table[s, :n] = ids[at:at + n]
+        at += n
+    return table, pool
+
+
+def _starts(news):
+    out = [0]
+    for n in news:
+        out.append(out[-1] + n)
+    return out
+
+
+def _pool(pages, heads, page, dim, layout, dtype, gen, spread=0.0):
+    """[pages, heads, page, dim] values, head-major or token-major in memory;
+    spread: the log-normal factor of each head's channels."""
+    shape = (pages, heads, page, dim) if layout == "heads" else (pages, page, heads, dim)
+    out = torch.empty(shape, dtype=dtype, device=DEV)
+    factor = torch.exp(spread * torch.randn((heads, dim), generator=gen, device=DEV))
+    factor = factor[None, :, None] if layout == "heads" else factor[None, None]
+    step = max(1, (1 << 26) // (heads * page * dim))
+    if pages > 1:
+        for p in range(0, pages, step):
+            part = out[p:p + step]
+            part.copy_(torch.randn(part.shape, generator=gen, device=DEV) * factor)
+    else:
+        out.copy_(torch.randn(shape, generator=gen, device=DEV) * factor)
+    return out if layout == "heads" else out.transpose(1, 2)
+
+
+def prepare(case, seed):
+    return {"attention": _prepare_attention, "qk": _prepare_qk, "pages": _prepare_pages}[case["kind"]](case, seed)
+
+
+def _prepare_attention(case, seed):
+    gen = _gen(seed)
+    lens, news = _ints(case["lens"]), _ints(case["news"])
+    H, G, D, page, dt = case["kv_heads"], case["groups"], case["dim"], case["page"], DTYPES[case["dtype"]]
+    start = _starts(news)
+    N = start[-1] + case["pad"]
+    state = dict(case=case, lens_host=lens, start_host=start)
+    # queries lean towards one direction per head that the first keys of a
+    # sequence share: the first tokens draw weight, as they do in practice
+    lean = torch.randn((H, D), generator=gen, device=DEV)
+    q = torch.randn((N, H, G, D), generator=gen, device=DEV) + lean[None, :, None]
+    state["q"] = q.view(N, H * G, D).to(dt)
+    if page:
+        state["table"], pool = _table(lens, page, gen)
+    else:
+        state["table"], pool, page = None, len(lens), max(max(lens), 1)
+    state["k"] = _pool(pool, H, page, D, case["layout"], dt, gen, 0.5)
+    state["v"] = _pool(pool, H, page, D, case["layout"], dt, gen)
+    for s, n in enumerate(lens):
+        first = s if state["table"] is None else int(state["table"][s, 0])
+        state["k"][first, :, :min(n, 4, page)] += (0.5 * lean[:, None]).to(dt)
+    state["lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    state["start"] = torch.tensor(start, dtype=torch.int32, device=DEV)
+    state["out"] = torch.zeros((N, H * G, D), dtype=dt, device=DEV)
+    state["lse"] = torch.zeros((N, H * G), dtype=torch.float32, device=DEV)
+    return state
+
+
+def _prepare_qk(case, seed):
+    gen = _gen(seed)
+    lens, news = _ints(case["lens"]), _ints(case["news"])
+    H, G, D, page, dt = case["kv_heads"], case["groups"], case["dim"], case["page"], DTYPES[case["dtype"]]
+    start = _starts(news)
+    N = start[-1] + case["pad"]
+    state = dict(case=case, lens_host=lens, start_host=start)
+    # one projection's output: queries, keys and values of a token in one row
+    qkv = (2.0 * torch.randn((N, (H * G + 2 * H) * D), generator=gen, device=DEV)).to(dt)
+    state["q"] = qkv[:, :H * G * D].view(N, H * G, D)
+    state["k"] = qkv[:, H * G * D:(H * G + H) * D].view(N, H, D)
+    state["v"] = qkv[:, (H * G + H) * D:].view(N, H, D)
+    weight = lambda: (1.0 + 0.2 * torch.randn((D,), generator=gen, device=DEV)).to(dt) if case["norm"] else None
+    state["qw"], state["kw"] = weight(), weight()
+    r = case["rotary"]
+    state["inv_freq"] = (THETA ** (-torch.arange(0, r // 2, dtype=torch.float64, device=DEV) * 2.0 / r)).float()
+    state["q_out"] = torch.zeros((N, H * G, D), dtype=dt, device=DEV)
+    pos = [lens[s] - news[s] + i for s in range(len(news)) for i in range(news[s])] + [0] * case["pad"]
+    if page:
+        state["table"], pool = _table(lens, page, gen)
+        state["key_pages"] = torch.zeros((pool, H, page, D), dtype=dt, device=DEV)
+        state["value_pages"] = torch.zeros_like(state["key_pages"])
+        seq = torch.tensor([s for s in range(len(news)) for _ in range(news[s])], device=DEV)
+        at = torch.tensor(pos[:start[-1]], device=DEV)
+        state["slots"] = (state["table"][seq, at // page].long(), at % page)   # the plain form's addresses
+    else:
+        state["k_out"] = torch.zeros((N, H, D), dtype=dt, device=DEV)
+    state["positions"] = torch.tensor(pos, dtype=torch.int32, device=DEV)
+    state["lens"] = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    state["start"] = torch.tensor(start, dtype=torch.int32, device=DEV)
+    return state
+
+
+def _prepare_pages(case, seed):
+    gen = _gen(seed)
+    lens = _ints(case["lens"])
+    S, page, width = len(lens), case["page"], case["width"]
+    held = [-(-n // page) for n in lens]
+    cols = max(held) + 2
+    # the beams of a prompt share its full pages, each has its own last page
+    pool = max(8, int(1.3 * (sum(held) // width + 3 * S)))
+    ids = torch.randperm(pool, generator=gen, device=DEV).cpu().tolist()
+    table = torch.full((S, cols), -1, dtype=torch.int32)
+    refs = torch.zeros((pool,), dtype=torch.int32)
+    take = iter(ids)
+    for s in range(S):
+        for j in range(held[s]):
+            if s % width and j < lens[s] // page:
+                table[s, j] = table[s - s % width, j]
+            else:
+                table[s, j] = next(take)
+            refs[table[s, j]] += 1
+    pick = torch.rand((S,), generator=gen, device=DEV).cpu().tolist()
+    if case["fork"] == "beam":   # a beam's new parent is one of its prompt's beams
+        parents = [s - s % width + int(pick[s] * width) for s in range(S)]
+    else:                        # a third of the sequences has ended
+        parents = [-1 if pick[s] < 0.33 else s for s in range(S)]
+    more = torch.randint(0, 2 * page, (S,), generator=gen, device=DEV).cpu().tolist()
+    counts = {"": [0] * S, "1": [1] * S, "3": [3] * S, "mixed": more}[case["new"]]
+    i32 = lambda x: torch.as_tensor(x, dtype=torch.int32).to(DEV)
+    state = dict(case=case, table=i32(table), lens=i32(lens), refs=i32(refs), parents=i32(parents),
+                 counts=i32(counts))
+    state["pools"] = [_pool(pool, case["kv_heads"], page, case["dim"], "heads", torch.bfloat16, gen)
+                      for _ in range(2 * case["layers"])]
+    state["work"] = (torch.empty_like(state["table"]), torch.empty_like(state["lens"]),
+                     torch.empty_like(state["refs"]))
+    return state
+
+
+# --------------------------------------------------------------------- run --
+
+def run(state):
+    kind = state["case"]["kind"]
+    if own:
+        return {"attention": _own_attention, "qk": _own_qk, "pages": _own_pages}[kind](state)
+    return {"attention": _plain_attention, "qk": _plain_qk, "pages": _plain_pages}[kind](state)
+
+
+def _own_batch(state):
+    from adaptiveimi_amd import ops
+
+    news = [b - a for a, b in zip(state["start_host"], state["start_host"][1:])]
+    return ops.PagedBatch(state.get("table"), state["lens"], state["start"], max_query=max(news),
+                          max_len=max(state["lens_host"]))
+
+
+def _own_attention(state):
+    from adaptiveimi_amd import ops
+
+    case = state["case"]
+    out, lse = ops.paged_attention(state["q"], state["k"], state["v"], _own_batch(state), window=case["window"],
+                                   sinks=case["sinks"], out=state["out"], lse=state["lse"])
+    return out, lse
+
+
+def _own_qk(state):
+    from adaptiveimi_amd import ops
+
+    case = state["case"]
+    kw = dict(inv_freq=state["inv_freq"], query_weight=state["qw"], key_weight=state["kw"], eps=EPS,
+              interleaved=case["interleaved"], query_out=state["q_out"])
+    if not case["page"]:
+        return ops.qk_norm_rope(state["q"], state["k"], positions=state["positions"], key_out=state["k_out"], **kw)
+    q, _ = ops.qk_norm_rope(state["q"], state["k"], value=state["v"], batch=_own_batch(state),
+                            key_pages=state["key_pages"], value_pages=state["value_pages"], **kw)
+    return q, state["key_pages"], state["value_pages"]
+
+
+def _own_pages(state):
+    from adaptiveimi_amd import ops
+
+    case = state["case"]
+    base = ops.PageTable(state["table"], state["lens"], state["refs"], case["page"])
+    table = ops.fork_pages(base, state["parents"], out=ops.PageTable(*state["work"], case["page"]))
+    result = [table.pages, table.lens, table.refs]
+    if case["new"]:
+        result.append(ops.extend_pages(table, state["counts"], state["pools"]))
+    if case["compact"]:
+        result.append(ops.compact_pages(table, state["pools"]))
+    return tuple(result) + tuple(state["pools"])
+
+
+# -------------------------------------------------------------- plain form --
+
+def _rows(state, s, n):
+    """The n cached rows of sequence s: keys and values [H, n, D]."""
+    if state["table"] is None:
+        return state["k"][s, :, :n], state["v"][s, :, :n]
+    page = state["case"]["page"]
+    ids = state["table"][s, :-(-n // page)].long()
+    flat = lambda pool: pool[ids].transpose(0, 1).flatten(1, 2)[:, :n]
+    return flat(state["k"]), flat(state["v"])
+
+
+def _plain_attention(state):
+    case = state["case"]
+    H, G, D = case["kv_heads"], case["groups"], case["dim"]
+    window, sinks = case["window"], case["sinks"]
+    out, lse = state["out"], state["lse"]
+    scale = 1.0 / math.sqrt(D)
+    for s, n in enumerate(state["lens_host"]):
+        lo, hi = state["start_host"][s], state["start_host"][s + 1]
+        if hi == lo:
+            continue
+        k, v = _rows(state, s, n)
+        k, v = k.float(), v.float()
+        step = max(1, (1 << 28) // (H * G * n))   # scores of a gigabyte at most
+        for a in range(lo, hi, step):
+            b = min(hi, a + step)
+            pos = torch.arange(n - hi + a, n - hi + b, device=DEV)
+            first, last = n - hi + a, n - hi + b   # the keys that these rows can see
+            lower = max(0, first - window + 1) if window else 0
+            col = torch.arange(lower, last, device=DEV)
+            ks, vs = k[:, lower:last], v[:, lower:last]
+            if lower > 0 and sinks:
+                head = min(sinks, lower)
+                col = torch.cat([torch.arange(head, device=DEV), col])
+                ks, vs = torch.cat([k[:, :head], ks], 1), torch.cat([v[:, :head], vs], 1)
+            q = state["q"][a:b].float().view(b - a, H, G, D).permute(1, 0, 2, 3).reshape(H, (b - a) * G, D)
+            x = torch.matmul(q, ks.transpose(1, 2)) * scale
+            seen = col[None] <= pos[:, None]
+            if window:
+                seen &= (col[None] > pos[:, None] - window) | (col[None] < sinks)
+            x = x.view(H, b - a, G, -1).masked_fill_(~seen[None, :, None], -math.inf)
+            top = x.amax(-1, keepdim=True)
+            w = torch.exp(x - top)
+            total = w.sum(-1, keepdim=True)
+            o = torch.matmul(w.view(H, (b - a) * G, -1), vs).view(H, b - a, G, D) / total
+            out[a:b] = o.permute(1, 0, 2, 3).reshape(b - a, H * G, D).to(out.dtype)
+            lse[a:b] = (top + torch.log(total))[..., 0].permute(1, 0, 2).reshape(b - a, H * G)
+    return out, lse
+
+
+def _rotate(x, cos, sin, interleaved):
+    half = cos.shape[-1]
+    c, s = cos[:, None], sin[:, None]
+    head, tail = x[..., :2 * half], x[..., 2 * half:]
+    if interleaved:
+        a, b = head[..., 0::2], head[..., 1::2]
+        head = torch.stack([a * c - b * s, b * c + a * s], -1).flatten(-2)
+    else:
+        a, b = head[..., :half], head[..., half:]
+        head = torch.cat([a * c - b * s, b * c + a * s], -1)
+    return torch.cat([head, tail], -1)
+
+
+def _plain_qk(state):
+    case = state["case"]
+    n = state["start_host"][-1]
+    ang = state["positions"][:n].double()[:, None] * state["inv_freq"].double()
+    cos, sin = torch.cos(ang).float(), torch.sin(ang).float()
+
+    def one(x, w):
+        x = x[:n].float()
+        x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + EPS)
+        if w is not None:
+            x = x * w.float()
+        return _rotate(x, cos, sin, case["interleaved"]).to(state["q"].dtype)
+
+    if not case["norm"]:   # no weights: no norm either
+        one = lambda x, w: _rotate(x[:n].float(), cos, sin, case["interleaved"]).to(state["q"].dtype)
+    state["q_out"][:n] = one(state["q"], state["qw"])
+    k = one(state["k"], state["kw"])
+    if not case["page"]:
+        state["k_out"][:n] = k
+        return state["q_out"], state["k_out"]
+    pages, slot = state["slots"]
+    state["key_pages"][pages, :, slot] = k
+    state["value_pages"][pages, :, slot] = state["v"][:n]
+    return state["q_out"], state["key_pages"], state["value_pages"]
+
+
+def _plain_pages(state):
+    case = state["case"]
+    page = case["page"]
+    table, lens, refs, parents = state["table"], state["lens"], state["refs"], state["parents"].long()
+    S, cols = table.shape
+    P = refs.shape[0]
+    col = torch.arange(cols, device=DEV)[None]
+    # fork
+    held = (lens + page - 1) // page
+    kept = (parents >= 0) & (parents < S)
+    src = parents.clamp(0, S - 1)
+    children = torch.zeros((S,), dtype=torch.int32, device=DEV).index_add_(0, src, kept.to(torch.int32))
+    valid = col < held[:, None]
+    delta = torch.where(valid, (children - 1)[:, None], 0).to(torch.int32)
+    refs = refs.clone().index_add_(0, table.clamp(min=0).long().flatten(), delta.flatten())
+    lens = torch.where(kept, lens[src], 0)
+    held = (lens + page - 1) // page
+    table = torch.where(col < held[:, None], table[src], -1)
+    result = []
+    if case["new"]:
+        count = state["counts"].clamp(min=0)
+        after = (lens + count + page - 1) // page
+        last = table.gather(1, (held - 1).clamp(min=0).long()[:, None])[:, 0].clamp(min=0).long()
+        copy = (count > 0) & (lens % page != 0) & (refs[last] > 1)
+        fits = after <= cols
+        need = torch.where(fits, after - held + copy, 0)
+        upto = need.cumsum(0)
+        free = refs == 0
+        granted = fits & ((need == 0) | (upto <= free.sum()))
+        copy &= granted
+        order = torch.where(free, free.cumsum(0) - 1, P)
+        ids = torch.zeros((P + 1,), dtype=torch.int32, device=DEV)
+        ids[order] = torch.arange(P, dtype=torch.int32, device=DEV)
+        new = granted[:, None] & (((col >= held[:, None]) & (col < after[:, None]))
+                                  | (copy[:, None] & (col == held[:, None] - 1)))
+        at = (upto - need)[:, None] + new.cumsum(1) - 1
+        table = torch.where(new, ids[at.clamp(0, P)], table)
+        rows = copy.nonzero()[:, 0]
+        old, fresh = last[rows], table[rows, held[rows].long() - 1].long()
+        refs.index_add_(0, table.clamp(min=0).long().flatten(), new.to(torch.int32).flatten())
+        refs.index_add_(0, last, -copy.to(torch.int32))
+        lens = torch.where(granted, lens + count, lens)
+        for pool in state["pools"]:
+            pool[fresh] = pool[old]
+        result.append(granted)
+    if case["compact"]:
+        live = refs > 0
+        n = live.sum()
+        ids = torch.arange(P, device=DEV)
+        to, fro = (~live & (ids < n)).nonzero()[:, 0], (live & (ids >= n)).nonzero()[:, 0]
+        where = torch.arange(P, dtype=torch.int32, device=DEV)
+        where[fro] = to.to(torch.int32)
+        table = torch.where(table >= 0, where[table.clamp(min=0).long()], -1)
+        refs[to] = refs[fro]
+        refs[fro] = 0
+        for pool in state["pools"]:
+            pool[to] = pool[fro]
+        result.append(n.to(torch.int32).view(1))
+    out_table, out_lens, out_refs = state["work"]
+    out_table.copy_(table)
+    out_lens.copy_(lens)
+    out_refs.copy_(refs)
+    return (out_table, out_lens, out_refs) + tuple(result) + tuple(state["pools"])
+
+
+# ------------------------------------------------------------------- exact --
+
+def exact(case, seed):
+    """The definition in 64 bits; None for the page tables (whole numbers)."""
+    if case["kind"] == "pages":
+        return None
+    state = prepare(case, seed)
+    return _exact_attention(state) if case["kind"] == "attention" else _exact_qk(state)
+
+
+def _exact_attention(state):
+    case = state["case"]
+    H, G, D, page = case["kv_heads"], case["groups"], case["dim"], case["page"]
+    out, lse = state["out"].double(), state["lse"].double()
+    for s, n in enumerate(state["lens_host"]):
+        lo, hi = state["start_host"][s], state["start_host"][s + 1]
+        row = torch.arange(n, device=DEV)
+        for h in range(H):
+            if page:
+                ids = state["table"][s].long()[row // page]
+                k, v = state["k"][ids, h, row % page].double(), state["v"][ids, h, row % page].double()
+            else:
+                k, v = state["k"][s, h, :n].double(), state["v"][s, h, :n].double()
+            for a in range(lo, hi, 1024):
+                b = min(hi, a + 1024)
+                pos = (n - hi + torch.arange(a, b, device=DEV))[:, None]
+                hidden = row[None] > pos
+                if case["window"]:
+                    hidden |= (row[None] <= pos - case["window"]) & (row[None] >= case["sinks"])
+                for g in range(h * G, h * G + G):
+                    x = (state["q"][a:b, g].double() @ k.T) / math.sqrt(D)
+                    x[hidden] = -math.inf
+                    lse[a:b, g] = torch.logsumexp(x, -1)
+                    out[a:b, g] = torch.softmax(x, -1) @ v
+    return out, lse
+
+
+def _exact_qk(state):
+    case = state["case"]
+    n, r = state["start_host"][-1], case["rotary"]
+    turn = torch.polar(torch.ones((n, r // 2), dtype=torch.float64, device=DEV),
+                       state["positions"][:n].double()[:, None] * state["inv_freq"].double()[None])
+
+    def one(x, w):
+        y = x[:n].double()
+        if w is not None:
+            y = y / torch.sqrt((y ** 2).sum(-1, keepdim=True) / y.shape[-1] + EPS) * w.double()
+        even, odd = (slice(0, r, 2), slice(1, r, 2)) if case["interleaved"] else (slice(0, r // 2), slice(r // 2, r))
+        z = torch.complex(y[..., even], y[..., odd]) * turn[:, None]
+        y[..., even], y[..., odd] = z.real, z.imag
+        return y
+
+    q = state["q_out"].double()
+    q[:n] = one(state["q"], state["qw"])
+    k = one(state["k"], state["kw"])
+    if not case["page"]:
+        keys = state["k_out"].double()
+        keys[:n] = k
+        return q, keys
+    kp, vp = state["key_pages"].double(), state["value_pages"].double()
+    seq = 0
+    for t in range(len(state["lens_host"])):
+        lo, hi = state["start_host"][t], state["start_host"][t + 1]
+        at = state["positions"][lo:hi].long()
+        ids = state["table"][seq + t].long()[at // case["page"]]
+        kp[ids, :, at % case["page"]] = k[lo:hi]
+        vp[ids, :, at % case["page"]] = state["v"][lo:hi].double()
+    return q, kp, vp
+
+
+# -------------------------------------------------------------------- work --
+
+def work(case):
+    return {"attention": _work_attention, "qk": _work_qk, "pages": _work_pages}[case["kind"]](case)
+
+
+def _work_attention(case):
+    H, G, D, window, sinks = case["kv_heads"], case["groups"], case["dim"], case["window"], case["sinks"]
+    pairs = rows = tokens = 0
+    for n, m in zip(_ints(case["lens"]), _ints(case["news"])):
+        tokens += m
+        first = n - m
+        if not window:
+            pairs += m * first + m * (m + 1) // 2
+            rows += n
+            continue
+        for p in range(first, n):
+            low = max(0, p - window + 1)
+            pairs += p + 1 - low + min(sinks, low)
+        low = max(0, first - window + 1)
+        rows += n - low + min(sinks, low)
+    return {"bytes": 2 * D * (2 * tokens * H * G + 2 * rows * H) + 4 * tokens * H * G, "flops": 4 * D * H * G * pairs}
+
+
+def _work_qk(case):
+    H, G, D = case["kv_heads"], case["groups"], case["dim"]
+    tokens = sum(_ints(case["news"]))
+    heads = H * G + (2 * H if case["page"] else H)
+    return {"bytes": 2 * 2 * D * heads * tokens, "flops": 8 * D * (H * G + H) * tokens}
+
+
+def _work_pages(case):
+    """Tables and counts read and written once; copied pages are at least one
+    per forked beam, or a sixth of the live ones (what a third freed leaves
+    above the new end)."""
+    lens, page = _ints(case["lens"]), case["page"]
+    held = sum(-(-n // page) for n in lens)
+    size = 2 * case["layers"] * case["kv_heads"] * page * case["dim"] * 2
+    moved = held // 6 if case["compact"] else sum(1 for n in lens if n % page) // 2
+    return {"bytes": 2 * 4 * held + 2 * moved * size, "flops": 0}
