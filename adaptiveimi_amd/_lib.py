@@ -99,6 +99,22 @@ class HostcacheGatherArgs(ctypes.Structure):
                 ("n_rows", _vp), ("sel_cap", _i32)]
 
 
+class PagedBatchArgs(ctypes.Structure):
+    _fields_ = [("page_table", _vp), ("table_stride", _i64), ("max_pages", _i32), ("n_pages", _i32),
+                ("page_size", _i32), ("lens", _vp), ("query_start", _vp), ("n_seqs", _i32), ("n_tokens", _i32),
+                ("max_query", _i32), ("max_len", _i32)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatchArgs), ("dtype", _i32), ("kv_heads", _i32), ("groups", _i32), ("dim", _i32),
+                ("query", _vp), ("query_token_stride", _i64), ("query_head_stride", _i64),
+                ("keys", _vp), ("values", _vp), ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("scale", _f32), ("window", _i32), ("sinks", _i32),
+                ("out", _vp), ("out_token_stride", _i64), ("out_head_stride", _i64),
+                ("out_lse", _vp), ("lse_token_stride", _i64),
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 EXPORTS = {
     "imi_last_error": (ctypes.c_char_p, []),
     "imi_version": (ctypes.c_int, []),
@@ -130,6 +146,9 @@ EXPORTS = {
     "imi_hostcache_admit": (ctypes.c_int, [_vp, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
                                            _vp]),
     "imi_host_device_pointer": (ctypes.c_int, [_vp, ctypes.POINTER(_vp)]),
+    "imi_paged_attention_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs),
+                                                          ctypes.POINTER(ctypes.c_size_t)]),
+    "imi_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs), _vp]),
 }
 
 _lib = None

@@ -1,0 +1,1116 @@
+// Attention of a batch of new tokens over a paged KV cache on gfx950.
+//
+// Sequence s has len rows, of which the last n = start[s + 1] - start[s] are
+// new; its new token i stands at position p = len - n + i and sees the rows
+//   V(p) = { j : 0 <= j <= p, and j > p - window or j < sinks }
+// (window 0: no limit).  For query head x of KV head h = x / G:
+//   out = sum_{j in V} w_j v_j,  w = softmax over V of scale * q . k_j,
+//   lse = ln sum_{j in V} exp(scale * q . k_j);  V empty: out 0, lse -inf.
+//
+// The G query heads of a KV head and the new tokens of a sequence form the
+// rows r = i * G + g of one problem.  Both kernels compute the transposed
+// scores S^T = K Q^T, so that a lane holds one query row (a column of S^T):
+// the running maximum, the sum and the rescaling of that row need no lane
+// exchange but the last steps of the maximum, and P^T in the registers of S^T
+// is the second operand of O^T += V^T P^T as it stands: the keys of a matrix
+// instruction are summed over, so their order is free, and V^T is read from
+// LDS (ds_read_b64_tr_b16) in the order that the registers of S^T have.
+//
+// The rows that a tile of new tokens sees are numbered without gaps: the
+// first min(sinks, lo) rows, then lo .. hi - 1, lo being the first row inside
+// the window of the tile's first token.
+//
+// Softmax statistics and sums are fp32 in base 2; P is rounded to the cache's
+// type for the matrix instruction (half a step of that type relative to each
+// weight, the rounding that the output itself takes), unnormalised and at
+// most 2^8: the running maximum moves only when it grows by more than 8 in
+// base 2, which leaves the sums exact to fp32 and saves most rescalings.
+#include <algorithm>
+
+#include "imi_common.hpp"
+
+namespace imi {
+namespace {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(16))) float f32x16_t;
+typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 8.0f;   // growth of a running maximum (base 2) that is left unapplied
+
+// The two element types: pairs rounded to nearest even, matrix instructions.
+struct BF16 {
+    typedef bf16x8_t v8;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef __attribute__((ext_vector_type(2))) float f2;
+        typedef __attribute__((ext_vector_type(2))) __bf16 b2;
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+    }
+    static __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+};
+struct FP16 {
+    typedef f16x8_t v8;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+        return __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
+    }
+    static __device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
+    }
+};
+
+// LDS row of D elements plus a pad: eight rows' 16-byte pieces (the K reads)
+// and four rows' 32-byte pieces (the transposed V reads) fall on different
+// banks.
+template <int D>
+constexpr int kRow = D == 128 ? 144 : 72;
+
+struct PagedParams {
+    const uint16_t* q;
+    const uint16_t* k;
+    const uint16_t* v;
+    uint16_t* out;
+    float* lse;                // or null
+    const int32_t* table;      // or null: sequence s's rows are "page" s
+    const int32_t* lens;
+    const int32_t* start;
+    int64_t q_ts, q_hs;        // strides in elements: token, head
+    int64_t o_ts, o_hs;
+    int64_t l_ts;              // lse token stride (heads are adjacent)
+    int64_t page_s, head_s, tok_s;
+    int64_t table_s;
+    int S, N, H, G;
+    int n_pages;               // pages in the pool
+    int page_shift;            // 31 with no table
+    int capacity;              // rows a sequence can have
+    int window, sinks;
+    float c;                   // scale * log2(e)
+    int min_rows, max_rows;    // rows (n * G) of the sequences this launch takes
+    int W;                     // workgroups that share the work
+    float* part;               // [2 W][rows][D]
+    float* part_ml;            // [2 W][rows][2]
+    int32_t* plan;             // tile kernel: see plan_kernel
+    int slots;                 // tile kernel: tiles that the plan can hold
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// New tokens [t0, t0 + n) and length of sequence s, forced into the tensors.
+struct Seq {
+    int t0, n, len;
+};
+__device__ __forceinline__ Seq seq_of(const PagedParams& a, int s) {
+    const int b = clampi(a.start[s], 0, a.N), e = clampi(a.start[s + 1], 0, a.N);
+    return Seq{b, max(e - b, 0), clampi(a.lens[s], 0, a.capacity)};
+}
+
+// Rows visible to the new tokens at positions p0 .. p1: [0, sink) and [lo, hi).
+struct Span {
+    int lo, hi, sink;
+    __device__ __forceinline__ int count() const { return sink + hi - lo; }
+    __device__ __forceinline__ int row(int v) const { return v < sink ? v : v - sink + lo; }
+};
+__device__ __forceinline__ Span span_of(const PagedParams& a, int len, int p0, int p1) {
+    Span r;
+    r.hi = clampi(p1 + 1, 0, len);
+    r.lo = a.window > 0 ? clampi(p0 - a.window + 1, 0, r.hi) : 0;
+    r.sink = min(a.sinks, r.lo);
+    return r;
+}
+
+// Element offset of cached row j of sequence s (head offset not included).
+// A page id outside the pool is forced into it.
+__device__ __forceinline__ int page_of(const PagedParams& a, int s, int j) {
+    return a.table ? a.table[static_cast<int64_t>(s) * a.table_s + (j >> a.page_shift)] : s;
+}
+__device__ __forceinline__ int64_t row_offset(const PagedParams& a, int page, int j) {
+    const int slot = j & ((1u << a.page_shift) - 1u);
+    return static_cast<int64_t>(clampi(page, 0, a.n_pages - 1)) * a.page_s + static_cast<int64_t>(slot) * a.tok_s;
+}
+
+__device__ __forceinline__ void wave_lds_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ u32x4_t load16(const uint16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
+
+__device__ __forceinline__ s16x4_t read_tr(const uint16_t* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(p));
+}
+__device__ __forceinline__ u32x4_t join(s16x4_t a, s16x4_t b) {
+    return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ float exp2_weight(float m, float M, float c) {
+    return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
+}
+
+// ---------------------------------------------------------- few rows ------
+// Sequences of at most 16 NB rows (decode, verification of a few tokens):
+// the rows fit one matrix tile, so K and V are streamed once and the kernel
+// is bound by that stream.  Work is counted in units of kUnit cached rows of
+// one (sequence, KV head); the units of all, in order, are cut into W equal
+// ranges, one per workgroup, whatever the lengths (each workgroup adds the
+// lengths up itself: no host knows them).  A workgroup whose range covers a
+// whole (sequence, head) writes its output; the others (its first and its
+// last at most) write a partial that few_merge_kernel joins in order.
+constexpr int kFewWaves = 4;
+constexpr int kFewTile = 32;                       // rows of K / V per wave and step
+constexpr int kUnit = kFewTile * kFewWaves;
+
+__device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
+    const int rows = q.n * a.G;
+    if (q.n <= 0 || rows < a.min_rows || rows > a.max_rows) return 0;
+    const Span sp = span_of(a, q.len, max(q.len - q.n, 0), q.len - 1);
+    return max((sp.count() + kUnit - 1) / kUnit, 1);
+}
+
+// Units of all sequences (per KV head), and where unit `at` falls: the
+// sequence and the units before it.
+struct FewPlace {
+    int s;
+    int64_t before;
+};
+__device__ __forceinline__ int64_t few_total(const PagedParams& a) {
+    int64_t total = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        const int s = s0 + lane_id();
+        total += wave_sum_i(s < a.S ? few_units(a, seq_of(a, s)) : 0);
+    }
+    return total;
+}
+// First sequence whose units (times H) reach past `at`; units before it.
+__device__ __forceinline__ FewPlace few_find(const PagedParams& a, int64_t at) {
+    int64_t before = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        const int s = s0 + lane_id();
+        const int u = s < a.S ? few_units(a, seq_of(a, s)) : 0;
+        const int incl = wave_incl_scan(u);
+        const uint64_t past = __ballot((before + incl) * a.H > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            return FewPlace{s0 + l, before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(u, l)};
+        }
+        before += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return FewPlace{a.S, before};
+}
+
+template <typename T, int D, int NB>
+__global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) {
+    constexpr int KK = D / 32;     // matrix instructions over the head dim
+    constexpr int DB = D / 16;     // output blocks of 16 dims
+    constexpr int LR = kRow<D>;
+    constexpr int kWaveLds = kFewTile * LR > 16 * D * 2 ? kFewTile * LR : 16 * D * 2;   // u16
+    __shared__ uint16_t s_buf[kFewWaves * kWaveLds];
+    __shared__ float s_ml[kFewWaves][16 * NB][2];
+    const int tid = threadIdx.x, lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ln = lane & 15, lg = lane >> 4;
+    uint16_t* const sv = s_buf + wave * kWaveLds;
+
+    int64_t g0, g1;   // this workgroup's units
+    FewPlace at;
+    if (direct) {     // a workgroup per (sequence, head): nothing to join
+        at.s = blockIdx.x / a.H;
+        at.before = 0;
+        const int u = few_units(a, seq_of(a, at.s));
+        if (u == 0) return;
+        g0 = static_cast<int64_t>(blockIdx.x % a.H) * u;
+        g1 = g0 + u;
+    } else {
+        const int64_t U = few_total(a) * a.H;
+        g0 = U * blockIdx.x / a.W;
+        g1 = U * (blockIdx.x + 1) / a.W;
+        if (g0 >= g1) return;
+        at = few_find(a, g0);
+    }
+    int s = at.s;
+    int64_t base = at.before * a.H;   // units before sequence s, all heads
+    bool first = true;
+    while (g0 < g1) {
+        const Seq sq = seq_of(a, s);
+        const int units = few_units(a, sq);
+        if (g0 >= base + static_cast<int64_t>(units) * a.H) {   // next sequence
+            base += static_cast<int64_t>(units) * a.H;
+            ++s;
+            continue;
+        }
+        const int h = static_cast<int>((g0 - base) / units);
+        const int u0 = static_cast<int>(g0 - base - static_cast<int64_t>(h) * units);
+        const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + g1 - g0));
+        const int rows = sq.n * a.G;
+        const int p0 = sq.len - sq.n;
+        const Span sp = span_of(a, sq.len, max(p0, 0), sq.len - 1);
+        const int vis = sp.count();
+
+        // queries: row r = 16 b + ln of lane, dims 32 c + 8 lg ..
+        u32x4_t qf[NB][KK];
+        int pos[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const int r = 16 * b + ln;
+            const int i = r / a.G;
+            pos[b] = r < rows ? p0 + i : -1;
+            const int rr = min(r, rows - 1);
+            const uint16_t* qp = a.q + static_cast<int64_t>(sq.t0 + rr / a.G) * a.q_ts +
+                                 static_cast<int64_t>(h * a.G + rr % a.G) * a.q_hs + 8 * lg;
+#pragma unroll
+            for (int c = 0; c < KK; ++c) qf[b][c] = load16(qp + 32 * c);
+        }
+        f32x4_t acc[NB][DB];
+        float m[NB], l[NB];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            m[b] = -INFINITY;
+            l[b] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) acc[b][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s + 8 * lg;
+        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * lg;
+        // lane's two rows of a step's tile: ln and 16 + ln
+        auto row_at = [&](int u, int e) { return min(u * kUnit + wave * kFewTile + 16 * e + ln, vis - 1); };
+        int id[2];
+        auto fetch_ids = [&](int u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) id[e] = page_of(a, s, sp.row(row_at(u, e)));
+        };
+        u32x4_t kb[2][KK], vb[2][KK];
+        auto fetch = [&](int u) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int64_t o = row_offset(a, id[e], sp.row(row_at(u, e)));
+#pragma unroll
+                for (int c = 0; c < KK; ++c) kb[e][c] = load16(kh + o + 32 * c);
+#pragma unroll
+                for (int c = 0; c < KK; ++c) vb[e][c] = load16(vh + o + 32 * c);
+            }
+        };
+        // a wave with no row in its share of a unit still runs the step (all
+        // of its keys masked): only a unit's tail has such waves
+        const bool any = vis > 0;
+        if (any) {
+            fetch_ids(u0);
+            fetch(u0);
+            fetch_ids(min(u0 + 1, u1 - 1));
+        }
+        for (int u = u0; any && u < u1; ++u) {
+            const int v0 = u * kUnit + wave * kFewTile;   // first row of the tile
+            if (v0 + kFewTile > vis) {   // rows past the end weigh nothing: no NaN may enter through V
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (v0 + 16 * e + ln >= vis)
+#pragma unroll
+                        for (int c = 0; c < KK; ++c) vb[e][c] = u32x4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int c = 0; c < KK; ++c)
+                    *reinterpret_cast<u32x4_t*>(sv + (16 * e + ln) * LR + 32 * c + 8 * lg) = vb[e][c];
+            f32x4_t sc[NB][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    sc[b][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < KK; ++c) sc[b][e] = T::mma16(kb[e][c], qf[b][c], sc[b][e]);
+                }
+            if (u + 1 < u1) {
+                fetch(u + 1);
+                fetch_ids(min(u + 2, u1 - 1));
+            }
+            wave_lds_sync();
+            // lane: keys v0 + 16 e + 4 lg + i of row ln
+            const bool edge = v0 + kFewTile > vis;
+            u32x4_t pf[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                if (edge || sq.n > 1 || NB > 1) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int v = v0 + 16 * e + 4 * lg + i;
+                            const int j = sp.row(v);
+                            const bool seen = v < vis && j <= pos[b] &&
+                                              (a.window == 0 || j > pos[b] - a.window || j < a.sinks);
+                            sc[b][e][i] = seen ? sc[b][e][i] : -INFINITY;
+                        }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[b][e][i]);
+                mx = fmaxf(mx, xor16(mx));
+                mx = fmaxf(mx, xor32(mx));
+                const bool grow = (mx - m[b]) * a.c > kSlack;
+                if (__builtin_amdgcn_ballot_w64(grow)) {
+                    const float f = grow ? __builtin_amdgcn_exp2f((m[b] - mx) * a.c) : 1.0f;
+                    m[b] = grow ? mx : m[b];
+                    l[b] *= f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[b][d] *= f;
+                }
+                const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+                float p[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 2][i & 3], a.c, -mc));
+                l[b] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                pf[b] = u32x4_t{T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+            }
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                const uint16_t* vp = sv + (4 * lg + (ln >> 2)) * LR + 16 * d + 4 * (ln & 3);
+                const u32x4_t vt = join(read_tr(vp), read_tr(vp + 16 * LR));
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[b][d] = T::mma16(vt, pf[b], acc[b][d]);
+            }
+            wave_lds_sync();
+        }
+        // join the waves: sums over the lane groups, then LDS, block by block
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            l[b] += xor16(l[b]);
+            l[b] += xor32(l[b]);
+            if (lg == 0) {
+                s_ml[wave][16 * b + ln][0] = m[b];
+                s_ml[wave][16 * b + ln][1] = l[b];
+            }
+        }
+        const bool whole = u0 == 0 && u1 == units;
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
+        float* const so = reinterpret_cast<float*>(sv);   // [16 rows][D]
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (16 * b >= rows) break;
+            if (b) __syncthreads();
+            // O^T: lane has dims 16 d + 4 lg + i of row ln
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+                *reinterpret_cast<f32x4_t*>(so + ln * D + 16 * d + 4 * lg) = acc[b][d];
+            __syncthreads();
+            for (int x = tid; x < 16 * D / 4; x += 256) {
+                const int rr = x / (D / 4), d4 = x % (D / 4), r = 16 * b + rr;
+                if (r >= rows) break;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kFewWaves; ++w) M = fmaxf(M, s_ml[w][r][0]);
+                float L = 0.0f;
+                f32x4_t A = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int w = 0; w < kFewWaves; ++w) {
+                    const float wt = exp2_weight(s_ml[w][r][0], M, a.c);
+                    L += s_ml[w][r][1] * wt;
+                    A += *reinterpret_cast<const f32x4_t*>(reinterpret_cast<float*>(s_buf + w * kWaveLds) + rr * D +
+                                                           4 * d4) *
+                         wt;
+                }
+                if (whole) {
+                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                    const int64_t t = sq.t0 + r / a.G;
+                    const int x_head = h * a.G + r % a.G;
+                    uint2 o;
+                    o.x = T::pack(A[0] * inv, A[1] * inv);
+                    o.y = T::pack(A[2] * inv, A[3] * inv);
+                    *reinterpret_cast<uint2*>(a.out + t * a.o_ts + x_head * a.o_hs + 4 * d4) = o;
+                    if (a.lse && d4 == 0)
+                        a.lse[t * a.l_ts + x_head] = L == 0.0f ? -INFINITY : (M * a.c + __log2f(L)) * kLn2;
+                } else {
+                    *reinterpret_cast<f32x4_t*>(a.part + (slot * a.max_rows + r) * D + 4 * d4) = A;
+                    if (d4 == 0) {
+                        a.part_ml[(slot * a.max_rows + r) * 2] = M;
+                        a.part_ml[(slot * a.max_rows + r) * 2 + 1] = L;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        g0 += u1 - u0;
+        first = false;
+    }
+}
+
+// What the joins share.  Cut w lies at unit U w / W; a (sequence, head) or
+// tile with units [lo, hi) was shared when a cut falls inside, and the join
+// belongs to the first such cut, so a launch over the cuts covers all of them
+// whatever the batch is.  Range w - 1 holds lo, the ranges from w on continue;
+// each wrote its first partial, but w - 1 its second if it begins before lo.
+struct Join {
+    int w;             // first cut inside
+    int64_t lo, hi;
+};
+__device__ __forceinline__ int64_t cut(int64_t U, int64_t w, int W) { return U * w / W; }
+
+template <int D>
+struct Partial {
+    float M = -INFINITY, L = 0.0f;
+    f32x4_t A = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    __device__ __forceinline__ void add(float m, float l, f32x4_t x, float c) {
+        const float Mn = fmaxf(M, m);
+        const float f0 = exp2_weight(M, Mn, c), f1 = exp2_weight(m, Mn, c);
+        L = L * f0 + l * f1;
+        A = A * f0 + x * f1;
+        M = Mn;
+    }
+    // partials first, first + step, ... of a join, in order
+    __device__ __forceinline__ void gather(const PagedParams& a, int64_t U, const Join& j, int cap, int r, int d4,
+                                           int first, int step) {
+        for (int w = j.w - 1 + first; w < a.W && cut(U, w, a.W) < j.hi; w += step) {
+            const int64_t b = cut(U, w, a.W);
+            if (b == cut(U, w + 1, a.W)) continue;   // an empty range
+            const int64_t e = (2 * static_cast<int64_t>(w) + (b < j.lo ? 1 : 0)) * cap + r;
+            add(a.part_ml[2 * e], a.part_ml[2 * e + 1], *reinterpret_cast<const f32x4_t*>(a.part + e * D + 4 * d4),
+                a.c);
+        }
+    }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void write_row(const PagedParams& a, const Partial<D>& p, int64_t tok, int x_head, int d4) {
+    const float inv = p.L == 0.0f ? 0.0f : 1.0f / p.L;
+    uint2 o;
+    o.x = T::pack(p.A[0] * inv, p.A[1] * inv);
+    o.y = T::pack(p.A[2] * inv, p.A[3] * inv);
+    *reinterpret_cast<uint2*>(a.out + tok * a.o_ts + x_head * a.o_hs + 4 * d4) = o;
+    if (a.lse && d4 == 0) a.lse[tok * a.l_ts + x_head] = p.L == 0.0f ? -INFINITY : (p.M * a.c + __log2f(p.L)) * kLn2;
+}
+
+// One workgroup per (cut, row): a row has many partials (a long sequence is
+// cut often), which D / 4 threads at a time take in turn.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void few_merge_kernel(PagedParams a) {
+    constexpr int Q = D / 4;            // threads that hold a row
+    constexpr int P = 256 / Q;          // partials in flight
+    __shared__ float s_ml[P][2];
+    __shared__ float s_acc[P][D];
+    const int w = blockIdx.x + 1, r = blockIdx.y;
+    const int64_t U = few_total(a) * a.H;
+    const int64_t at = cut(U, w, a.W);
+    if (at >= U || at == cut(U, w - 1, a.W)) return;
+    const FewPlace f = few_find(a, at);
+    const Seq sq = seq_of(a, f.s);
+    const int units = few_units(a, sq);
+    const int h = static_cast<int>((at - f.before * a.H) / units);
+    Join j;
+    j.w = w;
+    j.lo = f.before * a.H + static_cast<int64_t>(h) * units;
+    j.hi = j.lo + units;
+    if (r >= sq.n * a.G || at == j.lo || cut(U, w - 1, a.W) > j.lo) return;
+    const int tid = threadIdx.x, d4 = tid % Q, g = tid / Q;
+    Partial<D> p;
+    p.gather(a, U, j, a.max_rows, r, d4, g, P);
+    if (d4 == 0) {
+        s_ml[g][0] = p.M;
+        s_ml[g][1] = p.L;
+    }
+    *reinterpret_cast<f32x4_t*>(&s_acc[g][4 * d4]) = p.A;
+    __syncthreads();
+    if (g == 0) {
+        Partial<D> t;
+        for (int x = 0; x < P; ++x)
+            t.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
+        write_row<T, D>(a, t, sq.t0 + r / a.G, h * a.G + r % a.G, d4);
+    }
+}
+
+// --------------------------------------------------------- many rows ------
+// Sequences of more rows (prefill chunks): tiles of kTileRows rows of one
+// (sequence, KV head), 32 per wave; the waves share each step's kStep rows of
+// K and V in LDS.  The steps of all tiles, KV head by KV head, are again cut
+// into W equal ranges, so a causal triangle, a short prompt and a chunk over
+// a long prefix load the chip evenly; partials as above.
+constexpr int kTileRows = 128;
+constexpr int kStep = 64;
+
+__device__ __forceinline__ int seq_tiles(const PagedParams& a, const Seq& q) {
+    const int64_t rows = static_cast<int64_t>(q.n) * a.G;
+    if (q.n <= 0 || rows < a.min_rows || rows > a.max_rows) return 0;
+    return static_cast<int>((rows + kTileRows - 1) / kTileRows);
+}
+
+__device__ __forceinline__ Span tile_span(const PagedParams& a, const Seq& q, int first) {
+    const int p0 = q.len - q.n;
+    const int i0 = first / a.G;
+    const int i1 = min((first + kTileRows - 1) / a.G, q.n - 1);
+    return span_of(a, q.len, max(p0 + i0, 0), p0 + i1);
+}
+
+// The plan: tiles in use; per tile its sequence and first row, and the
+// inclusive prefix of the steps; per sequence the inclusive prefix of the
+// tiles (scratch of plan_kernel).
+struct Plan {
+    int32_t* n;
+    int2* tiles;       // [slots]
+    int64_t* steps;    // [slots]
+    int32_t* seqs;     // [S]
+};
+__host__ __device__ inline size_t plan_bytes(int slots, int S) { return 16 + size_t(slots) * 16 + size_t(S) * 4; }
+__device__ __forceinline__ Plan plan_of(const PagedParams& a) {
+    Plan p;
+    p.n = a.plan;
+    p.tiles = reinterpret_cast<int2*>(a.plan + 4);
+    p.steps = reinterpret_cast<int64_t*>(p.tiles + a.slots);
+    p.seqs = reinterpret_cast<int32_t*>(p.steps + a.slots);
+    return p;
+}
+
+template <typename V>
+__device__ __forceinline__ V block_incl_scan(V x, V* s_wave, V& total) {
+    const int lane = lane_id(), wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const V y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) s_wave[wave] = x;
+    __syncthreads();
+    V before = 0;
+    total = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
+        if (w < wave) before += s_wave[w];
+        total += s_wave[w];
+    }
+    return x + before;
+}
+
+__global__ __launch_bounds__(1024) void plan_kernel(PagedParams a) {
+    __shared__ int64_t s_wave[16];
+    const Plan p = plan_of(a);
+    int64_t n = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 1024) {
+        const int s = s0 + threadIdx.x;
+        int64_t total;
+        const int64_t incl = block_incl_scan<int64_t>(s < a.S ? seq_tiles(a, seq_of(a, s)) : 0, s_wave, total);
+        if (s < a.S) p.seqs[s] = static_cast<int32_t>(min(n + incl, static_cast<int64_t>(a.slots)));
+        n += total;
+    }
+    const int n_tiles = static_cast<int>(min(n, static_cast<int64_t>(a.slots)));
+    __syncthreads();   // the prefix is read by other threads of this workgroup
+    int64_t before = 0;
+    for (int t0 = 0; t0 < n_tiles; t0 += 1024) {
+        const int t = t0 + threadIdx.x;
+        int64_t u = 0;
+        if (t < n_tiles) {
+            int lo = 0, hi = a.S - 1;   // first sequence whose prefix is past t
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (p.seqs[mid] > t) hi = mid;
+                else lo = mid + 1;
+            }
+            const int row = (t - (lo ? p.seqs[lo - 1] : 0)) * kTileRows;
+            p.tiles[t] = make_int2(lo, row);
+            u = max((tile_span(a, seq_of(a, lo), row).count() + kStep - 1) / kStep, 1);
+        }
+        int64_t total;
+        const int64_t incl = block_incl_scan<int64_t>(u, s_wave, total);
+        if (t < n_tiles) p.steps[t] = before + incl;
+        before += total;
+    }
+    if (threadIdx.x == 0) *p.n = n_tiles;
+}
+
+// First tile whose steps reach past x.
+__device__ __forceinline__ int find_tile(const int64_t* steps, int n, int64_t x) {
+    int lo = 0, hi = n;   // steps[lo - 1] <= x < steps[hi - 1]
+    while (hi - lo > 1) {
+        const int stride = (hi - lo + 63) / 64;
+        const int i = lo + (lane_id() + 1) * stride - 1;
+        const uint64_t past = __ballot(i >= hi - 1 || steps[i] > x);
+        const int l = __builtin_ctzll(past);
+        const int nlo = lo + l * stride;
+        hi = min(hi, nlo + stride);
+        lo = nlo;
+    }
+    return lo;
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void tile_kernel(PagedParams a) {
+    constexpr int KK = D / 16;
+    constexpr int DB = D / 32;
+    constexpr int LR = kRow<D>;
+    constexpr int CH = D / 8;               // 16-byte pieces of a row
+    constexpr int RP = 256 / CH;            // rows that one load of the workgroup covers
+    constexpr int NR = kStep / RP;
+    __shared__ uint16_t s_k[2][kStep * LR];
+    __shared__ uint16_t s_v[2][kStep * LR];
+    const int tid = threadIdx.x, lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q32 = lane & 31, hi = lane >> 5, ln = lane & 15;
+    const int l_row = tid / CH, l_ch = tid % CH;
+
+    const Plan plan = plan_of(a);
+    const int n_tiles = *plan.n;
+    const int64_t* const steps = plan.steps;
+    if (n_tiles == 0) return;
+    const int64_t per_head = steps[n_tiles - 1];
+    const int64_t U = per_head * a.H;
+    // workgroups go round robin over the 8 dies: die x takes the x-th eighth
+    // of the steps, so that its workgroups read the same head's K and V
+    const int wg = a.W % 8 == 0 ? (blockIdx.x % 8) * (a.W / 8) + blockIdx.x / 8 : blockIdx.x;
+    int64_t g0 = U * wg / a.W;
+    const int64_t g1 = U * (wg + 1) / a.W;
+    bool first = true;
+    int h = static_cast<int>(g0 / per_head);
+    int t = g0 < g1 ? find_tile(steps, n_tiles, g0 - h * per_head) : 0;
+    while (g0 < g1) {
+        const int2 tile = plan.tiles[t];
+        const int64_t t_lo = h * per_head + (t ? steps[t - 1] : 0);
+        const int units = static_cast<int>(h * per_head + steps[t] - t_lo);
+        const int u0 = static_cast<int>(g0 - t_lo);
+        const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + g1 - g0));
+        const int s = tile.x;
+        const Seq sq = seq_of(a, s);
+        const int64_t rows = static_cast<int64_t>(sq.n) * a.G;
+        const int p0 = sq.len - sq.n;
+        const Span sp = tile_span(a, sq, tile.y);
+        const int vis = sp.count();
+
+        // this lane's query row (both halves of the wave), dims 16 c + 8 hi ..
+        const int r = tile.y + wave * 32 + q32;
+        const bool live = r < rows;
+        const int rr = live ? r : static_cast<int>(rows) - 1;
+        const int tok = rr / a.G;
+        const int pos = live ? p0 + tok : -1;
+        const int64_t q_tok = sq.t0 + tok;
+        const int x_head = h * a.G + rr % a.G;
+        const uint16_t* qp = a.q + q_tok * a.q_ts + x_head * a.q_hs + 8 * hi;
+        u32x4_t qf[KK];
+#pragma unroll
+        for (int c = 0; c < KK; ++c) qf[c] = load16(qp + 16 * c);
+        // the wave's positions, for steps that need no mask
+        const int w_first = tile.y + wave * 32;
+        const bool idle = w_first >= rows;
+        const int p_min = p0 + min(w_first, static_cast<int>(rows) - 1) / a.G;
+        const int p_max = p0 + static_cast<int>(min(static_cast<int64_t>(w_first) + 31, rows - 1)) / a.G;
+
+        f32x16_t acc[DB];
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+
+        const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s + 8 * l_ch;
+        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * l_ch;
+        int id[NR];
+        auto row_at = [&](int u, int i) { return sp.row(min(u * kStep + l_row + RP * i, vis - 1)); };
+        auto fetch_ids = [&](int u) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) id[i] = page_of(a, s, row_at(u, i));
+        };
+        u32x4_t kb[NR], vb[NR];
+        auto fetch = [&](int u) {
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int64_t o = row_offset(a, id[i], row_at(u, i));
+                kb[i] = load16(kh + o);
+                vb[i] = load16(vh + o);
+            }
+        };
+        auto store = [&](int u) {
+            uint16_t* const sk = s_k[u & 1];
+            uint16_t* const sv = s_v[u & 1];
+            const bool tail = (u + 1) * kStep > vis;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int row = l_row + RP * i;
+                *reinterpret_cast<u32x4_t*>(sk + row * LR + 8 * l_ch) = kb[i];
+                // rows past the end weigh nothing: no NaN may enter through V
+                if (tail && u * kStep + row >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
+                *reinterpret_cast<u32x4_t*>(sv + row * LR + 8 * l_ch) = vb[i];
+            }
+        };
+        if (vis > 0) {
+            fetch_ids(u0);
+            fetch(u0);
+            fetch_ids(min(u0 + 1, u1 - 1));
+            store(u0);
+        }
+        for (int u = u0; vis > 0 && u < u1; ++u) {
+            const bool more = u + 1 < u1;
+            if (more) {
+                fetch(u + 1);
+                fetch_ids(min(u + 2, u1 - 1));
+            }
+            __syncthreads();
+            const uint16_t* const sk = s_k[u & 1];
+            const uint16_t* const sv = s_v[u & 1];
+            const int v0 = u * kStep;
+            const int j_lo = sp.row(v0), j_hi = sp.row(min(v0 + kStep, vis) - 1);
+            // a step whose rows none of the wave's tokens sees is skipped
+            const bool skip = idle || j_lo > p_max ||
+                              (a.window > 0 && v0 >= sp.sink && j_hi <= p_min - a.window);
+            if (!skip) {
+                f32x16_t sc[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) sc[e][i] = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < KK; ++c)
+                        sc[e] = T::mma32(load16(sk + (32 * e + q32) * LR + 16 * c + 8 * hi), qf[c], sc[e]);
+                }
+                // lane: keys v0 + 32 e + 8 (i / 4) + 4 hi + i % 4 of row q32
+                const bool full = v0 + kStep <= vis && j_hi <= p_min &&
+                                  (a.window == 0 || j_lo > p_max - a.window || j_hi < a.sinks) &&
+                                  w_first + 32 <= rows;
+                if (!full) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int v = v0 + 32 * e + 8 * (i >> 2) + 4 * hi + (i & 3);
+                            const int j = sp.row(v);
+                            const bool seen = v < vis && j <= pos &&
+                                              (a.window == 0 || j > pos - a.window || j < a.sinks);
+                            sc[e][i] = seen ? sc[e][i] : -INFINITY;
+                        }
+                }
+                float mx = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[e][i]);
+                mx = fmaxf(mx, xor32(mx));
+                const bool grow = (mx - m) * a.c > kSlack;
+                if (__builtin_amdgcn_ballot_w64(grow)) {
+                    const float f = grow ? __builtin_amdgcn_exp2f((m - mx) * a.c) : 1.0f;
+                    m = grow ? mx : m;
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) acc[d] *= f;
+                }
+                const float mc = m == -INFINITY ? 0.0f : m * a.c;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        sc[e][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e][i], a.c, -mc));
+                float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) ls[i & 3] += sc[e][i];
+                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const u32x4_t pf = u32x4_t{T::pack(sc[e][8 * c], sc[e][8 * c + 1]),
+                                                   T::pack(sc[e][8 * c + 2], sc[e][8 * c + 3]),
+                                                   T::pack(sc[e][8 * c + 4], sc[e][8 * c + 5]),
+                                                   T::pack(sc[e][8 * c + 6], sc[e][8 * c + 7])};
+                        const uint16_t* vp = sv + (32 * e + 16 * c + 4 * hi + (ln >> 2)) * LR +
+                                             16 * ((lane >> 4) & 1) + 4 * (ln & 3);
+#pragma unroll
+                        for (int d = 0; d < DB; ++d)
+                            acc[d] = T::mma32(join(read_tr(vp + 32 * d), read_tr(vp + 8 * LR + 32 * d)), pf, acc[d]);
+                    }
+            }
+            if (more) store(u + 1);
+        }
+        l += xor32(l);
+        if (live) {
+            if (u0 == 0 && u1 == units) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                uint16_t* const op = a.out + q_tok * a.o_ts + x_head * a.o_hs + 4 * hi;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint2 o;
+                        o.x = T::pack(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv);
+                        o.y = T::pack(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv);
+                        *reinterpret_cast<uint2*>(op + 32 * d + 8 * i) = o;
+                    }
+                if (a.lse && hi == 0)
+                    a.lse[q_tok * a.l_ts + x_head] = l == 0.0f ? -INFINITY : (m * a.c + __log2f(l)) * kLn2;
+            } else {
+                const int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * kTileRows + wave * 32 + q32;
+                float* const op = a.part + e * D + 4 * hi;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * i) =
+                            f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+                if (hi == 0) {
+                    a.part_ml[2 * e] = m;
+                    a.part_ml[2 * e + 1] = l;
+                }
+            }
+        }
+        __syncthreads();   // the next range's first store reuses the tiles
+        g0 += u1 - u0;
+        first = false;
+        if (++t == n_tiles) {
+            t = 0;
+            ++h;
+        }
+    }
+}
+
+// One workgroup per (cut, 256 / (D / 4) rows).
+template <typename T, int D>
+__global__ __launch_bounds__(256) void tile_merge_kernel(PagedParams a) {
+    constexpr int Q = D / 4;
+    const Plan plan = plan_of(a);
+    const int n_tiles = *plan.n;
+    if (n_tiles == 0) return;
+    const int64_t per_head = plan.steps[n_tiles - 1];
+    const int64_t U = per_head * a.H;
+    const int w = blockIdx.x + 1;
+    const int64_t at = cut(U, w, a.W);
+    if (at >= U || at == cut(U, w - 1, a.W)) return;
+    const int h = static_cast<int>(at / per_head);
+    const int t = find_tile(plan.steps, n_tiles, at - h * per_head);
+    const int2 tile = plan.tiles[t];
+    const Seq sq = seq_of(a, tile.x);
+    Join j;
+    j.w = w;
+    j.lo = h * per_head + (t ? plan.steps[t - 1] : 0);
+    j.hi = h * per_head + plan.steps[t];
+    const int r = blockIdx.y * (256 / Q) + threadIdx.x / Q, d4 = threadIdx.x % Q;
+    const int row = tile.y + r;
+    if (at == j.lo || cut(U, w - 1, a.W) > j.lo || row >= static_cast<int64_t>(sq.n) * a.G) return;
+    Partial<D> p;
+    p.gather(a, U, j, kTileRows, r, d4, 0, 1);
+    write_row<T, D>(a, p, sq.t0 + row / a.G, h * a.G + row % a.G, d4);
+}
+
+// ------------------------------------------------------------- host -------
+
+int validate_batch(const imi_paged_batch* b) {
+    IMI_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0, IMI_ERR_INVALID, "negative batch (n_seqs=%d, n_tokens=%d)",
+                b->n_seqs, b->n_tokens);
+    if (b->n_seqs == 0 || b->n_tokens == 0) return IMI_OK;
+    IMI_REQUIRE(b->lens && b->query_start, IMI_ERR_INVALID, "null lens or query_start");
+    IMI_REQUIRE(b->max_query >= 1, IMI_ERR_INVALID, "max_query=%d must be >= 1", b->max_query);
+    IMI_REQUIRE(b->n_pages >= 1, IMI_ERR_INVALID, "n_pages=%d must be >= 1", b->n_pages);
+    IMI_REQUIRE(b->page_size >= 1, IMI_ERR_INVALID, "page_size=%d must be >= 1", b->page_size);
+    if (b->page_table) {
+        IMI_REQUIRE((b->page_size & (b->page_size - 1)) == 0, IMI_ERR_UNSUPPORTED,
+                    "page_size=%d must be a power of two", b->page_size);
+        IMI_REQUIRE(b->max_pages >= 0 && b->table_stride >= b->max_pages, IMI_ERR_INVALID,
+                    "table_stride=%lld < max_pages=%d", static_cast<long long>(b->table_stride), b->max_pages);
+    } else {
+        IMI_REQUIRE(b->n_pages >= b->n_seqs, IMI_ERR_INVALID, "n_pages=%d < n_seqs=%d with no page table", b->n_pages,
+                    b->n_seqs);
+    }
+    return IMI_OK;
+}
+
+// Rows a sequence can have: what the page table (or the page) holds.
+int64_t batch_capacity(const imi_paged_batch* b) {
+    return b->page_table ? static_cast<int64_t>(b->max_pages) * b->page_size : b->page_size;
+}
+
+int validate(const imi_paged_attention_args* a) {
+    if (const int rc = validate_batch(&a->batch)) return rc;
+    IMI_REQUIRE(a->dtype == IMI_BF16 || a->dtype == IMI_FP16, IMI_ERR_UNSUPPORTED, "dtype=%d is not bf16 or fp16",
+                a->dtype);
+    IMI_REQUIRE(a->dim == 64 || a->dim == 128, IMI_ERR_UNSUPPORTED, "dim=%d is not 64 or 128", a->dim);
+    IMI_REQUIRE(a->kv_heads >= 1 && a->groups >= 1 && static_cast<int64_t>(a->kv_heads) * a->groups <= 65535,
+                IMI_ERR_INVALID, "bad heads (kv_heads=%d, groups=%d)", a->kv_heads, a->groups);
+    IMI_REQUIRE(a->window >= 0 && a->sinks >= 0, IMI_ERR_INVALID, "window=%d and sinks=%d must be >= 0", a->window,
+                a->sinks);
+    IMI_REQUIRE(a->scale > 0.0f && a->scale <= 1e30f, IMI_ERR_INVALID, "scale=%g must be positive and finite",
+                static_cast<double>(a->scale));
+    if (a->batch.n_seqs == 0 || a->batch.n_tokens == 0) return IMI_OK;
+    IMI_REQUIRE(a->query && a->keys && a->values && a->out, IMI_ERR_INVALID, "null query, keys, values or out");
+    const int64_t strides[] = {a->query_token_stride, a->query_head_stride, a->out_token_stride, a->out_head_stride,
+                               a->page_stride,        a->head_stride,       a->row_stride};
+    for (const int64_t s : strides)
+        IMI_REQUIRE(s >= 0 && s % 8 == 0, IMI_ERR_INVALID, "strides must be multiples of 8 elements (got %lld)",
+                    static_cast<long long>(s));
+    const void* ptrs[] = {a->query, a->keys, a->values, a->out};
+    for (const void* p : ptrs)
+        IMI_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, IMI_ERR_INVALID,
+                    "query, keys, values and out must be 16-byte aligned");
+    IMI_REQUIRE(batch_capacity(&a->batch) <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
+                "more than 2^30 rows in a sequence");
+    IMI_REQUIRE(static_cast<int64_t>(a->batch.n_tokens) * a->groups <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
+                "more than 2^30 query rows per KV head");
+    return IMI_OK;
+}
+
+// The launches of one call.  Sequences of at most few_rows rows go to the
+// few-row kernel (blocks of 16 rows), the others to the tile kernel.
+struct Shape {
+    int few_rows = 0;       // 0: no few-row launch
+    int few_wg = 0;
+    int most = 0;           // rows a few-row sequence can have
+    bool direct = false;    // a workgroup per (sequence, head), no join
+    bool tiles = false;
+    int tile_wg = 0;
+    int slots = 0;
+    size_t few_part = 0, tile_part = 0, plan = 0;   // workspace bytes
+};
+
+constexpr int kDirectUnits = 8;
+
+Shape shape_of(const imi_paged_attention_args* a) {
+    Shape p;
+    const imi_paged_batch& b = a->batch;
+    if (b.n_seqs == 0 || b.n_tokens == 0) return p;
+    const int64_t most = static_cast<int64_t>(std::min(b.max_query, b.n_tokens)) * a->groups;
+    if (most <= 32) {
+        p.few_rows = most <= 16 ? 16 : 32;
+    } else {
+        p.tiles = true;
+        if (b.n_seqs > 1 && a->groups <= 32) p.few_rows = a->groups <= 16 ? 16 : 32;
+    }
+    if (p.few_rows) {
+        p.most = static_cast<int>(std::min<int64_t>(most, p.few_rows));
+        const int64_t cap = std::min<int64_t>(batch_capacity(&b), b.max_len > 0 ? b.max_len : INT_MAX);
+        int64_t longest = cap;   // visible rows of the longest sequence
+        if (a->window > 0)
+            longest = std::min<int64_t>(cap, static_cast<int64_t>(a->window) + a->sinks + p.few_rows / a->groups);
+        p.direct = (longest + kUnit - 1) / kUnit <= kDirectUnits;
+        p.few_wg = 2 * device_cus();
+        if (!p.direct) p.few_part = size_t(2) * p.few_wg * p.few_rows * (a->dim + 2) * sizeof(float);
+    }
+    if (p.tiles) {
+        p.slots = static_cast<int>(static_cast<int64_t>(b.n_tokens) * a->groups / kTileRows + b.n_seqs);
+        p.tile_wg = 2 * device_cus();
+        p.tile_part = size_t(2) * p.tile_wg * kTileRows * (a->dim + 2) * sizeof(float);
+        p.plan = plan_bytes(p.slots, b.n_seqs);
+    }
+    return p;
+}
+
+size_t carve(const Shape& p, void* base, float** few, float** tile, int32_t** plan) {
+    Carver c(base);
+    *few = c.take<float>(p.few_part / sizeof(float));
+    *tile = c.take<float>(p.tile_part / sizeof(float));
+    *plan = c.take<int32_t>(p.plan / sizeof(int32_t));
+    return p.few_part || p.tile_part ? c.used() : 0;
+}
+
+template <typename T, int D>
+int launch(const imi_paged_attention_args* a, const Shape& p, PagedParams P, float* few, float* tile, int32_t* plan,
+           hipStream_t stream) {
+    if (p.tiles) {
+        PagedParams Q = P;
+        Q.min_rows = p.few_rows + 1;
+        Q.max_rows = INT_MAX;
+        Q.W = p.tile_wg;
+        Q.part = tile;
+        Q.part_ml = tile + size_t(2) * p.tile_wg * kTileRows * D;
+        Q.plan = plan;
+        Q.slots = p.slots;
+        plan_kernel<<<1, 1024, 0, stream>>>(Q);
+        IMI_LAUNCH_CHECK("plan_kernel");
+        tile_kernel<T, D><<<p.tile_wg, 256, 0, stream>>>(Q);
+        IMI_LAUNCH_CHECK("tile_kernel");
+        tile_merge_kernel<T, D><<<dim3(p.tile_wg - 1, kTileRows * D / 1024), 256, 0, stream>>>(Q);
+        IMI_LAUNCH_CHECK("tile_merge_kernel");
+    }
+    if (p.few_rows) {
+        PagedParams Q = P;
+        Q.min_rows = 1;
+        Q.max_rows = p.few_rows;
+        Q.W = p.few_wg;
+        Q.part = few;
+        Q.part_ml = few + size_t(2) * p.few_wg * p.few_rows * D;
+        const int grid = p.direct ? P.S * P.H : p.few_wg;
+        if (p.few_rows == 16)
+            few_kernel<T, D, 1><<<grid, 256, 0, stream>>>(Q, p.direct ? 1 : 0);
+        else
+            few_kernel<T, D, 2><<<grid, 256, 0, stream>>>(Q, p.direct ? 1 : 0);
+        IMI_LAUNCH_CHECK("few_kernel");
+        if (!p.direct) {
+            few_merge_kernel<T, D><<<dim3(p.few_wg - 1, p.most), 256, 0, stream>>>(Q);
+            IMI_LAUNCH_CHECK("few_merge_kernel");
+        }
+    }
+    return IMI_OK;
+}
+
+}  // namespace
+}  // namespace imi
+
+extern "C" int imi_paged_attention_workspace_size(const imi_paged_attention_args* a, size_t* bytes) {
+    using namespace imi;
+    clear_error();
+    IMI_REQUIRE(a && bytes, IMI_ERR_INVALID, "null argument");
+    if (const int rc = validate(a)) return rc;
+    float *f, *t;
+    int32_t* p;
+    *bytes = carve(shape_of(a), nullptr, &f, &t, &p);
+    return IMI_OK;
+}
+
+extern "C" int imi_paged_attention(const imi_paged_attention_args* a, imi_stream_t stream) {
+    using namespace imi;
+    clear_error();
+    IMI_REQUIRE(a, IMI_ERR_INVALID, "null argument");
+    if (const int rc = validate(a)) return rc;
+    const imi_paged_batch& b = a->batch;
+    if (b.n_seqs == 0 || b.n_tokens == 0) return IMI_OK;
+    const Shape p = shape_of(a);
+    float *few, *tile;
+    int32_t* plan;
+    const size_t need = carve(p, nullptr, &few, &tile, &plan);
+    IMI_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), IMI_ERR_WORKSPACE,
+                "workspace of %zu bytes, need %zu", a->workspace_bytes, need);
+    carve(p, a->workspace, &few, &tile, &plan);
+    PagedParams P{};
+    P.q = a->query;
+    P.k = a->keys;
+    P.v = a->values;
+    P.out = a->out;
+    P.lse = a->out_lse;
+    P.table = b.page_table;
+    P.lens = b.lens;
+    P.start = b.query_start;
+    P.q_ts = a->query_token_stride;
+    P.q_hs = a->query_head_stride;
+    P.o_ts = a->out_token_stride;
+    P.o_hs = a->out_head_stride;
+    P.l_ts = a->lse_token_stride;
+    P.page_s = a->page_stride;
+    P.head_s = a->head_stride;
+    P.tok_s = a->row_stride;
+    P.table_s = b.table_stride;
+    P.S = b.n_seqs;
+    P.N = b.n_tokens;
+    P.H = a->kv_heads;
+    P.G = a->groups;
+    P.n_pages = b.n_pages;
+    P.page_shift = b.page_table ? __builtin_ctz(static_cast<unsigned>(b.page_size)) : 31;
+    P.capacity = static_cast<int>(batch_capacity(&b));
+    P.window = a->window;
+    P.sinks = a->window > 0 ? a->sinks : 0;
+    P.c = a->scale * kLog2e;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (a->dtype == IMI_BF16)
+        return a->dim == 128 ? launch<BF16, 128>(a, p, P, few, tile, plan, st)
+                             : launch<BF16, 64>(a, p, P, few, tile, plan, st);
+    return a->dim == 128 ? launch<FP16, 128>(a, p, P, few, tile, plan, st)
+                         : launch<FP16, 64>(a, p, P, few, tile, plan, st);
+}

@@ -7,6 +7,7 @@ zero-filled once on allocation (the kernels leave them reusable).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -15,7 +16,8 @@ from typing import Dict, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import AttentionArgs, DecodeArgs, IndexArgs, KmeansArgs, SelectArgs, UpdateArgs, check
+from ._lib import (AttentionArgs, DecodeArgs, IndexArgs, KmeansArgs, PagedAttentionArgs, PagedBatchArgs, SelectArgs,
+                   UpdateArgs, check)
 
 _WS: Dict[Tuple[str, int], torch.Tensor] = {}
 
@@ -948,3 +950,160 @@ class HostTierPlan:
                                     self.d_nums[1, 0].data_ptr(), stream), "imi_hostcache_admit")
         self.plan.run(query, out, static_len, stream=stream, phases=2, exec_rows=exec_rows)   # attention + merge
         return out
+
+
+# ------------------------------------------------------------- paged cache --
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}   # IMI_BF16, IMI_FP16
+
+
+def _on(dev: torch.device):
+    """Make dev current for launches (None: it is)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _same_device(dev: torch.device, **ts: Optional[torch.Tensor]) -> None:
+    for name, t in ts.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+
+
+def _i32_tensor(name: str, t: torch.Tensor, dim: int) -> None:
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+        raise ValueError(f"{name} must have {dim} dimension(s) and unit stride on the last")
+
+
+def _stride(t: torch.Tensor, d: int) -> int:
+    """Stride of dimension d; 0 where it has one entry (torch leaves the
+    stride of such a dimension open)."""
+    return t.stride(d) if t.shape[d] > 1 else 0
+
+
+def _write_strides(name: str, t: torch.Tensor) -> None:
+    if any(t.stride(d) == 0 and t.shape[d] > 1 for d in range(t.dim())):
+        raise ValueError(f"{name} is written, so no two of its elements may share memory")
+
+
+class PagedBatch:
+    """A ragged batch of new tokens over cached rows, one object for every
+    layer of a step.
+
+    page_table: int32 [S, max_pages], the pages of each sequence in row order
+    (entries past its last page are not read), or None: sequence s's rows are
+    "page" s of the key and value tensors (contiguous rows, e.g. a steady
+    zone [S, H, rows, D]).  lens: int32 [S] cached rows, new tokens included.
+    query_start: int32 [S + 1], sequence s's new tokens are the query rows
+    query_start[s] .. query_start[s + 1] - 1; query rows behind the last
+    sequence belong to none.  max_query: at least every sequence's new tokens
+    (sequences with more are not served).  max_len: a hint, about the longest
+    sequence (default: what the table holds); only the split of short batches
+    depends on it."""
+
+    __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device")
+
+    def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
+                 max_query: int, max_len: Optional[int] = None):
+        dev = _require_device(lens, query_start, page_table)
+        _same_device(dev, page_table=page_table, query_start=query_start)
+        _i32_tensor("lens", lens, 1)
+        _i32_tensor("query_start", query_start, 1)
+        S = lens.shape[0]
+        if query_start.shape[0] != S + 1:
+            raise ValueError(f"query_start has {query_start.shape[0]} entries for {S} sequences")
+        self.page_table, self.lens, self.query_start = page_table, lens, query_start
+        self.max_query, self.max_len, self.device = int(max_query), max_len, dev
+        self.args = PagedBatchArgs(lens=lens.data_ptr(), query_start=query_start.data_ptr(), n_seqs=S,
+                                   max_query=self.max_query, max_len=int(max_len or 0))
+        if page_table is not None:
+            _i32_tensor("page_table", page_table, 2)
+            if page_table.shape[0] != S:
+                raise ValueError(f"page_table has {page_table.shape[0]} rows for {S} sequences")
+            self.args.page_table = page_table.data_ptr()
+            self.args.max_pages = page_table.shape[1]
+            self.args.table_stride = page_table.stride(0) if S > 1 else page_table.shape[1]
+
+    def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
+        """The C struct for pools of n_pages pages and n_tokens query rows."""
+        a = self.args
+        a.n_pages, a.page_size, a.n_tokens = n_pages, page_size, n_tokens
+        return a
+
+
+def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch, dim: int, dtype: torch.dtype):
+    """Checks a key and a value pool [pages, kv_heads, page_size, D] of any
+    memory order with the head dim adjacent."""
+    for name, t in (("key_pages", key_pages), ("value_pages", value_pages)):
+        if t.dtype != dtype:
+            raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+        if t.dim() != 4 or t.shape[3] != dim or t.stride(3) != 1:
+            raise ValueError(f"{name} must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
+    if value_pages.shape != key_pages.shape or value_pages.stride() != key_pages.stride():
+        raise ValueError("key_pages and value_pages must share shape and strides")
+    _same_device(batch.device, key_pages=key_pages, value_pages=value_pages)
+    P, H, page, _ = key_pages.shape
+    if batch.page_table is None and P < batch.lens.shape[0]:
+        raise ValueError(f"{P} contiguous key rows sets for {batch.lens.shape[0]} sequences")
+    return P, H, page
+
+
+def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch,
+                    scale: Optional[float] = None, window: int = 0, sinks: int = 0,
+                    out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """Causal GQA attention of a batch of new tokens over their sequences'
+    cached rows (the new tokens' own among them): decode, verification of a
+    few tokens and prefill chunks, mixed in one call as they come.
+
+    query: bf16 or fp16 [N, Hq, D], D 64 or 128, any token and head strides.
+    key_pages / value_pages: [pages, Hkv, page_size, D] (a power of two of
+    rows per page with a page table), e.g. ``pool.transpose(1, 2)`` of a
+    token-major pool; Hq a multiple of Hkv.  A token at position p sees rows
+    j <= p; with ``window`` of these the last ``window`` and the first
+    ``sinks``.  A token that sees no row gets 0 (lse -inf).  ``out`` [N, Hq,
+    D] and ``lse`` f32 [N, Hq] (natural log) may be given; rows behind the
+    last sequence are left as they are in them (unset in a tensor made here).
+    Returns out, or (out, lse) with ``lse`` or ``return_lse``."""
+    dev = batch.device
+    if query.dim() != 3 or query.stride(2) != 1:
+        raise ValueError("query must be [tokens, heads, dim] with unit stride on dim")
+    code = _DTYPES.get(query.dtype)
+    if code is None:
+        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
+    N, Hq, D = query.shape
+    P, H, page = _pools(key_pages, value_pages, batch, D, query.dtype)
+    if H == 0 or Hq % H:
+        raise ValueError(f"{Hq} query heads are not a multiple of {H} KV heads")
+    _same_device(dev, query=query, out=out, lse=lse)
+    if out is None:
+        out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    else:
+        if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
+            raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} with unit stride on dim")
+        _write_strides("out", out)
+    if lse is None and return_lse:
+        lse = torch.empty((N, Hq), dtype=torch.float32, device=dev)
+    elif lse is not None:
+        if lse.shape != (N, Hq) or lse.dtype != torch.float32 or (Hq > 1 and lse.stride(1) != 1):
+            raise ValueError(f"lse must be float32 {(N, Hq)} with unit stride on heads")
+        _write_strides("lse", lse)
+    a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D,
+                           query.data_ptr(), _stride(query, 0), _stride(query, 1),
+                           key_pages.data_ptr(), value_pages.data_ptr(), _stride(key_pages, 0),
+                           _stride(key_pages, 1), _stride(key_pages, 2),
+                           1.0 / math.sqrt(D) if scale is None else scale, window, sinks,
+                           out.data_ptr(), _stride(out, 0), _stride(out, 1),
+                           _ptr(lse), 0 if lse is None else _stride(lse, 0))
+    L = _lib.lib()
+    ref = ctypes.byref(a)
+    with _on(dev):
+        need = ctypes.c_size_t()
+        check(L.imi_paged_attention_workspace_size(ref, ctypes.byref(need)), "imi_paged_attention")
+        if need.value:   # this call's own: calls on other streams and captured graphs share nothing
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
+        check(L.imi_paged_attention(ref, _stream(dev)), "imi_paged_attention")
+    return out if lse is None else (out, lse)

@@ -475,6 +475,67 @@ int imi_hostcache_admit(const uint16_t* exec_keys, const uint16_t* exec_values, 
  * addressing hands the host pointer to the kernel). */
 int imi_host_device_pointer(const void* host, void** device);
 
+/* ------------------------------------------------------- paged KV cache
+ * Attention of new tokens over cached rows that lie in pages, the norm and
+ * rotation that fill them, and the page tables.  No counterpart in the
+ * reference (its dense layers attend a contiguous cache through flash_attn,
+ * attn_hub/full.py:20-81; its prefill runs in chunks, model_hub/
+ * prefill.py:232-343).
+ *
+ * A ragged batch of new tokens: sequence s has lens[s] cached rows, the last
+ * of them its new tokens, which are rows query_start[s] .. query_start[s + 1]
+ * - 1 of the query.  Row j lies in slot j % page_size of page
+ * page_table[s][j / page_size]; with page_table NULL in slot j of page s
+ * (contiguous rows, page_size of them).  Values of query_start outside 0 ..
+ * n_tokens, of lens outside the table's rows and page ids outside 0 ..
+ * n_pages - 1 are forced into these ranges by attention, and rows that they
+ * would lead to are not written by imi_qk_norm_rope: no access leaves the
+ * tensors. */
+enum { IMI_BF16 = 0, IMI_FP16 = 1 };
+
+typedef struct {
+    const int32_t* page_table;   /* device [n_seqs][table_stride], or NULL */
+    int64_t table_stride;        /* >= max_pages */
+    int32_t max_pages;           /* table entries per sequence */
+    int32_t n_pages;             /* pages in the pool */
+    int32_t page_size;           /* rows per page, a power of two (any number with no table) */
+    const int32_t* lens;         /* device [n_seqs] rows, new tokens included */
+    const int32_t* query_start;  /* device [n_seqs + 1], ascending */
+    int32_t n_seqs, n_tokens;    /* n_tokens: rows of the query tensor */
+    int32_t max_query;           /* at least every sequence's new tokens */
+    int32_t max_len;             /* hint: about the longest sequence; 0 = what the table holds */
+} imi_paged_batch;
+
+/* out[t][x] = softmax over the visible rows of scale * q . k, times v, for
+ * query head x of KV head x / groups.  A new token at position p sees rows
+ * j <= p and, with window > 0, of these the last `window` (its own among
+ * them) and the first `sinks`.  A token that sees nothing gets 0 and an lse
+ * of -inf.  Query rows behind the last sequence are neither read nor
+ * written.  Strides in elements, multiples of 8; the head dim is adjacent.
+ * Keys and values share their strides.  fp32 accumulation. */
+typedef struct {
+    imi_paged_batch batch;
+    int32_t dtype;               /* IMI_BF16 or IMI_FP16: query, keys, values, out */
+    int32_t kv_heads, groups, dim;   /* groups = query heads per KV head; dim 64 or 128 */
+    const uint16_t* query;       /* device [n_tokens][kv_heads * groups][dim] */
+    int64_t query_token_stride, query_head_stride;
+    const uint16_t* keys;        /* device [n_pages][kv_heads][page_size][dim] */
+    const uint16_t* values;
+    int64_t page_stride, head_stride, row_stride;
+    float scale;                 /* > 0 */
+    int32_t window;              /* 0: every earlier row */
+    int32_t sinks;
+    uint16_t* out;               /* device [n_tokens][kv_heads * groups][dim] */
+    int64_t out_token_stride, out_head_stride;
+    float* out_lse;              /* device [n_tokens][kv_heads * groups] natural log, or NULL */
+    int64_t lse_token_stride;
+    void* workspace;             /* device, >= imi_paged_attention_workspace_size() bytes; any content */
+    size_t workspace_bytes;
+} imi_paged_attention_args;
+
+int imi_paged_attention_workspace_size(const imi_paged_attention_args* a, size_t* bytes);
+int imi_paged_attention(const imi_paged_attention_args* a, imi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,161 @@
+"""ops.paged_attention against the definition in 64 bits on the CPU.
+
+Tolerance.  With w the exact weights and A = sum w |v|, the kernel differs from
+the exact output by: its weights rounded to the tensor type before the product
+(half a step, eps / 2, relative to each weight: eps / 2 * A; in fp16 a weight
+under 2^-14 keeps an absolute 2^-25 instead, against a sum of at least 1), the
+scores' fp32 sums (at most (D + 2) 2^-24 sum |q k| scale each, which scales a
+weight by as much, numerator and sum: twice), exp2 and its argument (2^-21 for
+scores up to 8), the sums over n rows (n 2^-24 twice), and the output's own
+rounding (eps / 2 relative)."""
+import math
+
+import pytest
+import torch
+
+from conftest import gpu_available
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
+
+DEV = "cuda:0"
+
+
+def make(lens, news, H, G, D, page, dtype, layout="heads", seed=0, packed=False, pad=0, junk=float("nan"), slack=3):
+    """Tensors on the device and their 64-bit copies.  Everything that no
+    sequence owns (unused pages, slots behind a last row, table entries behind
+    a last page) is junk."""
+    g = torch.Generator().manual_seed(seed)
+    S, N = len(lens), sum(news) + pad
+    start = [0]
+    for n in news:
+        start.append(start[-1] + n)
+    width = Hw = H * G
+    if packed:
+        Hw = width + 2 * H
+    q = torch.randn((N, Hw, D), generator=g).to(dtype)
+    rows = [(torch.randn((H, n, D), generator=g).to(dtype), torch.randn((H, n, D), generator=g).to(dtype))
+            for n in lens]
+    if page:
+        held = [-(-n // page) for n in lens]
+        P = sum(held) + slack
+        ids = torch.randperm(P, generator=g).tolist()
+        table = torch.full((S, max(held + [0]) + 2), 2 ** 31 - 1, dtype=torch.int32)
+        k = torch.full((P, H, page, D), junk, dtype=dtype)
+        v = torch.full((P, H, page, D), junk, dtype=dtype)
+        at = 0
+        for s, n in enumerate(lens):
+            for j in range(held[s]):
+                p = ids[at]
+                at += 1
+                table[s, j] = p
+                part = slice(j * page, min(n, (j + 1) * page))
+                k[p, :, :part.stop - part.start] = rows[s][0][:, part]
+                v[p, :, :part.stop - part.start] = rows[s][1][:, part]
+        table = table.to(DEV)
+    else:
+        table = None
+        k = torch.full((S, H, max(lens + [1]) + slack, D), junk, dtype=dtype)
+        v = k.clone()
+        for s, n in enumerate(lens):
+            k[s, :, :n], v[s, :, :n] = rows[s]
+    if layout == "tokens":
+        k, v = (t.transpose(1, 2).contiguous().to(DEV).transpose(1, 2) for t in (k, v))
+    else:
+        k, v = k.to(DEV), v.to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    return dict(q=q.to(DEV)[:, :width], k=k, v=v, table=table, lens=i32(lens), start=i32(start), rows=rows,
+                q64=q[:, :width].double(), lens_host=lens, start_host=start, H=H, G=G, D=D, dtype=dtype)
+
+
+def batch_of(ops, x, **kw):
+    news = [b - a for a, b in zip(x["start_host"], x["start_host"][1:])]
+    return ops.PagedBatch(x["table"], x["lens"], x["start"], max_query=max(news + [1]), **kw)
+
+
+def expected(x, window=0, sinks=0, scale=None):
+    """(out, lse, tolerance of out, tolerance of lse) in 64 bits; rows of no
+    sequence are None in the mask."""
+    H, G, D = x["H"], x["G"], x["D"]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    eps = torch.finfo(x["dtype"]).eps
+    N = x["q64"].shape[0]
+    out = torch.zeros((N, H * G, D), dtype=torch.float64)
+    lse = torch.full((N, H * G), -math.inf, dtype=torch.float64)
+    tol, ltol = torch.zeros_like(out), torch.zeros_like(lse)
+    mine = torch.zeros(N, dtype=torch.bool)
+    for s, n in enumerate(x["lens_host"]):
+        a, b = x["start_host"][s], x["start_host"][s + 1]
+        mine[a:b] = True
+        k, v = x["rows"][s][0].double(), x["rows"][s][1].double()
+        for t in range(a, b):
+            p = n - (b - a) + t - a
+            seen = [j for j in range(0, p + 1) if window == 0 or j > p - window or j < sinks]
+            if not seen:
+                continue
+            for h in range(H):
+                ks, vs = k[h, seen], v[h, seen]
+                q = x["q64"][t, h * G:(h + 1) * G]
+                sc = scale * q @ ks.T
+                w = torch.softmax(sc, -1)
+                o = w @ vs
+                A = w @ vs.abs()
+                ds = (D + 2) * 2.0 ** -24 * scale * (q.abs() @ ks.abs().T).amax(-1, keepdim=True) + 2.0 ** -21
+                m = len(seen)
+                err = (eps / 2 + 2 * ds + 2 * m * 2.0 ** -24) * A + eps / 2 * o.abs() + 1e-6
+                if x["dtype"] == torch.float16:
+                    err = err + 2.0 ** -25 * vs.abs().sum(0) + 2.0 ** -25
+                hs = slice(h * G, (h + 1) * G)
+                out[t, hs], tol[t, hs] = o, err
+                lse[t, hs] = torch.logsumexp(sc, -1)
+                ltol[t, hs] = (2 * ds[:, 0] + m * 2.0 ** -24) + 2.0 ** -22 * lse[t, hs].abs() + 1e-6
+    return out, lse, tol, ltol, mine
+
+
+def check(x, got, got_lse, window=0, sinks=0, scale=None):
+    out, lse, tol, ltol, mine = expected(x, window, sinks, scale)
+    got, got_lse = got.double().cpu(), got_lse.double().cpu()
+    err = (got - out).abs()[mine]
+    assert torch.all(err <= tol[mine]), f"out: {err.max()} (worst excess {(err - tol[mine]).max()})"
+    empty = torch.isinf(lse) & mine[:, None]
+    assert torch.all(got_lse[empty] == -math.inf) and torch.all(got[empty] == 0)
+    live = ~torch.isinf(lse) & mine[:, None]
+    lerr = (got_lse - lse).abs()[live]
+    assert torch.all(lerr <= ltol[live]), f"lse: {lerr.max()}"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from adaptiveimi_amd import ops
+
+    return ops
+
+
+BF, HF = torch.bfloat16, torch.float16
+CASES = [
+    # lens, news, H, G, D, page, dtype, window, sinks, layout
+    ([1], [1], 1, 1, 128, 8, BF, 0, 0, "heads"),
+    ([519], [1], 2, 4, 128, 8, BF, 0, 0, "heads"),
+    ([2500], [1], 2, 4, 128, 16, BF, 0, 0, "heads"),           # several workgroups, joined
+    ([2500, 3, 129, 1, 4000], [1] * 5, 2, 8, 128, 16, BF, 0, 0, "tokens"),
+    ([700, 64, 1290], [1, 1, 1], 1, 16, 64, 32, HF, 0, 0, "heads"),
+    ([700, 64, 1290], [5, 4, 3], 2, 3, 128, 64, HF, 100, 7, "tokens"),
+    ([2000, 300], [5, 5], 2, 4, 64, 32, HF, 150, 32, "heads"),
+    ([300, 40, 9], [8, 8, 8], 1, 4, 128, 1, BF, 0, 0, "heads"),
+    ([300], [300], 1, 1, 128, 16, BF, 0, 0, "heads"),
+    ([300], [300], 2, 4, 64, 16, HF, 0, 0, "tokens"),
+    ([450], [130], 1, 7, 128, 16, BF, 0, 0, "heads"),
+    ([450], [450], 1, 2, 128, 0, BF, 64, 4, "tokens"),
+    ([450], [200], 1, 2, 128, 8, BF, 1, 0, "heads"),            # a token sees itself alone
+    ([333], [333], 1, 3, 128, 8, HF, 5, 40, "heads"),           # more sinks than window
+    ([200, 1, 333, 77, 64, 500], [1, 1, 150, 77, 2, 1], 2, 5, 128, 16, BF, 0, 0, "heads"),
+    ([200, 1, 333, 77, 64, 500], [1, 1, 150, 77, 2, 1], 1, 33, 64, 16, BF, 90, 3, "tokens"),   # more than 32 rows a token
+    ([64, 129, 31], [64, 129, 31], 1, 4, 128, 0, HF, 0, 0, "heads"),
+]
+
+
+@pytest.mark.parametrize("lens,news,H,G,D,page,dtype,window,sinks,layout", CASES)
+def test_matches_definition(ops, lens, news, H, G, D, page, dtype, window, sinks, layout):
+    x = make(lens, news, H, G, D, page, dtype, layout)
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window, sinks=sinks,
+                                   return_lse=True)
+    check(x, out, lse, window, sinks)
