@@ -115,6 +115,28 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class QkNormRopeArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatchArgs), ("dtype", _i32), ("query_heads", _i32), ("kv_heads", _i32), ("dim", _i32),
+                ("query", _vp), ("query_token_stride", _i64), ("query_head_stride", _i64),
+                ("key", _vp), ("key_token_stride", _i64), ("key_head_stride", _i64),
+                ("value", _vp), ("value_token_stride", _i64), ("value_head_stride", _i64),
+                ("positions", _vp), ("positions_64", _i32), ("inv_freq", _vp), ("rotary", _i32),
+                ("interleaved", _i32), ("query_weight", _vp), ("key_weight", _vp), ("weight_fp32", _i32),
+                ("eps", _f32), ("query_out", _vp), ("query_out_token_stride", _i64), ("query_out_head_stride", _i64),
+                ("key_out", _vp), ("key_out_token_stride", _i64), ("key_out_head_stride", _i64),
+                ("key_pages", _vp), ("value_pages", _vp),
+                ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64)]
+
+
+class PageTableArgs(ctypes.Structure):
+    _fields_ = [("pages", _vp), ("stride", _i64), ("lens", _vp), ("refs", _vp), ("n_seqs", _i32),
+                ("max_pages", _i32), ("n_pages", _i32), ("page_size", _i32)]
+
+
+class PagePool(ctypes.Structure):
+    _fields_ = [("base", _vp), ("page_stride", _i64), ("page_bytes", _i64)]
+
+
 EXPORTS = {
     "imi_last_error": (ctypes.c_char_p, []),
     "imi_version": (ctypes.c_int, []),
@@ -149,6 +171,16 @@ EXPORTS = {
     "imi_paged_attention_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs),
                                                           ctypes.POINTER(ctypes.c_size_t)]),
     "imi_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs), _vp]),
+    "imi_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), _vp]),
+    "imi_fork_pages": (ctypes.c_int, [ctypes.POINTER(PageTableArgs), _vp, ctypes.POINTER(PageTableArgs), _vp]),
+    "imi_extend_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(PageTableArgs),
+                                                       ctypes.POINTER(ctypes.c_size_t)]),
+    "imi_extend_pages": (ctypes.c_int, [ctypes.POINTER(PageTableArgs), _vp, _vp, ctypes.POINTER(PagePool), _i32, _vp,
+                                        ctypes.c_size_t, _vp]),
+    "imi_compact_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(PageTableArgs),
+                                                        ctypes.POINTER(ctypes.c_size_t)]),
+    "imi_compact_pages": (ctypes.c_int, [ctypes.POINTER(PageTableArgs), _vp, ctypes.POINTER(PagePool), _i32, _vp,
+                                         ctypes.c_size_t, _vp]),
 }
 
 _lib = None

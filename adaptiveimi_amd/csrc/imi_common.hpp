@@ -47,6 +47,11 @@ void clear_error();
         }                                                                                  \
     } while (0)
 
+// Checks of a paged batch, and the rows that one of its sequences can have
+// (imi_paged.hip).
+int validate_batch(const imi_paged_batch* b);
+int64_t batch_capacity(const imi_paged_batch* b);
+
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Carves aligned sub-buffers out of one caller-provided workspace.

@@ -30,6 +30,32 @@
 #include "imi_common.hpp"
 
 namespace imi {
+
+int validate_batch(const imi_paged_batch* b) {
+    IMI_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0, IMI_ERR_INVALID, "negative batch (n_seqs=%d, n_tokens=%d)",
+                b->n_seqs, b->n_tokens);
+    if (b->n_seqs == 0 || b->n_tokens == 0) return IMI_OK;
+    IMI_REQUIRE(b->lens && b->query_start, IMI_ERR_INVALID, "null lens or query_start");
+    IMI_REQUIRE(b->max_query >= 1, IMI_ERR_INVALID, "max_query=%d must be >= 1", b->max_query);
+    IMI_REQUIRE(b->n_pages >= 1, IMI_ERR_INVALID, "n_pages=%d must be >= 1", b->n_pages);
+    IMI_REQUIRE(b->page_size >= 1, IMI_ERR_INVALID, "page_size=%d must be >= 1", b->page_size);
+    if (b->page_table) {
+        IMI_REQUIRE((b->page_size & (b->page_size - 1)) == 0, IMI_ERR_UNSUPPORTED,
+                    "page_size=%d must be a power of two", b->page_size);
+        IMI_REQUIRE(b->max_pages >= 0 && b->table_stride >= b->max_pages, IMI_ERR_INVALID,
+                    "table_stride=%lld < max_pages=%d", static_cast<long long>(b->table_stride), b->max_pages);
+    } else {
+        IMI_REQUIRE(b->n_pages >= b->n_seqs, IMI_ERR_INVALID, "n_pages=%d < n_seqs=%d with no page table", b->n_pages,
+                    b->n_seqs);
+    }
+    return IMI_OK;
+}
+
+// Rows a sequence can have: what the page table (or the page) holds.
+int64_t batch_capacity(const imi_paged_batch* b) {
+    return b->page_table ? static_cast<int64_t>(b->max_pages) * b->page_size : b->page_size;
+}
+
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8_t;
@@ -903,31 +929,6 @@ __global__ __launch_bounds__(256) void tile_merge_kernel(PagedParams a) {
 }
 
 // ------------------------------------------------------------- host -------
-
-int validate_batch(const imi_paged_batch* b) {
-    IMI_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0, IMI_ERR_INVALID, "negative batch (n_seqs=%d, n_tokens=%d)",
-                b->n_seqs, b->n_tokens);
-    if (b->n_seqs == 0 || b->n_tokens == 0) return IMI_OK;
-    IMI_REQUIRE(b->lens && b->query_start, IMI_ERR_INVALID, "null lens or query_start");
-    IMI_REQUIRE(b->max_query >= 1, IMI_ERR_INVALID, "max_query=%d must be >= 1", b->max_query);
-    IMI_REQUIRE(b->n_pages >= 1, IMI_ERR_INVALID, "n_pages=%d must be >= 1", b->n_pages);
-    IMI_REQUIRE(b->page_size >= 1, IMI_ERR_INVALID, "page_size=%d must be >= 1", b->page_size);
-    if (b->page_table) {
-        IMI_REQUIRE((b->page_size & (b->page_size - 1)) == 0, IMI_ERR_UNSUPPORTED,
-                    "page_size=%d must be a power of two", b->page_size);
-        IMI_REQUIRE(b->max_pages >= 0 && b->table_stride >= b->max_pages, IMI_ERR_INVALID,
-                    "table_stride=%lld < max_pages=%d", static_cast<long long>(b->table_stride), b->max_pages);
-    } else {
-        IMI_REQUIRE(b->n_pages >= b->n_seqs, IMI_ERR_INVALID, "n_pages=%d < n_seqs=%d with no page table", b->n_pages,
-                    b->n_seqs);
-    }
-    return IMI_OK;
-}
-
-// Rows a sequence can have: what the page table (or the page) holds.
-int64_t batch_capacity(const imi_paged_batch* b) {
-    return b->page_table ? static_cast<int64_t>(b->max_pages) * b->page_size : b->page_size;
-}
 
 int validate(const imi_paged_attention_args* a) {
     if (const int rc = validate_batch(&a->batch)) return rc;

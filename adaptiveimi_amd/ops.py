@@ -16,8 +16,8 @@ from typing import Dict, Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from ._lib import (AttentionArgs, DecodeArgs, IndexArgs, KmeansArgs, PagedAttentionArgs, PagedBatchArgs, SelectArgs,
-                   UpdateArgs, check)
+from ._lib import (AttentionArgs, DecodeArgs, IndexArgs, KmeansArgs, PagedAttentionArgs, PagedBatchArgs, PagePool,
+                   PageTableArgs, QkNormRopeArgs, SelectArgs, UpdateArgs, check)
 
 _WS: Dict[Tuple[str, int], torch.Tensor] = {}
 
@@ -1046,7 +1046,7 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch
     _same_device(batch.device, key_pages=key_pages, value_pages=value_pages)
     P, H, page, _ = key_pages.shape
     if batch.page_table is None and P < batch.lens.shape[0]:
-        raise ValueError(f"{P} contiguous key rows sets for {batch.lens.shape[0]} sequences")
+        raise ValueError(f"{P} sets of contiguous rows for {batch.lens.shape[0]} sequences")
     return P, H, page
 
 
@@ -1107,3 +1107,218 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
             a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
         check(L.imi_paged_attention(ref, _stream(dev)), "imi_paged_attention")
     return out if lse is None else (out, lse)
+
+
+def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[torch.Tensor] = None, *,
+                 inv_freq: Optional[torch.Tensor] = None, query_weight: Optional[torch.Tensor] = None,
+                 key_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                 query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
+                 value: Optional[torch.Tensor] = None, batch: Optional[PagedBatch] = None,
+                 key_pages: Optional[torch.Tensor] = None, value_pages: Optional[torch.Tensor] = None):
+    """RMS norm of each query and key head and the rotation by position, in
+    one pass.
+
+    query [N, Hq, D] and key [N, Hkv, D]: bf16 or fp16, D 64 or 128, any token
+    and head strides (views of one projection's output).  query_weight /
+    key_weight [D] (their dtype or float32): x / sqrt(mean(x^2) + eps) * w per
+    head; a tensor without weight is not normed.  inv_freq float32 [r / 2], r
+    a multiple of 16 up to D: the first r dims of a head turn by position *
+    inv_freq[i], pairs (i, i + r / 2) or, interleaved, (2i, 2i + 1).  No
+    inv_freq: no rotation.
+
+    Either ``positions`` (int32 or int64 [N], at most 2^31 - 1 in magnitude)
+    are given: returns (query_out, key_out), made here or given (the inputs
+    themselves are allowed).  Or ``batch``, ``value`` [N, Hkv, D] and the
+    pools (as in paged_attention) are: new token i of a sequence stands at
+    lens - (its new tokens) + i, its key and value are stored in that row, and
+    (query_out, None) is returned; tokens behind the last sequence, and rows
+    that the table has no page for, are left as they are."""
+    dev = _require_device(query, key)
+    code = _DTYPES.get(query.dtype)
+    if code is None:
+        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
+    if query.dim() != 3:
+        raise ValueError("query must be [tokens, heads, dim]")
+    N, Hq, D = query.shape
+
+    def rows(name, t, heads, written):
+        if t.dtype != query.dtype:
+            raise TypeError(f"{name} is {t.dtype}, expected {query.dtype}")
+        if t.dim() != 3 or t.shape != (N, heads, D) or t.stride(2) != 1:
+            raise ValueError(f"{name} must be [{N}, {heads}, {D}] with unit stride on dim")
+        if written:
+            _write_strides(name, t)
+        return t.data_ptr(), _stride(t, 0), _stride(t, 1)
+
+    Hk = key.shape[1] if key.dim() == 3 else -1
+    paged = batch is not None
+    if paged == (positions is not None):
+        raise ValueError("give either positions or a batch with pages")
+    if paged and (value is None or key_pages is None or value_pages is None or key_out is not None):
+        raise ValueError("a batch needs value, key_pages and value_pages, and no key_out")
+    if not paged and (value is not None or key_pages is not None or value_pages is not None):
+        raise ValueError("value and pages need a batch")
+    _same_device(dev, key=key, positions=positions, inv_freq=inv_freq, query_weight=query_weight,
+                 key_weight=key_weight, query_out=query_out, key_out=key_out, value=value)
+    a = QkNormRopeArgs(dtype=code, query_heads=Hq, kv_heads=Hk, dim=D, eps=eps, interleaved=int(interleaved))
+    if query_out is None:
+        query_out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
+    a.query, a.query_token_stride, a.query_head_stride = rows("query", query, Hq, False)
+    a.key, a.key_token_stride, a.key_head_stride = rows("key", key, Hk, False)
+    a.query_out, a.query_out_token_stride, a.query_out_head_stride = rows("query_out", query_out, Hq, True)
+    weights = [w for w in (query_weight, key_weight) if w is not None]
+    for w in weights:
+        if w.dtype not in (torch.float32, query.dtype) or w.dtype != weights[0].dtype:
+            raise TypeError(f"weights must both be float32 or both {query.dtype}")
+        if w.shape != (D,) or not w.is_contiguous():
+            raise ValueError(f"weights must be contiguous [{D}]")
+    a.query_weight, a.key_weight = _ptr(query_weight), _ptr(key_weight)
+    a.weight_fp32 = int(bool(weights) and weights[0].dtype == torch.float32)
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise ValueError("inv_freq must be a contiguous float32 vector")
+        a.inv_freq, a.rotary = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+    if paged:
+        _same_device(dev, lens=batch.lens)
+        P, H, page = _pools(key_pages, value_pages, batch, D, query.dtype)
+        if H != Hk:
+            raise ValueError(f"pages hold {H} KV heads, key has {Hk}")
+        _write_strides("key_pages", key_pages)
+        a.batch = batch.bind(P, page, N)
+        a.value, a.value_token_stride, a.value_head_stride = rows("value", value, Hk, False)
+        a.key_pages, a.value_pages = key_pages.data_ptr(), value_pages.data_ptr()
+        a.page_stride, a.head_stride, a.row_stride = (_stride(key_pages, 0), _stride(key_pages, 1),
+                                                      _stride(key_pages, 2))
+    else:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+        if positions.shape != (N,) or not positions.is_contiguous():
+            raise ValueError(f"positions must be contiguous [{N}]")
+        a.batch.n_tokens = N
+        a.positions, a.positions_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        if key_out is None:
+            key_out = torch.empty((N, Hk, D), dtype=key.dtype, device=dev)
+        a.key_out, a.key_out_token_stride, a.key_out_head_stride = rows("key_out", key_out, Hk, True)
+    with _on(dev):
+        check(_lib.lib().imi_qk_norm_rope(ctypes.byref(a), _stream(dev)), "imi_qk_norm_rope")
+    return query_out, key_out
+
+
+class PageTable:
+    """Which pages each sequence of a paged cache holds, on the device.
+
+    pages int32 [S, max_pages]: sequence s holds its first ceil(lens[s] /
+    page_size) entries; lens int32 [S]; refs int32 [n_pages]: sequences that
+    hold each page (0: free).  fork_pages, extend_pages and compact_pages work
+    on it without a host synchronisation and can be captured in a graph."""
+
+    __slots__ = ("pages", "lens", "refs", "page_size", "args", "device")
+
+    def __init__(self, pages: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page_size: int):
+        dev = _require_device(pages, lens, refs)
+        _same_device(dev, lens=lens, refs=refs)
+        _i32_tensor("pages", pages, 2)
+        _i32_tensor("lens", lens, 1)
+        _i32_tensor("refs", refs, 1)
+        if lens.shape[0] != pages.shape[0]:
+            raise ValueError(f"lens has {lens.shape[0]} entries for {pages.shape[0]} sequences")
+        _write_strides("pages", pages)
+        self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
+        S, M = pages.shape
+        self.args = PageTableArgs(pages.data_ptr(), pages.stride(0) if S > 1 else M, lens.data_ptr(),
+                                  refs.data_ptr(), S, M, refs.shape[0], self.page_size)
+
+    @classmethod
+    def empty(cls, n_seqs: int, max_pages: int, n_pages: int, page_size: int, device) -> "PageTable":
+        """n_seqs sequences of no rows over a pool of n_pages free pages."""
+        i32 = dict(dtype=torch.int32, device=device)
+        return cls(torch.full((n_seqs, max_pages), -1, **i32), torch.zeros((n_seqs,), **i32),
+                   torch.zeros((n_pages,), **i32), page_size)
+
+    def batch(self, query_start: torch.Tensor, max_query: int, max_len: Optional[int] = None) -> PagedBatch:
+        """The batch whose new tokens are the last rows of each sequence
+        (after extend_pages)."""
+        return PagedBatch(self.pages, self.lens, query_start, max_query, max_len)
+
+
+def _pool_args(table: PageTable, pools: Sequence[torch.Tensor]):
+    arr = (PagePool * max(len(pools), 1))()
+    for i, t in enumerate(pools):
+        _same_device(table.device, **{f"pool {i}": t})
+        if t.dim() < 2 or t.shape[0] != table.refs.shape[0]:
+            raise ValueError(f"pool {i} must have {table.refs.shape[0]} pages as its first dimension")
+        n = t[0].numel() if t.shape[0] else 0
+        span = 1 + sum((k - 1) * s for k, s in zip(t.shape[1:], t.stride()[1:]))
+        if n == 0 or span != n or (t.shape[0] > 1 and t.stride(0) < n):
+            raise ValueError(f"pool {i}: each page must be one dense block of memory")
+        size = t.element_size()
+        arr[i] = PagePool(t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else n) * size, n * size)
+    return arr, len(pools)
+
+
+def fork_pages(table: PageTable, parents: torch.Tensor, out: Optional[PageTable] = None) -> PageTable:
+    """The table in which sequence s goes on as sequence parents[s] (int32
+    [S]) of ``table`` and shares its pages: beams re-parented, a prompt forked,
+    or a sequence freed (a parent outside 0 .. S - 1).  ``out``: a table of
+    the same sizes and other memory to write to (two tables in turn serve a
+    loop); ``table`` itself is not changed."""
+    if parents.shape != table.lens.shape:
+        raise ValueError(f"parents has shape {tuple(parents.shape)} for {table.lens.shape[0]} sequences")
+    _i32_tensor("parents", parents, 1)
+    _same_device(table.device, parents=parents)
+    if out is None:
+        out = PageTable(torch.empty_like(table.pages, memory_format=torch.contiguous_format),
+                        torch.empty_like(table.lens), torch.empty_like(table.refs), table.page_size)
+    else:
+        _same_device(table.device, out=out.lens)
+        spans = [(t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+                 for x in (table, out) for t in (x.pages, x.lens, x.refs) if t.numel()]
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("out must share no memory with the table")
+    with _on(table.device):
+        check(_lib.lib().imi_fork_pages(ctypes.byref(table.args), parents.data_ptr(), ctypes.byref(out.args),
+                                        _stream(table.device)), "imi_fork_pages")
+    return out
+
+
+def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.Tensor] = ()) -> torch.Tensor:
+    """Grow sequence s by counts[s] tokens (int32 [S]), in place: the lowest
+    free pages go to the sequences in order.  A partly filled last page that
+    another sequence holds too is replaced by a copy, in every pool (tensors
+    [n_pages, ...], each page one dense block, e.g. the keys and the values of
+    every layer).  Returns bool [S]: False, with the sequence unchanged, where
+    its row of the table is too short or the pages that were free before the
+    call do not last for the sequences up to it."""
+    if counts.shape != table.lens.shape:
+        raise ValueError(f"counts has shape {tuple(counts.shape)} for {table.lens.shape[0]} sequences")
+    _i32_tensor("counts", counts, 1)
+    _same_device(table.device, counts=counts)
+    arr, n = _pool_args(table, pools)
+    dev = table.device
+    granted = torch.empty(counts.shape, dtype=torch.bool, device=dev)
+    L = _lib.lib()
+    with _on(dev):
+        need = ctypes.c_size_t()
+        check(L.imi_extend_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_extend_pages")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(L.imi_extend_pages(ctypes.byref(table.args), counts.data_ptr(), granted.data_ptr(), arr, n,
+                                 ws.data_ptr(), need.value, _stream(dev)), "imi_extend_pages")
+    return granted
+
+
+def compact_pages(table: PageTable, pools: Sequence[torch.Tensor] = ()) -> torch.Tensor:
+    """Move live pages to the lowest ids, in place (the table, refs and every
+    pool, as in extend_pages): the i-th live page from id n_live on goes to
+    the i-th free id below.  Returns n_live, int32 [1]."""
+    arr, n = _pool_args(table, pools)
+    dev = table.device
+    n_live = torch.empty((1,), dtype=torch.int32, device=dev)
+    L = _lib.lib()
+    with _on(dev):
+        need = ctypes.c_size_t()
+        check(L.imi_compact_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_compact_pages")
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        check(L.imi_compact_pages(ctypes.byref(table.args), n_live.data_ptr(), arr, n, ws.data_ptr(), need.value,
+                                  _stream(dev)), "imi_compact_pages")
+    return n_live

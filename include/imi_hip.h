@@ -536,6 +536,87 @@ typedef struct {
 int imi_paged_attention_workspace_size(const imi_paged_attention_args* a, size_t* bytes);
 int imi_paged_attention(const imi_paged_attention_args* a, imi_stream_t stream);
 
+/* RMS norm of each query and key head (over dim; skipped for a tensor without
+ * a weight) and rotation by position of the first `rotary` dims: pairs
+ * (i, i + rotary / 2), or (2i, 2i + 1) interleaved, by the angle position *
+ * inv_freq[i].  Either positions are given and keys go to key_out, or the
+ * batch gives them (the i-th new token of a sequence stands at lens - new
+ * tokens + i) and keys and values go to their rows of the pages; tokens
+ * behind the last sequence are then left alone.  fp32 arithmetic (angles
+ * fp64), one rounding.  Outputs may be the inputs. */
+typedef struct {
+    imi_paged_batch batch;       /* n_tokens always; the rest with key_pages */
+    int32_t dtype;               /* IMI_BF16 or IMI_FP16: every tensor but the weights */
+    int32_t query_heads, kv_heads, dim;   /* dim 64 or 128 */
+    const uint16_t* query;       /* device [n_tokens][query_heads][dim] */
+    int64_t query_token_stride, query_head_stride;
+    const uint16_t* key;         /* device [n_tokens][kv_heads][dim] */
+    int64_t key_token_stride, key_head_stride;
+    const uint16_t* value;       /* as key; with key_pages only */
+    int64_t value_token_stride, value_head_stride;
+    const void* positions;       /* device [n_tokens] int32 or int64, or NULL */
+    int32_t positions_64;
+    const float* inv_freq;       /* device [rotary / 2], or NULL with rotary 0 */
+    int32_t rotary;              /* a multiple of 16 up to dim */
+    int32_t interleaved;
+    const void* query_weight;    /* device [dim], or NULL: no norm of the queries */
+    const void* key_weight;
+    int32_t weight_fp32;         /* weights are float32 (else dtype) */
+    float eps;
+    uint16_t* query_out;
+    int64_t query_out_token_stride, query_out_head_stride;
+    uint16_t* key_out;           /* with positions */
+    int64_t key_out_token_stride, key_out_head_stride;
+    uint16_t* key_pages;         /* with the batch: [n_pages][kv_heads][page_size][dim] */
+    uint16_t* value_pages;
+    int64_t page_stride, head_stride, row_stride;
+} imi_qk_norm_rope_args;
+
+int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t stream);
+
+/* The page tables.  Sequence s holds the first ceil(lens[s] / page_size)
+ * entries of its row; refs[p] counts the sequences that hold page p, 0 =
+ * free.  Entries outside 0 .. n_pages - 1 are ignored. */
+typedef struct {
+    int32_t* pages;              /* device [n_seqs][stride] */
+    int64_t stride;              /* >= max_pages */
+    int32_t* lens;               /* device [n_seqs] */
+    int32_t* refs;               /* device [n_pages] */
+    int32_t n_seqs, max_pages, n_pages;
+    int32_t page_size;
+} imi_page_table;
+
+/* A tensor of pages whose contents follow the table (keys or values of a
+ * layer). */
+typedef struct {
+    void* base;                  /* device, 16-byte aligned */
+    int64_t page_stride;         /* bytes, a multiple of 16 */
+    int64_t page_bytes;          /* bytes of a page, a multiple of 16 */
+} imi_page_pool;
+
+/* out: sequence s becomes sequence parents[s] of in, sharing its pages; a
+ * parent outside 0 .. n_seqs - 1 leaves s empty.  Pages that no sequence
+ * holds any more are free.  Entries past a sequence's pages become -1.  out
+ * shares no memory with in. */
+int imi_fork_pages(const imi_page_table* in, const int32_t* parents, const imi_page_table* out, imi_stream_t stream);
+
+/* Grows sequence s by counts[s] tokens (< 0: 0), in place.  It takes the
+ * lowest free pages, sequences in order, for the entries it lacks, and for a
+ * partly filled last page that other sequences hold too: that page is copied
+ * in every pool.  granted[s] = 0, with the sequence as it was, where the row
+ * of the table is too short or the free pages (those free before the call)
+ * do not last for the sequences up to s. */
+int imi_extend_pages_workspace_size(const imi_page_table* t, size_t* bytes);
+int imi_extend_pages(const imi_page_table* t, const int32_t* counts, uint8_t* granted, const imi_page_pool* pools,
+                     int32_t n_pools, void* workspace, size_t workspace_bytes, imi_stream_t stream);
+
+/* Moves the live pages from id n_live on (n_live = pages with refs > 0) to
+ * the free ids below it, in ascending order both, in place: tables, refs and
+ * every pool. */
+int imi_compact_pages_workspace_size(const imi_page_table* t, size_t* bytes);
+int imi_compact_pages(const imi_page_table* t, int32_t* n_live, const imi_page_pool* pools, int32_t n_pools,
+                      void* workspace, size_t workspace_bytes, imi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
