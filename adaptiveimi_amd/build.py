@@ -35,9 +35,12 @@ HIPCC_FLAGS = [
 
 # Per-source additions.  k-means: matrix-core results go straight to VGPRs
 # (its E-step reads every accumulator with VALU code; the AGPR form costs one
-# copy per value).
+# copy per value).  Paged attention: a masked step's scores stay one register
+# tuple where the masked and the unmasked path meet (split into 32 values, each
+# is copied on the path that every step takes).
 EXTRA_FLAGS = {
     "imi_kmeans.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "imi_paged.hip": ["-mllvm", "-amdgpu-codegenprepare-break-large-phis=0"],
 }
 
 

@@ -175,6 +175,10 @@ __device__ __forceinline__ void wave_lds_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
+// The loads into LDS that this wave has under way are done.  The compiler
+// counts only those whose result it sees in a register.
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ u32x4_t load16(const uint16_t* p) { return *reinterpret_cast<const u32x4_t*>(p); }
 
 __device__ __forceinline__ s16x4_t read_tr(const uint16_t* p) {
@@ -562,13 +566,95 @@ __global__ __launch_bounds__(256) void few_merge_kernel(PagedParams a) {
 }
 
 // --------------------------------------------------------- many rows ------
-// Sequences of more rows (prefill chunks): tiles of kTileRows rows of one
-// (sequence, KV head), 32 per wave; the waves share each step's kStep rows of
-// K and V in LDS.  The steps of all tiles, KV head by KV head, are again cut
+// Sequences of more rows (prefill chunks): tiles of 256 rows of one (sequence,
+// KV head), 32 per wave; the waves share each step's 128 rows of K and V in
+// LDS.  The steps of all tiles, KV head by KV head, are again cut
 // into W equal ranges, so a causal triangle, a short prompt and a chunk over
 // a long prefix load the chip evenly; partials as above.
-constexpr int kTileRows = 128;
-constexpr int kStep = 64;
+constexpr int kTileRows = 256;
+constexpr int kStage = 64;            // cached rows of a stage in LDS
+constexpr int kStep = 2 * kStage;     // and of a step
+
+// A step's cached rows in LDS, two stages of 64, shared by the eight waves;
+// waves 0-3 fill the first stage, waves 4-7 the second.
+//
+// Thread (g, ch) of a wave holds piece ch (16 bytes, 8 dims) of NR rows in a
+// row, 16 wave + NR g + i, so one page lookup and one address serve K and V.
+// K goes from memory to LDS without registers (global_load_lds writes 64 x 16
+// bytes in lane order): load i of a wave is a block of consecutive LDS rows,
+// and a row's pieces lie at piece ^ k_swz(row).  A 16-byte read takes the lanes
+// 0-3, 12-15, 20-27 of a half wave together, then 4-11, 16-19, 28-31: sixteen
+// rows whose pieces then cover the 64 banks once.  V is transposed in registers on its way to LDS
+// ([dim][64 rows], 128 bytes a dim): the matrix instruction wants eight rows
+// of one dim per lane, and stored in the order that the registers of S^T have
+// (rows 4 hi .. and 8 + 4 hi .. of 16) they are one 16-byte read.  Dim d's
+// pieces lie at piece ^ ((d ^ d / 8) & 7): so do a read's dims, and the dims 8
+// apart of a write fall on different banks.
+template <int D>
+struct Stage {
+    static constexpr int CH = D / 8;          // 16-byte pieces of a row
+    static constexpr int NR = kStage * CH / 256;   // (four waves fill a stage)
+    static constexpr int G = 64 / CH;         // lane groups of a wave
+    static constexpr int kBytes = kStage * D * 2;   // of K, and of V
+    // what a lane adds to a stage's base, for the pieces that differ in the
+    // low bits xored in
+    static constexpr int KX = CH / 2;
+    int k_read[KX], v_read[4], v_write, v_swz, k_piece, l_ch, l_row;
+
+    // what row r's pieces of K are xored with
+    static __device__ __forceinline__ int k_swz(int r) { return D == 128 ? r & 15 : (r & 1) | ((r >> 1) & 6); }
+
+    __device__ __forceinline__ void init() {
+        const int lane = lane_id(), wave = threadIdx.x >> 6;
+        const int g = lane / CH;
+        l_ch = lane % CH;
+        l_row = 16 * wave + NR * g;   // in the step; the waves of a stage: 16 (wave & 3)
+        k_piece = l_ch ^ k_swz(NR * g);
+        const int q = lane & 31, hi = lane >> 5;
+        // LDS row of cached row q (of 16): load i = q % NR, lane group q / NR
+        const int slot = (q & 16) + (q % NR) * G + (q / NR) % G;
+        const int f = (q & 7) ^ (q >> 3);
+#pragma unroll
+        for (int x = 0; x < KX; ++x) k_read[x] = slot * (2 * D) + 16 * ((2 * x + hi) ^ k_swz(q));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) v_read[x] = q * 128 + 16 * ((f ^ hi) ^ (2 * x));
+        // this thread's rows in the transposed order
+        const int y = l_row & 15;
+        const int piece = 2 * (wave & 3) + ((y >> 2) & 1);
+        v_write = l_ch * 8 * 128 + 8 * ((y >> 3) & 1) + 2 * (y & 3);
+        v_swz = 16 * ((piece ^ l_ch) & 7);
+    }
+    // K: row i of the thread, from the row's first element to its LDS place
+    __device__ __forceinline__ void load_k(const uint16_t* row, int i, char* stage) const {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        typedef __attribute__((address_space(1))) const void gvoid;
+        typedef __attribute__((address_space(3))) void lvoid;
+        __builtin_amdgcn_global_load_lds((gvoid*)(row + 8 * (k_piece ^ i)), (lvoid*)(stage + (wave >> 2) * kBytes + ((wave & 3) * NR + i) * 1024), 16,
+                                         0, 0);
+    }
+    __device__ __forceinline__ void store_v(const u32x4_t (&r)[NR], char* stage) const {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            char* const at = stage + (threadIdx.x >> 8) * kBytes + v_write + (v_swz ^ (16 * d)) + 128 * d;
+            const uint32_t sel = d & 1 ? 0x07060302u : 0x05040100u;
+            const uint32_t lo = __builtin_amdgcn_perm(r[1][d >> 1], r[0][d >> 1], sel);
+            if constexpr (NR == 4) {
+                const uint32_t up = __builtin_amdgcn_perm(r[3][d >> 1], r[2][d >> 1], sel);
+                *reinterpret_cast<uint2*>(at) = make_uint2(lo, up);
+            } else {
+                *reinterpret_cast<uint32_t*>(at) = lo;
+            }
+        }
+    }
+    // S^T operand: rows 32 e .. of the step, dims 16 c ..
+    __device__ __forceinline__ u32x4_t k_frag(const char* stage, int e, int c) const {
+        return *reinterpret_cast<const u32x4_t*>(stage + k_read[c] + 32 * e * 2 * D);
+    }
+    // O^T operand: dims 32 d .., rows 32 e + 16 c ..
+    __device__ __forceinline__ u32x4_t v_frag(const char* stage, int e, int c, int d) const {
+        return *reinterpret_cast<const u32x4_t*>(stage + v_read[((2 * e + c) ^ (2 * (d & 1))) & 3] + 32 * d * 128);
+    }
+};
 
 __device__ __forceinline__ int seq_tiles(const PagedParams& a, const Seq& q) {
     const int64_t rows = static_cast<int64_t>(q.n) * a.G;
@@ -576,11 +662,35 @@ __device__ __forceinline__ int seq_tiles(const PagedParams& a, const Seq& q) {
     return static_cast<int>((rows + kTileRows - 1) / kTileRows);
 }
 
-__device__ __forceinline__ Span tile_span(const PagedParams& a, const Seq& q, int first) {
+// Rows of a tile of new tokens, bounds moved out to multiples of 8 so that
+// four rows from a multiple of 4 on are neighbours in memory (pages of four
+// rows or more): row v of the span is cached row v, v < pad, or v + shift.
+// The rows in between that no token sees (dead) weigh nothing.
+struct TileSpan {
+    int sink, lo, hi;     // visible: [0, sink) and [lo, hi)
+    int pad, shift, vis;  // rows of the span: vis
+    int edge;             // dead rows but for those past vis come before
+    __device__ __forceinline__ int row(int v) const { return v < pad ? v : v + shift; }
+    __device__ __forceinline__ bool dead(int v) const {
+        const int j = row(v);
+        return v >= vis || (j >= sink && j < lo);
+    }
+};
+__device__ __forceinline__ TileSpan tile_span(const PagedParams& a, const Seq& q, int first) {
     const int p0 = q.len - q.n;
     const int i0 = first / a.G;
     const int i1 = min((first + kTileRows - 1) / a.G, q.n - 1);
-    return span_of(a, q.len, max(p0 + i0, 0), p0 + i1);
+    const Span x = span_of(a, q.len, max(p0 + i0, 0), p0 + i1);
+    TileSpan r;
+    r.sink = x.sink;
+    r.lo = x.lo;
+    r.hi = x.hi;
+    r.pad = (x.sink + 7) & ~7;
+    r.shift = max((x.lo & ~7) - r.pad, 0);
+    r.vis = x.hi - r.shift;
+    if (r.shift == 0) r.pad = 0;
+    r.edge = x.lo > x.sink ? x.lo - r.shift : 0;
+    return r;
 }
 
 // The plan: tiles in use; per tile its sequence and first row, and the
@@ -648,7 +758,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(PagedParams a) {
             }
             const int row = (t - (lo ? p.seqs[lo - 1] : 0)) * kTileRows;
             p.tiles[t] = make_int2(lo, row);
-            u = max((tile_span(a, seq_of(a, lo), row).count() + kStep - 1) / kStep, 1);
+            u = max((tile_span(a, seq_of(a, lo), row).vis + kStep - 1) / kStep, 1);
         }
         int64_t total;
         const int64_t incl = block_incl_scan<int64_t>(u, s_wave, total);
@@ -674,19 +784,22 @@ __device__ __forceinline__ int find_tile(const int64_t* steps, int n, int64_t x)
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void tile_kernel(PagedParams a) {
+__global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     constexpr int KK = D / 16;
     constexpr int DB = D / 32;
-    constexpr int LR = kRow<D>;
-    constexpr int CH = D / 8;               // 16-byte pieces of a row
-    constexpr int RP = 256 / CH;            // rows that one load of the workgroup covers
-    constexpr int NR = kStep / RP;
-    __shared__ uint16_t s_k[2][kStep * LR];
-    __shared__ uint16_t s_v[2][kStep * LR];
+    constexpr int NF = 6;                   // operand blocks read ahead of their use (2, 4, 8: 940, 959, 918 TFLOP/s; 6: 962)
+    constexpr int NR = Stage<D>::NR;
+    constexpr int SB = Stage<D>::kBytes;
+    // one array: with two, the compiler makes every read of K wait for the
+    // loads into LDS that are under way for the next step
+    __shared__ __align__(1024) char s_stage[8 * SB];
+    char* const s_k = s_stage;
+    char* const s_v = s_stage + 4 * SB;
+    Stage<D> st;
+    st.init();
     const int tid = threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int q32 = lane & 31, hi = lane >> 5, ln = lane & 15;
-    const int l_row = tid / CH, l_ch = tid % CH;
+    const int q32 = lane & 31, hi = lane >> 5;
 
     const Plan plan = plan_of(a);
     const int n_tiles = *plan.n;
@@ -712,8 +825,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(PagedParams a) {
         const Seq sq = seq_of(a, s);
         const int64_t rows = static_cast<int64_t>(sq.n) * a.G;
         const int p0 = sq.len - sq.n;
-        const Span sp = tile_span(a, sq, tile.y);
-        const int vis = sp.count();
+        const TileSpan sp = tile_span(a, sq, tile.y);
+        const int vis = sp.vis;
 
         // this lane's query row (both halves of the wave), dims 16 c + 8 hi ..
         const int r = tile.y + wave * 32 + q32;
@@ -740,124 +853,150 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(PagedParams a) {
             for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
-        const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s + 8 * l_ch;
-        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * l_ch;
-        int id[NR];
-        auto row_at = [&](int u, int i) { return sp.row(min(u * kStep + l_row + RP * i, vis - 1)); };
-        auto fetch_ids = [&](int u) {
-#pragma unroll
-            for (int i = 0; i < NR; ++i) id[i] = page_of(a, s, row_at(u, i));
+        const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s;
+        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * st.l_ch;
+        // a whole step's rows are neighbours, four by four: one page lookup, one
+        // step ahead of its use, and one address per thread
+        auto neighbours = [&](int u) {
+            return a.page_shift >= 2 && (u + 1) * kStep <= vis && (u * kStep >= sp.pad || (u + 1) * kStep <= sp.pad);
         };
-        u32x4_t kb[NR], vb[NR];
+        int id = s;
+        auto fetch_id = [&](int u) {
+            if (a.table) id = page_of(a, s, sp.row(min(u * kStep + st.l_row, vis - 1)));
+        };
+        u32x4_t vb[NR];
         auto fetch = [&](int u) {
+            char* const sk = s_k + (u & 1) * 2 * SB;
+            if (neighbours(u)) {
+                const int64_t o = row_offset(a, id, sp.row(u * kStep + st.l_row));
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int64_t o = row_offset(a, id[i], row_at(u, i));
-                kb[i] = load16(kh + o);
-                vb[i] = load16(vh + o);
+                for (int i = 0; i < NR; ++i) {
+                    st.load_k(kh + o + i * a.tok_s, i, sk);
+                    vb[i] = load16(vh + o + i * a.tok_s);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    const int j = sp.row(min(u * kStep + st.l_row + i, vis - 1));
+                    const int64_t o = row_offset(a, page_of(a, s, j), j);
+                    st.load_k(kh + o, i, sk);
+                    vb[i] = load16(vh + o);
+                }
             }
         };
         auto store = [&](int u) {
-            uint16_t* const sk = s_k[u & 1];
-            uint16_t* const sv = s_v[u & 1];
-            const bool tail = (u + 1) * kStep > vis;
+            if ((u + 1) * kStep > vis || u * kStep < sp.edge) {   // no NaN may enter through a dead row's V
 #pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const int row = l_row + RP * i;
-                *reinterpret_cast<u32x4_t*>(sk + row * LR + 8 * l_ch) = kb[i];
-                // rows past the end weigh nothing: no NaN may enter through V
-                if (tail && u * kStep + row >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
-                *reinterpret_cast<u32x4_t*>(sv + row * LR + 8 * l_ch) = vb[i];
+                for (int i = 0; i < NR; ++i)
+                    if (sp.dead(u * kStep + st.l_row + i)) vb[i] = u32x4_t{0, 0, 0, 0};
             }
+            st.store_v(vb, s_v + (u & 1) * 2 * SB);
+            wait_loads();   // K is in LDS
         };
+        // block n of a step's V: rows 16 (n / DB), dims 32 (n % DB)
+        auto v_at = [&](const char* sv, int n) { return st.v_frag(sv, n / DB >> 1, n / DB & 1, n % DB); };
+        auto order = [] { __builtin_amdgcn_sched_barrier(0); };   // reads stay ahead of their use
+#pragma unroll
+        for (int c = 0; c < KK; ++c) asm volatile("" : "+v"(qf[c]));   // loaded here, not waited for in every step
         if (vis > 0) {
-            fetch_ids(u0);
+            fetch_id(u0);
             fetch(u0);
-            fetch_ids(min(u0 + 1, u1 - 1));
+            fetch_id(min(u0 + 1, u1 - 1));
             store(u0);
         }
         for (int u = u0; vis > 0 && u < u1; ++u) {
             const bool more = u + 1 < u1;
+            __syncthreads();
             if (more) {
                 fetch(u + 1);
-                fetch_ids(min(u + 2, u1 - 1));
+                fetch_id(min(u + 2, u1 - 1));
             }
-            __syncthreads();
-            const uint16_t* const sk = s_k[u & 1];
-            const uint16_t* const sv = s_v[u & 1];
-            const int v0 = u * kStep;
-            const int j_lo = sp.row(v0), j_hi = sp.row(min(v0 + kStep, vis) - 1);
-            // a step whose rows none of the wave's tokens sees is skipped
-            const bool skip = idle || j_lo > p_max ||
-                              (a.window > 0 && v0 >= sp.sink && j_hi <= p_min - a.window);
-            if (!skip) {
-                f32x16_t sc[2];
+#pragma unroll 1
+            for (int sub = 0; sub < 2; ++sub) {
+                const char* const sk = s_k + ((u & 1) * 2 + sub) * SB;
+                const char* const sv = s_v + ((u & 1) * 2 + sub) * SB;
+                const int v0 = u * kStep + sub * kStage;
+                if (sub > 0 && more) store(u + 1);   // between two stages, not where the waves meet
+                if (v0 >= vis) break;
+                const int j_lo = sp.row(v0), j_hi = sp.row(min(v0 + kStage, vis) - 1);
+                // a step whose rows none of the wave's tokens sees is skipped
+                const bool skip = idle || j_lo > p_max ||
+                                  (a.window > 0 && j_lo >= a.sinks && j_hi <= p_min - a.window);
+                if (!skip) {
+                    f32x16_t sc[2];
+                    // K's blocks (32 rows, 16 dims), then V's, NF reads ahead
+                    u32x4_t fr[NF];
+                    auto frag = [&](int n) {
+                        return n < 2 * KK ? st.k_frag(sk, n & 1, n >> 1) : v_at(sv, n - 2 * KK);
+                    };
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) sc[e][i] = 0.0f;
-#pragma unroll
-                    for (int c = 0; c < KK; ++c)
-                        sc[e] = T::mma32(load16(sk + (32 * e + q32) * LR + 16 * c + 8 * hi), qf[c], sc[e]);
-                }
-                // lane: keys v0 + 32 e + 8 (i / 4) + 4 hi + i % 4 of row q32
-                const bool full = v0 + kStep <= vis && j_hi <= p_min &&
-                                  (a.window == 0 || j_lo > p_max - a.window || j_hi < a.sinks) &&
-                                  w_first + 32 <= rows;
-                if (!full) {
+                    for (int n = 0; n < NF; ++n) fr[n] = frag(n);
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int v = v0 + 32 * e + 8 * (i >> 2) + 4 * hi + (i & 3);
-                            const int j = sp.row(v);
-                            const bool seen = v < vis && j <= pos &&
-                                              (a.window == 0 || j > pos - a.window || j < a.sinks);
-                            sc[e][i] = seen ? sc[e][i] : -INFINITY;
-                        }
-                }
-                float mx = -INFINITY;
+                        for (int i = 0; i < 16; ++i) sc[e][i] = 0.0f;
+                    order();
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[e][i]);
-                mx = fmaxf(mx, xor32(mx));
-                const bool grow = (mx - m) * a.c > kSlack;
-                if (__builtin_amdgcn_ballot_w64(grow)) {
-                    const float f = grow ? __builtin_amdgcn_exp2f((m - mx) * a.c) : 1.0f;
-                    m = grow ? mx : m;
-                    l *= f;
-#pragma unroll
-                    for (int d = 0; d < DB; ++d) acc[d] *= f;
-                }
-                const float mc = m == -INFINITY ? 0.0f : m * a.c;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        sc[e][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e][i], a.c, -mc));
-                float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) ls[i & 3] += sc[e][i];
-                l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const u32x4_t pf = u32x4_t{T::pack(sc[e][8 * c], sc[e][8 * c + 1]),
-                                                   T::pack(sc[e][8 * c + 2], sc[e][8 * c + 3]),
-                                                   T::pack(sc[e][8 * c + 4], sc[e][8 * c + 5]),
-                                                   T::pack(sc[e][8 * c + 6], sc[e][8 * c + 7])};
-                        const uint16_t* vp = sv + (32 * e + 16 * c + 4 * hi + (ln >> 2)) * LR +
-                                             16 * ((lane >> 4) & 1) + 4 * (ln & 3);
-#pragma unroll
-                        for (int d = 0; d < DB; ++d)
-                            acc[d] = T::mma32(join(read_tr(vp + 32 * d), read_tr(vp + 8 * LR + 32 * d)), pf, acc[d]);
+                    for (int n = 0; n < 2 * KK; ++n) {
+                        sc[n & 1] = T::mma32(fr[n % NF], qf[n >> 1], sc[n & 1]);
+                        fr[n % NF] = frag(n + NF);
+                        order();
                     }
+                    // lane: keys v0 + 32 e + 8 (i / 4) + 4 hi + i % 4 of row q32
+                    const bool full = v0 + kStage <= vis && j_hi <= p_min &&
+                                      (a.window == 0 || j_lo > p_max - a.window || j_hi < a.sinks) &&
+                                      w_first + 32 <= rows;
+                    u32x4_t pf[4];   // weights of 16 rows each
+                    {
+                        if (!full) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const int v = v0 + 32 * e + 8 * (i >> 2) + 4 * hi + (i & 3);
+                                    const int j = sp.row(v);
+                                    const bool seen = v < vis && j <= pos &&
+                                                      (a.window == 0 || j > pos - a.window || j < a.sinks);
+                                    sc[e][i] = seen ? sc[e][i] : -INFINITY;
+                                }
+                        }
+                        float mx = sc[0][0];
+#pragma unroll
+                        for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sc[i >> 4][i & 15]);
+                        mx = fmaxf(mx, xor32(mx));
+                        const bool grow = (mx - m) * a.c > kSlack;
+                        if (__builtin_amdgcn_ballot_w64(grow)) {
+                            const float f = grow ? __builtin_amdgcn_exp2f((m - mx) * a.c) : 1.0f;
+                            m = grow ? mx : m;
+                            l *= f;
+#pragma unroll
+                            for (int d = 0; d < DB; ++d) acc[d] *= f;
+                        }
+                        const float mc = m == -INFINITY ? 0.0f : m * a.c;
+                        float ls[2] = {0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], a.c, -mc));
+                            const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], a.c, -mc));
+                            pf[i >> 2][i & 3] = T::pack(w0, w1);
+                            ls[0] += w0;
+                            ls[1] += w1;
+                        }
+                        l += ls[0] + ls[1];
+                    }
+                    order();
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                        for (int d = 0; d < DB; ++d) {
+                            const int n = 2 * KK + DB * x + d;
+                            acc[d] = T::mma32(fr[n % NF], pf[x], acc[d]);
+                            if (n + NF < 2 * KK + 4 * DB) fr[n % NF] = frag(n + NF);
+                            order();
+                        }
+                    }
+                }
             }
-            if (more) store(u + 1);
         }
         l += xor32(l);
         if (live) {
@@ -996,8 +1135,8 @@ Shape shape_of(const imi_paged_attention_args* a) {
         if (!p.direct) p.few_part = size_t(2) * p.few_wg * p.few_rows * (a->dim + 2) * sizeof(float);
     }
     if (p.tiles) {
+        p.tile_wg = device_cus();
         p.slots = static_cast<int>(static_cast<int64_t>(b.n_tokens) * a->groups / kTileRows + b.n_seqs);
-        p.tile_wg = 2 * device_cus();
         p.tile_part = size_t(2) * p.tile_wg * kTileRows * (a->dim + 2) * sizeof(float);
         p.plan = plan_bytes(p.slots, b.n_seqs);
     }
@@ -1026,7 +1165,7 @@ int launch(const imi_paged_attention_args* a, const Shape& p, PagedParams P, flo
         Q.slots = p.slots;
         plan_kernel<<<1, 1024, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("plan_kernel");
-        tile_kernel<T, D><<<p.tile_wg, 256, 0, stream>>>(Q);
+        tile_kernel<T, D><<<p.tile_wg, 512, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("tile_kernel");
         tile_merge_kernel<T, D><<<dim3(p.tile_wg - 1, kTileRows * D / 1024), 256, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("tile_merge_kernel");

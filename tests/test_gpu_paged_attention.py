@@ -150,6 +150,11 @@ CASES = [
     ([200, 1, 333, 77, 64, 500], [1, 1, 150, 77, 2, 1], 2, 5, 128, 16, BF, 0, 0, "heads"),
     ([200, 1, 333, 77, 64, 500], [1, 1, 150, 77, 2, 1], 1, 33, 64, 16, BF, 90, 3, "tokens"),   # more than 32 rows a token
     ([64, 129, 31], [64, 129, 31], 1, 4, 128, 0, HF, 0, 0, "heads"),
+    ([600], [100], 1, 4, 128, 8, BF, 301, 100, "heads"),        # sinks and window with a few rows between them
+    ([700], [100], 1, 2, 64, 16, HF, 203, 69, "tokens"),        # a gap of more
+    ([500], [90], 1, 4, 128, 1, BF, 0, 0, "heads"),             # pages of one row and of two
+    ([500], [90], 1, 4, 128, 2, HF, 77, 5, "heads"),
+    ([1500], [700], 1, 4, 128, 16, BF, 0, 0, "heads"),
 ]
 
 
