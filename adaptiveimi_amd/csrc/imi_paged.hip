@@ -106,6 +106,8 @@ struct FP16 {
 template <int D>
 constexpr int kRow = D == 128 ? 144 : 72;
 
+struct Join;
+
 struct PagedParams {
     const uint16_t* q;
     const uint16_t* k;
@@ -127,9 +129,11 @@ struct PagedParams {
     int window, sinks;
     float c;                   // scale * log2(e)
     int min_rows, max_rows;    // rows (n * G) of the sequences this launch takes
-    int W;                     // workgroups that share the work
-    float* part;               // [2 W][rows][D]
-    float* part_ml;            // [2 W][rows][2]
+    int w_log;                 // 2^w_log workgroups share the work
+    Join* joins;        // [W]
+    float* part;               // [2 W][cap][D]
+    float* part_ml;            // [2 W][cap][2]
+    int cap;                   // rows of a partial
     int32_t* plan;             // tile kernel: see plan_kernel
     int slots;                 // tile kernel: tiles that the plan can hold
 };
@@ -200,10 +204,25 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
 // ranges, one per workgroup, whatever the lengths (each workgroup adds the
 // lengths up itself: no host knows them).  A workgroup whose range covers a
 // whole (sequence, head) writes its output; the others (its first and its
-// last at most) write a partial that few_merge_kernel joins in order.
-constexpr int kFewWaves = 4;
+// last at most) write a partial that merge_kernel joins.
+constexpr int kFewWaves = 8;
 constexpr int kFewTile = 32;                       // rows of K / V per wave and step
 constexpr int kUnit = kFewTile * kFewWaves;
+
+// How both kernels cut their work: range w of 2^w_log is the units
+// [cut(w), cut(w + 1)).  What one range holds of a (sequence, head) or tile
+// with units [lo, hi) that it does not hold whole goes to a partial: 2 w for
+// the first that the range meets, 2 w + 1 for the last.  The range that holds
+// unit lo leaves a Join where hi lies past its end, and merge_kernel joins the
+// partials of the ranges from there on, in order.
+struct Join {
+    int64_t total;      // units in all
+    int64_t lo, hi;     // lo = hi: nothing to join
+    int t0;             // the sequence's first query row
+    int first, end;     // rows (token, head of the group) [first, end)
+    int h;
+};
+__device__ __forceinline__ int64_t cut(int64_t total, int64_t w, int w_log) { return (total * w) >> w_log; }
 
 __device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
     const int rows = q.n * a.G;
@@ -212,39 +231,51 @@ __device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
     return max((sp.count() + kUnit - 1) / kUnit, 1);
 }
 
-// Units of all sequences (per KV head), and where unit `at` falls: the
-// sequence and the units before it.
-struct FewPlace {
-    int s;
-    int64_t before;
-};
-__device__ __forceinline__ int64_t few_total(const PagedParams& a) {
-    int64_t total = 0;
-    for (int s0 = 0; s0 < a.S; s0 += 64) {
-        const int s = s0 + lane_id();
-        total += wave_sum_i(s < a.S ? few_units(a, seq_of(a, s)) : 0);
-    }
-    return total;
+// a / b, fast where it fits 32 bits
+__device__ __forceinline__ int quotient(int64_t a, int b) {
+    return a <= UINT_MAX ? static_cast<int>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b))
+                         : static_cast<int>(a / b);
 }
-// First sequence whose units (times H) reach past `at`; units before it.
-__device__ __forceinline__ FewPlace few_find(const PagedParams& a, int64_t at) {
-    int64_t before = 0;
+
+// This workgroup's range of the units of all sequences, the sequence in which
+// it begins and the units (of one KV head) before that sequence.
+struct FewRange {
+    int64_t total, g0, g1, before;
+    int s;
+};
+__device__ __forceinline__ FewRange few_range(const PagedParams& a) {
+    FewRange r{0, 0, 0, 0, 0};
+    int u = 0, incl = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         const int s = s0 + lane_id();
-        const int u = s < a.S ? few_units(a, seq_of(a, s)) : 0;
-        const int incl = wave_incl_scan(u);
-        const uint64_t past = __ballot((before + incl) * a.H > at);
+        u = s < a.S ? few_units(a, seq_of(a, s)) : 0;
+        incl = wave_incl_scan(u);
+        r.total += __builtin_amdgcn_readlane(incl, 63);
+    }
+    r.total *= a.H;
+    r.g0 = cut(r.total, blockIdx.x, a.w_log);
+    r.g1 = cut(r.total, blockIdx.x + 1, a.w_log);
+    if (r.g0 >= r.g1) return r;
+    for (int s0 = 0; s0 < a.S; s0 += 64) {
+        if (a.S > 64) {   // else the only 64 are still at hand
+            const int s = s0 + lane_id();
+            u = s < a.S ? few_units(a, seq_of(a, s)) : 0;
+            incl = wave_incl_scan(u);
+        }
+        const uint64_t past = __ballot((r.before + incl) * a.H > r.g0);
         if (past) {
             const int l = __builtin_ctzll(past);
-            return FewPlace{s0 + l, before + __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(u, l)};
+            r.s = s0 + l;
+            r.before += __builtin_amdgcn_readlane(incl, l) - __builtin_amdgcn_readlane(u, l);
+            return r;
         }
-        before += __builtin_amdgcn_readlane(incl, 63);
+        r.before += __builtin_amdgcn_readlane(incl, 63);
     }
-    return FewPlace{a.S, before};
+    return r;
 }
 
 template <typename T, int D, int NB>
-__global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) {
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, int direct) {
     constexpr int KK = D / 32;     // matrix instructions over the head dim
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
@@ -256,25 +287,23 @@ __global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) 
     const int ln = lane & 15, lg = lane >> 4;
     uint16_t* const sv = s_buf + wave * kWaveLds;
 
-    int64_t g0, g1;   // this workgroup's units
-    FewPlace at;
+    FewRange range;
     if (direct) {     // a workgroup per (sequence, head): nothing to join
-        at.s = blockIdx.x / a.H;
-        at.before = 0;
-        const int u = few_units(a, seq_of(a, at.s));
+        range.s = blockIdx.x / a.H;
+        range.before = 0;
+        const int u = few_units(a, seq_of(a, range.s));
         if (u == 0) return;
-        g0 = static_cast<int64_t>(blockIdx.x % a.H) * u;
-        g1 = g0 + u;
+        range.g0 = static_cast<int64_t>(blockIdx.x % a.H) * u;
+        range.g1 = range.g0 + u;
     } else {
-        const int64_t U = few_total(a) * a.H;
-        g0 = U * blockIdx.x / a.W;
-        g1 = U * (blockIdx.x + 1) / a.W;
-        if (g0 >= g1) return;
-        at = few_find(a, g0);
+        range = few_range(a);
     }
-    int s = at.s;
-    int64_t base = at.before * a.H;   // units before sequence s, all heads
+    int64_t g0 = range.g0;
+    const int64_t g1 = range.g1;
+    int s = range.s;
+    int64_t base = range.before * a.H;   // units before sequence s, all heads
     bool first = true;
+    Join rest{0, 0, 0, 0, 0, 0, 0};
     while (g0 < g1) {
         const Seq sq = seq_of(a, s);
         const int units = few_units(a, sq);
@@ -283,7 +312,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) 
             ++s;
             continue;
         }
-        const int h = static_cast<int>((g0 - base) / units);
+        const int h = direct ? blockIdx.x % a.H : quotient(g0 - base, units);
         const int u0 = static_cast<int>(g0 - base - static_cast<int64_t>(h) * units);
         const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + g1 - g0));
         const int rows = sq.n * a.G;
@@ -318,8 +347,9 @@ __global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) 
         const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * lg;
         // lane's two rows of a step's tile: ln and 16 + ln
         auto row_at = [&](int u, int e) { return min(u * kUnit + wave * kFewTile + 16 * e + ln, vis - 1); };
-        int id[2];
+        int id[2] = {s, s};
         auto fetch_ids = [&](int u) {
+            if (!a.table) return;
 #pragma unroll
             for (int e = 0; e < 2; ++e) id[e] = page_of(a, s, sp.row(row_at(u, e)));
         };
@@ -441,7 +471,7 @@ __global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) 
             for (int d = 0; d < DB; ++d)
                 *reinterpret_cast<f32x4_t*>(so + ln * D + 16 * d + 4 * lg) = acc[b][d];
             __syncthreads();
-            for (int x = tid; x < 16 * D / 4; x += 256) {
+            for (int x = tid; x < 16 * D / 4; x += 64 * kFewWaves) {
                 const int rr = x / (D / 4), d4 = x % (D / 4), r = 16 * b + rr;
                 if (r >= rows) break;
                 float M = -INFINITY;
@@ -468,30 +498,22 @@ __global__ __launch_bounds__(256, 2) void few_kernel(PagedParams a, int direct) 
                     if (a.lse && d4 == 0)
                         a.lse[t * a.l_ts + x_head] = L == 0.0f ? -INFINITY : (M * a.c + __log2f(L)) * kLn2;
                 } else {
-                    *reinterpret_cast<f32x4_t*>(a.part + (slot * a.max_rows + r) * D + 4 * d4) = A;
+                    *reinterpret_cast<f32x4_t*>(a.part + (slot * a.cap + r) * D + 4 * d4) = A;
                     if (d4 == 0) {
-                        a.part_ml[(slot * a.max_rows + r) * 2] = M;
-                        a.part_ml[(slot * a.max_rows + r) * 2 + 1] = L;
+                        a.part_ml[(slot * a.cap + r) * 2] = M;
+                        a.part_ml[(slot * a.cap + r) * 2 + 1] = L;
                     }
                 }
             }
         }
         __syncthreads();
+        if (u0 == 0 && u1 < units)
+            rest = Join{range.total, g0, g0 + units, sq.t0, 0, rows, h};
         g0 += u1 - u0;
         first = false;
     }
+    if (!direct && tid == 0) a.joins[blockIdx.x] = rest;
 }
-
-// What the joins share.  Cut w lies at unit U w / W; a (sequence, head) or
-// tile with units [lo, hi) was shared when a cut falls inside, and the join
-// belongs to the first such cut, so a launch over the cuts covers all of them
-// whatever the batch is.  Range w - 1 holds lo, the ranges from w on continue;
-// each wrote its first partial, but w - 1 its second if it begins before lo.
-struct Join {
-    int w;             // first cut inside
-    int64_t lo, hi;
-};
-__device__ __forceinline__ int64_t cut(int64_t U, int64_t w, int W) { return U * w / W; }
 
 template <int D>
 struct Partial {
@@ -504,64 +526,85 @@ struct Partial {
         A = A * f0 + x * f1;
         M = Mn;
     }
-    // partials first, first + step, ... of a join, in order
-    __device__ __forceinline__ void gather(const PagedParams& a, int64_t U, const Join& j, int cap, int r, int d4,
-                                           int first, int step) {
-        for (int w = j.w - 1 + first; w < a.W && cut(U, w, a.W) < j.hi; w += step) {
-            const int64_t b = cut(U, w, a.W);
-            if (b == cut(U, w + 1, a.W)) continue;   // an empty range
-            const int64_t e = (2 * static_cast<int64_t>(w) + (b < j.lo ? 1 : 0)) * cap + r;
-            add(a.part_ml[2 * e], a.part_ml[2 * e + 1], *reinterpret_cast<const f32x4_t*>(a.part + e * D + 4 * d4),
-                a.c);
+    // row r's partials of ranges w0 + first, w0 + first + step .. w1, four
+    // loads under way at a time; an empty range (its slot holds anything) and
+    // one past w1 weigh nothing
+    __device__ __forceinline__ void gather(const PagedParams& a, const Join& j, int w0, int w1, int r, int d4, int first,
+                                           int step) {
+        for (int w = w0 + first; w <= w1; w += 4 * step) {
+            float m[4], l[4];
+            f32x4_t x[4];
+            bool use[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int wi = min(w + i * step, w1);
+                const int64_t b = cut(j.total, wi, a.w_log);
+                use[i] = w + i * step <= w1 && b != cut(j.total, wi + 1, a.w_log);
+                const int64_t e = (2 * static_cast<int64_t>(wi) + (b < j.lo ? 1 : 0)) * a.cap + r;
+                m[i] = a.part_ml[2 * e];
+                l[i] = a.part_ml[2 * e + 1];
+                x[i] = *reinterpret_cast<const f32x4_t*>(a.part + e * D + 4 * d4);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (use[i]) add(m[i], l[i], x[i], a.c);
         }
+    }
+    template <typename T>
+    __device__ __forceinline__ void write(const PagedParams& a, const Join& j, int row, int d4) const {
+        const int64_t tok = j.t0 + row / a.G;
+        const int head = j.h * a.G + row % a.G;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        uint2 o;
+        o.x = T::pack(A[0] * inv, A[1] * inv);
+        o.y = T::pack(A[2] * inv, A[3] * inv);
+        *reinterpret_cast<uint2*>(a.out + tok * a.o_ts + head * a.o_hs + 4 * d4) = o;
+        if (a.lse && d4 == 0) a.lse[tok * a.l_ts + head] = L == 0.0f ? -INFINITY : (M * a.c + __log2f(L)) * kLn2;
     }
 };
 
-template <typename T, int D>
-__device__ __forceinline__ void write_row(const PagedParams& a, const Partial<D>& p, int64_t tok, int x_head, int d4) {
-    const float inv = p.L == 0.0f ? 0.0f : 1.0f / p.L;
-    uint2 o;
-    o.x = T::pack(p.A[0] * inv, p.A[1] * inv);
-    o.y = T::pack(p.A[2] * inv, p.A[3] * inv);
-    *reinterpret_cast<uint2*>(a.out + tok * a.o_ts + x_head * a.o_hs + 4 * d4) = o;
-    if (a.lse && d4 == 0) a.lse[tok * a.l_ts + x_head] = p.L == 0.0f ? -INFINITY : (p.M * a.c + __log2f(p.L)) * kLn2;
-}
+// One workgroup per (range, y).  D / 4 threads hold a row's partial; with few of
+// them the groups take a row each, with many (a long sequence of few rows) all
+// take a row's partials in turn, one row after another or (spread) one per y.
+constexpr int kManyParts = 4;
 
-// One workgroup per (cut, row): a row has many partials (a long sequence is
-// cut often), which D / 4 threads at a time take in turn.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void few_merge_kernel(PagedParams a) {
-    constexpr int Q = D / 4;            // threads that hold a row
-    constexpr int P = 256 / Q;          // partials in flight
+__global__ __launch_bounds__(256) void merge_kernel(PagedParams a, bool spread) {
+    constexpr int Q = D / 4, P = 256 / Q;
     __shared__ float s_ml[P][2];
     __shared__ float s_acc[P][D];
-    const int w = blockIdx.x + 1, r = blockIdx.y;
-    const int64_t U = few_total(a) * a.H;
-    const int64_t at = cut(U, w, a.W);
-    if (at >= U || at == cut(U, w - 1, a.W)) return;
-    const FewPlace f = few_find(a, at);
-    const Seq sq = seq_of(a, f.s);
-    const int units = few_units(a, sq);
-    const int h = static_cast<int>((at - f.before * a.H) / units);
-    Join j;
-    j.w = w;
-    j.lo = f.before * a.H + static_cast<int64_t>(h) * units;
-    j.hi = j.lo + units;
-    if (r >= sq.n * a.G || at == j.lo || cut(U, w - 1, a.W) > j.lo) return;
-    const int tid = threadIdx.x, d4 = tid % Q, g = tid / Q;
-    Partial<D> p;
-    p.gather(a, U, j, a.max_rows, r, d4, g, P);
-    if (d4 == 0) {
-        s_ml[g][0] = p.M;
-        s_ml[g][1] = p.L;
+    const Join j = a.joins[blockIdx.x];
+    const int r0 = blockIdx.y * P;
+    if (j.lo == j.hi || (spread ? static_cast<int>(blockIdx.y) : r0) >= j.end - j.first) return;
+    const int w0 = blockIdx.x, d4 = threadIdx.x % Q, g = threadIdx.x / Q;
+    // the last range that holds some: about hi W / total, then exactly
+    int w1 = static_cast<int>(((j.hi - 1) << a.w_log) / j.total);
+    while (cut(j.total, w1 + 1, a.w_log) < j.hi) ++w1;
+    if (w1 - w0 < kManyParts) {
+        const int r = r0 + g;
+        if (r >= j.end - j.first) return;
+        Partial<D> p;
+        p.gather(a, j, w0, w1, r, d4, 0, 1);
+        p.template write<T>(a, j, j.first + r, d4);
+        return;
     }
-    *reinterpret_cast<f32x4_t*>(&s_acc[g][4 * d4]) = p.A;
-    __syncthreads();
-    if (g == 0) {
-        Partial<D> t;
-        for (int x = 0; x < P; ++x)
-            t.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
-        write_row<T, D>(a, t, sq.t0 + r / a.G, h * a.G + r % a.G, d4);
+    const int r_lo = spread ? blockIdx.y : r0, r_hi = spread ? r_lo + 1 : min(r0 + P, j.end - j.first);
+    for (int r = r_lo; r < r_hi; ++r) {
+        Partial<D> p;
+        p.gather(a, j, w0, w1, r, d4, g, P);
+        __syncthreads();
+        if (d4 == 0) {
+            s_ml[g][0] = p.M;
+            s_ml[g][1] = p.L;
+        }
+        *reinterpret_cast<f32x4_t*>(&s_acc[g][4 * d4]) = p.A;
+        __syncthreads();
+        if (g == 0) {
+            Partial<D> t;
+            for (int x = 0; x < P; ++x)
+                t.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
+            t.template write<T>(a, j, j.first + r, d4);
+        }
     }
 }
 
@@ -804,15 +847,16 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     const Plan plan = plan_of(a);
     const int n_tiles = *plan.n;
     const int64_t* const steps = plan.steps;
-    if (n_tiles == 0) return;
-    const int64_t per_head = steps[n_tiles - 1];
-    const int64_t U = per_head * a.H;
+    const int64_t per_head = n_tiles ? steps[n_tiles - 1] : 1;
+    const int64_t total = n_tiles ? per_head * a.H : 0;
     // workgroups go round robin over the 8 dies: die x takes the x-th eighth
     // of the steps, so that its workgroups read the same head's K and V
-    const int wg = a.W % 8 == 0 ? (blockIdx.x % 8) * (a.W / 8) + blockIdx.x / 8 : blockIdx.x;
-    int64_t g0 = U * wg / a.W;
-    const int64_t g1 = U * (wg + 1) / a.W;
+    const int W = 1 << a.w_log;
+    const int wg = W >= 8 ? (blockIdx.x % 8) * (W / 8) + blockIdx.x / 8 : blockIdx.x;
+    int64_t g0 = cut(total, wg, a.w_log);
+    const int64_t g1 = cut(total, wg + 1, a.w_log);
     bool first = true;
+    Join rest{0, 0, 0, 0, 0, 0, 0};
     int h = static_cast<int>(g0 / per_head);
     int t = g0 < g1 ? find_tile(steps, n_tiles, g0 - h * per_head) : 0;
     while (g0 < g1) {
@@ -1030,6 +1074,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
             }
         }
         __syncthreads();   // the next range's first store reuses the tiles
+        if (u0 == 0 && u1 < units)
+            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, static_cast<int>(min(rows, static_cast<int64_t>(tile.y) + kTileRows)), h};
         g0 += u1 - u0;
         first = false;
         if (++t == n_tiles) {
@@ -1037,34 +1083,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
             ++h;
         }
     }
-}
-
-// One workgroup per (cut, 256 / (D / 4) rows).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void tile_merge_kernel(PagedParams a) {
-    constexpr int Q = D / 4;
-    const Plan plan = plan_of(a);
-    const int n_tiles = *plan.n;
-    if (n_tiles == 0) return;
-    const int64_t per_head = plan.steps[n_tiles - 1];
-    const int64_t U = per_head * a.H;
-    const int w = blockIdx.x + 1;
-    const int64_t at = cut(U, w, a.W);
-    if (at >= U || at == cut(U, w - 1, a.W)) return;
-    const int h = static_cast<int>(at / per_head);
-    const int t = find_tile(plan.steps, n_tiles, at - h * per_head);
-    const int2 tile = plan.tiles[t];
-    const Seq sq = seq_of(a, tile.x);
-    Join j;
-    j.w = w;
-    j.lo = h * per_head + (t ? plan.steps[t - 1] : 0);
-    j.hi = h * per_head + plan.steps[t];
-    const int r = blockIdx.y * (256 / Q) + threadIdx.x / Q, d4 = threadIdx.x % Q;
-    const int row = tile.y + r;
-    if (at == j.lo || cut(U, w - 1, a.W) > j.lo || row >= static_cast<int64_t>(sq.n) * a.G) return;
-    Partial<D> p;
-    p.gather(a, U, j, kTileRows, r, d4, 0, 1);
-    write_row<T, D>(a, p, sq.t0 + row / a.G, h * a.G + row % a.G, d4);
+    if (tid == 0) a.joins[wg] = rest;
 }
 
 // ------------------------------------------------------------- host -------
@@ -1102,22 +1121,24 @@ int validate(const imi_paged_attention_args* a) {
 // few-row kernel (blocks of 16 rows), the others to the tile kernel.
 struct Shape {
     int few_rows = 0;       // 0: no few-row launch
-    int few_wg = 0;
+    int w_log = 0;          // 2^w_log workgroups
     int most = 0;           // rows a few-row sequence can have
     bool direct = false;    // a workgroup per (sequence, head), no join
     bool tiles = false;
-    int tile_wg = 0;
     int slots = 0;
-    size_t few_part = 0, tile_part = 0, plan = 0;   // workspace bytes
+    size_t few_part = 0, tile_part = 0, plan = 0, joins = 0;   // workspace bytes
 };
 
-constexpr int kDirectUnits = 8;
+constexpr int kDirectUnits = 4;
 
 Shape shape_of(const imi_paged_attention_args* a) {
     Shape p;
     const imi_paged_batch& b = a->batch;
     if (b.n_seqs == 0 || b.n_tokens == 0) return p;
     const int64_t most = static_cast<int64_t>(std::min(b.max_query, b.n_tokens)) * a->groups;
+    // a workgroup of eight waves per CU: its registers and LDS fill one
+    while ((2 << p.w_log) <= device_cus()) ++p.w_log;
+    p.joins = sizeof(Join) << p.w_log;
     if (most <= 32) {
         p.few_rows = most <= 16 ? 16 : 32;
     } else {
@@ -1131,20 +1152,19 @@ Shape shape_of(const imi_paged_attention_args* a) {
         if (a->window > 0)
             longest = std::min<int64_t>(cap, static_cast<int64_t>(a->window) + a->sinks + p.few_rows / a->groups);
         p.direct = (longest + kUnit - 1) / kUnit <= kDirectUnits;
-        p.few_wg = 2 * device_cus();
-        if (!p.direct) p.few_part = size_t(2) * p.few_wg * p.few_rows * (a->dim + 2) * sizeof(float);
+        if (!p.direct) p.few_part = (size_t(2) << p.w_log) * p.most * (a->dim + 2) * sizeof(float);
     }
     if (p.tiles) {
-        p.tile_wg = device_cus();
         p.slots = static_cast<int>(static_cast<int64_t>(b.n_tokens) * a->groups / kTileRows + b.n_seqs);
-        p.tile_part = size_t(2) * p.tile_wg * kTileRows * (a->dim + 2) * sizeof(float);
+        p.tile_part = (size_t(2) << p.w_log) * kTileRows * (a->dim + 2) * sizeof(float);
         p.plan = plan_bytes(p.slots, b.n_seqs);
     }
     return p;
 }
 
-size_t carve(const Shape& p, void* base, float** few, float** tile, int32_t** plan) {
+size_t carve(const Shape& p, void* base, float** few, float** tile, int32_t** plan, Join** joins) {
     Carver c(base);
+    *joins = c.take<Join>(2 * (p.joins / sizeof(Join)));   // of the few-row launch, of the tile launch
     *few = c.take<float>(p.few_part / sizeof(float));
     *tile = c.take<float>(p.tile_part / sizeof(float));
     *plan = c.take<int32_t>(p.plan / sizeof(int32_t));
@@ -1153,39 +1173,43 @@ size_t carve(const Shape& p, void* base, float** few, float** tile, int32_t** pl
 
 template <typename T, int D>
 int launch(const imi_paged_attention_args* a, const Shape& p, PagedParams P, float* few, float* tile, int32_t* plan,
-           hipStream_t stream) {
+           Join* joins, hipStream_t stream) {
+    const int W = 1 << p.w_log;
+    P.w_log = p.w_log;
     if (p.tiles) {
         PagedParams Q = P;
         Q.min_rows = p.few_rows + 1;
         Q.max_rows = INT_MAX;
-        Q.W = p.tile_wg;
+        Q.cap = kTileRows;
+        Q.joins = joins + W;
         Q.part = tile;
-        Q.part_ml = tile + size_t(2) * p.tile_wg * kTileRows * D;
+        Q.part_ml = tile + size_t(2) * W * kTileRows * D;
         Q.plan = plan;
         Q.slots = p.slots;
         plan_kernel<<<1, 1024, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("plan_kernel");
-        tile_kernel<T, D><<<p.tile_wg, 512, 0, stream>>>(Q);
+        tile_kernel<T, D><<<W, 512, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("tile_kernel");
-        tile_merge_kernel<T, D><<<dim3(p.tile_wg - 1, kTileRows * D / 1024), 256, 0, stream>>>(Q);
-        IMI_LAUNCH_CHECK("tile_merge_kernel");
+        merge_kernel<T, D><<<dim3(W, kTileRows * D / 1024), 256, 0, stream>>>(Q, false);
+        IMI_LAUNCH_CHECK("merge_kernel");
     }
     if (p.few_rows) {
         PagedParams Q = P;
         Q.min_rows = 1;
         Q.max_rows = p.few_rows;
-        Q.W = p.few_wg;
+        Q.cap = p.most;
+        Q.joins = joins;
         Q.part = few;
-        Q.part_ml = few + size_t(2) * p.few_wg * p.few_rows * D;
-        const int grid = p.direct ? P.S * P.H : p.few_wg;
+        Q.part_ml = few + size_t(2) * W * p.most * D;
+        const int grid = p.direct ? P.S * P.H : W;
         if (p.few_rows == 16)
-            few_kernel<T, D, 1><<<grid, 256, 0, stream>>>(Q, p.direct ? 1 : 0);
+            few_kernel<T, D, 1><<<grid, 64 * kFewWaves, 0, stream>>>(Q, p.direct ? 1 : 0);
         else
-            few_kernel<T, D, 2><<<grid, 256, 0, stream>>>(Q, p.direct ? 1 : 0);
+            few_kernel<T, D, 2><<<grid, 64 * kFewWaves, 0, stream>>>(Q, p.direct ? 1 : 0);
         IMI_LAUNCH_CHECK("few_kernel");
         if (!p.direct) {
-            few_merge_kernel<T, D><<<dim3(p.few_wg - 1, p.most), 256, 0, stream>>>(Q);
-            IMI_LAUNCH_CHECK("few_merge_kernel");
+            merge_kernel<T, D><<<dim3(W, p.most), 256, 0, stream>>>(Q, true);
+            IMI_LAUNCH_CHECK("merge_kernel");
         }
     }
     return IMI_OK;
@@ -1201,7 +1225,8 @@ extern "C" int imi_paged_attention_workspace_size(const imi_paged_attention_args
     if (const int rc = validate(a)) return rc;
     float *f, *t;
     int32_t* p;
-    *bytes = carve(shape_of(a), nullptr, &f, &t, &p);
+    Join* j;
+    *bytes = carve(shape_of(a), nullptr, &f, &t, &p, &j);
     return IMI_OK;
 }
 
@@ -1215,10 +1240,11 @@ extern "C" int imi_paged_attention(const imi_paged_attention_args* a, imi_stream
     const Shape p = shape_of(a);
     float *few, *tile;
     int32_t* plan;
-    const size_t need = carve(p, nullptr, &few, &tile, &plan);
+    Join* joins;
+    const size_t need = carve(p, nullptr, &few, &tile, &plan, &joins);
     IMI_REQUIRE(need == 0 || (a->workspace && a->workspace_bytes >= need), IMI_ERR_WORKSPACE,
                 "workspace of %zu bytes, need %zu", a->workspace_bytes, need);
-    carve(p, a->workspace, &few, &tile, &plan);
+    carve(p, a->workspace, &few, &tile, &plan, &joins);
     PagedParams P{};
     P.q = a->query;
     P.k = a->keys;
@@ -1249,8 +1275,8 @@ extern "C" int imi_paged_attention(const imi_paged_attention_args* a, imi_stream
     P.c = a->scale * kLog2e;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == IMI_BF16)
-        return a->dim == 128 ? launch<BF16, 128>(a, p, P, few, tile, plan, st)
-                             : launch<BF16, 64>(a, p, P, few, tile, plan, st);
-    return a->dim == 128 ? launch<FP16, 128>(a, p, P, few, tile, plan, st)
-                         : launch<FP16, 64>(a, p, P, few, tile, plan, st);
+        return a->dim == 128 ? launch<BF16, 128>(a, p, P, few, tile, plan, joins, st)
+                             : launch<BF16, 64>(a, p, P, few, tile, plan, joins, st);
+    return a->dim == 128 ? launch<FP16, 128>(a, p, P, few, tile, plan, joins, st)
+                         : launch<FP16, 64>(a, p, P, few, tile, plan, joins, st);
 }
