@@ -955,37 +955,53 @@ class HostTierPlan:
 # ------------------------------------------------------------- paged cache --
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}   # IMI_BF16, IMI_FP16
+_raw_stream = torch._C._cuda_getCurrentRawStream   # by device index; a few hundred ns less than the Stream object
+_no_guard = contextlib.nullcontext()
 
 
 def _on(dev: torch.device):
-    """Make dev current for launches (None: it is)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    """Make dev current for launches."""
+    return _no_guard if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _same_device(dev: torch.device, **ts: Optional[torch.Tensor]) -> None:
-    for name, t in ts.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+def _device_of(name: str, t: torch.Tensor) -> torch.device:
+    dev = t.device
+    if dev.type != "cuda":
+        raise ValueError(f"{name}: adaptiveimi_amd kernels need HIP device tensors (no CPU path)")
+    return dev
 
 
-def _i32_tensor(name: str, t: torch.Tensor, dim: int) -> None:
-    if t.dtype != torch.int32:
+def _i32_tensor(name: str, t: torch.Tensor, dim: int, dev: torch.device) -> None:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.dim() != dim or (t.numel() and t.stride(-1) != 1):
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if t.dim() != dim or (t.stride(-1) != 1 and t.shape[-1] > 1):
         raise ValueError(f"{name} must have {dim} dimension(s) and unit stride on the last")
 
 
-def _stride(t: torch.Tensor, d: int) -> int:
-    """Stride of dimension d; 0 where it has one entry (torch leaves the
-    stride of such a dimension open)."""
-    return t.stride(d) if t.shape[d] > 1 else 0
+def _steps(t: torch.Tensor) -> Tuple[int, ...]:
+    """Strides, 0 where a dimension has one entry (torch leaves them open)."""
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)])
 
 
-def _write_strides(name: str, t: torch.Tensor) -> None:
-    if any(t.stride(d) == 0 and t.shape[d] > 1 for d in range(t.dim())):
+def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: torch.device, written: bool = False):
+    """(address, token stride, head stride) of a [tokens, heads, dim] tensor."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if t.shape != shape or t.stride(2) != 1:
+        raise ValueError(f"{name} must be {list(shape)} with unit stride on dim")
+    st, sh, _ = t.stride()
+    N, H, _ = shape
+    if N < 2:
+        st = 0
+    if H < 2:
+        sh = 0
+    if written and ((st == 0 and N > 1) or (sh == 0 and H > 1)):
         raise ValueError(f"{name} is written, so no two of its elements may share memory")
+    return t.data_ptr(), st, sh
 
 
 class PagedBatch:
@@ -999,32 +1015,31 @@ class PagedBatch:
     query_start: int32 [S + 1], sequence s's new tokens are the query rows
     query_start[s] .. query_start[s + 1] - 1; query rows behind the last
     sequence belong to none.  max_query: at least every sequence's new tokens
-    (sequences with more are not served).  max_len: a hint, about the longest
-    sequence (default: what the table holds); only the split of short batches
-    depends on it."""
+    (sequences with more may not be served).  max_len: a hint, about the
+    longest sequence (default: what the table holds); only the split of short
+    batches depends on it."""
 
     __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
-        dev = _require_device(lens, query_start, page_table)
-        _same_device(dev, page_table=page_table, query_start=query_start)
-        _i32_tensor("lens", lens, 1)
-        _i32_tensor("query_start", query_start, 1)
+        dev = _device_of("lens", lens)
+        _i32_tensor("lens", lens, 1, dev)
+        _i32_tensor("query_start", query_start, 1, dev)
         S = lens.shape[0]
         if query_start.shape[0] != S + 1:
             raise ValueError(f"query_start has {query_start.shape[0]} entries for {S} sequences")
+        table = stride = cols = 0
+        if page_table is not None:
+            _i32_tensor("page_table", page_table, 2, dev)
+            rows, cols = page_table.shape
+            if rows != S:
+                raise ValueError(f"page_table has {rows} rows for {S} sequences")
+            table, stride = page_table.data_ptr(), page_table.stride(0) if S > 1 else cols
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
-        self.args = PagedBatchArgs(lens=lens.data_ptr(), query_start=query_start.data_ptr(), n_seqs=S,
-                                   max_query=self.max_query, max_len=int(max_len or 0))
-        if page_table is not None:
-            _i32_tensor("page_table", page_table, 2)
-            if page_table.shape[0] != S:
-                raise ValueError(f"page_table has {page_table.shape[0]} rows for {S} sequences")
-            self.args.page_table = page_table.data_ptr()
-            self.args.max_pages = page_table.shape[1]
-            self.args.table_stride = page_table.stride(0) if S > 1 else page_table.shape[1]
+        self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
+                                   self.max_query, max_len or 0)
 
     def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
         """The C struct for pools of n_pages pages and n_tokens query rows."""
@@ -1035,19 +1050,21 @@ class PagedBatch:
 
 def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch, dim: int, dtype: torch.dtype):
     """Checks a key and a value pool [pages, kv_heads, page_size, D] of any
-    memory order with the head dim adjacent."""
-    for name, t in (("key_pages", key_pages), ("value_pages", value_pages)):
-        if t.dtype != dtype:
-            raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-        if t.dim() != 4 or t.shape[3] != dim or t.stride(3) != 1:
-            raise ValueError(f"{name} must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
+    memory order with the head dim adjacent.  Returns (pages, heads, rows,
+    page, head and row strides)."""
+    if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
+        raise TypeError(f"pages are {key_pages.dtype} and {value_pages.dtype}, expected {dtype}")
+    if key_pages.dim() != 4 or key_pages.shape[3] != dim or key_pages.stride(3) != 1:
+        raise ValueError(f"key_pages must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
     if value_pages.shape != key_pages.shape or value_pages.stride() != key_pages.stride():
         raise ValueError("key_pages and value_pages must share shape and strides")
-    _same_device(batch.device, key_pages=key_pages, value_pages=value_pages)
+    if key_pages.device != batch.device or value_pages.device != batch.device:
+        raise ValueError(f"pages are on {key_pages.device} and {value_pages.device}, expected {batch.device}")
     P, H, page, _ = key_pages.shape
-    if batch.page_table is None and P < batch.lens.shape[0]:
-        raise ValueError(f"{P} sets of contiguous rows for {batch.lens.shape[0]} sequences")
-    return P, H, page
+    if batch.page_table is None and P < batch.args.n_seqs:
+        raise ValueError(f"{P} sets of contiguous rows for {batch.args.n_seqs} sequences")
+    sp, sh, sr, _ = _steps(key_pages)
+    return P, H, page, sp, sh, sr
 
 
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch,
@@ -1068,44 +1085,42 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     last sequence are left as they are in them (unset in a tensor made here).
     Returns out, or (out, lse) with ``lse`` or ``return_lse``."""
     dev = batch.device
-    if query.dim() != 3 or query.stride(2) != 1:
-        raise ValueError("query must be [tokens, heads, dim] with unit stride on dim")
-    code = _DTYPES.get(query.dtype)
+    dtype = query.dtype
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
-    N, Hq, D = query.shape
-    P, H, page = _pools(key_pages, value_pages, batch, D, query.dtype)
+        raise TypeError(f"query must be bfloat16 or float16, got {dtype}")
+    shape = query.shape
+    if len(shape) != 3:
+        raise ValueError("query must be [tokens, heads, dim]")
+    N, Hq, D = shape
+    q, q_ts, q_hs = _rows("query", query, shape, dtype, dev)
+    P, H, page, sp, sh, sr = _pools(key_pages, value_pages, batch, D, dtype)
     if H == 0 or Hq % H:
         raise ValueError(f"{Hq} query heads are not a multiple of {H} KV heads")
-    _same_device(dev, query=query, out=out, lse=lse)
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
-    else:
-        if out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1:
-            raise ValueError(f"out must be {query.dtype} {tuple(query.shape)} with unit stride on dim")
-        _write_strides("out", out)
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    o, o_ts, o_hs = _rows("out", out, shape, dtype, dev, True)
+    l = l_ts = 0
     if lse is None and return_lse:
         lse = torch.empty((N, Hq), dtype=torch.float32, device=dev)
-    elif lse is not None:
-        if lse.shape != (N, Hq) or lse.dtype != torch.float32 or (Hq > 1 and lse.stride(1) != 1):
-            raise ValueError(f"lse must be float32 {(N, Hq)} with unit stride on heads")
-        _write_strides("lse", lse)
-    a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D,
-                           query.data_ptr(), _stride(query, 0), _stride(query, 1),
-                           key_pages.data_ptr(), value_pages.data_ptr(), _stride(key_pages, 0),
-                           _stride(key_pages, 1), _stride(key_pages, 2),
-                           1.0 / math.sqrt(D) if scale is None else scale, window, sinks,
-                           out.data_ptr(), _stride(out, 0), _stride(out, 1),
-                           _ptr(lse), 0 if lse is None else _stride(lse, 0))
+    if lse is not None:
+        l_ts, one = lse.stride() if lse.dim() == 2 else (0, 0)
+        if (lse.shape != (N, Hq) or lse.dtype is not torch.float32 or lse.device != dev or (Hq > 1 and one != 1)
+                or (N > 1 and l_ts == 0)):
+            raise ValueError(f"lse must be float32 {(N, Hq)} on {dev}, with unit stride on heads")
+        l = lse.data_ptr()
+    a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, key_pages.data_ptr(),
+                           value_pages.data_ptr(), sp, sh, sr, D ** -0.5 if scale is None else scale, window, sinks,
+                           o, o_ts, o_hs, l, l_ts)
     L = _lib.lib()
     ref = ctypes.byref(a)
+    need = ctypes.c_size_t()
     with _on(dev):
-        need = ctypes.c_size_t()
         check(L.imi_paged_attention_workspace_size(ref, ctypes.byref(need)), "imi_paged_attention")
         if need.value:   # this call's own: calls on other streams and captured graphs share nothing
             ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
             a.workspace, a.workspace_bytes = ws.data_ptr(), need.value
-        check(L.imi_paged_attention(ref, _stream(dev)), "imi_paged_attention")
+        check(L.imi_paged_attention(ref, _raw_stream(dev.index)), "imi_paged_attention")
     return out if lse is None else (out, lse)
 
 
@@ -1133,24 +1148,17 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
     lens - (its new tokens) + i, its key and value are stored in that row, and
     (query_out, None) is returned; tokens behind the last sequence, and rows
     that the table has no page for, are left as they are."""
-    dev = _require_device(query, key)
-    code = _DTYPES.get(query.dtype)
+    dev = _device_of("query", query)
+    dtype = query.dtype
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
-    if query.dim() != 3:
-        raise ValueError("query must be [tokens, heads, dim]")
-    N, Hq, D = query.shape
-
-    def rows(name, t, heads, written):
-        if t.dtype != query.dtype:
-            raise TypeError(f"{name} is {t.dtype}, expected {query.dtype}")
-        if t.dim() != 3 or t.shape != (N, heads, D) or t.stride(2) != 1:
-            raise ValueError(f"{name} must be [{N}, {heads}, {D}] with unit stride on dim")
-        if written:
-            _write_strides(name, t)
-        return t.data_ptr(), _stride(t, 0), _stride(t, 1)
-
-    Hk = key.shape[1] if key.dim() == 3 else -1
+        raise TypeError(f"query must be bfloat16 or float16, got {dtype}")
+    shape = query.shape
+    if len(shape) != 3 or key.dim() != 3:
+        raise ValueError("query and key must be [tokens, heads, dim]")
+    N, Hq, D = shape
+    Hk = key.shape[1]
+    k_shape = (N, Hk, D)
     paged = batch is not None
     if paged == (positions is not None):
         raise ValueError("give either positions or a batch with pages")
@@ -1158,49 +1166,51 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
         raise ValueError("a batch needs value, key_pages and value_pages, and no key_out")
     if not paged and (value is not None or key_pages is not None or value_pages is not None):
         raise ValueError("value and pages need a batch")
-    _same_device(dev, key=key, positions=positions, inv_freq=inv_freq, query_weight=query_weight,
-                 key_weight=key_weight, query_out=query_out, key_out=key_out, value=value)
-    a = QkNormRopeArgs(dtype=code, query_heads=Hq, kv_heads=Hk, dim=D, eps=eps, interleaved=int(interleaved))
     if query_out is None:
-        query_out = torch.empty((N, Hq, D), dtype=query.dtype, device=dev)
-    a.query, a.query_token_stride, a.query_head_stride = rows("query", query, Hq, False)
-    a.key, a.key_token_stride, a.key_head_stride = rows("key", key, Hk, False)
-    a.query_out, a.query_out_token_stride, a.query_out_head_stride = rows("query_out", query_out, Hq, True)
-    weights = [w for w in (query_weight, key_weight) if w is not None]
-    for w in weights:
-        if w.dtype not in (torch.float32, query.dtype) or w.dtype != weights[0].dtype:
-            raise TypeError(f"weights must both be float32 or both {query.dtype}")
-        if w.shape != (D,) or not w.is_contiguous():
-            raise ValueError(f"weights must be contiguous [{D}]")
-    a.query_weight, a.key_weight = _ptr(query_weight), _ptr(key_weight)
-    a.weight_fp32 = int(bool(weights) and weights[0].dtype == torch.float32)
+        query_out = torch.empty(shape, dtype=dtype, device=dev)
+    rotary = f = w32 = qw = kw = 0
     if inv_freq is not None:
-        if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
-            raise ValueError("inv_freq must be a contiguous float32 vector")
-        a.inv_freq, a.rotary = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+        if (inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or not inv_freq.is_contiguous()
+                or inv_freq.device != dev):
+            raise ValueError(f"inv_freq must be a contiguous float32 vector on {dev}")
+        f, rotary = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+    if query_weight is not None or key_weight is not None:
+        w_type = (key_weight if query_weight is None else query_weight).dtype
+        for w in (query_weight, key_weight):
+            if w is None:
+                continue
+            if w.dtype is not w_type or (w_type is not dtype and w_type is not torch.float32):
+                raise TypeError(f"weights must both be float32 or both {dtype}")
+            if w.shape != (D,) or not w.is_contiguous() or w.device != dev:
+                raise ValueError(f"weights must be contiguous [{D}] on {dev}")
+        w32, qw, kw = int(w_type is torch.float32), _ptr(query_weight), _ptr(key_weight)
     if paged:
-        _same_device(dev, lens=batch.lens)
-        P, H, page = _pools(key_pages, value_pages, batch, D, query.dtype)
+        if batch.device != dev:
+            raise ValueError(f"batch is on {batch.device}, expected {dev}")
+        P, H, page, sp, sh, sr = _pools(key_pages, value_pages, batch, D, dtype)
         if H != Hk:
             raise ValueError(f"pages hold {H} KV heads, key has {Hk}")
-        _write_strides("key_pages", key_pages)
-        a.batch = batch.bind(P, page, N)
-        a.value, a.value_token_stride, a.value_head_stride = rows("value", value, Hk, False)
-        a.key_pages, a.value_pages = key_pages.data_ptr(), value_pages.data_ptr()
-        a.page_stride, a.head_stride, a.row_stride = (_stride(key_pages, 0), _stride(key_pages, 1),
-                                                      _stride(key_pages, 2))
+        if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1):
+            raise ValueError("pages are written, so no two of their elements may share memory")
+        a = QkNormRopeArgs(batch.bind(P, page, N), code, Hq, Hk, D, *_rows("query", query, shape, dtype, dev),
+                           *_rows("key", key, k_shape, dtype, dev), *_rows("value", value, k_shape, dtype, dev), 0, 0,
+                           f, rotary, int(interleaved), qw, kw, w32, eps,
+                           *_rows("query_out", query_out, shape, dtype, dev, True), 0, 0, 0, key_pages.data_ptr(),
+                           value_pages.data_ptr(), sp, sh, sr)
     else:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-        if positions.shape != (N,) or not positions.is_contiguous():
-            raise ValueError(f"positions must be contiguous [{N}]")
-        a.batch.n_tokens = N
-        a.positions, a.positions_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
+        if positions.shape != (N,) or not positions.is_contiguous() or positions.device != dev:
+            raise ValueError(f"positions must be contiguous [{N}] on {dev}")
         if key_out is None:
-            key_out = torch.empty((N, Hk, D), dtype=key.dtype, device=dev)
-        a.key_out, a.key_out_token_stride, a.key_out_head_stride = rows("key_out", key_out, Hk, True)
+            key_out = torch.empty(k_shape, dtype=dtype, device=dev)
+        a = QkNormRopeArgs(PagedBatchArgs(n_tokens=N), code, Hq, Hk, D, *_rows("query", query, shape, dtype, dev),
+                           *_rows("key", key, k_shape, dtype, dev), 0, 0, 0, positions.data_ptr(),
+                           int(positions.dtype is torch.int64), f, rotary, int(interleaved), qw, kw, w32, eps,
+                           *_rows("query_out", query_out, shape, dtype, dev, True),
+                           *_rows("key_out", key_out, k_shape, dtype, dev, True))
     with _on(dev):
-        check(_lib.lib().imi_qk_norm_rope(ctypes.byref(a), _stream(dev)), "imi_qk_norm_rope")
+        check(_lib.lib().imi_qk_norm_rope(ctypes.byref(a), _raw_stream(dev.index)), "imi_qk_norm_rope")
     return query_out, key_out
 
 
@@ -1215,18 +1225,19 @@ class PageTable:
     __slots__ = ("pages", "lens", "refs", "page_size", "args", "device")
 
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page_size: int):
-        dev = _require_device(pages, lens, refs)
-        _same_device(dev, lens=lens, refs=refs)
-        _i32_tensor("pages", pages, 2)
-        _i32_tensor("lens", lens, 1)
-        _i32_tensor("refs", refs, 1)
-        if lens.shape[0] != pages.shape[0]:
-            raise ValueError(f"lens has {lens.shape[0]} entries for {pages.shape[0]} sequences")
-        _write_strides("pages", pages)
-        self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
+        dev = _device_of("pages", pages)
+        _i32_tensor("pages", pages, 2, dev)
+        _i32_tensor("lens", lens, 1, dev)
+        _i32_tensor("refs", refs, 1, dev)
         S, M = pages.shape
-        self.args = PageTableArgs(pages.data_ptr(), pages.stride(0) if S > 1 else M, lens.data_ptr(),
-                                  refs.data_ptr(), S, M, refs.shape[0], self.page_size)
+        if lens.shape[0] != S:
+            raise ValueError(f"lens has {lens.shape[0]} entries for {S} sequences")
+        stride = pages.stride(0) if S > 1 else M
+        if stride < M:
+            raise ValueError("pages is written, so no two of its rows may share memory")
+        self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
+        self.args = PageTableArgs(pages.data_ptr(), stride, lens.data_ptr(), refs.data_ptr(), S, M, refs.shape[0],
+                                  self.page_size)
 
     @classmethod
     def empty(cls, n_seqs: int, max_pages: int, n_pages: int, page_size: int, device) -> "PageTable":
@@ -1243,16 +1254,21 @@ class PageTable:
 
 def _pool_args(table: PageTable, pools: Sequence[torch.Tensor]):
     arr = (PagePool * max(len(pools), 1))()
+    P = table.args.n_pages
     for i, t in enumerate(pools):
-        _same_device(table.device, **{f"pool {i}": t})
-        if t.dim() < 2 or t.shape[0] != table.refs.shape[0]:
-            raise ValueError(f"pool {i} must have {table.refs.shape[0]} pages as its first dimension")
-        n = t[0].numel() if t.shape[0] else 0
-        span = 1 + sum((k - 1) * s for k, s in zip(t.shape[1:], t.stride()[1:]))
-        if n == 0 or span != n or (t.shape[0] > 1 and t.stride(0) < n):
+        shape, stride = t.shape, t.stride()
+        if t.device != table.device:
+            raise ValueError(f"pool {i} is on {t.device}, expected {table.device}")
+        if len(shape) < 2 or shape[0] != P:
+            raise ValueError(f"pool {i} must have {P} pages as its first dimension")
+        n, span = 1, 1
+        for k, s in zip(shape[1:], stride[1:]):
+            n *= k
+            span += (k - 1) * s
+        if n == 0 or span != n or (P > 1 and stride[0] < n):
             raise ValueError(f"pool {i}: each page must be one dense block of memory")
         size = t.element_size()
-        arr[i] = PagePool(t.data_ptr(), (t.stride(0) if t.shape[0] > 1 else n) * size, n * size)
+        arr[i] = (t.data_ptr(), (stride[0] if P > 1 else n) * size, n * size)
     return arr, len(pools)
 
 
@@ -1264,21 +1280,23 @@ def fork_pages(table: PageTable, parents: torch.Tensor, out: Optional[PageTable]
     loop); ``table`` itself is not changed."""
     if parents.shape != table.lens.shape:
         raise ValueError(f"parents has shape {tuple(parents.shape)} for {table.lens.shape[0]} sequences")
-    _i32_tensor("parents", parents, 1)
-    _same_device(table.device, parents=parents)
+    _i32_tensor("parents", parents, 1, table.device)
     if out is None:
         out = PageTable(torch.empty_like(table.pages, memory_format=torch.contiguous_format),
                         torch.empty_like(table.lens), torch.empty_like(table.refs), table.page_size)
     else:
-        _same_device(table.device, out=out.lens)
-        spans = [(t.data_ptr(), t.data_ptr() + 4 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
-                 for x in (table, out) for t in (x.pages, x.lens, x.refs) if t.numel()]
-        spans.sort()
-        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        if out.device != table.device:
+            raise ValueError(f"out is on {out.device}, expected {table.device}")
+        spans = []
+        for x in (table.args, out.args):   # (an array of no entries has address 0)
+            spans += [(x.pages or 0, max(x.n_seqs - 1, 0) * x.stride + x.max_pages), (x.lens or 0, x.n_seqs),
+                      (x.refs or 0, x.n_pages)]
+        spans = sorted([(p, p + 4 * n) for p, n in spans if p and n > 0])
+        if any([a[1] > b[0] for a, b in zip(spans, spans[1:])]):
             raise ValueError("out must share no memory with the table")
     with _on(table.device):
         check(_lib.lib().imi_fork_pages(ctypes.byref(table.args), parents.data_ptr(), ctypes.byref(out.args),
-                                        _stream(table.device)), "imi_fork_pages")
+                                        _raw_stream(table.device.index)), "imi_fork_pages")
     return out
 
 
@@ -1292,8 +1310,7 @@ def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.T
     call do not last for the sequences up to it."""
     if counts.shape != table.lens.shape:
         raise ValueError(f"counts has shape {tuple(counts.shape)} for {table.lens.shape[0]} sequences")
-    _i32_tensor("counts", counts, 1)
-    _same_device(table.device, counts=counts)
+    _i32_tensor("counts", counts, 1, table.device)
     arr, n = _pool_args(table, pools)
     dev = table.device
     granted = torch.empty(counts.shape, dtype=torch.bool, device=dev)
@@ -1303,7 +1320,7 @@ def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.T
         check(L.imi_extend_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_extend_pages")
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
         check(L.imi_extend_pages(ctypes.byref(table.args), counts.data_ptr(), granted.data_ptr(), arr, n,
-                                 ws.data_ptr(), need.value, _stream(dev)), "imi_extend_pages")
+                                 ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_extend_pages")
     return granted
 
 
@@ -1320,5 +1337,5 @@ def compact_pages(table: PageTable, pools: Sequence[torch.Tensor] = ()) -> torch
         check(L.imi_compact_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_compact_pages")
         ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
         check(L.imi_compact_pages(ctypes.byref(table.args), n_live.data_ptr(), arr, n, ws.data_ptr(), need.value,
-                                  _stream(dev)), "imi_compact_pages")
+                                  _raw_stream(dev.index)), "imi_compact_pages")
     return n_live
