@@ -25,7 +25,12 @@ namespace {
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
 
 constexpr int kMaxTokens = 8;   // tokens of a workgroup
-constexpr int kInFlight = 4;    // heads a lane group loads before it computes
+// Heads a lane group loads before it computes, and twice as many in a
+// workgroup's share, where there are tokens enough to fill the chip: 58 us for
+// 10529 tokens of 48 heads (4.45 TB/s, a large copy runs at 4.84).  With 4 at a
+// time 60, 6 at a time 76, one batch per workgroup 71; a batch loaded ahead of
+// its use costs the registers that six waves per SIMD need (104).
+constexpr int kInFlight = 3;
 
 struct QkParams {
     const uint16_t *q, *k, *v;
@@ -41,6 +46,7 @@ struct QkParams {
     int S, N, Hq, Hk, n_pages, page_shift, capacity;
     int half;                              // r / 2, 0: no rotation
     int tokens;                            // per workgroup
+    uint32_t div;                          // floor(2^32 / heads) + 1: x / heads = (x div) >> 32
     float eps;
     bool w32, pos64, interleaved, paged;
 };
@@ -74,20 +80,10 @@ __device__ __forceinline__ void unpack8(u32x4_t x, float (&y)[8]) {
     }
 }
 
-// Eight weights of a head from dim d on.
 template <typename T>
-__device__ __forceinline__ void load_weight(const void* w, bool w32, int d, float (&y)[8]) {
-    if (!w) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = 1.0f;
-    } else if (w32) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = static_cast<const float*>(w)[d + i];
-    } else {
-        const uint16_t* p = static_cast<const uint16_t*>(w) + d;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = T::lo(p[i]);
-    }
+__device__ __forceinline__ float weight_at(const void* w, bool w32, int d) {
+    if (!w) return 1.0f;
+    return w32 ? static_cast<const float*>(w)[d] : T::lo(static_cast<const uint16_t*>(w)[d]);
 }
 
 // Sequence that owns token t (the last one that starts at or before it), or -1.
@@ -106,11 +102,12 @@ __device__ __forceinline__ int owner_of(const QkParams& a, int t) {
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams a) {
+__global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
     constexpr int L = D / 8;        // lanes of a head
     constexpr int NG = 256 / L;     // heads at a time
     __shared__ float2 s_cs[kMaxTokens][D / 2];
     __shared__ int64_t s_slot[kMaxTokens];   // element offset of the token's row in the pages, -1: not stored
+    __shared__ __align__(16) float s_w[2][D];
     __shared__ int s_pos[kMaxTokens];
     __shared__ int s_own[kMaxTokens];
     const int tid = threadIdx.x, c = tid % L, g = tid / L;
@@ -121,9 +118,11 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams a) {
 
     // heads of this lane group: loads first
     u32x4_t x[kInFlight];
+    auto token_of = [&](int p) { return HT > 1 ? static_cast<int>(__umulhi(static_cast<uint32_t>(p), a.div)) : p; };
     auto source = [&](int p) -> const uint16_t* {
-        const int64_t t = t0 + p / HT;
-        const int h = p % HT;
+        const int ti = token_of(p);
+        const int64_t t = t0 + ti;
+        const int h = p - ti * HT;
         if (h < a.Hq) return a.q + t * a.q_ts + h * a.q_hs + 8 * c;
         if (h < a.Hq + a.Hk) return a.k + t * a.k_ts + (h - a.Hq) * a.k_hs + 8 * c;
         return a.v + t * a.v_ts + (h - a.Hq - a.Hk) * a.v_hs + 8 * c;
@@ -136,9 +135,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams a) {
         }
     };
     fetch(g);
-    float wq[8], wk[8];
-    load_weight<T>(a.qw, a.w32, 8 * c, wq);
-    load_weight<T>(a.kw, a.w32, 8 * c, wk);
+    if (tid < 2 * D) s_w[tid / D][tid % D] = weight_at<T>(tid < D ? a.qw : a.kw, a.w32, tid % D);
 
     // positions and slots: a wave per token
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -189,7 +186,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams a) {
         for (int i = 0; i < kInFlight; ++i) {
             const int p = p0 + i * NG;
             if (p >= pairs) break;
-            const int ti = p / HT, h = p % HT;
+            const int ti = token_of(p), h = p - ti * HT;
             const int64_t t = t0 + ti;
             if (!s_own[ti]) continue;
             if (h >= a.Hq + a.Hk) {   // a value head: copied
@@ -210,7 +207,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkParams a) {
                 if (L == 16) ss += dpp_f32<0x140>(ss);
                 const float inv = 1.0f / sqrtf(ss * (1.0f / D) + a.eps);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * (is_q ? wq[j] : wk[j]);
+                for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * s_w[is_q ? 0 : 1][8 * c + j];
             }
             if (a.half) {
                 if (a.interleaved) {
@@ -333,8 +330,9 @@ extern "C" int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t str
     P.eps = a->eps;
     const int heads = P.Hq + P.Hk * (paged ? 2 : 1);
     const int at_once = 256 / (a->dim / 8);
-    P.tokens = std::min(kMaxTokens, std::max(1, 2 * at_once / heads));
+    P.tokens = std::min(kMaxTokens, std::max(1, 2 * kInFlight * at_once / heads));
     P.tokens = std::max(1, std::min(P.tokens, P.N / (2 * device_cus())));
+    P.div = static_cast<uint32_t>((uint64_t(1) << 32) / heads + 1);
     const int grid = (P.N + P.tokens - 1) / P.tokens;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == IMI_BF16) {
