@@ -74,6 +74,8 @@ constexpr float kSlack = 8.0f;   // growth of a running maximum (base 2) that is
 // The two element types: pairs rounded to nearest even, matrix instructions.
 struct BF16 {
     typedef bf16x8_t v8;
+    static constexpr uint32_t kExp = 0x7F80;
+    static __device__ __forceinline__ float wide(uint32_t h) { return __uint_as_float(h << 16); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         typedef __attribute__((ext_vector_type(2))) float f2;
         typedef __attribute__((ext_vector_type(2))) __bf16 b2;
@@ -88,6 +90,10 @@ struct BF16 {
 };
 struct FP16 {
     typedef f16x8_t v8;
+    static constexpr uint32_t kExp = 0x7C00;
+    static __device__ __forceinline__ float wide(uint32_t h) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
+    }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         typedef __attribute__((ext_vector_type(2))) _Float16 h2;
         return __builtin_bit_cast(uint32_t, (h2{static_cast<_Float16>(a), static_cast<_Float16>(b)}));
@@ -192,6 +198,66 @@ __device__ __forceinline__ u32x4_t join(s16x4_t a, s16x4_t b) {
     return __builtin_bit_cast(u32x4_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// A row of V that only some of a workgroup's tokens see meets the others with
+// weight 0 in the matrix instruction, and 0 times an infinity or a NaN would
+// reach them.  Where rows are masked in part such values are looked for and
+// replaced by 0; a workgroup that found one adds it, after its rows are
+// written, to those that see it (patch_rows: slow, for data that is broken).
+template <typename T>
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {   // 0xFFFF per finite half
+    return ((x & T::kExp) == T::kExp ? 0u : 0xFFFFu) | (((x >> 16) & T::kExp) == T::kExp ? 0u : 0xFFFF0000u);
+}
+template <typename T, int N>
+__device__ __forceinline__ bool all_finite(const u32x4_t (&x)[N]) {
+    uint32_t m = ~0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m &= finite_halves<T>(x[i][k]);
+    return m == ~0u;
+}
+template <typename T, int N>
+__device__ __forceinline__ void keep_finite(u32x4_t (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[i][k] &= finite_halves<T>(x[i][k]);
+}
+
+// Rows [first, end) of one (sequence s, KV head h): adds the infinities and NaN
+// of the span's rows [v0, v1) that each sees, to the output (slot < 0) or to
+// the partial.  The workgroup's own writes of these rows are done.
+template <typename T, int D, typename SpanT>
+__device__ __forceinline__ void patch_rows(const PagedParams& a, const Seq& sq, int s, int h, const SpanT& sp, int first,
+                                           int end, int v0, int v1, int64_t slot) {
+    for (int x = threadIdx.x; x < (end - first) * (D / 2); x += blockDim.x) {
+        const int r = first + x / (D / 2), d = 2 * (x % (D / 2));
+        const int p = sq.len - sq.n + r / a.G;
+        float add[2] = {0.0f, 0.0f};
+        for (int v = v0; v < v1; ++v) {
+            const int j = sp.row(v);
+            if (j > p || (a.window > 0 && j <= p - a.window && j >= a.sinks)) continue;
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(
+                a.v + row_offset(a, page_of(a, s, j), j) + static_cast<int64_t>(h) * a.head_s + d);
+            const uint32_t m = finite_halves<T>(w);
+            if (!(m & 0xFFFFu)) add[0] += T::wide(w & 0xFFFFu);
+            if (!(m >> 16)) add[1] += T::wide(w >> 16);
+        }
+        if (add[0] == 0.0f && add[1] == 0.0f) continue;
+        if (slot >= 0) {
+            float* const o = a.part + (slot * a.cap + r - first) * D + d;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                o[i] = __hip_atomic_load(o + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + add[i];
+        } else {
+            uint32_t* const o = reinterpret_cast<uint32_t*>(a.out + static_cast<int64_t>(sq.t0 + r / a.G) * a.o_ts +
+                                                            static_cast<int64_t>(h * a.G + r % a.G) * a.o_hs + d);
+            const uint32_t w = __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *o = T::pack(T::wide(w & 0xFFFFu) + add[0], T::wide(w >> 16) + add[1]);
+        }
+    }
+}
+
 __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
 }
@@ -282,10 +348,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     constexpr int kWaveLds = kFewTile * LR > 16 * D * 2 ? kFewTile * LR : 16 * D * 2;   // u16
     __shared__ uint16_t s_buf[kFewWaves * kWaveLds];
     __shared__ float s_ml[kFewWaves][16 * NB][2];
+    __shared__ int s_odd;   // a masked tile held infinities or NaN
     const int tid = threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 15, lg = lane >> 4;
     uint16_t* const sv = s_buf + wave * kWaveLds;
+    if (tid == 0) s_odd = 0;
+    __syncthreads();
 
     FewRange range;
     if (direct) {     // a workgroup per (sequence, head): nothing to join
@@ -381,6 +450,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
                         for (int c = 0; c < KK; ++c) vb[e][c] = u32x4_t{0, 0, 0, 0};
             }
+            const int j_lo = sp.row(v0), j_hi = sp.row(v0 + kFewTile - 1);
+            const bool full = v0 + kFewTile <= vis && j_hi <= p0 &&
+                              (a.window == 0 || j_lo >= sq.len - a.window || j_hi < a.sinks);
+            if (!full && sq.n > 1) {   // (one token sees every row of its span)
+                const bool odd = !all_finite<T>(vb[0]) || !all_finite<T>(vb[1]);
+                if (__builtin_amdgcn_ballot_w64(odd)) {
+                    keep_finite<T>(vb[0]);
+                    keep_finite<T>(vb[1]);
+                    s_odd = 1;
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -401,9 +481,6 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             }
             wave_lds_sync();
             // lane: keys v0 + 16 e + 4 lg + i of row ln
-            const int j_lo = sp.row(v0), j_hi = sp.row(v0 + kFewTile - 1);
-            const bool full = v0 + kFewTile <= vis && j_hi <= p0 &&
-                              (a.window == 0 || j_lo >= sq.len - a.window || j_hi < a.sinks);
             u32x4_t pf[NB];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
@@ -462,6 +539,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             }
         }
         const bool whole = u0 == 0 && u1 == units;
+        bool odd = false;
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
         float* const so = reinterpret_cast<float*>(sv);   // [16 rows][D]
 #pragma unroll
@@ -473,6 +551,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             for (int d = 0; d < DB; ++d)
                 *reinterpret_cast<f32x4_t*>(so + ln * D + 16 * d + 4 * lg) = acc[b][d];
             __syncthreads();
+            odd = s_odd != 0;   // set before, and not again until all are past the loop
             for (int x = tid; x < 16 * D / 4; x += 64 * kFewWaves) {
                 const int rr = x / (D / 4), d4 = x % (D / 4), r = 16 * b + rr;
                 if (r >= rows) break;
@@ -509,6 +588,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             }
         }
         __syncthreads();
+        if (odd) {
+            __threadfence();
+            __syncthreads();
+            patch_rows<T, D>(a, sq, s, h, sp, 0, rows, u0 * kUnit, min(u1 * kUnit, vis), whole ? -1 : slot);
+            __syncthreads();
+            if (tid == 0) s_odd = 0;
+            __syncthreads();
+        }
         if (u0 == 0 && u1 < units)
             rest = Join{range.total, g0, g0 + units, sq.t0, 0, rows, h};
         g0 += u1 - u0;
@@ -837,9 +924,13 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     constexpr int SB = Stage<D>::kBytes;
     // one array: with two, the compiler makes every read of K wait for the
     // loads into LDS that are under way for the next step
-    __shared__ __align__(1024) char s_stage[8 * SB];
+    __shared__ __align__(1024) char s_stage[8 * SB + 16];
     char* const s_k = s_stage;
     char* const s_v = s_stage + 4 * SB;
+    // a masked step held infinities or NaN: this tile's word and the next one's
+    int* const s_odd = reinterpret_cast<int*>(s_stage + 8 * SB);
+    int turn = 0;
+    if (threadIdx.x == 0) s_odd[0] = 0;
     Stage<D> st;
     st.init();
     const int tid = threadIdx.x, lane = lane_id();
@@ -891,6 +982,14 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         const bool idle = w_first >= rows;
         const int p_min = p0 + min(w_first, static_cast<int>(rows) - 1) / a.G;
         const int p_max = p0 + static_cast<int>(min(static_cast<int64_t>(w_first) + 31, rows - 1)) / a.G;
+        // steps with rows that some of the tile's tokens do not see
+        const int t_end = static_cast<int>(min(static_cast<int64_t>(tile.y) + kTileRows, rows));
+        const int t_min = p0 + tile.y / a.G, t_max = p0 + (t_end - 1) / a.G;
+        auto masked = [&](int u) {
+            return sp.row(min((u + 1) * kStep, vis) - 1) > t_min || (a.window > 0 && sp.row(u * kStep) <= t_max - a.window);
+        };
+        __syncthreads();   // all have read the last tile's word: it is the next one's
+        if (tid == 0) s_odd[turn ^ 1] = 0;
 
         f32x16_t acc[DB];
 #pragma unroll
@@ -935,6 +1034,10 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
                     if (sp.dead(u * kStep + st.l_row + i)) vb[i] = u32x4_t{0, 0, 0, 0};
+            }
+            if (masked(u) && __builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
+                keep_finite<T>(vb);
+                s_odd[turn] = 1;
             }
             st.store_v(vb, s_v + (u & 1) * 2 * SB);
             wait_loads();   // K is in LDS
@@ -1075,9 +1178,18 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                 }
             }
         }
-        __syncthreads();   // the next range's first store reuses the tiles
+        __syncthreads();   // the next tile's first store reuses the stages
+        if (s_odd[turn]) {
+            __threadfence();
+            __syncthreads();
+            for (int u = u0; u < u1; ++u)
+                if (masked(u))
+                    patch_rows<T, D>(a, sq, s, h, sp, tile.y, t_end, u * kStep, min((u + 1) * kStep, vis),
+                                     u0 == 0 && u1 == units ? -1 : 2 * static_cast<int64_t>(wg) + (first ? 0 : 1));
+        }
+        turn ^= 1;
         if (u0 == 0 && u1 < units)
-            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, static_cast<int>(min(rows, static_cast<int64_t>(tile.y) + kTileRows)), h};
+            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, t_end, h};
         g0 += u1 - u0;
         first = false;
         if (++t == n_tiles) {

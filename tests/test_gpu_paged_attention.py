@@ -164,3 +164,60 @@ def test_matches_definition(ops, lens, news, H, G, D, page, dtype, window, sinks
     out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window, sinks=sinks,
                                    return_lse=True)
     check(x, out, lse, window, sinks)
+
+
+def same_class(got, want, tol):
+    """Equal infinities and NaN, and within tol elsewhere."""
+    nan, inf = torch.isnan(want), torch.isinf(want)
+    assert torch.equal(torch.isnan(got), nan)
+    assert torch.equal(got[inf], want[inf])
+    fin = ~nan & ~inf
+    assert torch.all((got - want).abs()[fin] <= tol[fin])
+
+
+@pytest.mark.parametrize("lens,news,H,G,D,page,dtype,window,sinks", [
+    ([120], [120], 1, 4, 128, 16, BF, 0, 0),
+    ([300], [300], 2, 2, 64, 16, HF, 0, 0),
+    ([500], [300], 1, 5, 128, 8, BF, 70, 9),       # rows that leave a tile's window
+    ([400, 90], [6, 5], 2, 4, 128, 16, HF, 0, 0),  # few rows
+    ([400, 90], [3, 5], 1, 4, 64, 16, BF, 30, 2),
+])
+def test_infinities_and_nan_reach_only_what_sees_them(ops, lens, news, H, G, D, page, dtype, window, sinks):
+    """Rows of V that hold infinities or NaN, the last rows among them, change
+    the outputs of the tokens that see them and no other's."""
+    x = make(lens, news, H, G, D, page, dtype)
+    g = torch.Generator().manual_seed(7)
+    for s, n in enumerate(lens):
+        first = max(n - news[s], 0)
+        for j in [n - 1, n - 2] + torch.randint(max(first - 3, 0), n, (6,), generator=g).tolist() + [0]:
+            d = int(torch.randint(0, D, (1,), generator=g))
+            h = int(torch.randint(0, H, (1,), generator=g))
+            val = [math.inf, -math.inf, math.nan][int(torch.randint(0, 3, (1,), generator=g))]
+            x["rows"][s][1][h, j, d] = val
+            if j != 0 or window:   # a first row that every token sees makes for few finite outputs
+                x["v"][int(x["table"][s, j // page]), h, j % page, d] = val
+            else:
+                x["rows"][s][1][h, j, d] = x["v"][int(x["table"][s, 0]), h, 0, d].cpu()
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window, sinks=sinks,
+                                   return_lse=True)
+    want, want_lse, tol, ltol, mine = expected(x, window, sinks)
+    assert torch.isfinite(want).any() and not torch.isfinite(want).all()
+    same_class(out.double().cpu(), want, torch.nan_to_num(tol, nan=0.0, posinf=0.0))
+    assert torch.all((lse.double().cpu() - want_lse).abs() <= ltol)
+
+
+def test_nan_keys_reach_only_what_sees_them(ops):
+    """A NaN key makes NaN of the tokens that see it; earlier ones, and those
+    whose window has left it, stay as they are."""
+    for news, window in ((150, 0), (150, 40), (5, 0), (5, 3)):
+        x = make([200], [news], 2, 3, 128, 16, BF)
+        clean = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window)
+        j = 200 - news + news // 2
+        x["k"][int(x["table"][0, j // 16]), 1, j % 16, 5] = math.nan
+        out = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window)
+        p = torch.arange(200 - news, 200)
+        hit = (p >= j) & ((p < j + window) if window else True)
+        assert torch.isnan(out[hit.to(DEV)][:, 3:]).all()
+        keep = torch.ones((news, 6), dtype=torch.bool)
+        keep[hit, 3:] = False
+        assert torch.equal(out[keep.to(DEV)], clean[keep.to(DEV)])
