@@ -126,7 +126,8 @@ struct PagedParams {
     int64_t q_ts, q_hs;        // strides in elements: token, head
     int64_t o_ts, o_hs;
     int64_t l_ts;              // lse token stride (heads are adjacent)
-    int64_t page_s, head_s, tok_s;
+    int64_t head_s;
+    uint32_t page_s, tok_s;    // from page to page, from row to row
     int64_t table_s;
     int S, N, H, G;
     int n_pages;               // pages in the pool
@@ -169,14 +170,29 @@ __device__ __forceinline__ Span span_of(const PagedParams& a, int len, int p0, i
     return r;
 }
 
+// The rows of a span (row v is cached row v up to the sinks, v + shift from
+// there on) that a token at position pos (-1: none) sees: v <= last, and from
+// `from` on or under `sinks`.
+struct Sees {
+    int last, from, sinks;
+    __device__ __forceinline__ Sees(const PagedParams& a, int pos, int shift, int sink, int vis)
+        : last(min(pos - shift, vis - 1)),
+          from(a.window > 0 ? pos - a.window + 1 - shift : 0),
+          sinks(shift ? sink : a.sinks) {}
+    __device__ __forceinline__ bool row(int k, int base) const {   // v = base + k
+        return (k <= last - base) & ((k >= from - base) | (k < sinks - base));
+    }
+};
+
 // Element offset of cached row j of sequence s (head offset not included).
 // A page id outside the pool is forced into it.
 __device__ __forceinline__ int page_of(const PagedParams& a, int s, int j) {
     return a.table ? a.table[static_cast<int64_t>(s) * a.table_s + (j >> a.page_shift)] : s;
 }
 __device__ __forceinline__ int64_t row_offset(const PagedParams& a, int page, int j) {
-    const int slot = j & ((1u << a.page_shift) - 1u);
-    return static_cast<int64_t>(clampi(page, 0, a.n_pages - 1)) * a.page_s + static_cast<int64_t>(slot) * a.tok_s;
+    const uint32_t slot = static_cast<uint32_t>(j) & ((1u << a.page_shift) - 1u);
+    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(clampi(page, 0, a.n_pages - 1))) * a.page_s +
+                                slot * a.tok_s);
 }
 
 __device__ __forceinline__ void wave_lds_sync() {
@@ -485,16 +501,12 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (!full) {
+                    const Sees sees(a, pos[b], sp.lo - sp.sink, sp.sink, vis);
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int v = v0 + 16 * e + 4 * lg + i;
-                            const int j = sp.row(v);
-                            const bool seen = v < vis && j <= pos[b] &&
-                                              (a.window == 0 || j > pos[b] - a.window || j < a.sinks);
-                            sc[b][e][i] = seen ? sc[b][e][i] : -INFINITY;
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            sc[b][e][i] = sees.row(16 * e + i, v0 + 4 * lg) ? sc[b][e][i] : -INFINITY;
                 }
                 float mx = -INFINITY;
 #pragma unroll
@@ -919,7 +931,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     constexpr int KK = D / 16;
     constexpr int DB = D / 32;
-    constexpr int NF = 6;                   // operand blocks read ahead of their use (2, 4, 8: 940, 959, 918 TFLOP/s; 6: 962)
+    constexpr int NF = 4;                   // operand blocks read ahead of their use (2, 6, 8 cost 2, 0, 4 percent)
     constexpr int NR = Stage<D>::NR;
     constexpr int SB = Stage<D>::kBytes;
     // one array: with two, the compiler makes every read of K wait for the
@@ -977,17 +989,27 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         u32x4_t qf[KK];
 #pragma unroll
         for (int c = 0; c < KK; ++c) qf[c] = load16(qp + 16 * c);
-        // the wave's positions, for steps that need no mask
         const int w_first = tile.y + wave * 32;
         const bool idle = w_first >= rows;
+        const int t_end = static_cast<int>(min(static_cast<int64_t>(tile.y) + kTileRows, rows));
+        // Which steps need what, once per tile.  Row v of the span is cached row
+        // v + shift (from pad on), so a bound on rows is one on steps.
+        // A step whose rows are all there, and neighbours four by four:
+        const int easy_lo = (sp.pad + kStep - 1) / kStep, easy_hi = a.page_shift >= 2 ? vis / kStep : 0;
+        // a step with nothing to look for in V: no dead row, no row that only
+        // some of the tile's tokens see
+        const int t_min = p0 + tile.y / a.G, t_max = p0 + (t_end - 1) / a.G;
+        const int gone = a.window > 0 ? max(t_max - a.window - sp.shift + 1, sp.pad) : 0;
+        const int plain_lo = (max(gone, sp.edge) + kStep - 1) / kStep;
+        const int plain_hi = min(vis, max(t_min + 1 - sp.shift, 0)) / kStep;
+        // stages (64 rows) that all of the wave's tokens see, and that some do
         const int p_min = p0 + min(w_first, static_cast<int>(rows) - 1) / a.G;
         const int p_max = p0 + static_cast<int>(min(static_cast<int64_t>(w_first) + 31, rows - 1)) / a.G;
-        // steps with rows that some of the tile's tokens do not see
-        const int t_end = static_cast<int>(min(static_cast<int64_t>(tile.y) + kTileRows, rows));
-        const int t_min = p0 + tile.y / a.G, t_max = p0 + (t_end - 1) / a.G;
-        auto masked = [&](int u) {
-            return sp.row(min((u + 1) * kStep, vis) - 1) > t_min || (a.window > 0 && sp.row(u * kStep) <= t_max - a.window);
-        };
+        const int full_lo = a.window > 0 ? (max(p_max - a.window + 1 - sp.shift, sp.pad) + kStage - 1) / kStage : 0;
+        const int full_hi = w_first + 32 <= rows ? min(vis, max(p_min + 1 - sp.shift, 0)) / kStage : 0;
+        const int seen_hi = idle ? 0 : (p_max - sp.shift) / kStage + 1;
+        // of the rows before, first tokens that stay visible: full up to here
+        const int sink_hi = w_first + 32 <= rows ? min(a.sinks, sp.shift ? sp.sink : p_min + 1) / kStage : 0;
         __syncthreads();   // all have read the last tile's word: it is the next one's
         if (tid == 0) s_odd[turn ^ 1] = 0;
 
@@ -1000,11 +1022,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 
         const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s;
         const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * st.l_ch;
-        // a whole step's rows are neighbours, four by four: one page lookup, one
-        // step ahead of its use, and one address per thread
-        auto neighbours = [&](int u) {
-            return a.page_shift >= 2 && (u + 1) * kStep <= vis && (u * kStep >= sp.pad || (u + 1) * kStep <= sp.pad);
-        };
+        // an easy step: one page lookup, one step ahead of its use, and one
+        // address per thread
         int id = s;
         auto fetch_id = [&](int u) {
             if (a.table) id = page_of(a, s, sp.row(min(u * kStep + st.l_row, vis - 1)));
@@ -1012,8 +1031,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         u32x4_t vb[NR];
         auto fetch = [&](int u) {
             char* const sk = s_k + (u & 1) * 2 * SB;
-            if (neighbours(u)) {
-                const int64_t o = row_offset(a, id, sp.row(u * kStep + st.l_row));
+            if (u >= easy_lo && u < easy_hi) {
+                const int64_t o = row_offset(a, id, u * kStep + st.l_row + sp.shift);
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     st.load_k(kh + o + i * a.tok_s, i, sk);
@@ -1030,14 +1049,14 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
             }
         };
         auto store = [&](int u) {
-            if ((u + 1) * kStep > vis || u * kStep < sp.edge) {   // no NaN may enter through a dead row's V
+            if (u < plain_lo || u >= plain_hi) {   // no NaN may enter through a row that is not seen
 #pragma unroll
                 for (int i = 0; i < NR; ++i)
                     if (sp.dead(u * kStep + st.l_row + i)) vb[i] = u32x4_t{0, 0, 0, 0};
-            }
-            if (masked(u) && __builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
-                keep_finite<T>(vb);
-                s_odd[turn] = 1;
+                if (__builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
+                    keep_finite<T>(vb);
+                    s_odd[turn] = 1;
+                }
             }
             st.store_v(vb, s_v + (u & 1) * 2 * SB);
             wait_loads();   // K is in LDS
@@ -1067,10 +1086,9 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                 const int v0 = u * kStep + sub * kStage;
                 if (sub > 0 && more) store(u + 1);   // between two stages, not where the waves meet
                 if (v0 >= vis) break;
-                const int j_lo = sp.row(v0), j_hi = sp.row(min(v0 + kStage, vis) - 1);
-                // a step whose rows none of the wave's tokens sees is skipped
-                const bool skip = idle || j_lo > p_max ||
-                                  (a.window > 0 && j_lo >= a.sinks && j_hi <= p_min - a.window);
+                const int stage = 2 * u + sub;
+                // rows that none of the wave's tokens sees are skipped
+                const bool skip = stage >= seen_hi;
                 if (!skip) {
                     f32x16_t sc[2];
                     // K's blocks (32 rows, 16 dims), then V's, NF reads ahead
@@ -1092,21 +1110,17 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         order();
                     }
                     // lane: keys v0 + 32 e + 8 (i / 4) + 4 hi + i % 4 of row q32
-                    const bool full = v0 + kStage <= vis && j_hi <= p_min &&
-                                      (a.window == 0 || j_lo > p_max - a.window || j_hi < a.sinks) &&
-                                      w_first + 32 <= rows;
+                    const bool full = (stage >= full_lo && stage < full_hi) || stage < sink_hi;
                     u32x4_t pf[4];   // weights of 16 rows each
                     {
                         if (!full) {
+                            const Sees sees(a, pos, sp.shift, sp.sink, vis);
 #pragma unroll
                             for (int e = 0; e < 2; ++e)
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) {
-                                    const int v = v0 + 32 * e + 8 * (i >> 2) + 4 * hi + (i & 3);
-                                    const int j = sp.row(v);
-                                    const bool seen = v < vis && j <= pos &&
-                                                      (a.window == 0 || j > pos - a.window || j < a.sinks);
-                                    sc[e][i] = seen ? sc[e][i] : -INFINITY;
+                                    const int k = 32 * e + 8 * (i >> 2) + (i & 3);
+                                    sc[e][i] = sees.row(k, v0 + 4 * hi) ? sc[e][i] : -INFINITY;
                                 }
                         }
                         float mx = sc[0][0];
@@ -1183,7 +1197,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
             __threadfence();
             __syncthreads();
             for (int u = u0; u < u1; ++u)
-                if (masked(u))
+                if (u < plain_lo || u >= plain_hi)
                     patch_rows<T, D>(a, sq, s, h, sp, tile.y, t_end, u * kStep, min((u + 1) * kStep, vis),
                                      u0 == 0 && u1 == units ? -1 : 2 * static_cast<int64_t>(wg) + (first ? 0 : 1));
         }
@@ -1224,6 +1238,8 @@ int validate(const imi_paged_attention_args* a) {
     for (const void* p : ptrs)
         IMI_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, IMI_ERR_INVALID,
                     "query, keys, values and out must be 16-byte aligned");
+    IMI_REQUIRE(a->page_stride <= UINT_MAX && (a->batch.page_size - 1) * a->row_stride <= UINT_MAX, IMI_ERR_UNSUPPORTED,
+                "a page spans more than 2^32 elements");
     IMI_REQUIRE(batch_capacity(&a->batch) <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
                 "more than 2^30 rows in a sequence");
     IMI_REQUIRE(static_cast<int64_t>(a->batch.n_tokens) * a->groups <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
@@ -1375,9 +1391,9 @@ extern "C" int imi_paged_attention(const imi_paged_attention_args* a, imi_stream
     P.o_ts = a->out_token_stride;
     P.o_hs = a->out_head_stride;
     P.l_ts = a->lse_token_stride;
-    P.page_s = a->page_stride;
+    P.page_s = static_cast<uint32_t>(a->page_stride);
     P.head_s = a->head_stride;
-    P.tok_s = a->row_stride;
+    P.tok_s = static_cast<uint32_t>(a->row_stride);
     P.table_s = b.table_stride;
     P.S = b.n_seqs;
     P.N = b.n_tokens;
