@@ -221,3 +221,176 @@ def test_nan_keys_reach_only_what_sees_them(ops):
         keep = torch.ones((news, 6), dtype=torch.bool)
         keep[hit, 3:] = False
         assert torch.equal(out[keep.to(DEV)], clean[keep.to(DEV)])
+
+
+def test_empty_sequences_and_rows(ops):
+    """Sequences of no rows, of no new tokens, more new tokens than rows; rows
+    of no sequence keep what the given outputs hold."""
+    lens, news = [0, 7, 50, 3, 0, 200], [0, 0, 2, 5, 3, 150]
+    for G in (1, 4):
+        x = make(lens, news, 2, G, 128, 8, BF, pad=11)
+        out = torch.full((sum(news) + 11, 2 * G, 128), 5.0, dtype=BF, device=DEV)
+        lse = torch.full((sum(news) + 11, 2 * G), 6.0, device=DEV)
+        a, b = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), out=out, lse=lse)
+        assert a is out and b is lse
+        check(x, out, lse)
+        assert torch.all(out[sum(news):] == 5.0) and torch.all(lse[sum(news):] == 6.0)
+    # nothing to do at all
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    out = ops.paged_attention(x["q"][:0], x["k"], x["v"], batch_of(ops, x))
+    assert out.shape == (0, 8, 128)
+    none = ops.PagedBatch(None, i32([]), i32([0]), max_query=1)
+    assert ops.paged_attention(x["q"], x["k"], x["v"], none).shape == x["q"].shape
+
+
+@pytest.mark.parametrize("news", [[1, 1, 1], [40, 3, 130]])
+def test_strides(ops, news):
+    """Queries inside a projection's rows, outputs inside a wider tensor, heads
+    and tokens in either order."""
+    lens = [300, 64, 500]
+    x = make(lens, news, 2, 4, 64, 16, HF, layout="tokens", packed=True)
+    assert not x["q"].is_contiguous()
+    N = x["q"].shape[0]
+    wide = torch.full((N, 3, 8, 64), 2.0, dtype=HF, device=DEV)
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), out=wide[:, 1], return_lse=True)
+    check(x, out, lse)
+    assert torch.all(wide[:, 0] == 2.0) and torch.all(wide[:, 2] == 2.0)
+    by_head = torch.empty((8, N, 64), dtype=HF, device=DEV).transpose(0, 1)
+    q2 = x["q"].transpose(0, 1).contiguous().transpose(0, 1)
+    again = ops.paged_attention(q2, x["k"], x["v"], batch_of(ops, x), out=by_head)
+    assert torch.equal(again, out)
+
+
+def test_lies_about_lengths_stay_in_bounds(ops):
+    """Lengths past the table, starts past the tensor and pages outside the
+    pool are forced into range: the call returns, and what is well described
+    is right."""
+    x = make([100, 90], [1, 1], 1, 4, 128, 16, BF, junk=0.0)
+    good = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x))
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    table = x["table"].clone()
+    table[1] = -7
+    b = ops.PagedBatch(table, i32([100, 10 ** 9]), i32([0, 1, 2 ** 30]), max_query=1)
+    out = ops.paged_attention(x["q"], x["k"], x["v"], b)
+    assert torch.equal(out[0], good[0])
+    b = ops.PagedBatch(table, i32([100, -5]), i32([0, 1, -3]), max_query=1)
+    out = ops.paged_attention(x["q"], x["k"], x["v"], b)
+    assert torch.equal(out[0], good[0])
+
+
+@pytest.mark.parametrize("S,n,news", [(1, 30000, 1), (1, 30000, 6), (70, 900, 1), (3, 9000, 33), (200, 40, 1)])
+def test_splits_agree_with_one_call_per_sequence(ops, S, n, news):
+    """Many sequences in one call, cut into ranges and joined, against each
+    sequence alone with a hint that keeps it whole where that path exists."""
+    g = torch.Generator().manual_seed(3)
+    lens = [max(news, int(n * (0.3 + 0.7 * float(torch.rand((), generator=g))))) for _ in range(S)]
+    x = make(lens, [news] * S, 1, 4, 64, 32, HF, seed=4)
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), return_lse=True)
+    for s in range(0, S, max(1, S // 5)):
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+        b = ops.PagedBatch(x["table"][s:s + 1], i32([lens[s]]), i32([0, news]), max_query=news, max_len=1)
+        one, one_lse = ops.paged_attention(x["q"][s * news:(s + 1) * news], x["k"], x["v"], b, return_lse=True)
+        got, got_lse = out[s * news:(s + 1) * news], lse[s * news:(s + 1) * news]
+        # each within eps of the same value (weights and output rounded), so within two of each other
+        scale = one.double().abs().amax()
+        assert (got.double() - one.double()).abs().max() <= 2 * 2.0 ** -10 * (scale + 1)
+        assert (got_lse - one_lse).abs().max() <= 1e-4
+    again = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x))
+    assert torch.equal(again, out)   # the same call gives the same bits
+
+
+def test_large_pages_offsets_past_32_bits(ops):
+    """A pool of more than 2^32 bytes: pages far apart."""
+    page, H, D = 128, 8, 128
+    P = (5 << 30) // (page * H * D * 2)
+    k = torch.zeros((P, H, page, D), dtype=BF, device=DEV)
+    v = torch.zeros_like(k)
+    x = make([500], [1], H, 4, D, page, BF, seed=8)
+    far = [P - 1, 3, P - 7, P // 2]
+    for j, p in enumerate(far):
+        src = int(x["table"][0, j])
+        k[p], v[p] = x["k"][src].nan_to_num(0.0), x["v"][src].nan_to_num(0.0)
+    table = torch.tensor([far], dtype=torch.int32, device=DEV)
+    for news in (1, 100):
+        y = make([500], [news], H, 4, D, page, BF, seed=8)
+        y["rows"] = x["rows"]
+        b = ops.PagedBatch(table, y["lens"], y["start"], max_query=news)
+        out, lse = ops.paged_attention(y["q"], k, v, b, return_lse=True)
+        check(y, out, lse)
+
+
+@pytest.mark.parametrize("lens,news", [([600, 40, 1], [1, 1, 1]), ([700, 90], [200, 5])])
+def test_captured_replays_and_streams(ops, lens, news):
+    """One captured call replayed as the batch changes, then the same call on
+    two streams at once: every result equals the eager one."""
+    x = make(lens, news, 2, 4, 128, 16, BF, junk=0.0)
+    cap = x["table"].shape[1] * 16
+    b = ops.PagedBatch(x["table"], x["lens"], x["start"], max_query=max(news))
+    eager = lambda: ops.paged_attention(x["q"], x["k"], x["v"], b, return_lse=True)
+    eager()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out, lse = eager()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=stream):   # a second capture on the stream
+        eager()
+    for step in range(4):
+        x["q"].normal_()
+        x["lens"].copy_(torch.tensor([max(1, n - 7 * step) for n in lens], dtype=torch.int32))
+        graph.replay()
+        want, want_lse = eager()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), step
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    results = []
+    for _ in range(5):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(eager())
+    graph.replay()
+    torch.cuda.synchronize()
+    for r, l in results:
+        assert torch.equal(r, want) and torch.equal(l, want_lse)
+    assert torch.equal(out, want)
+
+
+def test_refusals(ops):
+    x = make([40, 9], [2, 1], 2, 2, 64, 8, BF)
+    b = batch_of(ops, x)
+    call = lambda **kw: ops.paged_attention(**{**dict(query=x["q"], key_pages=x["k"], value_pages=x["v"], batch=b), **kw})
+    with pytest.raises(TypeError):
+        call(query=x["q"].float())
+    with pytest.raises(TypeError):
+        call(key_pages=x["k"].half())
+    with pytest.raises(ValueError):
+        call(query=x["q"][:, :3])
+    with pytest.raises(ValueError):
+        call(value_pages=x["v"][:, :, :4])
+    with pytest.raises(ValueError):
+        call(out=torch.empty_like(x["q"])[:1].expand(x["q"].shape))
+    with pytest.raises(ValueError):
+        call(lse=torch.empty((3, 4), device=DEV).double())
+    with pytest.raises(ValueError):
+        call(query=x["q"].cpu())
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=DEV)
+    with pytest.raises(TypeError):
+        ops.PagedBatch(x["table"], x["lens"].long(), x["start"], 2)
+    with pytest.raises(ValueError):
+        ops.PagedBatch(x["table"], x["lens"], x["start"][:2], 2)
+    with pytest.raises(ValueError):
+        ops.PagedBatch(x["table"][:1], x["lens"], x["start"], 2)
+    with pytest.raises(ValueError):
+        ops.PagedBatch(x["table"].T.contiguous().T, x["lens"], x["start"], 2)
+    with pytest.raises(ValueError, match="contiguous rows"):
+        ops.paged_attention(x["q"], x["k"][:1], x["v"][:1], ops.PagedBatch(None, x["lens"], x["start"], 2))
+    from adaptiveimi_amd._lib import IMIError
+
+    for kw in (dict(scale=0.0), dict(scale=-1.0), dict(window=-1), dict(sinks=-2)):
+        with pytest.raises(IMIError):
+            call(**kw)
+    with pytest.raises(IMIError, match="power of two"):
+        call(key_pages=x["k"][:, :, :6], value_pages=x["v"][:, :, :6])
+    with pytest.raises(IMIError, match="max_query"):
+        call(batch=ops.PagedBatch(x["table"], x["lens"], x["start"], 0))
