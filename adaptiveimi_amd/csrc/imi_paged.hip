@@ -34,6 +34,8 @@ namespace imi {
 int validate_batch(const imi_paged_batch* b) {
     IMI_REQUIRE(b->n_seqs >= 0 && b->n_tokens >= 0, IMI_ERR_INVALID, "negative batch (n_seqs=%d, n_tokens=%d)",
                 b->n_seqs, b->n_tokens);
+    IMI_REQUIRE(b->n_seqs <= 1 << 30 && b->n_tokens <= 1 << 30, IMI_ERR_UNSUPPORTED,
+                "more than 2^30 sequences or tokens (n_seqs=%d, n_tokens=%d)", b->n_seqs, b->n_tokens);
     if (b->n_seqs == 0 || b->n_tokens == 0) return IMI_OK;
     IMI_REQUIRE(b->lens && b->query_start, IMI_ERR_INVALID, "null lens or query_start");
     IMI_REQUIRE(b->max_query >= 1, IMI_ERR_INVALID, "max_query=%d must be >= 1", b->max_query);
@@ -48,6 +50,7 @@ int validate_batch(const imi_paged_batch* b) {
         IMI_REQUIRE(b->n_pages >= b->n_seqs, IMI_ERR_INVALID, "n_pages=%d < n_seqs=%d with no page table", b->n_pages,
                     b->n_seqs);
     }
+    IMI_REQUIRE(batch_capacity(b) <= int64_t(1) << 30, IMI_ERR_UNSUPPORTED, "more than 2^30 rows in a sequence");
     return IMI_OK;
 }
 
@@ -1240,10 +1243,12 @@ int validate(const imi_paged_attention_args* a) {
                     "query, keys, values and out must be 16-byte aligned");
     IMI_REQUIRE(a->page_stride <= UINT_MAX && (a->batch.page_size - 1) * a->row_stride <= UINT_MAX, IMI_ERR_UNSUPPORTED,
                 "a page spans more than 2^32 elements");
-    IMI_REQUIRE(batch_capacity(&a->batch) <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
-                "more than 2^30 rows in a sequence");
     IMI_REQUIRE(static_cast<int64_t>(a->batch.n_tokens) * a->groups <= (int64_t(1) << 30), IMI_ERR_UNSUPPORTED,
                 "more than 2^30 query rows per KV head");
+    // the units that are shared out (each at least 128 rows of a sequence), times workgroups, in 64 bits
+    const double units = (static_cast<double>(a->batch.n_tokens) * a->groups / kTileRows + a->batch.n_seqs) *
+                         (batch_capacity(&a->batch) / 128 + 1) * a->kv_heads;
+    IMI_REQUIRE(units <= 1e15, IMI_ERR_UNSUPPORTED, "too much work for one call");
     return IMI_OK;
 }
 
@@ -1262,6 +1267,7 @@ struct Shape {
 // A workgroup per (sequence, head) up to this many units: 512, 768, 1024 rows of
 // one sequence take 13, 17, 20 us that way, 15 with a join.
 constexpr int kDirectUnits = 3;
+constexpr int kDirectGrid = 1 << 22;   // workgroups of 512 threads in a launch of at most 2^32 - 1
 
 Shape shape_of(const imi_paged_attention_args* a) {
     Shape p;
@@ -1283,7 +1289,8 @@ Shape shape_of(const imi_paged_attention_args* a) {
         int64_t longest = cap;   // visible rows of the longest sequence
         if (a->window > 0)
             longest = std::min<int64_t>(cap, static_cast<int64_t>(a->window) + a->sinks + p.few_rows / a->groups);
-        p.direct = (longest + kUnit - 1) / kUnit <= kDirectUnits;
+        p.direct = (longest + kUnit - 1) / kUnit <= kDirectUnits &&
+                   static_cast<int64_t>(b.n_seqs) * a->kv_heads <= kDirectGrid;
         if (!p.direct) p.few_part = (size_t(2) << p.w_log) * p.most * (a->dim + 2) * sizeof(float);
     }
     if (p.tiles) {
@@ -1328,7 +1335,7 @@ int launch(const imi_paged_attention_args* a, const Shape& p, PagedParams P, flo
     if (p.few_rows) {
         PagedParams Q = P;
         Q.min_rows = 1;
-        Q.max_rows = p.few_rows;
+        Q.max_rows = p.most;   // (one with more new tokens than max_query has no room in the partials)
         Q.cap = p.most;
         Q.joins = joins;
         Q.part = few;
@@ -1402,8 +1409,8 @@ extern "C" int imi_paged_attention(const imi_paged_attention_args* a, imi_stream
     P.n_pages = b.n_pages;
     P.page_shift = b.page_table ? __builtin_ctz(static_cast<unsigned>(b.page_size)) : 31;
     P.capacity = static_cast<int>(batch_capacity(&b));
-    P.window = a->window;
-    P.sinks = a->window > 0 ? a->sinks : 0;
+    P.window = a->window < P.capacity ? a->window : 0;   // (a window of all rows is none)
+    P.sinks = P.window > 0 ? a->sinks : 0;
     P.c = a->scale * kLog2e;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == IMI_BF16)

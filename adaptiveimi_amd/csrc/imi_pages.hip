@@ -327,14 +327,17 @@ __global__ __launch_bounds__(256) void compact_move_kernel(TableParams t, const 
 // ---------------------------------------------------------------- host ----
 int check_table(const imi_page_table* t, const char* what) {
     IMI_REQUIRE(t->n_seqs >= 0 && t->max_pages >= 0 && t->n_pages >= 0, IMI_ERR_INVALID, "%s: negative size", what);
+    IMI_REQUIRE(t->n_pages <= 1 << 30 && t->n_seqs <= 1 << 30, IMI_ERR_UNSUPPORTED,
+                "%s: more than 2^30 pages or sequences", what);
     IMI_REQUIRE(t->page_size >= 1, IMI_ERR_INVALID, "%s: page_size=%d must be >= 1", what, t->page_size);
     IMI_REQUIRE(t->stride >= t->max_pages, IMI_ERR_INVALID, "%s: stride=%lld < max_pages=%d", what,
                 static_cast<long long>(t->stride), t->max_pages);
     IMI_REQUIRE(t->n_seqs == 0 || (t->lens && (t->pages || t->max_pages == 0)), IMI_ERR_INVALID, "%s: null pointer",
                 what);
     IMI_REQUIRE(t->n_pages == 0 || t->refs, IMI_ERR_INVALID, "%s: null refs", what);
-    IMI_REQUIRE(static_cast<int64_t>(t->max_pages) * t->page_size <= INT_MAX, IMI_ERR_UNSUPPORTED,
-                "%s: more than 2^31 - 1 rows in a sequence", what);
+    // (a page more than the table holds, for the rounding up to whole pages)
+    IMI_REQUIRE((static_cast<int64_t>(t->max_pages) + 1) * t->page_size <= INT_MAX, IMI_ERR_UNSUPPORTED,
+                "%s: 2^31 rows or more in a sequence and a page (max_pages=%d, page_size=%d)", what, t->max_pages, t->page_size);
     return IMI_OK;
 }
 

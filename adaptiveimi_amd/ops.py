@@ -1015,7 +1015,7 @@ class PagedBatch:
     query_start: int32 [S + 1], sequence s's new tokens are the query rows
     query_start[s] .. query_start[s + 1] - 1; query rows behind the last
     sequence belong to none.  max_query: at least every sequence's new tokens
-    (sequences with more may not be served).  max_len: a hint, about the
+    (the rows of one with more may be left as they are).  max_len: a hint, about the
     longest sequence (default: what the table holds); only the split of short
     batches depends on it."""
 
@@ -1042,8 +1042,9 @@ class PagedBatch:
                                    self.max_query, max_len or 0)
 
     def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
-        """The C struct for pools of n_pages pages and n_tokens query rows."""
-        a = self.args
+        """The C struct for pools of n_pages pages and n_tokens query rows: a
+        copy, so that threads can use one batch."""
+        a = PagedBatchArgs.from_buffer_copy(self.args)
         a.n_pages, a.page_size, a.n_tokens = n_pages, page_size, n_tokens
         return a
 
@@ -1288,12 +1289,13 @@ def fork_pages(table: PageTable, parents: torch.Tensor, out: Optional[PageTable]
         if out.device != table.device:
             raise ValueError(f"out is on {out.device}, expected {table.device}")
         spans = []
+        spans.append((parents.data_ptr(), parents.shape[0]))
         for x in (table.args, out.args):   # (an array of no entries has address 0)
             spans += [(x.pages or 0, max(x.n_seqs - 1, 0) * x.stride + x.max_pages), (x.lens or 0, x.n_seqs),
                       (x.refs or 0, x.n_pages)]
         spans = sorted([(p, p + 4 * n) for p, n in spans if p and n > 0])
         if any([a[1] > b[0] for a, b in zip(spans, spans[1:])]):
-            raise ValueError("out must share no memory with the table")
+            raise ValueError("out must share no memory with the table or parents")
     with _on(table.device):
         check(_lib.lib().imi_fork_pages(ctypes.byref(table.args), parents.data_ptr(), ctypes.byref(out.args),
                                         _raw_stream(table.device.index)), "imi_fork_pages")

@@ -394,3 +394,67 @@ def test_refusals(ops):
         call(key_pages=x["k"][:, :, :6], value_pages=x["v"][:, :, :6])
     with pytest.raises(IMIError, match="max_query"):
         call(batch=ops.PagedBatch(x["table"], x["lens"], x["start"], 0))
+
+
+@pytest.mark.parametrize("G,news,max_query", [(4, [1, 2, 1], 1), (1, [3, 9, 2], 3), (8, [4, 2, 3], 3)])
+def test_more_new_tokens_than_max_query(ops, G, news, max_query):
+    """Sequences within max_query are right; rows of the others may be left,
+    and nothing else is written."""
+    lens = [3000, 2000, 900]
+    x = make(lens, news, 2, G, 128, 16, BF, junk=0.0)
+    b = ops.PagedBatch(x["table"], x["lens"], x["start"], max_query=max_query)
+    N = sum(news)
+    wide = torch.full((N + 2, 2 * G, 128), 7.0, dtype=BF, device=DEV)
+    out = ops.paged_attention(x["q"], x["k"], x["v"], b, out=wide[1:-1])
+    want, _, tol, _, _ = expected(x)
+    for s, n in enumerate(news):
+        rows = slice(x["start_host"][s], x["start_host"][s + 1])
+        if n <= max_query:
+            assert torch.all((out[rows].double().cpu() - want[rows]).abs() <= tol[rows])
+        else:
+            got = out[rows].double().cpu()
+            assert torch.all((got == 7.0) | ((got - want[rows]).abs() <= tol[rows]))
+    assert torch.all(wide[0] == 7.0) and torch.all(wide[-1] == 7.0)
+
+
+def test_window_of_every_row_is_none(ops):
+    for lens, news in (([900, 70], [1, 1]), ([900, 70], [300, 70])):
+        x = make(lens, news, 1, 4, 64, 16, HF)
+        cap = x["table"].shape[1] * 16
+        want = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x))
+        for window in (900, cap - 1, cap, 2 ** 31 - 1):
+            got = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), window=window, sinks=2 ** 31 - 1)
+            assert (got.double() - want.double()).abs().max() <= 2 * 2.0 ** -10 * (want.double().abs().max() + 1)
+
+
+def test_more_heads_than_a_launch_has_workgroups(ops):
+    """Half a million short sequences: their units are shared out."""
+    S, H = (1 << 16) + 1, 64
+    g = torch.Generator(device=DEV).manual_seed(0)
+    k, v = (torch.randn((3, H, 16, 64), generator=g, device=DEV).to(HF) for _ in range(2))
+    q = torch.randn((S, H, 64), generator=g, device=DEV).to(HF)
+    ids = torch.arange(S, device=DEV)
+    lens, page = ids % 17, ids % 3
+    b = ops.PagedBatch(page.int()[:, None].contiguous(), lens.int(), torch.arange(S + 1, device=DEV).int(), 1)
+    out = ops.paged_attention(q, k, v, b)
+    for n in (0, 1, 9, 16):
+        for p in range(3):
+            rows = ids[(lens == n) & (page == p)][:200]
+            if n == 0:
+                assert torch.all(out[rows] == 0)
+                continue
+            for h in (0, 63):
+                qs, ks, vs = q[rows, h].double().cpu(), k[p, h, :n].double().cpu(), v[p, h, :n].double().cpu()
+                w = torch.softmax(qs @ ks.T / 8, -1)
+                err = (out[rows, h].double().cpu() - w @ vs).abs()
+                # weights and output rounded: half a step each, and the scores' fp32 sums
+                assert torch.all(err <= (2.0 ** -11 + 2.0 ** -17) * (w @ vs.abs()) + 2.0 ** -11 * (w @ vs).abs() + 1e-5)
+
+
+def test_a_batch_serves_pools_of_its_own_sizes(ops):
+    x = make([40], [1], 1, 1, 64, 8, HF)
+    b = batch_of(ops, x)
+    one = b.bind(5, 8, 1)
+    two = b.bind(9, 16, 3)
+    assert (one.n_pages, one.page_size, one.n_tokens) == (5, 8, 1)
+    assert (two.n_pages, two.page_size, two.n_tokens) == (9, 16, 3)

@@ -227,3 +227,31 @@ def test_captured_steps(ops):
         for a, b in ((base.pages, work.pages), (base.lens, work.lens), (base.refs, work.refs)):
             a.copy_(b)
         torch.cuda.synchronize()
+
+
+def test_fork_refuses_shared_memory(ops):
+    table, other = (ops.PageTable.empty(4, 8, 16, 4, DEV) for _ in range(2))
+    for parents in (other.lens, other.refs[3:7], other.pages.view(-1)[9:13]):
+        with pytest.raises(ValueError, match="share no memory"):
+            ops.fork_pages(table, parents, out=other)
+    with pytest.raises(ValueError, match="share no memory"):
+        ops.fork_pages(table, i32([0, 1, 2, 3]), out=table)
+
+
+def test_counts_may_be_the_lengths(ops):
+    """Every sequence doubled; the same pool listed twice moves once."""
+    m = Model(3, 40, 64, 4, n_pools=1)
+    table = ops.PageTable.empty(3, 40, 64, 4, DEV)
+    (pool,) = pools = [content((64, 8), 0)]
+    for counts in ([5, 9, 2], None, None):
+        given = m.lens[:] if counts is None else counts
+        ops.extend_pages(table, table.lens if counts is None else i32(counts), [pool, pool])
+        m.extend(given)
+        m.same(table)
+    m.fork([-1, 1, 1])
+    table = ops.fork_pages(table, i32([-1, 1, 1]))
+    ops.extend_pages(table, i32([1, 1, 1]), [pool, pool])
+    m.extend([1, 1, 1])
+    assert ops.compact_pages(table, [pool, pool]).item() == m.compact()
+    m.same(table)
+    pools_equal(m, pools)

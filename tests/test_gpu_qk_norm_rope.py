@@ -185,3 +185,77 @@ def test_far_positions(ops):
     for got, x in ((qo, q), (ko, k)):
         z, m = definition(x, None, 0.0, pos, f, False)
         close(got, z, m * 2, 128)
+
+
+def test_captured_and_on_streams(ops):
+    """A captured store replayed as positions move, and two streams at once."""
+    (_, _, _), (q, k, v) = inputs(6, 4, 2, 128, BF)
+    qw, kw = (w.to(DEV) for w in weights(128, BF))
+    f = freqs(128).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    lens, start = i32([30, 9, 50]), i32([0, 1, 5, 6])
+    table = torch.randperm(12, device=DEV).int().view(3, 4)
+    pools = [torch.zeros((12, 2, 16, 128), dtype=BF, device=DEV) for _ in range(4)]
+    batch = ops.PagedBatch(table, lens, start, 4)
+    call = lambda out, kp, vp: ops.qk_norm_rope(q, k, inv_freq=f, query_weight=qw, key_weight=kw, query_out=out,
+                                                value=v, batch=batch, key_pages=kp, value_pages=vp)
+    outs = [torch.zeros_like(q, memory_format=torch.contiguous_format) for _ in range(4)]
+    call(outs[0], *pools[:2])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        call(outs[1], *pools[2:])
+    for step in range(4):
+        q.normal_()
+        lens.copy_(i32([30 + step, 9 + 2 * step, 50 + step]))
+        graph.replay()
+        call(outs[0], *pools[:2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(pools[0], pools[2])
+        # (the first eager call, before the graph, stored the first step's values too)
+        assert torch.equal(pools[1], pools[3])
+    pos = torch.arange(6, device=DEV)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(ops.qk_norm_rope(q, k, pos, inv_freq=f, query_weight=qw, key_weight=kw))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, got[0][0]) and torch.equal(b, got[0][1]) for a, b in got)
+
+
+def test_refusals(ops):
+    from adaptiveimi_amd._lib import IMIError
+
+    (_, _, _), (q, k, v) = inputs(3, 4, 2, 128, BF, packed=False)
+    pos = torch.arange(3, device=DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    table = i32([[0, 1]])
+    pages = torch.zeros((2, 2, 16, 128), dtype=BF, device=DEV)
+    batch = ops.PagedBatch(table, i32([3]), i32([0, 3]), 3)
+    store = dict(value=v, batch=batch, key_pages=pages, value_pages=pages.clone())
+    for kw in (dict(), dict(positions=pos, **store), dict(batch=batch), dict(positions=pos, value=v),
+               dict(key_out=k, **store), dict(positions=pos[:2]), dict(positions=pos.cpu()),
+               dict(positions=pos, inv_freq=torch.ones(64, dtype=torch.float64, device=DEV)),
+               dict(positions=pos, query_weight=torch.ones(64, dtype=BF, device=DEV)),
+               dict(positions=pos, query_out=q[:1].expand(q.shape)),
+               dict(store, value=v[:2]), dict(store, key_pages=pages[:, :1], value_pages=pages[:, :1]),
+               dict(store, key_pages=pages[:1].expand(2, -1, -1, -1), value_pages=pages[:1].expand(2, -1, -1, -1))):
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope(q, k, **kw)
+    for kw in (dict(positions=pos.float()), dict(positions=pos, query_weight=torch.ones(128, dtype=HF, device=DEV)),
+               dict(positions=pos, query_weight=torch.ones(128, dtype=BF, device=DEV),
+                    key_weight=torch.ones(128, device=DEV)), dict(store, key_pages=pages.half())):
+        with pytest.raises(TypeError):
+            ops.qk_norm_rope(q, k, **kw)
+    with pytest.raises(IMIError, match="rotary"):
+        ops.qk_norm_rope(q, k, pos, inv_freq=torch.ones(4, device=DEV))
+    with pytest.raises(IMIError, match="eps"):
+        ops.qk_norm_rope(q, k, pos, eps=-1.0)
+    with pytest.raises(IMIError, match="dim=96"):
+        ops.qk_norm_rope(q[..., :96].contiguous(), k[..., :96].contiguous(), pos)
+    none = ops.qk_norm_rope(q[:0], k[:0], pos[:0])
+    assert none[0].shape == (0, 4, 128) and none[1].shape == (0, 2, 128)

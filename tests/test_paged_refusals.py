@@ -171,3 +171,33 @@ def test_python_layer_refuses_host_tensors():
     x = torch.zeros((2, 1, 128), dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="HIP device"):
         ops.qk_norm_rope(x, x, positions=i32)
+
+
+def test_sizes_past_the_kernels_indexes(L):
+    """Counts that 32-bit indexes of the kernels would not hold are refused."""
+    ref = ctypes.byref
+    need = ctypes.c_size_t()
+    for over in (dict(n_seqs=(1 << 30) + 1), dict(n_tokens=(1 << 30) + 1)):
+        a = attention(batch(**over))
+        assert L.imi_paged_attention_workspace_size(ref(a), ref(need)) == 3
+        assert "2^30" in L.imi_last_error().decode()
+        assert L.imi_qk_norm_rope(ref(norm(batch(**over))), None) == 3
+    long = dict(max_pages=1 << 27, table_stride=1 << 27)
+    assert L.imi_qk_norm_rope(ref(norm(batch(**long))), None) == 3
+    assert "2^30" in L.imi_last_error().decode()
+    a = attention(batch(n_seqs=1 << 28, max_pages=1 << 20, table_stride=1 << 20), kv_heads=1024, groups=1)
+    assert L.imi_paged_attention_workspace_size(ref(a), ref(need)) == 3
+    assert "too much work" in L.imi_last_error().decode()
+    for over in (dict(n_pages=(1 << 30) + 1), dict(n_seqs=(1 << 30) + 1), dict(max_pages=1, page_size=(1 << 31) - 1)):
+        assert L.imi_compact_pages_workspace_size(ref(table(**over)), ref(need)) == 3
+
+
+def test_attention_splits_more_heads_than_a_launch_has_workgroups(L):
+    """Short sequences take a workgroup per (sequence, head) and no workspace,
+    as long as a launch can hold them."""
+    need = ctypes.c_size_t()
+    short = dict(max_pages=2, table_stride=2, max_query=1)
+    for n, shared in ((1 << 19, False), ((1 << 19) + 1, True)):
+        a = attention(batch(n_seqs=n, n_tokens=n, **short))
+        assert L.imi_paged_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)) == 0
+        assert (need.value > 0) == shared
