@@ -349,7 +349,13 @@ def _own_qk(state):
     kw = dict(inv_freq=state["inv_freq"], query_weight=state["qw"], key_weight=state["kw"], eps=EPS,
               interleaved=case["interleaved"], query_out=state["q_out"])
     if not case["page"]:
-        return ops.qk_norm_rope(state["q"], state["k"], positions=state["positions"], key_out=state["k_out"], **kw)
+        if not case["pad"]:
+            return ops.qk_norm_rope(state["q"], state["k"], positions=state["positions"], key_out=state["k_out"], **kw)
+        n = state["start_host"][-1]   # the padding's rows are left alone
+        kw["query_out"] = state["q_out"][:n]
+        ops.qk_norm_rope(state["q"][:n], state["k"][:n], positions=state["positions"][:n], key_out=state["k_out"][:n],
+                         **kw)
+        return state["q_out"], state["k_out"]
     q, _ = ops.qk_norm_rope(state["q"], state["k"], value=state["v"], batch=_own_batch(state),
                             key_pages=state["key_pages"], value_pages=state["value_pages"], **kw)
     return q, state["key_pages"], state["value_pages"]
