@@ -294,8 +294,10 @@ constexpr int kFewWaves = 8;
 constexpr int kFewTile = 32;                       // rows of K / V per wave and step
 constexpr int kUnit = kFewTile * kFewWaves;
 
-// How both kernels cut their work: range w of 2^w_log is the units
-// [cut(w), cut(w + 1)).  What one range holds of a (sequence, head) or tile
+// How both kernels cut their work: range w of 2^log is the units
+// [cut(w), cut(w + 1)), with a range per workgroup, or for little work about
+// as many ranges as units (at most half of them empty: merge_kernel visits
+// every range of a tile).  What one range holds of a (sequence, head) or tile
 // with units [lo, hi) that it does not hold whole goes to a partial: 2 w for
 // the first that the range meets, 2 w + 1 for the last.  The range that holds
 // unit lo leaves a Join where hi lies past its end, and merge_kernel joins the
@@ -307,7 +309,10 @@ struct Join {
     int first, end;     // rows (token, head of the group) [first, end)
     int h;
 };
-__device__ __forceinline__ int64_t cut(int64_t total, int64_t w, int w_log) { return (total * w) >> w_log; }
+__device__ __forceinline__ int ranges_log(int w_log, int64_t total) {
+    return total <= 1 ? 0 : min(w_log, 64 - __builtin_clzll(static_cast<uint64_t>(total - 1)));
+}
+__device__ __forceinline__ int64_t cut(int64_t total, int64_t w, int log) { return (total * w) >> log; }
 
 __device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
     const int rows = q.n * a.G;
@@ -338,8 +343,10 @@ __device__ __forceinline__ FewRange few_range(const PagedParams& a) {
         r.total += __builtin_amdgcn_readlane(incl, 63);
     }
     r.total *= a.H;
-    r.g0 = cut(r.total, blockIdx.x, a.w_log);
-    r.g1 = cut(r.total, blockIdx.x + 1, a.w_log);
+    const int log = ranges_log(a.w_log, r.total);
+    if (blockIdx.x >> log) return r;
+    r.g0 = cut(r.total, blockIdx.x, log);
+    r.g1 = cut(r.total, blockIdx.x + 1, log);
     if (r.g0 >= r.g1) return r;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         if (a.S > 64) {   // else the only 64 are still at hand
@@ -619,6 +626,23 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     if (!direct && tid == 0) a.joins[blockIdx.x] = rest;
 }
 
+// What merge_kernel needs: the partials of the few-row launch and of the tiles.
+struct Parts {
+    const Join* joins;
+    const float* rows;   // [2 W][cap][D]
+    const float* ml;     // [2 W][cap][2]
+    int cap;
+};
+struct MergeParams {
+    Parts few, tiles;
+    uint16_t* out;
+    float* lse;
+    int64_t o_ts, o_hs, l_ts;
+    int few_blocks;      // workgroups for the few-row launch: W cap, or none
+    int G, w_log;
+    float c;
+};
+
 template <int D>
 struct Partial {
     float M = -INFINITY, L = 0.0f;
@@ -631,31 +655,32 @@ struct Partial {
         M = Mn;
     }
     // row r's partials of ranges w0 + first, w0 + first + step .. w1, four
-    // loads under way at a time; an empty range (its slot holds anything) and
-    // one past w1 weigh nothing
-    __device__ __forceinline__ void gather(const PagedParams& a, const Join& j, int w0, int w1, int r, int d4, int first,
-                                           int step) {
-        for (int w = w0 + first; w <= w1; w += 4 * step) {
-            float m[4], l[4];
-            f32x4_t x[4];
-            bool use[4];
+    // loads under way at a time (behind a branch each they would be one); an
+    // empty range, whose slot holds anything, and one past w1 are left out
+    __device__ __forceinline__ void gather(const Parts& p, const Join& j, int log, int w0, int w1, int r, int d4,
+                                           int first, int step, float c) {
+        constexpr int N = 4;
+        for (int w = w0 + first; w <= w1; w += N * step) {
+            float m[N], l[N];
+            f32x4_t x[N];
+            bool use[N];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < N; ++i) {
                 const int wi = min(w + i * step, w1);
-                const int64_t b = cut(j.total, wi, a.w_log);
-                use[i] = w + i * step <= w1 && b != cut(j.total, wi + 1, a.w_log);
-                const int64_t e = (2 * static_cast<int64_t>(wi) + (b < j.lo ? 1 : 0)) * a.cap + r;
-                m[i] = a.part_ml[2 * e];
-                l[i] = a.part_ml[2 * e + 1];
-                x[i] = *reinterpret_cast<const f32x4_t*>(a.part + e * D + 4 * d4);
+                const int64_t b = cut(j.total, wi, log);
+                use[i] = w + i * step <= w1 && b != cut(j.total, wi + 1, log);
+                const int64_t e = (2 * static_cast<int64_t>(wi) + (b < j.lo ? 1 : 0)) * p.cap + r;
+                m[i] = p.ml[2 * e];
+                l[i] = p.ml[2 * e + 1];
+                x[i] = *reinterpret_cast<const f32x4_t*>(p.rows + e * D + 4 * d4);
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (use[i]) add(m[i], l[i], x[i], a.c);
+            for (int i = 0; i < N; ++i)
+                if (use[i]) add(m[i], l[i], x[i], c);
         }
     }
     template <typename T>
-    __device__ __forceinline__ void write(const PagedParams& a, const Join& j, int row, int d4) const {
+    __device__ __forceinline__ void write(const MergeParams& a, const Join& j, int row, int d4) const {
         const int64_t tok = j.t0 + row / a.G;
         const int head = j.h * a.G + row % a.G;
         const float inv = L == 0.0f ? 0.0f : 1.0f / L;
@@ -667,48 +692,90 @@ struct Partial {
     }
 };
 
-// One workgroup per (range, y).  D / 4 threads hold a row's partial; with few of
-// them the groups take a row each, with many (a long sequence of few rows) all
-// take a row's partials in turn, one row after another or (spread) one per y.
-constexpr int kManyParts = 4;
+// Joins what the ranges left.  D / 4 threads hold a row's partial, so a
+// workgroup holds P of them: P / K rows with K groups each, K about a quarter
+// of a join's partials, so that a long sequence of few rows and a large chunk
+// both wait for one or two loads.
+//
+// The few-row launch has a workgroup per (range, P / K rows) and most find
+// nothing to do.  Tiles have up to 256 rows, far more such workgroups, so
+// theirs first list the joins and share out (join, rows) pairs: a tile of 120
+// rows in 38 ranges takes 6 us so, 73 with a fixed share of the rows per
+// workgroup.  Decoding takes 5 us the first way and 7 the second.
+constexpr int kMergeThreads = 256;
+constexpr int kMaxRanges = kMergeThreads;   // (a thread looks at one)
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void merge_kernel(PagedParams a, bool spread) {
-    constexpr int Q = D / 4, P = 256 / Q;
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
+    constexpr int Q = D / 4, P = kMergeThreads / Q;
     __shared__ float s_ml[P][2];
     __shared__ float s_acc[P][D];
-    const Join j = a.joins[blockIdx.x];
-    const int r0 = blockIdx.y * P;
-    if (j.lo == j.hi || (spread ? static_cast<int>(blockIdx.y) : r0) >= j.end - j.first) return;
-    const int w0 = blockIdx.x, d4 = threadIdx.x % Q, g = threadIdx.x / Q;
-    // the last range that holds some: about hi W / total, then exactly
-    int w1 = static_cast<int>(((j.hi - 1) << a.w_log) / j.total);
-    while (cut(j.total, w1 + 1, a.w_log) < j.hi) ++w1;
-    if (w1 - w0 < kManyParts) {
-        const int r = r0 + g;
-        if (r >= j.end - j.first) return;
+    __shared__ int s_range[kMaxRanges];
+    __shared__ int s_n[kMergeThreads / 64];
+    const int tid = threadIdx.x, W = 1 << a.w_log;
+    const int d4 = tid % Q, g = tid / Q;
+    // rows r0 .. of a join that range w0 left, K groups to a row
+    auto merge = [&](const Parts& from, const Join& j, int w0, int w1, int log, int r0, int K) {
+        const int r = r0 + g / K, k = g % K;
+        const bool live = r < j.end - j.first;
         Partial<D> p;
-        p.gather(a, j, w0, w1, r, d4, 0, 1);
-        p.template write<T>(a, j, j.first + r, d4);
+        if (live) p.gather(from, j, log, w0, w1, r, d4, k, K, a.c);
+        if (K > 1) {
+            __syncthreads();
+            if (d4 == 0) {
+                s_ml[g][0] = p.M;
+                s_ml[g][1] = p.L;
+            }
+            *reinterpret_cast<f32x4_t*>(&s_acc[g][4 * d4]) = p.A;
+            __syncthreads();
+            if (k == 0)
+                for (int x = g + 1; x < g + K; ++x)
+                    p.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
+        }
+        if (live && k == 0) p.template write<T>(a, j, j.first + r, d4);
+    };
+    // the last range that holds some of a join: about hi W / total, then exactly
+    auto last_of = [&](const Join& j, int w0, int log) {
+        int w1 = max(w0, static_cast<int>(static_cast<float>(j.hi - 1) / static_cast<float>(j.total) * (1 << log)) - 1);
+        while (cut(j.total, w1 + 1, log) < j.hi) ++w1;
+        return w1;
+    };
+    auto groups = [&](int parts) {
+        int K = 1;
+        while (K < P && 4 * K < parts) K *= 2;
+        return K;
+    };
+    if (static_cast<int>(blockIdx.x) < a.few_blocks) {
+        const int w0 = blockIdx.x % W, y = blockIdx.x / W;
+        const Join j = a.few.joins[w0];
+        if (j.lo == j.hi) return;
+        const int log = ranges_log(a.w_log, j.total), w1 = last_of(j, w0, log);
+        const int K = groups(w1 - w0 + 1), r0 = y * (P / K);
+        if (r0 < j.end - j.first) merge(a.few, j, w0, w1, log, r0, K);
         return;
     }
-    const int r_lo = spread ? blockIdx.y : r0, r_hi = spread ? r_lo + 1 : min(r0 + P, j.end - j.first);
-    for (int r = r_lo; r < r_hi; ++r) {
-        Partial<D> p;
-        p.gather(a, j, w0, w1, r, d4, g, P);
-        __syncthreads();
-        if (d4 == 0) {
-            s_ml[g][0] = p.M;
-            s_ml[g][1] = p.L;
-        }
-        *reinterpret_cast<f32x4_t*>(&s_acc[g][4 * d4]) = p.A;
-        __syncthreads();
-        if (g == 0) {
-            Partial<D> t;
-            for (int x = 0; x < P; ++x)
-                t.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
-            t.template write<T>(a, j, j.first + r, d4);
-        }
+    // the ranges that hold a join
+    const bool has = tid < W && a.tiles.joins[tid].lo != a.tiles.joins[tid].hi;
+    const uint64_t mask = __ballot(has);
+    if (lane_id() == 0) s_n[tid >> 6] = __builtin_popcountll(mask);
+    __syncthreads();
+    int before = 0, n = 0;
+#pragma unroll
+    for (int w = 0; w < kMergeThreads / 64; ++w) {
+        if (w < tid >> 6) before += s_n[w];
+        n += s_n[w];
+    }
+    if (n == 0) return;
+    if (has) s_range[before + __builtin_popcountll(mask & ((1ull << lane_id()) - 1))] = tid;
+    __syncthreads();
+    const int log = ranges_log(a.w_log, a.tiles.joins[s_range[0]].total);
+    const int K = groups(((1 << log) + n - 1) / n);
+    const int blocks = (a.tiles.cap * K + P - 1) / P;
+    for (int item = blockIdx.x - a.few_blocks; item < n * blocks; item += gridDim.x - a.few_blocks) {
+        const int w0 = __builtin_amdgcn_readfirstlane(s_range[item / blocks]);
+        const Join j = a.tiles.joins[w0];
+        const int r0 = item % blocks * (P / K);
+        if (r0 < j.end - j.first) merge(a.tiles, j, w0, last_of(j, w0, log), log, r0, K);
     }
 }
 
@@ -959,10 +1026,11 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     const int64_t total = n_tiles ? per_head * a.H : 0;
     // workgroups go round robin over the 8 dies: die x takes the x-th eighth
     // of the steps, so that its workgroups read the same head's K and V
-    const int W = 1 << a.w_log;
-    const int wg = W >= 8 ? (blockIdx.x % 8) * (W / 8) + blockIdx.x / 8 : blockIdx.x;
-    int64_t g0 = cut(total, wg, a.w_log);
-    const int64_t g1 = cut(total, wg + 1, a.w_log);
+    const int log = ranges_log(a.w_log, total), W = 1 << log;
+    const bool used = static_cast<int>(blockIdx.x) < W;
+    const int wg = W >= 8 && used ? (blockIdx.x % 8) * (W / 8) + blockIdx.x / 8 : blockIdx.x;
+    int64_t g0 = used ? cut(total, wg, log) : 0;
+    const int64_t g1 = used ? cut(total, wg + 1, log) : 0;
     bool first = true;
     Join rest{0, 0, 0, 0, 0, 0, 0};
     int h = static_cast<int>(g0 / per_head);
@@ -1181,7 +1249,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                 if (a.lse && hi == 0)
                     a.lse[q_tok * a.l_ts + x_head] = l == 0.0f ? -INFINITY : (m * a.c + __log2f(l)) * kLn2;
             } else {
-                const int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * kTileRows + wave * 32 + q32;
+                const int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
                 float* const op = a.part + e * D + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -1257,9 +1325,11 @@ int validate(const imi_paged_attention_args* a) {
 struct Shape {
     int few_rows = 0;       // 0: no few-row launch
     int w_log = 0;          // 2^w_log workgroups
+    int max_rows = 0;       // rows a sequence can have: one with more has no room in the partials and is left out
     int most = 0;           // rows a few-row sequence can have
     bool direct = false;    // a workgroup per (sequence, head), no join
     bool tiles = false;
+    int tile_most = 0;      // rows of a tile that can be in use
     int slots = 0;
     size_t few_part = 0, tile_part = 0, plan = 0, joins = 0;   // workspace bytes
 };
@@ -1274,8 +1344,9 @@ Shape shape_of(const imi_paged_attention_args* a) {
     const imi_paged_batch& b = a->batch;
     if (b.n_seqs == 0 || b.n_tokens == 0) return p;
     const int64_t most = static_cast<int64_t>(std::min(b.max_query, b.n_tokens)) * a->groups;
+    p.max_rows = static_cast<int>(most);
     // a workgroup of eight waves per CU: its registers and LDS fill one
-    while ((2 << p.w_log) <= device_cus()) ++p.w_log;
+    while ((2 << p.w_log) <= std::min(device_cus(), kMaxRanges)) ++p.w_log;
     p.joins = sizeof(Join) << p.w_log;
     if (most <= 32) {
         p.few_rows = most <= 16 ? 16 : 32;
@@ -1295,7 +1366,8 @@ Shape shape_of(const imi_paged_attention_args* a) {
     }
     if (p.tiles) {
         p.slots = static_cast<int>(static_cast<int64_t>(b.n_tokens) * a->groups / kTileRows + b.n_seqs);
-        p.tile_part = (size_t(2) << p.w_log) * kTileRows * (a->dim + 2) * sizeof(float);
+        p.tile_most = static_cast<int>(std::min<int64_t>(most, kTileRows));
+        p.tile_part = (size_t(2) << p.w_log) * p.tile_most * (a->dim + 2) * sizeof(float);
         p.plan = plan_bytes(p.slots, b.n_seqs);
     }
     return p;
@@ -1315,41 +1387,44 @@ int launch(const imi_paged_attention_args* a, const Shape& p, PagedParams P, flo
            Join* joins, hipStream_t stream) {
     const int W = 1 << p.w_log;
     P.w_log = p.w_log;
+    PagedParams F = P, Q = P;
     if (p.tiles) {
-        PagedParams Q = P;
         Q.min_rows = p.few_rows + 1;
-        Q.max_rows = INT_MAX;
-        Q.cap = kTileRows;
+        Q.max_rows = p.max_rows;
+        Q.cap = p.tile_most;
         Q.joins = joins + W;
         Q.part = tile;
-        Q.part_ml = tile + size_t(2) * W * kTileRows * D;
+        Q.part_ml = tile + size_t(2) * W * p.tile_most * D;
         Q.plan = plan;
         Q.slots = p.slots;
         plan_kernel<<<1, 1024, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("plan_kernel");
         tile_kernel<T, D><<<W, 512, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("tile_kernel");
-        merge_kernel<T, D><<<dim3(W, kTileRows * D / 1024), 256, 0, stream>>>(Q, false);
-        IMI_LAUNCH_CHECK("merge_kernel");
     }
     if (p.few_rows) {
-        PagedParams Q = P;
-        Q.min_rows = 1;
-        Q.max_rows = p.most;   // (one with more new tokens than max_query has no room in the partials)
-        Q.cap = p.most;
-        Q.joins = joins;
-        Q.part = few;
-        Q.part_ml = few + size_t(2) * W * p.most * D;
+        F.min_rows = 1;
+        F.max_rows = p.most;
+        F.cap = p.most;
+        F.joins = joins;
+        F.part = few;
+        F.part_ml = few + size_t(2) * W * p.most * D;
         const int grid = p.direct ? P.S * P.H : W;
         if (p.few_rows == 16)
-            few_kernel<T, D, 1><<<grid, 64 * kFewWaves, 0, stream>>>(Q, p.direct ? 1 : 0);
+            few_kernel<T, D, 1><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
         else
-            few_kernel<T, D, 2><<<grid, 64 * kFewWaves, 0, stream>>>(Q, p.direct ? 1 : 0);
+            few_kernel<T, D, 2><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
         IMI_LAUNCH_CHECK("few_kernel");
-        if (!p.direct) {
-            merge_kernel<T, D><<<dim3(W, p.most), 256, 0, stream>>>(Q, true);
-            IMI_LAUNCH_CHECK("merge_kernel");
-        }
+    }
+    const int few_blocks = p.few_rows && !p.direct ? W * p.most : 0;
+    if (few_blocks || p.tiles) {
+        const MergeParams M{{F.joins, F.part, F.part_ml, F.cap}, {Q.joins, Q.part, Q.part_ml, Q.cap}, P.out, P.lse,
+                            P.o_ts, P.o_hs, P.l_ts, few_blocks, P.G, P.w_log, P.c};
+        // for the tiles: the pairs there can be, as far as workgroups are worth it
+        const int64_t pairs = std::min<int64_t>(W, int64_t(p.slots) * P.H) * p.tile_most;
+        const int more = p.tiles ? static_cast<int>(std::min<int64_t>(8 * W, pairs)) : 0;
+        merge_kernel<T, D><<<few_blocks + more, kMergeThreads, 0, stream>>>(M);
+        IMI_LAUNCH_CHECK("merge_kernel");
     }
     return IMI_OK;
 }
