@@ -375,6 +375,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     __shared__ uint16_t s_buf[kFewWaves * kWaveLds];
     __shared__ float s_ml[kFewWaves][16 * NB][2];
     __shared__ int s_odd;   // a masked tile held infinities or NaN
+    // Queries: in registers, but for two blocks of 128 dims (32 registers more
+    // than there are) in LDS.
+    constexpr bool kQueryLds = NB * D > 128;
+    __shared__ __align__(16) uint16_t s_q[kQueryLds ? 16 * NB * LR : 8];
     const int tid = threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 15, lg = lane >> 4;
@@ -416,7 +420,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
         const int vis = sp.count();
 
         // queries: row r = 16 b + ln of lane, dims 32 c + 8 lg ..
-        u32x4_t qf[NB][KK];
+        u32x4_t qf[kQueryLds ? 1 : NB][KK];
         int pos[NB];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -426,9 +430,19 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             const int rr = min(r, rows - 1);
             const uint16_t* qp = a.q + static_cast<int64_t>(sq.t0 + rr / a.G) * a.q_ts +
                                  static_cast<int64_t>(h * a.G + rr % a.G) * a.q_hs + 8 * lg;
+            if constexpr (!kQueryLds)
 #pragma unroll
-            for (int c = 0; c < KK; ++c) qf[b][c] = load16(qp + 32 * c);
+                for (int c = 0; c < KK; ++c) qf[b][c] = load16(qp + 32 * c);
+            else if (wave == b)   // (a segment's end has a barrier)
+#pragma unroll
+                for (int c = 0; c < KK; ++c)
+                    *reinterpret_cast<u32x4_t*>(s_q + r * LR + 32 * c + 8 * lg) = load16(qp + 32 * c);
         }
+        if constexpr (kQueryLds) __syncthreads();
+        auto query = [&](int b, int c) {
+            if constexpr (kQueryLds) return *reinterpret_cast<const u32x4_t*>(s_q + (16 * b + ln) * LR + 32 * c + 8 * lg);
+            else return qf[b][c];
+        };
         f32x4_t acc[NB][DB];
         float m[NB], l[NB];
 #pragma unroll
@@ -499,7 +513,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                 for (int e = 0; e < 2; ++e) {
                     sc[b][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < KK; ++c) sc[b][e] = T::mma16(kb[e][c], qf[b][c], sc[b][e]);
+                    for (int c = 0; c < KK; ++c) sc[b][e] = T::mma16(kb[e][c], query(b, c), sc[b][e]);
                 }
             if (u + 1 < u1) {
                 fetch(u + 1);
