@@ -1371,8 +1371,10 @@ struct Shape {
     size_t few_part = 0, tile_part = 0, plan = 0, joins = 0;   // workspace bytes
 };
 
-// A workgroup per (sequence, head) up to this many units: 512, 768, 1024 rows of
-// one sequence take 13, 17, 20 us that way, 15 with a join.
+// A workgroup per (sequence, head) up to this many units.  One sequence of 519
+// rows of 128 dims called in a loop takes 14.3 us so, 16.0 with a join, whose
+// workspace and second launch cost the host more than the GPU gains (replayed
+// in a graph: 512, 768, 1024 rows 12.3, 16.0, 19.5 us without, 12.2 each with).
 constexpr int kDirectUnits = 3;
 constexpr int kDirectGrid = 1 << 22;   // workgroups of 512 threads in a launch of at most 2^32 - 1
 
