@@ -1223,7 +1223,7 @@ class PageTable:
     hold each page (0: free).  fork_pages, extend_pages and compact_pages work
     on it without a host synchronisation and can be captured in a graph."""
 
-    __slots__ = ("pages", "lens", "refs", "page_size", "args", "device")
+    __slots__ = ("pages", "lens", "refs", "page_size", "args", "device", "spans", "work_bytes")
 
     def __init__(self, pages: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, page_size: int):
         dev = _device_of("pages", pages)
@@ -1237,8 +1237,12 @@ class PageTable:
         if stride < M:
             raise ValueError("pages is written, so no two of its rows may share memory")
         self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
-        self.args = PageTableArgs(pages.data_ptr(), stride, lens.data_ptr(), refs.data_ptr(), S, M, refs.shape[0],
-                                  self.page_size)
+        P = refs.shape[0]
+        at = pages.data_ptr(), lens.data_ptr(), refs.data_ptr()
+        self.args = PageTableArgs(at[0], stride, at[1], at[2], S, M, P, self.page_size)
+        self.work_bytes = {}   # workspace of each operation: depends on the sizes alone
+        n = max(S - 1, 0) * stride + M if S else 0   # the memory the three take
+        self.spans = [(at[0], at[0] + 4 * n), (at[1], at[1] + 4 * S), (at[2], at[2] + 4 * P)]
 
     @classmethod
     def empty(cls, n_seqs: int, max_pages: int, n_pages: int, page_size: int, device) -> "PageTable":
@@ -1253,6 +1257,16 @@ class PageTable:
         return PagedBatch(self.pages, self.lens, query_start, max_query, max_len)
 
 
+def _table_work(table: PageTable, L, what: str) -> torch.Tensor:
+    """A workspace of this call's own for imi_<what>."""
+    n = table.work_bytes.get(what)
+    if n is None:
+        need = ctypes.c_size_t()
+        check(getattr(L, f"imi_{what}_workspace_size")(ctypes.byref(table.args), ctypes.byref(need)), f"imi_{what}")
+        n = table.work_bytes[what] = need.value
+    return torch.empty(n, dtype=torch.uint8, device=table.device)
+
+
 def _pool_args(table: PageTable, pools: Sequence[torch.Tensor]):
     arr = (PagePool * max(len(pools), 1))()
     P = table.args.n_pages
@@ -1262,14 +1276,20 @@ def _pool_args(table: PageTable, pools: Sequence[torch.Tensor]):
             raise ValueError(f"pool {i} is on {t.device}, expected {table.device}")
         if len(shape) < 2 or shape[0] != P:
             raise ValueError(f"pool {i} must have {P} pages as its first dimension")
-        n, span = 1, 1
-        for k, s in zip(shape[1:], stride[1:]):
-            n *= k
-            span += (k - 1) * s
-        if n == 0 or span != n or (P > 1 and stride[0] < n):
+        if t.is_contiguous() and P:
+            n = t.numel() // P
+            step, dense = n, n > 0
+        else:
+            n, span = 1, 1
+            for k, s in zip(shape[1:], stride[1:]):
+                n *= k
+                span += (k - 1) * s
+            step = stride[0] if P > 1 else n
+            dense = n > 0 and span == n and step >= n
+        if not dense:
             raise ValueError(f"pool {i}: each page must be one dense block of memory")
         size = t.element_size()
-        arr[i] = (t.data_ptr(), (stride[0] if P > 1 else n) * size, n * size)
+        arr[i] = (t.data_ptr(), step * size, n * size)
     return arr, len(pools)
 
 
@@ -1288,14 +1308,12 @@ def fork_pages(table: PageTable, parents: torch.Tensor, out: Optional[PageTable]
     else:
         if out.device != table.device:
             raise ValueError(f"out is on {out.device}, expected {table.device}")
-        spans = []
-        spans.append((parents.data_ptr(), parents.shape[0]))
-        for x in (table.args, out.args):   # (an array of no entries has address 0)
-            spans += [(x.pages or 0, max(x.n_seqs - 1, 0) * x.stride + x.max_pages), (x.lens or 0, x.n_seqs),
-                      (x.refs or 0, x.n_pages)]
-        spans = sorted([(p, p + 4 * n) for p, n in spans if p and n > 0])
-        if any([a[1] > b[0] for a, b in zip(spans, spans[1:])]):
-            raise ValueError("out must share no memory with the table or parents")
+        at = parents.data_ptr()
+        spans = table.spans + [(at, at + 4 * parents.shape[0])]
+        for a, b in out.spans:
+            for c, d in spans:
+                if a < d and c < b:
+                    raise ValueError("out must share no memory with the table or parents")
     with _on(table.device):
         check(_lib.lib().imi_fork_pages(ctypes.byref(table.args), parents.data_ptr(), ctypes.byref(out.args),
                                         _raw_stream(table.device.index)), "imi_fork_pages")
@@ -1318,11 +1336,9 @@ def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.T
     granted = torch.empty(counts.shape, dtype=torch.bool, device=dev)
     L = _lib.lib()
     with _on(dev):
-        need = ctypes.c_size_t()
-        check(L.imi_extend_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_extend_pages")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        ws = _table_work(table, L, "extend_pages")
         check(L.imi_extend_pages(ctypes.byref(table.args), counts.data_ptr(), granted.data_ptr(), arr, n,
-                                 ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_extend_pages")
+                                 ws.data_ptr(), ws.shape[0], _raw_stream(dev.index)), "imi_extend_pages")
     return granted
 
 
@@ -1335,9 +1351,7 @@ def compact_pages(table: PageTable, pools: Sequence[torch.Tensor] = ()) -> torch
     n_live = torch.empty((1,), dtype=torch.int32, device=dev)
     L = _lib.lib()
     with _on(dev):
-        need = ctypes.c_size_t()
-        check(L.imi_compact_pages_workspace_size(ctypes.byref(table.args), ctypes.byref(need)), "imi_compact_pages")
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        check(L.imi_compact_pages(ctypes.byref(table.args), n_live.data_ptr(), arr, n, ws.data_ptr(), need.value,
+        ws = _table_work(table, L, "compact_pages")
+        check(L.imi_compact_pages(ctypes.byref(table.args), n_live.data_ptr(), arr, n, ws.data_ptr(), ws.shape[0],
                                   _raw_stream(dev.index)), "imi_compact_pages")
     return n_live
