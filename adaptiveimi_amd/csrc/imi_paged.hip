@@ -294,9 +294,13 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
 //
 // A wave's 32 rows of the next unit are loaded while it computes on this one's:
 // 128 KB per CU under way (64 for 64 dims; twice the rows there, two
-// workgroups per CU, or loads two units ahead were no faster).  One token over
-// 131072 rows of 8 heads of 128: 97 us, 5.5 TB/s (a large copy runs at 4.84);
-// 64 dims, 4 x 30000 rows: 44 us with its join.
+// workgroups per CU, or loads two units ahead were no faster).  K is loaded as
+// the matrix instruction wants it, 64 bytes of 16 rows at a time; V goes through
+// LDS and is loaded in whole rows, which the cache serves faster (768 rows in a
+// workgroup 16.0 -> 14.1 us; K in the same way 12.0, but then the long streams
+// lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 94 us,
+// 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
+// join.
 constexpr int kFewWaves = 8;
 constexpr int kFewTile = 32;                       // rows of K / V per wave and step
 constexpr int kUnit = kFewTile * kFewWaves;
@@ -378,6 +382,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     constexpr int KK = D / 32;     // matrix instructions over the head dim
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
+    constexpr int CH = D / 8, NV = kFewTile * CH / 64;   // 16-byte pieces of a row, loads of a tile of V
     constexpr int kWaveLds = kFewTile * LR > 16 * D * 2 ? kFewTile * LR : 16 * D * 2;   // u16
     __shared__ uint16_t s_buf[kFewWaves * kWaveLds];
     __shared__ float s_ml[kFewWaves][16 * NB][2];
@@ -460,25 +465,32 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             for (int d = 0; d < DB; ++d) acc[b][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
         }
         const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s + 8 * lg;
-        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * lg;
-        // lane's two rows of a step's tile: ln and 16 + ln
-        auto row_at = [&](int u, int e) { return min(u * kUnit + wave * kFewTile + 16 * e + ln, vis - 1); };
-        int id[2] = {s, s};
+        const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * (lane % CH);
+        // lane's rows of a step's tile: of K ln and 16 + ln (the matrix
+        // instruction's), of V, which goes through LDS, whole rows of CH lanes
+        auto row_of = [&](int u, int r) { return sp.row(min(u * kUnit + wave * kFewTile + r, vis - 1)); };
+        auto k_row = [&](int u, int e) { return row_of(u, 16 * e + ln); };
+        auto v_row = [&](int u, int i) { return row_of(u, (64 / CH) * i + lane / CH); };
+        int idk[2] = {s, s}, idv[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) idv[i] = s;
         auto fetch_ids = [&](int u) {
             if (!a.table) return;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) id[e] = page_of(a, s, sp.row(row_at(u, e)));
+            for (int e = 0; e < 2; ++e) idk[e] = page_of(a, s, k_row(u, e));
+#pragma unroll
+            for (int i = 0; i < NV; ++i) idv[i] = page_of(a, s, v_row(u, i));
         };
-        u32x4_t kb[2][KK], vb[2][KK];
+        u32x4_t kb[2][KK], vb[NV];
         auto fetch = [&](int u) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int64_t o = row_offset(a, id[e], sp.row(row_at(u, e)));
+                const int64_t o = row_offset(a, idk[e], k_row(u, e));
 #pragma unroll
                 for (int c = 0; c < KK; ++c) kb[e][c] = load16(kh + o + 32 * c);
-#pragma unroll
-                for (int c = 0; c < KK; ++c) vb[e][c] = load16(vh + o + 32 * c);
             }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) vb[i] = load16(vh + row_offset(a, idv[i], v_row(u, i)));
         };
         // a wave with no row in its share of a unit still runs the step (all
         // of its keys masked): only a unit's tail has such waves
@@ -492,27 +504,21 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             const int v0 = u * kUnit + wave * kFewTile;   // first row of the tile
             if (v0 + kFewTile > vis) {   // rows past the end weigh nothing: no NaN may enter through V
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (v0 + 16 * e + ln >= vis)
-#pragma unroll
-                        for (int c = 0; c < KK; ++c) vb[e][c] = u32x4_t{0, 0, 0, 0};
+                for (int i = 0; i < NV; ++i)
+                    if (v0 + (64 / CH) * i + lane / CH >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
             }
             const int j_lo = sp.row(v0), j_hi = sp.row(v0 + kFewTile - 1);
             const bool full = v0 + kFewTile <= vis && j_hi <= p0 &&
                               (a.window == 0 || j_lo >= sq.len - a.window || j_hi < a.sinks);
             if (!full && sq.n > 1) {   // (one token sees every row of its span)
-                const bool odd = !all_finite<T>(vb[0]) || !all_finite<T>(vb[1]);
-                if (__builtin_amdgcn_ballot_w64(odd)) {
-                    keep_finite<T>(vb[0]);
-                    keep_finite<T>(vb[1]);
+                if (__builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
+                    keep_finite<T>(vb);
                     s_odd = 1;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int c = 0; c < KK; ++c)
-                    *reinterpret_cast<u32x4_t*>(sv + (16 * e + ln) * LR + 32 * c + 8 * lg) = vb[e][c];
+            for (int i = 0; i < NV; ++i)
+                *reinterpret_cast<u32x4_t*>(sv + ((64 / CH) * i + lane / CH) * LR + 8 * (lane % CH)) = vb[i];
             f32x4_t sc[NB][2];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
@@ -1387,9 +1393,9 @@ struct Shape {
 };
 
 // A workgroup per (sequence, head) up to this many units.  One sequence of 519
-// rows of 128 dims called in a loop takes 14.3 us so, 16.0 with a join, whose
+// rows of 128 dims called in a loop takes 13.3 us so, 15.4 with a join, whose
 // workspace and second launch cost the host more than the GPU gains (replayed
-// in a graph: 512, 768, 1024 rows 12.3, 16.0, 19.5 us without, 12.2 each with).
+// in a graph: 512, 768, 1024 rows 11.3, 14.1, 16.8 us without, 11.4 each with).
 constexpr int kDirectUnits = 3;
 constexpr int kDirectGrid = 1 << 22;   // workgroups of 512 threads in a launch of at most 2^32 - 1
 
