@@ -1004,6 +1004,9 @@ def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: torch.devi
     return t.data_ptr(), st, sh
 
 
+_I32_MAX = 2 ** 31 - 1   # (a C int takes more than that modulo 2^32)
+
+
 class PagedBatch:
     """A ragged batch of new tokens over cached rows, one object for every
     layer of a step.
@@ -1035,11 +1038,13 @@ class PagedBatch:
             rows, cols = page_table.shape
             if rows != S:
                 raise ValueError(f"page_table has {rows} rows for {S} sequences")
+            if cols == 0 and S > 0:
+                raise ValueError("page_table has no columns")
             table, stride = page_table.data_ptr(), page_table.stride(0) if S > 1 else cols
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
-                                   self.max_query, max_len or 0)
+                                   min(self.max_query, _I32_MAX), min(max_len or 0, _I32_MAX))
 
     def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
         """The C struct for pools of n_pages pages and n_tokens query rows: a
@@ -1082,7 +1087,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     token-major pool; Hq a multiple of Hkv.  A token at position p sees rows
     j <= p; with ``window`` of these the last ``window`` and the first
     ``sinks``.  A token that sees no row gets 0 (lse -inf).  ``out`` [N, Hq,
-    D] and ``lse`` f32 [N, Hq] (natural log) may be given; rows behind the
+    D] (the query itself is allowed) and ``lse`` f32 [N, Hq] (natural log) may be given; rows behind the
     last sequence are left as they are in them (unset in a tensor made here).
     Returns out, or (out, lse) with ``lse`` or ``return_lse``."""
     dev = batch.device
@@ -1111,7 +1116,8 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
             raise ValueError(f"lse must be float32 {(N, Hq)} on {dev}, with unit stride on heads")
         l = lse.data_ptr()
     a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, key_pages.data_ptr(),
-                           value_pages.data_ptr(), sp, sh, sr, D ** -0.5 if scale is None else scale, window, sinks,
+                           value_pages.data_ptr(), sp, sh, sr, D ** -0.5 if scale is None else scale,
+                           min(window, _I32_MAX), min(sinks, _I32_MAX),
                            o, o_ts, o_hs, l, l_ts)
     L = _lib.lib()
     ref = ctypes.byref(a)
@@ -1239,7 +1245,7 @@ class PageTable:
         self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
         P = refs.shape[0]
         at = pages.data_ptr(), lens.data_ptr(), refs.data_ptr()
-        self.args = PageTableArgs(at[0], stride, at[1], at[2], S, M, P, self.page_size)
+        self.args = PageTableArgs(at[0], stride, at[1], at[2], S, M, P, min(self.page_size, _I32_MAX))
         self.work_bytes = {}   # workspace of each operation: depends on the sizes alone
         n = max(S - 1, 0) * stride + M if S else 0   # the memory the three take
         self.spans = [(at[0], at[0] + 4 * n), (at[1], at[1] + 4 * S), (at[2], at[2] + 4 * P)]

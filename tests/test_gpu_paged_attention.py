@@ -458,3 +458,24 @@ def test_a_batch_serves_pools_of_its_own_sizes(ops):
     two = b.bind(9, 16, 3)
     assert (one.n_pages, one.page_size, one.n_tokens) == (5, 8, 1)
     assert (two.n_pages, two.page_size, two.n_tokens) == (9, 16, 3)
+
+
+def test_numbers_past_32_bits(ops):
+    """Windows, sinks and bounds are not taken modulo 2^32."""
+    x = make([90, 40], [1, 30], 1, 2, 64, 8, HF)
+    want = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x))
+    b = ops.PagedBatch(x["table"], x["lens"], x["start"], 2 ** 32 + 1, max_len=2 ** 32 + 1)
+    assert torch.equal(ops.paged_attention(x["q"], x["k"], x["v"], b, window=2 ** 32 + 5, sinks=2 ** 33), want)
+    assert torch.equal(ops.paged_attention(x["q"], x["k"], x["v"], b, window=10, sinks=2 ** 32 + 1),
+                       ops.paged_attention(x["q"], x["k"], x["v"], b, window=10, sinks=90))
+    with pytest.raises(ValueError, match="no columns"):
+        ops.PagedBatch(x["table"][:, :0], x["lens"], x["start"], 1)
+
+
+def test_out_may_be_the_queries(ops):
+    for lens, news in (([700, 30], [1, 1]), ([3000, 300], [150, 300])):
+        x = make(lens, news, 2, 4, 128, 16, BF)
+        want = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x))
+        q = x["q"].clone()
+        assert ops.paged_attention(q, x["k"], x["v"], batch_of(ops, x), out=q) is q
+        assert torch.equal(q, want)
