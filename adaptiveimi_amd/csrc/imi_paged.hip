@@ -1266,26 +1266,34 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         }
                         const float mc = m == -INFINITY ? 0.0f : m * a.c;
                         float ls[2] = {0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
+                        // weights 2 i, 2 i + 1 of the lane's 32; those of the next
+                        // 16 rows between the matrix instructions of these (one
+                        // percent of a chunk's time)
+                        auto weigh = [&](int i) {
                             const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], a.c, -mc));
                             const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], a.c, -mc));
                             pf[i >> 2][i & 3] = T::pack(w0, w1);
                             ls[0] += w0;
                             ls[1] += w1;
+                        };
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) weigh(i);
+                        order();
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+                            for (int d = 0; d < DB; ++d) {
+                                const int n = 2 * KK + DB * x + d;
+                                acc[d] = T::mma32(fr[n % NF], pf[x], acc[d]);
+                                if (n + NF < 2 * KK + 4 * DB) fr[n % NF] = frag(n + NF);
+                                if (x < 3) {
+#pragma unroll
+                                    for (int k = 0; k < 4 / DB; ++k) weigh(4 * (x + 1) + (4 / DB) * d + k);
+                                }
+                                order();
+                            }
                         }
                         l += ls[0] + ls[1];
-                    }
-                    order();
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-#pragma unroll
-                        for (int d = 0; d < DB; ++d) {
-                            const int n = 2 * KK + DB * x + d;
-                            acc[d] = T::mma32(fr[n % NF], pf[x], acc[d]);
-                            if (n + NF < 2 * KK + 4 * DB) fr[n % NF] = frag(n + NF);
-                            order();
-                        }
                     }
                 }
             }
