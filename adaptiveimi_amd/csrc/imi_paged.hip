@@ -816,7 +816,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
 // A CU's eight waves have its registers (acc, scores, queries: 245 of 256) and
 // LDS to themselves.  Bound by matrix and vector instructions together (49 and
 // 58 percent of a SIMD's time): 8192 tokens of 32 heads over 32768 rows take
-// 3.9-4.1 ms, 940-980 TFLOP/s (a large matrix product runs at 1381).  Without
+// 3.85-4.0 ms, 960-1000 TFLOP/s (a large matrix product runs at 1381).  Without
 // the staging the same loop runs at 1190, without the softmax at 1100.  Tiles
 // of 128 rows read K and V twice as often and were slower, 64 rows per wave
 // (half as many reads of LDS) no faster.
@@ -1267,8 +1267,9 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         const float mc = m == -INFINITY ? 0.0f : m * a.c;
                         float ls[2] = {0.0f, 0.0f};
                         // weights 2 i, 2 i + 1 of the lane's 32; those of the next
-                        // 16 rows between the matrix instructions of these (one
-                        // percent of a chunk's time)
+                        // 16 rows come between the matrix instructions of these, in
+                        // the compiler's order (1 percent of a chunk's time, 2 more
+                        // of a mixed batch than in this one's)
                         auto weigh = [&](int i) {
                             const float w0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], a.c, -mc));
                             const float w1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], a.c, -mc));
@@ -1290,7 +1291,6 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
                                     for (int k = 0; k < 4 / DB; ++k) weigh(4 * (x + 1) + (4 / DB) * d + k);
                                 }
-                                order();
                             }
                         }
                         l += ls[0] + ls[1];
