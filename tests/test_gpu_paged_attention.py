@@ -479,3 +479,17 @@ def test_out_may_be_the_queries(ops):
         q = x["q"].clone()
         assert ops.paged_attention(q, x["k"], x["v"], batch_of(ops, x), out=q) is q
         assert torch.equal(q, want)
+
+
+@pytest.mark.parametrize("S,long", [(600, 0), (1100, 700)])
+def test_many_sequences_of_many_rows(ops, S, long):
+    """More tiles than a workgroup plans for itself, more sequences than a
+    workgroup has threads; one sequence of many tiles among them."""
+    g = torch.Generator().manual_seed(S)
+    news = torch.randint(0, 11, (S,), generator=g).tolist()
+    lens = [n + int(torch.randint(0, 14, (), generator=g)) for n in news]
+    if long:
+        news[S // 2], lens[S // 2] = long, long + 300
+    x = make(lens, news, 1, 4, 64, 8, BF, seed=2)
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), return_lse=True)
+    check(x, out, lse)
