@@ -22,10 +22,18 @@
 // the window of the tile's first token.
 //
 // Softmax statistics and sums are fp32 in base 2; P is rounded to the cache's
-// type for the matrix instruction (half a step of that type relative to each
-// weight, the rounding that the output itself takes), unnormalised and at
-// most 2^8: the running maximum moves only when it grows by more than 8 in
-// base 2, which leaves the sums exact to fp32 and saves most rescalings.
+// type for the matrix instruction, unnormalised (half a step of that type
+// relative to each weight, the rounding that the output itself takes: bf16
+// outputs are 2.0e-3 off where an fp32 P leaves 1.7e-3, and P in two halves
+// would take the matrix instructions of the second product twice).  The running
+// maximum moves only when it grows by more than kSlack in base 2, which leaves
+// the sums exact to fp32 and saves most rescalings; a row's largest weight lies
+// in 2^kShift .. 2^(kShift + kSlack).  bf16 has fp32's range (shift 0, slack 8).
+// fp16 has steps of 2^-24 under 2^-14, so its weights use the range up to 2^15
+// (shift 11, slack 4): one under 2^-25 of the largest is off by at most 2^-36 of
+// it, and 131072 rows of such weights, which one row outweighs, by 2^-19 in all
+// (unshifted they would be lost: 2^-25 of it each, 2^-8 in all).  Either way 8192
+// fp16 tokens over 32768 rows take 3.91-4.0 ms.
 #include <algorithm>
 
 #include "imi_common.hpp"
@@ -73,12 +81,14 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kSlack = 8.0f;   // growth of a running maximum (base 2) that is left unapplied
 
-// The two element types: pairs rounded to nearest even, matrix instructions.
+// The two element types: pairs rounded to nearest even, matrix instructions;
+// kShift: base 2 exponent of the weight of a row at the running maximum, kSlack:
+// growth of a running maximum (base 2) that is left unapplied.
 struct BF16 {
     typedef bf16x8_t v8;
     static constexpr uint32_t kExp = 0x7F80;
+    static constexpr float kShift = 0.0f, kSlack = 8.0f;
     static __device__ __forceinline__ float wide(uint32_t h) { return __uint_as_float(h << 16); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         typedef __attribute__((ext_vector_type(2))) float f2;
@@ -95,6 +105,7 @@ struct BF16 {
 struct FP16 {
     typedef f16x8_t v8;
     static constexpr uint32_t kExp = 0x7C00;
+    static constexpr float kShift = 11.0f, kSlack = 4.0f;
     static __device__ __forceinline__ float wide(uint32_t h) {
         return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
     }
@@ -280,6 +291,12 @@ __device__ __forceinline__ void patch_rows(const PagedParams& a, const Seq& sq, 
 
 __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
+}
+
+// ln sum exp of a row: maximum M, sum L of its weights.
+template <typename T>
+__device__ __forceinline__ float log_sum(float M, float L, float c) {
+    return L == 0.0f ? -INFINITY : (M * c + (__log2f(L) - T::kShift)) * kLn2;
 }
 
 // ---------------------------------------------------------- few rows ------
@@ -552,7 +569,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[b][e][i]);
                 mx = fmaxf(mx, xor16(mx));
                 mx = fmaxf(mx, xor32(mx));
-                const bool grow = (mx - m[b]) * a.c > kSlack;
+                const bool grow = (mx - m[b]) * a.c > T::kSlack;
                 if (__builtin_amdgcn_ballot_w64(grow)) {
                     const float f = grow ? __builtin_amdgcn_exp2f((m[b] - mx) * a.c) : 1.0f;
                     m[b] = grow ? mx : m[b];
@@ -560,7 +577,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
                     for (int d = 0; d < DB; ++d) acc[b][d] *= f;
                 }
-                const float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+                const float mc = (m[b] == -INFINITY ? 0.0f : m[b] * a.c) - T::kShift;
                 float p[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -626,7 +643,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                     o.y = T::pack(A[2] * inv, A[3] * inv);
                     *reinterpret_cast<uint2*>(a.out + t * a.o_ts + x_head * a.o_hs + 4 * d4) = o;
                     if (a.lse && d4 == 0)
-                        a.lse[t * a.l_ts + x_head] = L == 0.0f ? -INFINITY : (M * a.c + __log2f(L)) * kLn2;
+                        a.lse[t * a.l_ts + x_head] = log_sum<T>(M, L, a.c);
                 } else {
                     *reinterpret_cast<f32x4_t*>(a.part + (slot * a.cap + r) * D + 4 * d4) = A;
                     if (d4 == 0) {
@@ -715,7 +732,7 @@ struct Partial {
         o.x = T::pack(A[0] * inv, A[1] * inv);
         o.y = T::pack(A[2] * inv, A[3] * inv);
         *reinterpret_cast<uint2*>(a.out + tok * a.o_ts + head * a.o_hs + 4 * d4) = o;
-        if (a.lse && d4 == 0) a.lse[tok * a.l_ts + head] = L == 0.0f ? -INFINITY : (M * a.c + __log2f(L)) * kLn2;
+        if (a.lse && d4 == 0) a.lse[tok * a.l_ts + head] = log_sum<T>(M, L, a.c);
     }
 };
 
@@ -1256,7 +1273,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
                         for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sc[i >> 4][i & 15]);
                         mx = fmaxf(mx, xor32(mx));
-                        const bool grow = (mx - m) * a.c > kSlack;
+                        const bool grow = (mx - m) * a.c > T::kSlack;
                         if (__builtin_amdgcn_ballot_w64(grow)) {
                             const float f = grow ? __builtin_amdgcn_exp2f((m - mx) * a.c) : 1.0f;
                             m = grow ? mx : m;
@@ -1264,7 +1281,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
                             for (int d = 0; d < DB; ++d) acc[d] *= f;
                         }
-                        const float mc = m == -INFINITY ? 0.0f : m * a.c;
+                        const float mc = (m == -INFINITY ? 0.0f : m * a.c) - T::kShift;
                         float ls[2] = {0.0f, 0.0f};
                         // weights 2 i, 2 i + 1 of the lane's 32; those of the next
                         // 16 rows come between the matrix instructions of these, in
@@ -1313,7 +1330,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         *reinterpret_cast<uint2*>(op + 32 * d + 8 * i) = o;
                     }
                 if (a.lse && hi == 0)
-                    a.lse[q_tok * a.l_ts + x_head] = l == 0.0f ? -INFINITY : (m * a.c + __log2f(l)) * kLn2;
+                    a.lse[q_tok * a.l_ts + x_head] = log_sum<T>(m, l, a.c);
             } else {
                 const int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
                 float* const op = a.part + e * D + 4 * hi;

@@ -493,3 +493,30 @@ def test_many_sequences_of_many_rows(ops, S, long):
     x = make(lens, news, 1, 4, 64, 8, BF, seed=2)
     out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), return_lse=True)
     check(x, out, lse)
+
+
+@pytest.mark.parametrize("n,news,H", [(700, 1, 1), (700, 5, 1), (6000, 3, 4), (600, 70, 1), (6000, 70, 2)])
+@pytest.mark.parametrize("first", [1.6, 2.2, 2.5])
+def test_many_small_weights_in_half_precision(ops, n, news, H, first):
+    """One row without a value outweighs every other by 2^18, 2^25 or 2^29;
+    what the others hold is the output.  A weight far under fp16's range keeps
+    an absolute 2^-36 of the largest, not the 2^-25 that expected() allows."""
+    G, D = 4, 64
+    x = make([n], [news], H, G, D, 0, HF, slack=0)
+    g = torch.Generator().manual_seed(12)
+    k, v = x["rows"][0]
+    k.copy_(0.05 * torch.randn(k.shape, generator=g))
+    v.copy_(64.0 + 32.0 * torch.randn(v.shape, generator=g))
+    q = (1.0 + 0.05 * torch.randn((news, H * G, D), generator=g)).to(HF)
+    k[:, 0], v[:, 0] = first, 0.0      # scores 64 first / 8 above the others'
+    x["k"][0], x["v"][0] = k.to(DEV), v.to(DEV)
+    x["q"], x["q64"] = q.to(DEV), q.double()
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), return_lse=True)
+    want, want_lse, tol, ltol, _ = expected(x)
+    last = [n - news + i for i in range(news)]
+    seen = torch.stack([v[:, :p + 1].double().abs().sum(1) for p in last]).repeat_interleave(G, 1)
+    tol = tol - (2.0 ** -25 - 2.0 ** -36) * seen
+    assert tol.min() > 0 and (want.abs() > 8 * tol).any()
+    err = (out.double().cpu() - want).abs()
+    assert torch.all(err <= tol), f"{err.max()} (worst excess {(err - tol).max()})"
+    assert torch.all((lse.double().cpu() - want_lse).abs() <= ltol)
