@@ -293,6 +293,13 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
 }
 
+// What a row's sum L of weights divides by.  No weight: the row sees nothing
+// (blind) and gets 0, or all that it sees has a score of -infinity and 0 / 0 is
+// NaN, as for a NaN among them.
+__device__ __forceinline__ float inverse(float L, bool blind) {
+    return L == 0.0f ? (blind ? 0.0f : __builtin_nanf("")) : 1.0f / L;
+}
+
 // ln sum exp of a row: maximum M, sum L of its weights.
 template <typename T>
 __device__ __forceinline__ float log_sum(float M, float L, float c) {
@@ -336,6 +343,7 @@ struct Join {
     int t0;             // the sequence's first query row
     int first, end;     // rows (token, head of the group) [first, end)
     int h;
+    int blind;          // the sequence's rows before this one see nothing (more new tokens than rows)
 };
 __device__ __forceinline__ int ranges_log(int w_log, int64_t total) {
     return total <= 1 ? 0 : min(w_log, 64 - __builtin_clzll(static_cast<uint64_t>(total - 1)));
@@ -431,7 +439,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     int s = range.s;
     int64_t base = range.before * a.H;   // units before sequence s, all heads
     bool first = true;
-    Join rest{0, 0, 0, 0, 0, 0, 0};
+    Join rest{};
     while (g0 < g1) {
         const Seq sq = seq_of(a, s);
         const int units = few_units(a, sq);
@@ -635,7 +643,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                          wt;
                 }
                 if (whole) {
-                    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+                    const float inv = inverse(L, p0 + r / a.G < 0);
                     const int64_t t = sq.t0 + r / a.G;
                     const int x_head = h * a.G + r % a.G;
                     uint2 o;
@@ -663,7 +671,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             __syncthreads();
         }
         if (u0 == 0 && u1 < units)
-            rest = Join{range.total, g0, g0 + units, sq.t0, 0, rows, h};
+            rest = Join{range.total, g0, g0 + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G};
         g0 += u1 - u0;
         first = false;
     }
@@ -727,7 +735,7 @@ struct Partial {
     __device__ __forceinline__ void write(const MergeParams& a, const Join& j, int row, int d4) const {
         const int64_t tok = j.t0 + row / a.G;
         const int head = j.h * a.G + row % a.G;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const float inv = inverse(L, row < j.blind);
         uint2 o;
         o.x = T::pack(A[0] * inv, A[1] * inv);
         o.y = T::pack(A[2] * inv, A[3] * inv);
@@ -1107,7 +1115,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     int64_t g0 = used ? cut(total, wg, log) : 0;
     const int64_t g1 = used ? cut(total, wg + 1, log) : 0;
     bool first = true;
-    Join rest{0, 0, 0, 0, 0, 0, 0};
+    Join rest{};
     int h = static_cast<int>(g0 / per_head);
     int t = g0 < g1 ? find_tile(steps, n_tiles, g0 - h * per_head) : 0;
     while (g0 < g1) {
@@ -1318,7 +1326,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         l += xor32(l);
         if (live) {
             if (u0 == 0 && u1 == units) {
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = inverse(l, pos < 0);
                 uint16_t* const op = a.out + q_tok * a.o_ts + x_head * a.o_hs + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
@@ -1357,7 +1365,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         }
         turn ^= 1;
         if (u0 == 0 && u1 < units)
-            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, t_end, h};
+            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, t_end, h, max(-p0, 0) * a.G};
         g0 += u1 - u0;
         first = false;
         if (++t == n_tiles) {

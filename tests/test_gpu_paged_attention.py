@@ -520,3 +520,25 @@ def test_many_small_weights_in_half_precision(ops, n, news, H, first):
     err = (out.double().cpu() - want).abs()
     assert torch.all(err <= tol), f"{err.max()} (worst excess {(err - tol).max()})"
     assert torch.all((lse.double().cpu() - want_lse).abs() <= ltol)
+
+
+@pytest.mark.parametrize("n,news,D,dtype,window", [
+    (300, 1, 128, BF, 0), (5000, 1, 64, HF, 0), (5000, 5, 128, BF, 0), (40, 45, 64, BF, 0), (3, 6, 128, HF, 0),
+    (900, 70, 128, BF, 0), (900, 150, 64, HF, 50), (70, 90, 64, BF, 0),
+])
+def test_scores_of_minus_infinity(ops, n, news, D, dtype, window):
+    """Softmax over scores that are all -infinity is 0 / 0: NaN, not the zeros of a
+    token that sees nothing."""
+    G = 4
+    x = make([n], [news], 2, G, D, 0, dtype, slack=0)
+    k = x["k"].clone()
+    k[..., 0] = -1.0
+    q = x["q"].clone()
+    hit = torch.zeros((news, 2 * G), dtype=torch.bool, device=DEV)
+    hit[::3, ::2] = True
+    q[..., 0] = torch.where(hit, math.inf, q[..., 0])
+    out, lse = ops.paged_attention(q, k, x["v"], batch_of(ops, x), window=window, return_lse=True)
+    none = (torch.arange(news, device=DEV) < news - n)[:, None].expand_as(hit)
+    assert torch.all(out[none] == 0) and torch.all(lse[none] == -math.inf)
+    assert torch.isnan(out[hit & ~none]).all() and torch.all(lse[hit & ~none] == -math.inf)
+    assert torch.isfinite(out[~hit]).all()
