@@ -81,6 +81,13 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// A weight is 2^(s c - m c) in one fma, whose m c is rounded: a common factor of
+// the weights of one maximum, of up to half a step of m c in base 2.  Past 2^12
+// (a factor of 1 + 2^-13) the maximum is subtracted from the scores instead, which
+// is exact next to it: from 2^24 on the factor could leave fp16's range, from 2^31
+// on fp32's (keys padded with the type's lowest value have such scores), and
+// before that it differs between the maxima that are joined.
+constexpr float kFar = 4096.0f;
 
 // The two element types: pairs rounded to nearest even, matrix instructions;
 // kShift: base 2 exponent of the weight of a row at the running maximum, kSlack:
@@ -303,7 +310,7 @@ __device__ __forceinline__ float inverse(float L, bool blind) {
 // ln sum exp of a row: maximum M, sum L of its weights.
 template <typename T>
 __device__ __forceinline__ float log_sum(float M, float L, float c) {
-    return L == 0.0f ? -INFINITY : (M * c + (__log2f(L) - T::kShift)) * kLn2;
+    return L == 0.0f ? -INFINITY : M * (c * kLn2) + (__log2f(L) - T::kShift) * kLn2;   // (M c may be past fp32)
 }
 
 // ---------------------------------------------------------- few rows ------
@@ -585,7 +592,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
                     for (int d = 0; d < DB; ++d) acc[b][d] *= f;
                 }
-                const float mc = (m[b] == -INFINITY ? 0.0f : m[b] * a.c) - T::kShift;
+                float mc = m[b] == -INFINITY ? 0.0f : m[b] * a.c;
+                if (__builtin_amdgcn_ballot_w64(fabsf(mc) > kFar)) {
+                    const float off = fabsf(mc) > kFar ? m[b] : 0.0f;
+                    mc = fabsf(mc) > kFar ? 0.0f : mc;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sc[b][i >> 2][i & 3] -= off;
+                }
+                mc -= T::kShift;
                 float p[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -1289,7 +1303,14 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
                             for (int d = 0; d < DB; ++d) acc[d] *= f;
                         }
-                        const float mc = (m == -INFINITY ? 0.0f : m * a.c) - T::kShift;
+                        float mc = m == -INFINITY ? 0.0f : m * a.c;
+                        if (__builtin_amdgcn_ballot_w64(fabsf(mc) > kFar)) {
+                            const float off = fabsf(mc) > kFar ? m : 0.0f;
+                            mc = fabsf(mc) > kFar ? 0.0f : mc;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] -= off;
+                        }
+                        mc -= T::kShift;
                         float ls[2] = {0.0f, 0.0f};
                         // weights 2 i, 2 i + 1 of the lane's 32; those of the next
                         // 16 rows come between the matrix instructions of these, in

@@ -542,3 +542,48 @@ def test_scores_of_minus_infinity(ops, n, news, D, dtype, window):
     assert torch.all(out[none] == 0) and torch.all(lse[none] == -math.inf)
     assert torch.isnan(out[hit & ~none]).all() and torch.all(lse[hit & ~none] == -math.inf)
     assert torch.isfinite(out[~hit]).all()
+
+
+@pytest.mark.parametrize("n,news,window", [(300, 1, 0), (5000, 1, 0), (5000, 5, 0), (600, 5, 90), (900, 70, 0), (900, 150, 50)])
+@pytest.mark.parametrize("dtype,size", [(HF, -2.0 ** 13), (HF, 2.0 ** 13), (BF, -2.0 ** 13), (BF, 2.0 ** 13), (BF, -2.0 ** 60),
+                                        (BF, 2.0 ** 60), (HF, None), (BF, None)])
+def test_scores_far_from_zero(ops, n, news, window, dtype, size):
+    """Scores of size^2 plus a few units, or rows padded with the type's lowest
+    value.  Every product and sum of them is exact in fp32, so what is left of the
+    tolerance is the weights' rounding and the output's, and for exponents of up
+    to 24 log2(e) their fp32 rounding (three of 2^-24 relative: 2^-17), the sums'
+    (n 2^-24, twice) and exp2's."""
+    H, G, D = 2, 4, 64
+    x = make([n], [news], H, G, D, 0, dtype, slack=0, seed=3)
+    g = torch.Generator().manual_seed(6)
+    k, v = x["rows"][0]
+    k.zero_()
+    q = torch.zeros((news, H * G, D), dtype=dtype)
+    q[..., 40] = 1.0
+    k[..., 40] = 8.0 * torch.randint(0, 4, (H, n), generator=g)
+    if size is None:     # seven of every ten blocks of 50 rows; not the last
+        q[..., 0] = 255.0 if dtype == HF else 1.0
+        block = torch.arange(n) // 50
+        k[:, (block % 10 < 7) & (block < n // 50 - 1), 0] = torch.finfo(dtype).min
+    else:
+        q[..., 0] = abs(size)
+        k[..., 0] = size
+    if size is not None and abs(size) > 2 ** 20:
+        k[..., 40] = 0.0     # (no sum of these is exact)
+    x["k"][0], x["v"][0] = k.to(DEV), v.to(DEV)
+    x["q"], x["q64"] = q.to(DEV), q.double()
+    out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch_of(ops, x), scale=1.0, window=window, return_lse=True)
+    want, want_lse, _, _, _ = expected(x, window, 0, 1.0)
+    eps = torch.finfo(dtype).eps
+    A = torch.zeros_like(want)
+    for i in range(news):
+        p = n - news + i
+        first = max(0, p - window + 1) if window else 0
+        for h in range(H):
+            w = torch.softmax(x["q64"][i, h * G:(h + 1) * G] @ k[h, first:p + 1].double().T, -1)
+            A[i, h * G:(h + 1) * G] = w @ v[h, first:p + 1].double().abs()
+    tol = (eps / 2 + 2.0 ** -17 + 2 * n * 2.0 ** -24 + 2.0 ** -21) * A + eps / 2 * want.abs() + 1e-6
+    err = (out.double().cpu() - want).abs()
+    assert torch.all(err <= tol), f"{err.max()} (worst excess {(err - tol).max()})"
+    lerr = (lse.double().cpu() - want_lse).abs()
+    assert torch.all(lerr <= 2.0 ** -22 * want_lse.abs() + 2.0 ** -16 + n * 2.0 ** -23)
