@@ -300,12 +300,10 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
 }
 
-// What a row's sum L of weights divides by.  No weight: the row sees nothing
-// (blind) and gets 0, or all that it sees has a score of -infinity and 0 / 0 is
-// NaN, as for a NaN among them.
-__device__ __forceinline__ float inverse(float L, bool blind) {
-    return L == 0.0f ? (blind ? 0.0f : __builtin_nanf("")) : 1.0f / L;
-}
+// What a row's sum L of weights divides by: nothing for a row that sees nothing
+// (blind: 0), and 1 / 0 where all that it sees has a score of -infinity, which
+// makes NaN of its zeros, as 0 / 0 is and as for a NaN among the scores.
+__device__ __forceinline__ float inverse(float L, bool blind) { return blind ? 0.0f : 1.0f / L; }
 
 // ln sum exp of a row: maximum M, sum L of its weights.
 template <typename T>
@@ -1187,6 +1185,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
+        float mc = -T::kShift;   // what a score's exponent loses, and whether a row of the wave is far (kFar)
+        bool far = false;
 
         const uint16_t* const kh = a.k + static_cast<int64_t>(h) * a.head_s;
         const uint16_t* const vh = a.v + static_cast<int64_t>(h) * a.head_s + 8 * st.l_ch;
@@ -1296,21 +1296,22 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         for (int i = 1; i < 32; ++i) mx = fmaxf(mx, sc[i >> 4][i & 15]);
                         mx = fmaxf(mx, xor32(mx));
                         const bool grow = (mx - m) * a.c > T::kSlack;
-                        if (__builtin_amdgcn_ballot_w64(grow)) {
+                        if (far || __builtin_amdgcn_ballot_w64(grow)) {
                             const float f = grow ? __builtin_amdgcn_exp2f((m - mx) * a.c) : 1.0f;
                             m = grow ? mx : m;
                             l *= f;
 #pragma unroll
                             for (int d = 0; d < DB; ++d) acc[d] *= f;
-                        }
-                        float mc = m == -INFINITY ? 0.0f : m * a.c;
-                        if (__builtin_amdgcn_ballot_w64(fabsf(mc) > kFar)) {
-                            const float off = fabsf(mc) > kFar ? m : 0.0f;
-                            mc = fabsf(mc) > kFar ? 0.0f : mc;
+                            mc = m == -INFINITY ? 0.0f : m * a.c;
+                            far = __builtin_amdgcn_ballot_w64(fabsf(mc) > kFar) != 0;
+                            if (far) {
+                                const float off = fabsf(mc) > kFar ? m : 0.0f;
+                                mc = fabsf(mc) > kFar ? 0.0f : mc;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] -= off;
+                                for (int i = 0; i < 32; ++i) sc[i >> 4][i & 15] -= off;
+                            }
+                            mc -= T::kShift;
                         }
-                        mc -= T::kShift;
                         float ls[2] = {0.0f, 0.0f};
                         // weights 2 i, 2 i + 1 of the lane's 32; those of the next
                         // 16 rows come between the matrix instructions of these, in
