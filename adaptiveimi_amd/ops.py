@@ -1004,7 +1004,9 @@ def _rows(name: str, t: torch.Tensor, shape, dtype: torch.dtype, dev: torch.devi
     return t.data_ptr(), st, sh
 
 
-_I32_MAX = 2 ** 31 - 1   # (a C int takes more than that modulo 2^32)
+def _c_int(x: int) -> int:
+    """x as a C int, which takes it modulo 2^32: the nearest it can hold."""
+    return max(-2 ** 31, min(x, 2 ** 31 - 1))
 
 
 class PagedBatch:
@@ -1044,7 +1046,7 @@ class PagedBatch:
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
-                                   min(self.max_query, _I32_MAX), min(max_len or 0, _I32_MAX))
+                                   _c_int(self.max_query), _c_int(max_len or 0))
 
     def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
         """The C struct for pools of n_pages pages and n_tokens query rows: a
@@ -1117,7 +1119,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         l = lse.data_ptr()
     a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, key_pages.data_ptr(),
                            value_pages.data_ptr(), sp, sh, sr, D ** -0.5 if scale is None else scale,
-                           min(window, _I32_MAX), min(sinks, _I32_MAX),
+                           _c_int(window), _c_int(sinks),
                            o, o_ts, o_hs, l, l_ts)
     L = _lib.lib()
     ref = ctypes.byref(a)
@@ -1245,7 +1247,7 @@ class PageTable:
         self.pages, self.lens, self.refs, self.page_size, self.device = pages, lens, refs, int(page_size), dev
         P = refs.shape[0]
         at = pages.data_ptr(), lens.data_ptr(), refs.data_ptr()
-        self.args = PageTableArgs(at[0], stride, at[1], at[2], S, M, P, min(self.page_size, _I32_MAX))
+        self.args = PageTableArgs(at[0], stride, at[1], at[2], S, M, P, _c_int(self.page_size))
         self.work_bytes = {}   # workspace of each operation: depends on the sizes alone
         n = max(S - 1, 0) * stride + M if S else 0   # the memory the three take
         self.spans = [(at[0], at[0] + 4 * n), (at[1], at[1] + 4 * S), (at[2], at[2] + 4 * P)]

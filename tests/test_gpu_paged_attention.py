@@ -587,3 +587,25 @@ def test_scores_far_from_zero(ops, n, news, window, dtype, size):
     assert torch.all(err <= tol), f"{err.max()} (worst excess {(err - tol).max()})"
     lerr = (lse.double().cpu() - want_lse).abs()
     assert torch.all(lerr <= 2.0 ** -22 * want_lse.abs() + 2.0 ** -16 + n * 2.0 ** -23)
+
+
+def test_numbers_under_32_bits(ops):
+    """Nor are negative ones: they are refused as -1 is, and a hint is none."""
+    from adaptiveimi_amd._lib import IMIError
+
+    x = make([90, 40], [1, 30], 1, 2, 64, 8, HF)
+    b = batch_of(ops, x)
+    call = lambda b, **kw: ops.paged_attention(x["q"], x["k"], x["v"], b, **kw)
+    for n in (-1, -2 ** 31, -2 ** 32 + 5, -2 ** 33):
+        for kw in (dict(window=n), dict(window=9, sinks=n)):
+            with pytest.raises(IMIError, match="must be >= 0"):
+                call(b, **kw)
+        with pytest.raises(IMIError, match="max_query"):
+            call(ops.PagedBatch(x["table"], x["lens"], x["start"], n))
+        assert torch.equal(call(ops.PagedBatch(x["table"], x["lens"], x["start"], 30, max_len=n)), call(b))
+        table = ops.PageTable(x["table"], x["lens"], torch.zeros((9,), dtype=torch.int32, device=DEV), n)
+        counts = torch.ones((2,), dtype=torch.int32, device=DEV)
+        for f in (lambda: ops.fork_pages(table, counts), lambda: ops.extend_pages(table, counts),
+                  lambda: ops.compact_pages(table)):
+            with pytest.raises(IMIError, match="page_size"):
+                f()

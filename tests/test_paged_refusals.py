@@ -201,3 +201,13 @@ def test_attention_splits_more_heads_than_a_launch_has_workgroups(L):
         a = attention(batch(n_seqs=n, n_tokens=n, **short))
         assert L.imi_paged_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)) == 0
         assert (need.value > 0) == shared
+
+
+def test_c_ints_are_not_taken_modulo():
+    from adaptiveimi_amd import ops
+
+    for x in (0, 1, -1, 2 ** 31 - 1, -2 ** 31):
+        assert ctypes.c_int32(ops._c_int(x)).value == x
+    for x in (2 ** 31, 2 ** 32 + 5, 2 ** 64):
+        assert ctypes.c_int32(ops._c_int(x)).value == 2 ** 31 - 1
+        assert ctypes.c_int32(ops._c_int(-x + 5 if x > 2 ** 31 else -x - 1)).value == -2 ** 31
