@@ -1024,7 +1024,8 @@ class PagedBatch:
     longest sequence (default: what the table holds); only the split of short
     batches depends on it."""
 
-    __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device")
+    __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device", "pool_pages",
+                 "page_size")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
@@ -1045,6 +1046,7 @@ class PagedBatch:
             table, stride = page_table.data_ptr(), page_table.stride(0) if S > 1 else cols
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
+        self.pool_pages, self.page_size = 0, None   # what a PageTable knows of the pools
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
                                    _c_int(self.max_query), _c_int(max_len or 0))
 
@@ -1071,6 +1073,9 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch
     P, H, page, _ = key_pages.shape
     if batch.page_table is None and P < batch.args.n_seqs:
         raise ValueError(f"{P} sets of contiguous rows for {batch.args.n_seqs} sequences")
+    if batch.page_size is not None and (page != batch.page_size or P < batch.pool_pages):
+        raise ValueError(f"{P} pages of {page} rows under a table of {batch.pool_pages} pages of {batch.page_size} rows "
+                         "(a token-major pool is given as pool.transpose(1, 2))")
     sp, sh, sr, _ = _steps(key_pages)
     return P, H, page, sp, sh, sr
 
@@ -1261,8 +1266,11 @@ class PageTable:
 
     def batch(self, query_start: torch.Tensor, max_query: int, max_len: Optional[int] = None) -> PagedBatch:
         """The batch whose new tokens are the last rows of each sequence
-        (after extend_pages)."""
-        return PagedBatch(self.pages, self.lens, query_start, max_query, max_len)
+        (after extend_pages).  Pools have to have the table's page size and
+        its pages."""
+        b = PagedBatch(self.pages, self.lens, query_start, max_query, max_len)
+        b.pool_pages, b.page_size = self.args.n_pages, self.page_size
+        return b
 
 
 def _table_work(table: PageTable, L, what: str) -> torch.Tensor:

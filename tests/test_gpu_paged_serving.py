@@ -131,3 +131,24 @@ def test_chunks_decode_beams_and_compaction(ops, page, Hq, Hk, D, dtype, window,
     s.fork([-1, 1, -1, -1])
     s.compact()
     s.step([90, 1, 40, 2])
+
+
+def test_a_batch_of_a_table_knows_its_pages(ops):
+    """Pools of another page size, as a token-major pool that is not transposed
+    looks like, and of fewer pages than the table's are refused."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    table = ops.PageTable.empty(2, 4, 12, 16, DEV)
+    pool = torch.randn((12, 16, 8, 64), device=DEV).to(torch.bfloat16)      # token-major, pages of 16 rows, 8 heads
+    assert ops.extend_pages(table, i32([20, 3]), [pool]).all()
+    batch = table.batch(i32([0, 1, 2]), max_query=1)
+    q = torch.randn((2, 32, 64), device=DEV).to(torch.bfloat16)
+    k = q[:, :8]
+    good = pool.transpose(1, 2)
+    out = ops.paged_attention(q, good, good, batch)
+    for bad, heads in ((pool, 16), (good[:11], 8)):
+        with pytest.raises(ValueError, match="pages of 16 rows"):
+            ops.paged_attention(q, bad, bad, batch)
+        with pytest.raises(ValueError, match="pages of 16 rows"):
+            ops.qk_norm_rope(q, q[:, :heads], value=q[:, :heads], batch=batch, key_pages=bad, value_pages=bad)
+    more = torch.cat([pool, pool]).transpose(1, 2)      # more pages than the table's are never reached
+    assert torch.equal(ops.paged_attention(q, more, more, batch), out)
