@@ -1066,7 +1066,8 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch
         raise TypeError(f"pages are {key_pages.dtype} and {value_pages.dtype}, expected {dtype}")
     if key_pages.dim() != 4 or key_pages.shape[3] != dim or key_pages.stride(3) != 1:
         raise ValueError(f"key_pages must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
-    if value_pages.shape != key_pages.shape or value_pages.stride() != key_pages.stride():
+    steps = _steps(key_pages)
+    if value_pages.shape != key_pages.shape or _steps(value_pages) != steps:
         raise ValueError("key_pages and value_pages must share shape and strides")
     if key_pages.device != batch.device or value_pages.device != batch.device:
         raise ValueError(f"pages are on {key_pages.device} and {value_pages.device}, expected {batch.device}")
@@ -1076,8 +1077,7 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch
     if batch.page_size is not None and (page != batch.page_size or P < batch.pool_pages):
         raise ValueError(f"{P} pages of {page} rows under a table of {batch.pool_pages} pages of {batch.page_size} rows "
                          "(a token-major pool is given as pool.transpose(1, 2))")
-    sp, sh, sr, _ = _steps(key_pages)
-    return P, H, page, sp, sh, sr
+    return (P, H, page) + steps[:3]
 
 
 def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch,

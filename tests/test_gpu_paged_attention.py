@@ -609,3 +609,17 @@ def test_numbers_under_32_bits(ops):
                   lambda: ops.compact_pages(table)):
             with pytest.raises(IMIError, match="page_size"):
                 f()
+
+
+@pytest.mark.parametrize("P,H,page", [(9, 1, 8), (9, 2, 1), (1, 2, 64)])
+def test_keys_and_values_of_one_layout(ops, P, H, page):
+    """Strides of a dimension with one entry are torch's to choose: a head-major
+    key pool and a token-major value pool of one head are the same layout."""
+    g = torch.Generator(device=DEV).manual_seed(1)
+    k, v = (torch.randn((P, H, page, 64), generator=g, device=DEV).to(BF) for _ in range(2))
+    other = v.as_strided(v.shape, [s if n > 1 else 8 for s, n in zip(v.stride(), v.shape)])
+    assert other.stride() != k.stride()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    b = ops.PagedBatch(i32([list(range(P))]), i32([P * page - 1]), i32([0, 1]), 1)
+    q = torch.randn((1, 2, 64), generator=g, device=DEV).to(BF)
+    assert torch.equal(ops.paged_attention(q, k, other, b), ops.paged_attention(q, k, v, b))
