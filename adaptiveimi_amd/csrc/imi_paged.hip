@@ -414,7 +414,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     constexpr int LR = kRow<D>;
     constexpr int CH = D / 8, NV = kFewTile * CH / 64;   // 16-byte pieces of a row, loads of a tile of V
     constexpr int kWaveLds = kFewTile * LR > 16 * D * 2 ? kFewTile * LR : 16 * D * 2;   // u16
-    __shared__ uint16_t s_buf[kFewWaves * kWaveLds];
+    __shared__ __align__(16) uint16_t s_buf[kFewWaves * kWaveLds];
+    static_assert(__alignof__(s_buf) >= 16 && kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0,
+                  "rows and partials are read and written 16 bytes at a time");
     __shared__ float s_ml[kFewWaves][16 * NB][2];
     __shared__ int s_odd;   // a masked tile held infinities or NaN
     // Queries: in registers, but for two blocks of 128 dims (32 registers more
@@ -773,7 +775,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
     constexpr int Q = D / 4, P = kMergeThreads / Q;
     __shared__ float s_ml[P][2];
-    __shared__ float s_acc[P][D];
+    __shared__ __align__(16) float s_acc[P][D];
+    static_assert(__alignof__(s_acc) >= 16 && D * 4 % 16 == 0, "rows are read and written 16 bytes at a time");
     __shared__ int s_range[kMaxRanges];
     __shared__ int s_n[kMergeThreads / 64];
     const int tid = threadIdx.x, W = 1 << a.w_log;
@@ -1096,6 +1099,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     char* const s_v = s_stage + 4 * SB;
     // a masked step held infinities or NaN: this tile's word and the next one's
     int* const s_odd = reinterpret_cast<int*>(s_stage + 8 * SB);
+    static_assert(__alignof__(s_stage) >= 16 && SB % 16 == 0, "read and written 16 bytes at a time");
     int turn = 0;
     if (threadIdx.x == 0) s_odd[0] = 0;
     Stage<D> st;
