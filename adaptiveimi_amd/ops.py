@@ -1234,7 +1234,12 @@ class PageTable:
     pages int32 [S, max_pages]: sequence s holds its first ceil(lens[s] /
     page_size) entries; lens int32 [S]; refs int32 [n_pages]: sequences that
     hold each page (0: free).  fork_pages, extend_pages and compact_pages work
-    on it without a host synchronisation and can be captured in a graph."""
+    on it without a host synchronisation and can be captured in a graph.
+
+    The caller may change the three as long as refs counts what lens and pages
+    say.  Rows taken back (drafted tokens that were not accepted) are a smaller
+    entry of lens; where it then holds fewer pages, refs of the others goes
+    down by one each, or they stay taken for good."""
 
     __slots__ = ("pages", "lens", "refs", "page_size", "args", "device", "spans", "work_bytes")
 

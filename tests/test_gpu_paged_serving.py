@@ -152,3 +152,71 @@ def test_a_batch_of_a_table_knows_its_pages(ops):
             ops.qk_norm_rope(q, q[:, :heads], value=q[:, :heads], batch=batch, key_pages=bad, value_pages=bad)
     more = torch.cat([pool, pool]).transpose(1, 2)      # more pages than the table's are never reached
     assert torch.equal(ops.paged_attention(q, more, more, batch), out)
+
+
+def take_back(table, rejected):
+    """Rows that verification rejected, as the integration notes give it."""
+    page, cols = table.page_size, torch.arange(table.pages.shape[1], device=table.device)
+    held = lambda lens: ((lens + page - 1) // page)[:, None]
+    lens = (table.lens - rejected).clamp_(min=0)
+    drop = (cols >= held(lens)) & (cols < held(table.lens))
+    table.refs.scatter_add_(0, table.pages.clamp(min=0).flatten().long(), -drop.flatten().int())
+    table.lens.copy_(lens)
+
+
+def counted(table):
+    """What refs has to be."""
+    refs = [0] * table.refs.shape[0]
+    for row, n in zip(table.pages.tolist(), table.lens.tolist()):
+        for p in row[:-(-n // table.page_size)]:
+            refs[p] += 1
+    return refs
+
+
+@pytest.mark.parametrize("page,dtype", [(4, torch.bfloat16), (16, torch.float16)])
+def test_drafted_tokens_taken_back(ops, page, dtype):
+    """Drafts verified and taken back across page borders, by sequences that
+    share pages too: no page is lost, rows that stayed are the bits that were
+    stored, and nobody writes into a page that another sequence holds."""
+    s = Server(ops, 4, 256 // page, 900 // page, page, 4, 2, 64, dtype)
+    s.step([50, 17, 0, 1])
+    s.fork([0, 0, 1, 3])
+    for news, rejected in (([5, 5, 5, 5], [5, 3, 0, 4]), ([9, 2, 7, 1], [8, 2, 1, 0]), ([1, 1, 1, 1], [0, 0, 0, 0]),
+                           ([6, 6, 6, 6], [20, 6, 11, 9]), ([7, 5, 3, 2], [40, 0, 3, 9])):
+        s.step(news)
+        take_back(s.tables[0], s.i32(rejected))
+        s.lens = [max(n - r, 0) for n, r in zip(s.lens, rejected)]
+        s.hist = [[(k[:, :n], v[:, :n]) for (k, v), n in zip(layer, s.lens)] for layer in s.hist]
+        assert s.tables[0].lens.tolist() == s.lens
+        assert s.tables[0].refs.tolist() == counted(s.tables[0])
+        if rejected[0] == 8:
+            s.fork([0, 0, 2, 1])   # the last page of each is shared again
+    s.compact()
+    s.step([3, 2, 1, 9])
+    s.fork([-1] * 4)
+    assert not s.tables[0].refs.any()
+
+
+def test_taking_back_in_a_graph(ops):
+    """Extension and taking back captured together, replayed; an eager copy of
+    the table follows."""
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    tables = [ops.PageTable.empty(5, 12, 40, 4, DEV) for _ in range(2)]
+    counts, rejected = i32([0] * 5), i32([0] * 5)
+    step = lambda t: (ops.extend_pages(t, counts), take_back(t, rejected))
+    step(tables[0])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(tables[0])
+    for new, back in (([9, 4, 1, 0, 17], [0, 0, 0, 0, 3]), ([5, 5, 5, 5, 5], [5, 4, 3, 2, 1]), ([1] * 5, [9, 0, 9, 0, 20]),
+                      ([7, 0, 0, 12, 2], [0] * 5)):
+        counts.copy_(i32(new))
+        rejected.copy_(i32(back))
+        graph.replay()
+        step(tables[1])
+        torch.cuda.synchronize()
+        a, b = tables
+        assert torch.equal(a.lens, b.lens) and torch.equal(a.refs, b.refs)
+        assert a.refs.tolist() == counted(a) == counted(b)
