@@ -1348,7 +1348,12 @@ def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.T
     [n_pages, ...], each page one dense block, e.g. the keys and the values of
     every layer).  Returns bool [S]: False, with the sequence unchanged, where
     its row of the table is too short or the pages that were free before the
-    call do not last for the sequences up to it."""
+    call do not last for the sequences up to it.
+
+    Copies go by refs as they are before the call: of n sequences that share a
+    last page and all grow, each takes a page and a copy, and the shared one is
+    free afterwards.  With a page less the last of them is refused, and asked
+    again it keeps the shared page, which is then its own."""
     if counts.shape != table.lens.shape:
         raise ValueError(f"counts has shape {tuple(counts.shape)} for {table.lens.shape[0]} sequences")
     _i32_tensor("counts", counts, 1, table.device)

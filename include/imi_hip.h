@@ -605,7 +605,9 @@ int imi_fork_pages(const imi_page_table* in, const int32_t* parents, const imi_p
  * partly filled last page that other sequences hold too: that page is copied
  * in every pool.  granted[s] = 0, with the sequence as it was, where the row
  * of the table is too short or the free pages (those free before the call)
- * do not last for the sequences up to s. */
+ * do not last for the sequences up to s.  Copies go by refs before the call:
+ * n sequences that share a last page and all grow take n pages and n copies,
+ * and the shared page is free afterwards. */
 int imi_extend_pages_workspace_size(const imi_page_table* t, size_t* bytes);
 int imi_extend_pages(const imi_page_table* t, const int32_t* counts, uint8_t* granted, const imi_page_pool* pools,
                      int32_t n_pools, void* workspace, size_t workspace_bytes, imi_stream_t stream);

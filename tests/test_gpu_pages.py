@@ -255,3 +255,18 @@ def test_counts_may_be_the_lengths(ops):
     assert ops.compact_pages(table, [pool, pool]).item() == m.compact()
     m.same(table)
     pools_equal(m, pools)
+
+
+def test_shared_last_page_takes_a_page_per_holder(ops):
+    """Two beams on one half-filled page with one free page left: the first gets
+    its copy, the second is refused and keeps the page for itself."""
+    m = Model(2, 4, 2, 8, 1)
+    table, pools = ops.PageTable.empty(2, 4, 2, 8, DEV), [content((2, 4), 0)]
+    assert ops.extend_pages(table, i32([5, 0]), pools).tolist() == m.extend([5, 0])
+    table = ops.fork_pages(table, i32([0, 0]))
+    m.fork([0, 0])
+    for counts, granted in (([1, 1], [True, False]), ([0, 1], [True, True]), ([2, 2], [True, True])):
+        assert ops.extend_pages(table, i32(counts), pools).tolist() == m.extend(counts) == granted
+        m.same(table)
+        pools_equal(m, pools)
+    assert table.refs.tolist() == [1, 1] and table.lens.tolist() == [8, 8]
