@@ -1470,6 +1470,15 @@ Shape shape_of(const imi_paged_attention_args* a) {
     if (most <= 32) {
         p.few_rows = most <= 16 ? 16 : 32;
     } else {
+        // Beside tiles the few-row kernel takes one block where it holds a token,
+        // so sequences of 17 to 32 rows become tiles: the batch says how long its
+        // chunks may be, not whether there are any, and what such steps mostly
+        // hold is single tokens.  With two blocks 40 of these over 300..40000 rows
+        // (4 heads of 128, 8 queries each) take 166 us instead of 146, 24 over
+        // 600..20000 (8 heads, 4 queries) 134 instead of 124, of 64 dims 71 instead
+        // of 65; with one block 24 sequences of 5 tokens (20 rows each) take 173
+        // instead of 148 (100 instead of 81 in a window of 4096; beside a chunk of
+        // 500 tokens 229 either way, of 64 dims 170 instead of 131).
         p.tiles = true;
         if (b.n_seqs > 1 && a->groups <= 32) p.few_rows = a->groups <= 16 ? 16 : 32;
     }

@@ -11,9 +11,12 @@
 // The counting (free pages, pages needed) is one workgroup's pass over refs
 // and lens (4 bytes per page, 16 pages per thread at a time: 7 us to extend 32
 // sequences, 15 us to compact a pool of 10401 pages, mostly the chain of
-// loads and scans); the table entries and the page copies, which are what
-// moves bytes, are spread over the chip (0.67 GB of pages moved in 256 us,
-// 5.3 TB/s both ways).
+// loads and scans).  It stays so at any size, 16384 pages to a turn of about 7 us:
+// extend looks no further than the free pages it needs, but in a full pool of
+// 100000 pages (one sequence of 128k rows takes 8192 of 16) a call takes 58 us, of
+// 10^6 pages 500, and compact, which always looks at all and twice, 105 and 975.
+// The table entries and the page copies, which are what moves bytes, are
+// spread over the chip (0.67 GB of pages moved in 256 us, 5.3 TB/s both ways).
 #include <algorithm>
 
 #include "imi_common.hpp"
