@@ -853,10 +853,10 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
 // into W equal ranges, so a causal triangle, a short prompt and a chunk over
 // a long prefix load the chip evenly; partials as above.
 //
-// A CU's eight waves have its registers (acc, scores, queries: 245 of 256) and
-// LDS to themselves.  Bound by matrix and vector instructions together (49 and
-// 58 percent of a SIMD's time): 8192 tokens of 32 heads over 32768 rows take
-// 3.85-4.0 ms, 960-1000 TFLOP/s (a large matrix product runs at 1381).  Without
+// A CU's eight waves have its registers (acc, scores, queries: 248 of 256) and
+// LDS to themselves.  Bound by matrix and vector instructions together (50 and
+// 60 percent of a SIMD's time): 8192 tokens of 32 heads over 32768 rows take
+// 3.8-4.0 ms, 960-1010 TFLOP/s (a large matrix product runs at 1381).  Without
 // the staging the same loop runs at 1190, without the softmax at 1100.  Tiles
 // of 128 rows read K and V twice as often and were slower, 64 rows per wave
 // (half as many reads of LDS) no faster.
@@ -1452,7 +1452,7 @@ struct Shape {
 };
 
 // A workgroup per (sequence, head) up to this many units.  One sequence of 519
-// rows of 128 dims called in a loop takes 13.3 us so, 15.4 with a join, whose
+// rows of 128 dims called in a loop takes 13.3 us so, 15.4-15.9 with a join, whose
 // workspace and second launch cost the host more than the GPU gains (replayed
 // in a graph: 512, 768, 1024 rows 11.3, 14.1, 16.8 us without, 11.4 each with).
 constexpr int kDirectUnits = 3;

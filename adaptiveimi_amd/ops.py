@@ -1067,7 +1067,8 @@ def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch
     if key_pages.dim() != 4 or key_pages.shape[3] != dim or key_pages.stride(3) != 1:
         raise ValueError(f"key_pages must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
     steps = _steps(key_pages)
-    if value_pages.shape != key_pages.shape or _steps(value_pages) != steps:
+    if value_pages.shape != key_pages.shape or (value_pages.stride() != key_pages.stride()
+                                                and _steps(value_pages) != steps):
         raise ValueError("key_pages and value_pages must share shape and strides")
     if key_pages.device != batch.device or value_pages.device != batch.device:
         raise ValueError(f"pages are on {key_pages.device} and {value_pages.device}, expected {batch.device}")
