@@ -425,7 +425,7 @@ def _own_read(state):
 def _own_shared(state):
     from adaptiveimi_amd import ops
 
-    batch = ops.share_prefixes(_own_batch(state, ops))
+    batch = ops.share_prefixes(_own_batch(state, ops), state["case"]["page"])
     return [ops.paged_attention(x["q"], _own_pages(x["k"], ops), _own_pages(x["v"], ops), batch, out=x["out"],
                                 lse=x["lse"]) for x in state["layers"]]
 
