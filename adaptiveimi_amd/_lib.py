@@ -102,7 +102,7 @@ class HostcacheGatherArgs(ctypes.Structure):
 class PagedBatchArgs(ctypes.Structure):
     _fields_ = [("page_table", _vp), ("table_stride", _i64), ("max_pages", _i32), ("n_pages", _i32),
                 ("page_size", _i32), ("lens", _vp), ("query_start", _vp), ("n_seqs", _i32), ("n_tokens", _i32),
-                ("max_query", _i32), ("max_len", _i32)]
+                ("max_query", _i32), ("max_len", _i32), ("shared", _vp), ("members", _vp)]
 
 
 class PagedAttentionArgs(ctypes.Structure):
@@ -112,7 +112,9 @@ class PagedAttentionArgs(ctypes.Structure):
                 ("scale", _f32), ("window", _i32), ("sinks", _i32),
                 ("out", _vp), ("out_token_stride", _i64), ("out_head_stride", _i64),
                 ("out_lse", _vp), ("lse_token_stride", _i64),
-                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t)]
+                ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+                ("format", _i32), ("key_exponents", _vp), ("value_exponents", _vp),
+                ("exponent_page_stride", _i64), ("exponent_head_stride", _i64), ("exponent_row_stride", _i64)]
 
 
 class QkNormRopeArgs(ctypes.Structure):
@@ -125,7 +127,19 @@ class QkNormRopeArgs(ctypes.Structure):
                 ("eps", _f32), ("query_out", _vp), ("query_out_token_stride", _i64), ("query_out_head_stride", _i64),
                 ("key_out", _vp), ("key_out_token_stride", _i64), ("key_out_head_stride", _i64),
                 ("key_pages", _vp), ("value_pages", _vp),
-                ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64)]
+                ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("format", _i32), ("key_exponents", _vp), ("value_exponents", _vp),
+                ("exponent_page_stride", _i64), ("exponent_head_stride", _i64), ("exponent_row_stride", _i64)]
+
+
+class ReadPagesArgs(ctypes.Structure):
+    _fields_ = [("batch", PagedBatchArgs), ("dtype", _i32), ("kv_heads", _i32), ("dim", _i32),
+                ("key_pages", _vp), ("value_pages", _vp),
+                ("page_stride", _i64), ("head_stride", _i64), ("row_stride", _i64),
+                ("format", _i32), ("key_exponents", _vp), ("value_exponents", _vp),
+                ("exponent_page_stride", _i64), ("exponent_head_stride", _i64), ("exponent_row_stride", _i64),
+                ("first", _vp), ("rows", _i32), ("keys", _vp), ("values", _vp),
+                ("out_seq_stride", _i64), ("out_head_stride", _i64), ("out_row_stride", _i64)]
 
 
 class PageTableArgs(ctypes.Structure):
@@ -172,6 +186,10 @@ EXPORTS = {
                                                           ctypes.POINTER(ctypes.c_size_t)]),
     "imi_paged_attention": (ctypes.c_int, [ctypes.POINTER(PagedAttentionArgs), _vp]),
     "imi_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(QkNormRopeArgs), _vp]),
+    "imi_read_pages": (ctypes.c_int, [ctypes.POINTER(ReadPagesArgs), _vp]),
+    "imi_share_prefixes_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedBatchArgs),
+                                                         ctypes.POINTER(ctypes.c_size_t)]),
+    "imi_share_prefixes": (ctypes.c_int, [ctypes.POINTER(PagedBatchArgs), _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "imi_fork_pages": (ctypes.c_int, [ctypes.POINTER(PageTableArgs), _vp, ctypes.POINTER(PageTableArgs), _vp]),
     "imi_extend_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(PageTableArgs),
                                                        ctypes.POINTER(ctypes.c_size_t)]),

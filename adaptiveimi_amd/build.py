@@ -40,7 +40,8 @@ HIPCC_FLAGS = [
 # is copied on the path that every step takes).
 EXTRA_FLAGS = {
     "imi_kmeans.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-    "imi_paged.hip": ["-mllvm", "-amdgpu-codegenprepare-break-large-phis=0"],
+    **{f"imi_paged{form}.hip": ["-mllvm", "-amdgpu-codegenprepare-break-large-phis=0"]
+       for form in ("", "_fp8", "_int8", "_fp4")},
 }
 
 
@@ -61,7 +62,7 @@ def sources():
     return sorted(CSRC.glob("*.hip"))
 
 
-def build(verbose: bool = False, jobs: int = 4, force: bool = False) -> Path:
+def build(verbose: bool = False, jobs: int = 8, force: bool = False) -> Path:
     """Compile every source (force) or the ones newer than their object."""
     BUILD_DIR.mkdir(exist_ok=True)
     hipcc = _hipcc()

@@ -51,6 +51,8 @@ void clear_error();
 // (imi_paged.hip).
 int validate_batch(const imi_paged_batch* b);
 int64_t batch_capacity(const imi_paged_batch* b);
+int validate_format(int format, int dim, const void* key_exps, const void* value_exps, int64_t page_s, int64_t head_s,
+                    int64_t row_s, int64_t e_page, int64_t e_head, int64_t e_row, int64_t page_size);
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

@@ -15,9 +15,13 @@
 // the partner of a pair is a lane exchange.  A workgroup takes a few tokens;
 // its sines and cosines are computed once into LDS while the loads of the
 // heads are in flight.
+//
+// Pages in 8 or 4 bits (C): a block of 32 dims is four lanes, whose largest
+// magnitude two lane exchanges find; the codes are made of the fp32 results, so
+// a key is rounded once there too.
 #include <algorithm>
 
-#include "imi_common.hpp"
+#include "imi_blocks.hpp"
 
 namespace imi {
 namespace {
@@ -49,11 +53,14 @@ struct QkParams {
     uint32_t div;                          // floor(2^32 / heads) + 1: x / heads = (x div) >> 32
     float eps;
     bool w32, pos64, interleaved, paged;
+    uint8_t *ke, *ve;                      // codes (page, head and row strides in bytes then): exponents
+    int64_t e_page_s, e_hs, e_ts;
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
 struct BF16 {
+    static constexpr bool kHalf = false;
     static __device__ __forceinline__ float lo(uint32_t x) { return bf16_lo(x); }
     static __device__ __forceinline__ float hi(uint32_t x) { return bf16_hi(x); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -63,6 +70,7 @@ struct BF16 {
     }
 };
 struct FP16 {
+    static constexpr bool kHalf = true;
     typedef __attribute__((ext_vector_type(2))) _Float16 h2;
     static __device__ __forceinline__ float lo(uint32_t x) { return __builtin_bit_cast(h2, x)[0]; }
     static __device__ __forceinline__ float hi(uint32_t x) { return __builtin_bit_cast(h2, x)[1]; }
@@ -101,12 +109,33 @@ __device__ __forceinline__ int owner_of(const QkParams& a, int t) {
     }
 }
 
-template <typename T, int D>
+// 8 dims of a lane to a row of codes and, by the first lane of a block, its
+// exponent.
+template <typename T, typename C>
+__device__ __forceinline__ void store_codes(const float (&y)[8], uint8_t* row, uint8_t* exps, int c) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(y[j]) & 0x7FFFFFFFu);
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xF, 0xF, true)));
+    top = max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0x4E, 0xF, 0xF, true)));
+    const uint32_t e = block_exponent<C, T::kHalf>(top);
+    uint32_t w[C::kWords];
+    block_encode<C, T::kHalf>(y, e, w);
+    if constexpr (C::kWords == 2)
+        *reinterpret_cast<uint2*>(row + 8 * c) = make_uint2(w[0], w[1]);
+    else
+        *reinterpret_cast<uint32_t*>(row + 4 * c) = w[0];
+    if (c % 4 == 0) exps[c / 4] = static_cast<uint8_t>(e);
+}
+
+template <typename T, int D, typename C>
 __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
     constexpr int L = D / 8;        // lanes of a head
     constexpr int NG = 256 / L;     // heads at a time
     __shared__ float2 s_cs[kMaxTokens][D / 2];
+    constexpr bool kCodes = C::kBits != 16;
     __shared__ int64_t s_slot[kMaxTokens];   // element offset of the token's row in the pages, -1: not stored
+    __shared__ int64_t s_exp[kCodes ? kMaxTokens : 1];   // and of its exponents
     __shared__ __align__(16) float s_w[2][D];
     __shared__ int s_pos[kMaxTokens];
     __shared__ int s_own[kMaxTokens];
@@ -142,7 +171,7 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
     for (int i = wave; i < nt; i += 4) {
         const int t = t0 + i;
         int pos = 0, own = 1;
-        int64_t slot = -1;
+        int64_t slot = -1, exp = 0;
         if (a.positions) {
             pos = a.pos64 ? static_cast<int>(static_cast<const int64_t*>(a.positions)[t])
                           : static_cast<const int32_t*>(a.positions)[t];
@@ -154,8 +183,10 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
                 pos = clampi(a.lens[s], 0, a.capacity) - (e - b) + (t - b);
                 if (pos >= 0) {
                     const int page = a.table ? a.table[s * a.table_s + (pos >> a.page_shift)] : s;
-                    if (page >= 0 && page < a.n_pages)
+                    if (page >= 0 && page < a.n_pages) {
                         slot = page * a.page_s + (pos & ((1u << a.page_shift) - 1u)) * a.ko_ts;
+                        if constexpr (kCodes) exp = page * a.e_page_s + (pos & ((1u << a.page_shift) - 1u)) * a.e_ts;
+                    }
                 }
             }
         }
@@ -163,6 +194,7 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
             s_pos[i] = pos;
             s_own[i] = own;
             s_slot[i] = slot;
+            if constexpr (kCodes) s_exp[i] = exp;
         }
     }
     __syncthreads();
@@ -190,8 +222,17 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
             const int64_t t = t0 + ti;
             if (!s_own[ti]) continue;
             if (h >= a.Hq + a.Hk) {   // a value head: copied
-                if (s_slot[ti] >= 0)
-                    *reinterpret_cast<u32x4_t*>(a.vo + s_slot[ti] + (h - a.Hq - a.Hk) * a.ko_hs + 8 * c) = x[i];
+                if (s_slot[ti] >= 0) {
+                    const int kv = h - a.Hq - a.Hk;
+                    if constexpr (kCodes) {
+                        float y[8];
+                        unpack8<T>(x[i], y);
+                        store_codes<T, C>(y, reinterpret_cast<uint8_t*>(a.vo) + s_slot[ti] + kv * a.ko_hs,
+                                          a.ve + s_exp[ti] + kv * a.e_hs, c);
+                    } else {
+                        *reinterpret_cast<u32x4_t*>(a.vo + s_slot[ti] + kv * a.ko_hs + 8 * c) = x[i];
+                    }
+                }
                 continue;
             }
             const bool is_q = h < a.Hq;
@@ -234,6 +275,14 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
                     }
                 }
             }
+            if constexpr (kCodes) {
+                if (!is_q) {
+                    if (s_slot[ti] >= 0)
+                        store_codes<T, C>(y, reinterpret_cast<uint8_t*>(a.ko) + s_slot[ti] + (h - a.Hq) * a.ko_hs,
+                                          a.ke + s_exp[ti] + (h - a.Hq) * a.e_hs, c);
+                    continue;
+                }
+            }
             const u32x4_t o = u32x4_t{T::pack(y[0], y[1]), T::pack(y[2], y[3]), T::pack(y[4], y[5]), T::pack(y[6], y[7])};
             if (is_q)
                 *reinterpret_cast<u32x4_t*>(a.qo + t * a.qo_ts + h * a.qo_hs + 8 * c) = o;
@@ -242,6 +291,16 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
             else if (s_slot[ti] >= 0)
                 *reinterpret_cast<u32x4_t*>(a.ko + s_slot[ti] + (h - a.Hq) * a.ko_hs + 8 * c) = o;
         }
+    }
+}
+
+template <typename T, int D>
+void launch(const QkParams& P, int format, int grid, hipStream_t st) {
+    switch (format) {
+        case IMI_FP8: qk_norm_rope_kernel<T, D, Fp8><<<grid, 256, 0, st>>>(P); break;
+        case IMI_INT8: qk_norm_rope_kernel<T, D, Int8><<<grid, 256, 0, st>>>(P); break;
+        case IMI_FP4: qk_norm_rope_kernel<T, D, Fp4><<<grid, 256, 0, st>>>(P); break;
+        default: qk_norm_rope_kernel<T, D, Raw16><<<grid, 256, 0, st>>>(P);
     }
 }
 
@@ -293,8 +352,17 @@ extern "C" int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t str
         P.n_pages = b.n_pages;
         P.page_shift = b.page_table ? __builtin_ctz(static_cast<unsigned>(b.page_size)) : 31;
         P.capacity = static_cast<int>(batch_capacity(&b));
-        P.ko = a->key_pages;
-        P.vo = a->value_pages;
+        if (const int rc = validate_format(a->format, a->dim, a->key_exponents, a->value_exponents, a->page_stride,
+                                           a->head_stride, a->row_stride, a->exponent_page_stride,
+                                           a->exponent_head_stride, a->exponent_row_stride, b.page_size))
+            return rc;
+        P.ko = static_cast<uint16_t*>(a->key_pages);
+        P.vo = static_cast<uint16_t*>(a->value_pages);
+        P.ke = a->key_exponents;
+        P.ve = a->value_exponents;
+        P.e_page_s = a->exponent_page_stride;
+        P.e_hs = a->exponent_head_stride;
+        P.e_ts = a->exponent_row_stride;
         P.ko_ts = a->row_stride;
         P.ko_hs = a->head_stride;
         P.page_s = a->page_stride;
@@ -335,13 +403,9 @@ extern "C" int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t str
     P.div = static_cast<uint32_t>((uint64_t(1) << 32) / heads + 1);
     const int grid = (P.N + P.tokens - 1) / P.tokens;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == IMI_BF16) {
-        if (a->dim == 128) qk_norm_rope_kernel<BF16, 128><<<grid, 256, 0, st>>>(P);
-        else qk_norm_rope_kernel<BF16, 64><<<grid, 256, 0, st>>>(P);
-    } else {
-        if (a->dim == 128) qk_norm_rope_kernel<FP16, 128><<<grid, 256, 0, st>>>(P);
-        else qk_norm_rope_kernel<FP16, 64><<<grid, 256, 0, st>>>(P);
-    }
+    const int format = paged ? a->format : IMI_ROWS;
+    if (a->dtype == IMI_BF16) a->dim == 128 ? launch<BF16, 128>(P, format, grid, st) : launch<BF16, 64>(P, format, grid, st);
+    else a->dim == 128 ? launch<FP16, 128>(P, format, grid, st) : launch<FP16, 64>(P, format, grid, st);
     IMI_LAUNCH_CHECK("qk_norm_rope_kernel");
     return IMI_OK;
 }

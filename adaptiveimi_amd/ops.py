@@ -17,7 +17,7 @@ import torch
 
 from . import _lib
 from ._lib import (AttentionArgs, DecodeArgs, IndexArgs, KmeansArgs, PagedAttentionArgs, PagedBatchArgs, PagePool,
-                   PageTableArgs, QkNormRopeArgs, SelectArgs, UpdateArgs, check)
+                   PageTableArgs, QkNormRopeArgs, ReadPagesArgs, SelectArgs, UpdateArgs, check)
 
 _WS: Dict[Tuple[str, int], torch.Tensor] = {}
 
@@ -1022,10 +1022,12 @@ class PagedBatch:
     sequence belong to none.  max_query: at least every sequence's new tokens
     (the rows of one with more may be left as they are).  max_len: a hint, about the
     longest sequence (default: what the table holds); only the split of short
-    batches depends on it."""
+    batches depends on it.
+
+    ``shared`` and ``members`` are None but in a batch of share_prefixes."""
 
     __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device", "pool_pages",
-                 "page_size")
+                 "page_size", "shared", "members")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
@@ -1047,6 +1049,7 @@ class PagedBatch:
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.pool_pages, self.page_size = 0, None   # what a PageTable knows of the pools
+        self.shared = self.members = None
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
                                    _c_int(self.max_query), _c_int(max_len or 0))
 
@@ -1058,30 +1061,104 @@ class PagedBatch:
         return a
 
 
-def _pools(key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch, dim: int, dtype: torch.dtype):
+# code type: (format, dims per element)
+_FORMATS = {torch.float8_e4m3fn: (1, 1), torch.int8: (2, 1), torch.uint8: (3, 2)}   # IMI_FP8, IMI_INT8, IMI_FP4
+_FORMAT_NAMES = {"fp8": torch.float8_e4m3fn, "int8": torch.int8, "fp4": torch.uint8}
+_BLOCK = 32   # dims that share an exponent
+
+
+class QuantizedPages:
+    """A pool of keys or values in 8 or 4 bits, given in a tensor's place.
+
+    codes [pages, kv_heads, page_size, D], float8_e4m3fn ("fp8") or int8, or
+    uint8 [..., D / 2] with two e2m1 numbers in a byte, the lower half first
+    ("fp4").  exponents uint8 [pages, kv_heads, page_size, D / 32]: value =
+    code * 2^(e - 127), NaN for e = 255.  Both of any memory order with the
+    last dimension adjacent (``codes.transpose(1, 2)`` of a token-major pool).
+
+    What is stored (qk_norm_rope) takes, for each 32 dims, the smallest power
+    of two that keeps their largest magnitude within 448, 127 or 6, at least
+    2^-117, and is rounded to the nearest code, ties to even; where that would
+    read back as an infinity, to the largest that does not.  A block that holds
+    an infinity or a NaN reads back as NaN."""
+
+    __slots__ = ("codes", "exponents", "format")
+
+    def __init__(self, codes: torch.Tensor, exponents: torch.Tensor):
+        form = _FORMATS.get(codes.dtype)
+        if form is None:
+            raise TypeError(f"codes must be float8_e4m3fn, int8 or uint8, got {codes.dtype}")
+        if exponents.dtype is not torch.uint8:
+            raise TypeError(f"exponents must be uint8, got {exponents.dtype}")
+        if codes.dim() != 4 or exponents.dim() != 4:
+            raise ValueError("codes and exponents must be [pages, kv_heads, page_size, ...]")
+        dim = codes.shape[3] * form[1]
+        if codes.shape[:3] != exponents.shape[:3] or exponents.shape[3] * _BLOCK != dim:
+            raise ValueError(f"exponents are {list(exponents.shape)} for codes of {list(codes.shape[:3])} rows of "
+                             f"{dim} dims (one for {_BLOCK} dims)")
+        if codes.device != exponents.device:
+            raise ValueError(f"codes are on {codes.device}, exponents on {exponents.device}")
+        if codes.stride(3) != 1 or (exponents.stride(3) != 1 and exponents.shape[3] > 1):
+            raise ValueError("codes and exponents must have unit stride on the last dimension")
+        self.codes, self.exponents, self.format = codes, exponents, form[0]
+
+    @classmethod
+    def zeros(cls, n_pages: int, kv_heads: int, page_size: int, dim: int, format: str, device) -> "QuantizedPages":
+        """A pool of zeros; format "fp8", "int8" or "fp4"."""
+        code = _FORMAT_NAMES.get(format)
+        if code is None:
+            raise ValueError(f"format must be one of {sorted(_FORMAT_NAMES)}, got {format!r}")
+        if dim % _BLOCK:
+            raise ValueError(f"dim={dim} is not a multiple of {_BLOCK}")
+        shape = (n_pages, kv_heads, page_size)
+        return cls(torch.zeros(shape + (dim // _FORMATS[code][1],), dtype=code, device=device),
+                   torch.full(shape + (dim // _BLOCK,), 127, dtype=torch.uint8, device=device))
+
+
+def _same_rows(name: str, a: torch.Tensor, b: torch.Tensor, dev: torch.device) -> Tuple[int, ...]:
+    """Strides of two tensors that have to be laid out alike, without the last."""
+    steps = _steps(a)
+    if b.shape != a.shape or (b.stride() != a.stride() and _steps(b) != steps):
+        raise ValueError(f"{name} must share shape and strides")
+    if a.device != dev or b.device != dev:
+        raise ValueError(f"pages are on {a.device} and {b.device}, expected {dev}")
+    return steps[:3]
+
+
+_NO_CODES = (0, 0, 0, 0, 0, 0)
+
+
+def _pools(key_pages, value_pages, batch: PagedBatch, dim: int, dtype: torch.dtype):
     """Checks a key and a value pool [pages, kv_heads, page_size, D] of any
-    memory order with the head dim adjacent.  Returns (pages, heads, rows,
-    page, head and row strides)."""
-    if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
-        raise TypeError(f"pages are {key_pages.dtype} and {value_pages.dtype}, expected {dtype}")
-    if key_pages.dim() != 4 or key_pages.shape[3] != dim or key_pages.stride(3) != 1:
-        raise ValueError(f"key_pages must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
-    steps = _steps(key_pages)
-    if value_pages.shape != key_pages.shape or (value_pages.stride() != key_pages.stride()
-                                                and _steps(value_pages) != steps):
-        raise ValueError("key_pages and value_pages must share shape and strides")
-    if key_pages.device != batch.device or value_pages.device != batch.device:
-        raise ValueError(f"pages are on {key_pages.device} and {value_pages.device}, expected {batch.device}")
+    memory order with the head dim adjacent.  Returns (pages, heads, rows), the
+    addresses and the page, head and row strides, and (format, addresses and
+    strides of the exponents)."""
+    codes = _NO_CODES
+    if type(key_pages) is QuantizedPages or type(value_pages) is QuantizedPages:
+        if type(key_pages) is not type(value_pages) or key_pages.format != value_pages.format:
+            raise TypeError("key_pages and value_pages must have the same format")
+        ke, ve = key_pages.exponents, value_pages.exponents
+        if ke.shape[3] * _BLOCK != dim:
+            raise ValueError(f"pages of {ke.shape[3] * _BLOCK} dims, expected {dim}")
+        codes = (key_pages.format, ke.data_ptr(), ve.data_ptr()) + _same_rows(
+            "exponents of key_pages and value_pages", ke, ve, batch.device)
+        key_pages, value_pages = key_pages.codes, value_pages.codes
+    else:
+        if key_pages.dtype is not dtype or value_pages.dtype is not dtype:
+            raise TypeError(f"pages are {key_pages.dtype} and {value_pages.dtype}, expected {dtype}")
+        if key_pages.dim() != 4 or key_pages.shape[3] != dim or key_pages.stride(3) != 1:
+            raise ValueError(f"key_pages must be [pages, kv_heads, page_size, {dim}] with unit stride on the last")
+    steps = _same_rows("key_pages and value_pages", key_pages, value_pages, batch.device)
     P, H, page, _ = key_pages.shape
     if batch.page_table is None and P < batch.args.n_seqs:
         raise ValueError(f"{P} sets of contiguous rows for {batch.args.n_seqs} sequences")
     if batch.page_size is not None and (page != batch.page_size or P < batch.pool_pages):
         raise ValueError(f"{P} pages of {page} rows under a table of {batch.pool_pages} pages of {batch.page_size} rows "
                          "(a token-major pool is given as pool.transpose(1, 2))")
-    return (P, H, page) + steps[:3]
+    return (P, H, page), (key_pages.data_ptr(), value_pages.data_ptr()) + steps, codes
 
 
-def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, batch: PagedBatch,
+def paged_attention(query: torch.Tensor, key_pages, value_pages, batch: PagedBatch,
                     scale: Optional[float] = None, window: int = 0, sinks: int = 0,
                     out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
                     return_lse: bool = False):
@@ -1092,7 +1169,9 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     query: bf16 or fp16 [N, Hq, D], D 64 or 128, any token and head strides.
     key_pages / value_pages: [pages, Hkv, page_size, D] (a power of two of
     rows per page with a page table), e.g. ``pool.transpose(1, 2)`` of a
-    token-major pool; Hq a multiple of Hkv.  A token at position p sees rows
+    token-major pool, or QuantizedPages, both in one format; Hq a multiple of
+    Hkv.  A batch of share_prefixes attends the rows that sequences share once
+    for all of them (without ``window``).  A token at position p sees rows
     j <= p; with ``window`` of these the last ``window`` and the first
     ``sinks``.  A token that sees no row gets 0 (lse -inf).  ``out`` [N, Hq,
     D] (the query itself is allowed) and ``lse`` f32 [N, Hq] (natural log) may be given; rows behind the
@@ -1108,7 +1187,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
         raise ValueError("query must be [tokens, heads, dim]")
     N, Hq, D = shape
     q, q_ts, q_hs = _rows("query", query, shape, dtype, dev)
-    P, H, page, sp, sh, sr = _pools(key_pages, value_pages, batch, D, dtype)
+    (P, H, page), pools, codes = _pools(key_pages, value_pages, batch, D, dtype)
     if H == 0 or Hq % H:
         raise ValueError(f"{Hq} query heads are not a multiple of {H} KV heads")
     if out is None:
@@ -1123,10 +1202,9 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
                 or (N > 1 and l_ts == 0)):
             raise ValueError(f"lse must be float32 {(N, Hq)} on {dev}, with unit stride on heads")
         l = lse.data_ptr()
-    a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, key_pages.data_ptr(),
-                           value_pages.data_ptr(), sp, sh, sr, D ** -0.5 if scale is None else scale,
-                           _c_int(window), _c_int(sinks),
-                           o, o_ts, o_hs, l, l_ts)
+    a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, *pools,
+                           D ** -0.5 if scale is None else scale, _c_int(window), _c_int(sinks),
+                           o, o_ts, o_hs, l, l_ts, 0, 0, *codes)
     L = _lib.lib()
     ref = ctypes.byref(a)
     need = ctypes.c_size_t()
@@ -1144,7 +1222,7 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
                  key_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
                  query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None,
                  value: Optional[torch.Tensor] = None, batch: Optional[PagedBatch] = None,
-                 key_pages: Optional[torch.Tensor] = None, value_pages: Optional[torch.Tensor] = None):
+                 key_pages=None, value_pages=None):
     """RMS norm of each query and key head and the rotation by position, in
     one pass.
 
@@ -1159,7 +1237,7 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
     Either ``positions`` (int32 or int64 [N], at most 2^31 - 1 in magnitude)
     are given: returns (query_out, key_out), made here or given (the inputs
     themselves are allowed).  Or ``batch``, ``value`` [N, Hkv, D] and the
-    pools (as in paged_attention) are: new token i of a sequence stands at
+    pools (as in paged_attention; QuantizedPages are quantised into) are: new token i of a sequence stands at
     lens - (its new tokens) + i, its key and value are stored in that row, and
     (query_out, None) is returned; tokens behind the last sequence, and rows
     that the table has no page for, are left as they are."""
@@ -1202,16 +1280,16 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
     if paged:
         if batch.device != dev:
             raise ValueError(f"batch is on {batch.device}, expected {dev}")
-        P, H, page, sp, sh, sr = _pools(key_pages, value_pages, batch, D, dtype)
+        (P, H, page), pools, codes = _pools(key_pages, value_pages, batch, D, dtype)
         if H != Hk:
             raise ValueError(f"pages hold {H} KV heads, key has {Hk}")
-        if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1):
-            raise ValueError("pages are written, so no two of their elements may share memory")
+        for sp, sh, sr in (pools[2:], codes[3:]) if codes[0] else (pools[2:],):
+            if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1):
+                raise ValueError("pages are written, so no two of their elements may share memory")
         a = QkNormRopeArgs(batch.bind(P, page, N), code, Hq, Hk, D, *_rows("query", query, shape, dtype, dev),
                            *_rows("key", key, k_shape, dtype, dev), *_rows("value", value, k_shape, dtype, dev), 0, 0,
                            f, rotary, int(interleaved), qw, kw, w32, eps,
-                           *_rows("query_out", query_out, shape, dtype, dev, True), 0, 0, 0, key_pages.data_ptr(),
-                           value_pages.data_ptr(), sp, sh, sr)
+                           *_rows("query_out", query_out, shape, dtype, dev, True), 0, 0, 0, *pools, *codes)
     else:
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
@@ -1227,6 +1305,118 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
     with _on(dev):
         check(_lib.lib().imi_qk_norm_rope(ctypes.byref(a), _raw_stream(dev.index)), "imi_qk_norm_rope")
     return query_out, key_out
+
+
+def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = None,
+               first: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
+               out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cached rows as contiguous ones: (keys, values) [S, Hkv, rows, D], row i
+    of a sequence its cached row first[s] + i (``first`` int32 [S], default 0),
+    e.g. ``keys[s]`` for kmeans and build_index, or for a cache elsewhere.
+
+    QuantizedPages are read as their values in ``dtype`` (bf16 unless given or
+    ``out`` says), a tensor's rows as they are.  ``rows``: by default what the
+    batch's max_len, or else the table, says.  ``out``: tensors of any sequence,
+    head and row strides to write to.  Rows that a sequence does not have are
+    left as they are (unset in tensors made here)."""
+    dev = batch.device
+    quantized = type(key_pages) is QuantizedPages
+    if out is not None:
+        keys, values = out
+        dtype = keys.dtype if dtype is None else dtype
+    elif dtype is None:
+        dtype = torch.bfloat16 if quantized else key_pages.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"rows are read as bfloat16 or float16, got {dtype}")
+    if quantized:
+        dim = key_pages.exponents.shape[3] * _BLOCK
+    elif key_pages.dim() == 4:
+        dim = key_pages.shape[3]
+    else:
+        raise ValueError("key_pages must be [pages, kv_heads, page_size, D]")
+    (P, H, page), pools, codes = _pools(key_pages, value_pages, batch, dim, dtype)
+    S = batch.args.n_seqs
+    if out is None:
+        if rows is None:
+            rows = batch.max_len or (page if batch.page_table is None else batch.args.max_pages * page)
+        if rows < 0:
+            raise ValueError(f"rows={rows}")
+        keys, values = (torch.empty((S, H, rows, dim), dtype=dtype, device=dev) for _ in range(2))
+    elif rows is None and keys.dim() == 4:
+        rows = keys.shape[2]
+    shape = (S, H, rows, dim)
+    for t in (keys, values):
+        if t.dtype is not dtype:
+            raise TypeError(f"out is {t.dtype}, expected {dtype}")
+        if t.shape != shape or (t.stride(3) != 1 and t.numel()):
+            raise ValueError(f"out must be two tensors {list(shape)} with unit stride on dim")
+    steps = _same_rows("the two tensors of out", keys, values, dev)
+    if any(step == 0 and n > 1 for step, n in zip(steps, shape)):
+        raise ValueError("out is written, so no two of its elements may share memory")
+    f = 0
+    if first is not None:
+        _i32_tensor("first", first, 1, dev)
+        if first.shape[0] != S:
+            raise ValueError(f"first has {first.shape[0]} entries for {S} sequences")
+        f = first.data_ptr()
+    a = ReadPagesArgs(batch.bind(P, page, 0), code, H, dim, *pools, *codes, f, rows, keys.data_ptr(),
+                      values.data_ptr(), *steps)
+    with _on(dev):
+        check(_lib.lib().imi_read_pages(ctypes.byref(a), _raw_stream(dev.index)), "imi_read_pages")
+    return keys, values
+
+
+def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
+                   labels: Optional[torch.Tensor] = None) -> PagedBatch:
+    """The batch, with what its sequences have in common: paged_attention then
+    attends common rows once for all sequences of a run, in every layer.
+
+    A run is a row of neighbouring sequences whose tables begin with the same
+    page (forked prompts, beams: fork_pages keeps them so); it shares the
+    leading pages that all of them have in common before their new tokens.
+    ``labels`` int32 [S]: neighbours of different labels are not put together
+    (all sequences begin with one system prompt, and the beams of a prompt share
+    more).  In the result ``shared`` int32 [S] are the rows that each sequence
+    shares (multiples of 8; 0 for those on their own, or with fewer than 64) and
+    ``members`` the sequences of the run that each leads.  ``page_size``: the
+    pools', where the batch was not made by a PageTable.
+
+    Found on the device, without a synchronisation; the result holds for the
+    tables, lens and query_start as they are now, so it is made anew in every
+    step (in the step's graph, if there is one)."""
+    if batch.page_table is None:
+        raise ValueError("sequences without a page table share no pages")
+    if page_size is None:
+        page_size = batch.page_size
+        if page_size is None:
+            raise ValueError("give the page_size of the pools")
+    elif batch.page_size not in (None, page_size):
+        raise ValueError(f"page_size={page_size} under a table of {batch.page_size} rows per page")
+    dev, S = batch.device, batch.args.n_seqs
+    f = 0
+    if labels is not None:
+        _i32_tensor("labels", labels, 1, dev)
+        if labels.shape[0] != S:
+            raise ValueError(f"labels has {labels.shape[0]} entries for {S} sequences")
+        f = labels.data_ptr()
+    new = PagedBatch.__new__(PagedBatch)
+    for name in PagedBatch.__slots__:
+        setattr(new, name, getattr(batch, name))
+    new.page_size = page_size
+    a = new.args = batch.bind(1, _c_int(page_size), 1)
+    if S:
+        L = _lib.lib()
+        ref = ctypes.byref(a)
+        need = ctypes.c_size_t()
+        new.shared, new.members = torch.empty((2, S), dtype=torch.int32, device=dev)
+        with _on(dev):
+            check(L.imi_share_prefixes_workspace_size(ref, ctypes.byref(need)), "imi_share_prefixes")
+            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+            check(L.imi_share_prefixes(ref, f, new.shared.data_ptr(), new.members.data_ptr(), ws.data_ptr(),
+                                       need.value, _raw_stream(dev.index)), "imi_share_prefixes")
+        a.shared, a.members = new.shared.data_ptr(), new.members.data_ptr()
+    return new
 
 
 class PageTable:
@@ -1289,7 +1479,9 @@ def _table_work(table: PageTable, L, what: str) -> torch.Tensor:
     return torch.empty(n, dtype=torch.uint8, device=table.device)
 
 
-def _pool_args(table: PageTable, pools: Sequence[torch.Tensor]):
+def _pool_args(table: PageTable, pools: Sequence):
+    pools = [t for pool in pools
+             for t in ((pool.codes, pool.exponents) if type(pool) is QuantizedPages else (pool,))]
     arr = (PagePool * max(len(pools), 1))()
     P = table.args.n_pages
     for i, t in enumerate(pools):
@@ -1342,12 +1534,12 @@ def fork_pages(table: PageTable, parents: torch.Tensor, out: Optional[PageTable]
     return out
 
 
-def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.Tensor] = ()) -> torch.Tensor:
+def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence = ()) -> torch.Tensor:
     """Grow sequence s by counts[s] tokens (int32 [S]), in place: the lowest
     free pages go to the sequences in order.  A partly filled last page that
     another sequence holds too is replaced by a copy, in every pool (tensors
     [n_pages, ...], each page one dense block, e.g. the keys and the values of
-    every layer).  Returns bool [S]: False, with the sequence unchanged, where
+    every layer, or QuantizedPages).  Returns bool [S]: False, with the sequence unchanged, where
     its row of the table is too short or the pages that were free before the
     call do not last for the sequences up to it.
 
@@ -1369,7 +1561,7 @@ def extend_pages(table: PageTable, counts: torch.Tensor, pools: Sequence[torch.T
     return granted
 
 
-def compact_pages(table: PageTable, pools: Sequence[torch.Tensor] = ()) -> torch.Tensor:
+def compact_pages(table: PageTable, pools: Sequence = ()) -> torch.Tensor:
     """Move live pages to the lowest ids, in place (the table, refs and every
     pool, as in extend_pages): the i-th live page from id n_live on goes to
     the i-th free id below.  Returns n_live, int32 [1]."""

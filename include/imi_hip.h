@@ -504,7 +504,17 @@ typedef struct {
     int32_t n_seqs, n_tokens;    /* n_tokens: rows of the query tensor */
     int32_t max_query;           /* at least every sequence's new tokens */
     int32_t max_len;             /* hint: about the longest sequence; 0 = what the table holds */
+    const int32_t* shared;       /* device [n_seqs], what imi_share_prefixes found, or NULL (with members) */
+    const int32_t* members;      /*   read by imi_paged_attention alone */
 } imi_paged_batch;
+
+/* How a pool holds its rows: IMI_ROWS as bf16 or fp16 (the call's dtype), the
+ * others as codes [n_pages][kv_heads][page_size][dim] (IMI_FP8: e4m3, IMI_INT8)
+ * or [..][dim / 2] bytes (IMI_FP4: e2m1, the lower half of a byte first), and an
+ * exponent byte e per 32 dims, [n_pages][kv_heads][page_size][dim / 32]: a
+ * value is code * 2^(e - 127), NaN where e is 255.  Strides of codes and of
+ * exponents in bytes: multiples of 16, and of dim / 32. */
+enum { IMI_ROWS = 0, IMI_FP8 = 1, IMI_INT8 = 2, IMI_FP4 = 3 };
 
 /* out[t][x] = softmax over the visible rows of scale * q . k, times v, for
  * query head x of KV head x / groups.  A new token at position p sees rows
@@ -519,8 +529,8 @@ typedef struct {
     int32_t kv_heads, groups, dim;   /* groups = query heads per KV head; dim 64 or 128 */
     const uint16_t* query;       /* device [n_tokens][kv_heads * groups][dim] */
     int64_t query_token_stride, query_head_stride;
-    const uint16_t* keys;        /* device [n_pages][kv_heads][page_size][dim] */
-    const uint16_t* values;
+    const void* keys;            /* device [n_pages][kv_heads][page_size][dim] */
+    const void* values;
     int64_t page_stride, head_stride, row_stride;
     float scale;                 /* > 0 */
     int32_t window;              /* 0: every earlier row */
@@ -531,6 +541,10 @@ typedef struct {
     int64_t lse_token_stride;
     void* workspace;             /* device, >= imi_paged_attention_workspace_size() bytes; any content */
     size_t workspace_bytes;
+    int32_t format;              /* of keys and values */
+    const uint8_t* key_exponents;    /* with codes */
+    const uint8_t* value_exponents;
+    int64_t exponent_page_stride, exponent_head_stride, exponent_row_stride;
 } imi_paged_attention_args;
 
 int imi_paged_attention_workspace_size(const imi_paged_attention_args* a, size_t* bytes);
@@ -567,12 +581,55 @@ typedef struct {
     int64_t query_out_token_stride, query_out_head_stride;
     uint16_t* key_out;           /* with positions */
     int64_t key_out_token_stride, key_out_head_stride;
-    uint16_t* key_pages;         /* with the batch: [n_pages][kv_heads][page_size][dim] */
-    uint16_t* value_pages;
+    void* key_pages;             /* with the batch: [n_pages][kv_heads][page_size][dim] */
+    void* value_pages;
     int64_t page_stride, head_stride, row_stride;
+    int32_t format;              /* of the pages: codes are made of the fp32 results and of the values */
+    uint8_t* key_exponents;      /* with codes */
+    uint8_t* value_exponents;
+    int64_t exponent_page_stride, exponent_head_stride, exponent_row_stride;
 } imi_qk_norm_rope_args;
 
 int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t stream);
+
+/* Cached rows read back: keys[s][h][i] and values[s][h][i], i < rows, are row
+ * first[s] + i of sequence s (first NULL: 0) in the call's dtype, codes as their
+ * values rounded to it.  Rows outside 0 .. lens[s] - 1 are left as they are in
+ * the outputs.  Of the batch, tables, lens and sizes are read, not the new
+ * tokens. */
+typedef struct {
+    imi_paged_batch batch;
+    int32_t dtype;               /* IMI_BF16 or IMI_FP16: outputs, and pages with IMI_ROWS */
+    int32_t kv_heads, dim;       /* dim 64 or 128 */
+    const void* key_pages;       /* as in imi_paged_attention_args */
+    const void* value_pages;
+    int64_t page_stride, head_stride, row_stride;
+    int32_t format;
+    const uint8_t* key_exponents;
+    const uint8_t* value_exponents;
+    int64_t exponent_page_stride, exponent_head_stride, exponent_row_stride;
+    const int32_t* first;        /* device [n_seqs], or NULL */
+    int32_t rows;
+    uint16_t* keys;              /* device [n_seqs][kv_heads][rows][dim]; strides shared by both, multiples of 8 */
+    uint16_t* values;
+    int64_t out_seq_stride, out_head_stride, out_row_stride;
+} imi_read_pages_args;
+
+int imi_read_pages(const imi_read_pages_args* a, imi_stream_t stream);
+
+/* Which sequences begin with the same pages.  A run is a row of neighbouring
+ * sequences of the batch whose tables begin with the same page (and, with
+ * labels, that have the same label); it shares the leading pages that all of
+ * them have in common, as far as they lie before the new tokens of each.
+ * shared[s] = rows that sequence s shares with its run, a multiple of 8, or 0
+ * where it is alone or they are fewer than 64; members[s] = sequences of the run
+ * that s is the first of, or 0.  The batch with both, imi_paged_attention
+ * attends those rows once for all sequences of a run (without a window): the
+ * results differ in their rounding alone.  They hold for the tables, lens and
+ * query_start that they were made of. */
+int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_t* bytes);
+int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
+                       void* workspace, size_t workspace_bytes, imi_stream_t stream);
 
 /* The page tables.  Sequence s holds the first ceil(lens[s] / page_size)
  * entries of its row; refs[p] counts the sequences that hold page p, 0 =
