@@ -41,10 +41,10 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
 // [0.5, 1) with kLead its fraction bits in fp32; kSafe is the largest under
 // 2^kSafeExp, see block_exponent.
 struct Raw16 {
-    static constexpr int kBits = 16, kWords = 4;
+    static constexpr int kFormat = IMI_ROWS, kBits = 16, kWords = 4;
 };
 struct Fp8 {   // e4m3
-    static constexpr int kBits = 8, kWords = 2;
+    static constexpr int kFormat = IMI_FP8, kBits = 8, kWords = 2;
     static constexpr uint32_t kLead = 0x600000;   // 448 = 0.875 * 2^9
     static constexpr int kExp = 9;
     static constexpr int kSafeExp = 8;            // codes from 2^8 on
@@ -75,7 +75,7 @@ struct Fp8 {   // e4m3
     }
 };
 struct Int8 {
-    static constexpr int kBits = 8, kWords = 2;
+    static constexpr int kFormat = IMI_INT8, kBits = 8, kWords = 2;
     static constexpr uint32_t kLead = 0x7E0000;   // 127 = 0.9921875 * 2^7
     static constexpr int kExp = 7;
     static constexpr int kSafeExp = 6;
@@ -103,7 +103,7 @@ struct Int8 {
     }
 };
 struct Fp4 {   // e2m1, two in a byte, the lower half first
-    static constexpr int kBits = 4, kWords = 1;
+    static constexpr int kFormat = IMI_FP4, kBits = 4, kWords = 1;
     static constexpr uint32_t kLead = 0x400000;   // 6 = 0.75 * 2^3
     static constexpr int kExp = 3;
     static constexpr int kSafeExp = 2;

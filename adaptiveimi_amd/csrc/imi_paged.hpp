@@ -403,7 +403,7 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // ---------------------------------------------------------- few rows ------
 // Sequences of at most 16 NB rows (decode, verification of a few tokens):
 // the rows fit one matrix tile, so K and V are streamed once and the kernel
-// is bound by that stream.  Work is counted in units of kUnit cached rows of
+// is bound by that stream.  Work is counted in units of UNIT cached rows of
 // one (sequence, KV head); the units of all, in order, are cut into W equal
 // ranges, one per workgroup, whatever the lengths (each workgroup adds the
 // lengths up itself: no host knows them).  A workgroup whose range covers a
@@ -420,8 +420,14 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
 // join.
 constexpr int kFewWaves = 8;
-constexpr int kFewTile = 32;                       // rows of K / V per wave and step
-constexpr int kUnit = kFewTile * kFewWaves;
+// Rows of K / V per wave and step: 32, or 64 of 64 dims in 4 bits, which then
+// have as many bytes under way as others (3 tokens each of 12 sequences over 4000 ..
+// 60000 rows, 8 heads: 46 us instead of 54, one over 131072 28.6 instead of 29.9).
+// At 64 bytes a row the larger step is no better (one token each of 40 sequences
+// over 300 .. 40000, 4 heads: 75 us instead of 71 in 4 bits, 71 instead of 67 in 8
+// of 64 dims), at 128 worse.
+template <int BITS, int D>
+constexpr int kFewTile = D * BITS <= 8 * 32 ? 64 : 32;
 
 // How both kernels cut their work: range w of 2^log is the units
 // [cut(w), cut(w + 1)), with a range per workgroup, or for little work about
@@ -431,6 +437,13 @@ constexpr int kUnit = kFewTile * kFewWaves;
 // the first that the range meets, 2 w + 1 for the last.  The range that holds
 // unit lo leaves a Join where hi lies past its end, and merge_kernel joins the
 // partials of the ranges from there on, in order.
+//
+// To begin and to end a (sequence, head) costs about as much time as two units
+// of codes (6 us: lookups, queries, first loads, the join of the waves), so
+// FewLoads::kLead units that hold no rows come before each in the count, and a
+// range that holds none but these has no part in it.  One token each of 40
+// sequences over 300 .. 40000 rows, 4 heads of 128 dims: int8 107 -> 82 us, fp8 98
+// -> 85, fp4 88 -> 72 (1: 91, 87, 78; 4: 85, 87, 73).
 struct Join {
     int64_t total;      // units in all
     int64_t lo, hi;     // lo = hi: nothing to join
@@ -445,11 +458,12 @@ __device__ __forceinline__ int ranges_log(int w_log, int64_t total) {
 }
 __device__ __forceinline__ int64_t cut(int64_t total, int64_t w, int log) { return (total * w) >> log; }
 
+template <int UNIT, int LEAD>
 __device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
     const int rows = q.n * a.G;
     if (q.n <= 0 || rows < a.min_rows || rows > a.max_rows) return 0;
     const Span sp = span_of(a, q, max(q.p0, 0), q.len - 1);
-    return max((sp.count() + kUnit - 1) / kUnit, 1);
+    return max((sp.count() + UNIT - 1) / UNIT, 1) + LEAD;
 }
 
 // a / b, fast where it fits 32 bits
@@ -464,13 +478,13 @@ struct FewRange {
     int64_t total, g0, g1, before;
     int s;
 };
-template <bool SH>
+template <bool SH, int UNIT, int LEAD>
 __device__ __forceinline__ FewRange few_range(const PagedParams& a) {
     FewRange r{0, 0, 0, 0, 0};
     int u = 0, incl = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         const int s = s0 + lane_id();
-        u = s < a.S ? few_units(a, seq_of<SH>(a, s)) : 0;
+        u = s < a.S ? few_units<UNIT, LEAD>(a, seq_of<SH>(a, s)) : 0;
         incl = wave_incl_scan(u);
         r.total += __builtin_amdgcn_readlane(incl, 63);
     }
@@ -483,7 +497,7 @@ __device__ __forceinline__ FewRange few_range(const PagedParams& a) {
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         if (a.S > 64) {   // else the only 64 are still at hand
             const int s = s0 + lane_id();
-            u = s < a.S ? few_units(a, seq_of<SH>(a, s)) : 0;
+            u = s < a.S ? few_units<UNIT, LEAD>(a, seq_of<SH>(a, s)) : 0;
             incl = wave_incl_scan(u);
         }
         const uint64_t past = __ballot((r.before + incl) * a.H > r.g0);
@@ -508,7 +522,9 @@ struct FewLoads {
     static constexpr int kPiece = (kWords < 4 ? kWords : 4) * 32 / C::kBits;     // dims of a piece
     static constexpr int kFrags = kPiece / 8;                                    // matrix instructions of a piece
     static constexpr int CH = D * C::kBits / 128;                                // 16-byte pieces of a V row
-    static constexpr int NV = kFewTile * CH / 64;                                // loads of a tile of V
+    static constexpr int kTile = kFewTile<C::kBits, D>;
+    static constexpr int kLead = C::kBits == 16 ? 0 : 2;
+    static constexpr int NV = kTile * CH / 64;                                   // loads of a tile of V
     static constexpr int kDims = 128 / C::kBits;                                 // dims of such a piece
     // first of the 8 dims that instruction c takes from lane group lg
     static __device__ __forceinline__ int frag_dim(int c, int lg) {
@@ -522,10 +538,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
     typedef FewLoads<C, D> Lo;
+    constexpr int LEAD = Lo::kLead;
     constexpr bool kCodes = C::kBits != 16;
     constexpr int CH = Lo::CH, NV = Lo::NV;          // 16-byte pieces of a row, loads of a tile of V
-    constexpr int NF = NV * Lo::kDims / 8;           // the tile's pieces of 8 dims
-    constexpr int kWaveLds = kFewTile * LR > 16 * D * 2 ? kFewTile * LR : 16 * D * 2;   // u16
+    constexpr int TILE = Lo::kTile, UNIT = TILE * kFewWaves, KB = TILE / 16;   // KB: blocks of 16 rows
+    constexpr int kWaveLds = TILE * LR > 16 * D * 2 ? TILE * LR : 16 * D * 2;   // u16
     __shared__ __align__(16) uint16_t s_buf[kFewWaves * kWaveLds];
     static_assert(__alignof__(s_buf) >= 16 && kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0,
                   "rows and partials are read and written 16 bytes at a time");
@@ -546,12 +563,12 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     if (direct) {     // a workgroup per (sequence, head): nothing to join
         range.s = blockIdx.x / a.H;
         range.before = 0;
-        const int u = few_units(a, seq_of<SH>(a, range.s));
+        const int u = few_units<UNIT, LEAD>(a, seq_of<SH>(a, range.s));
         if (u == 0) return;
         range.g0 = static_cast<int64_t>(blockIdx.x % a.H) * u;
         range.g1 = range.g0 + u;
     } else {
-        range = few_range<SH>(a);
+        range = few_range<SH, UNIT, LEAD>(a);
     }
     int64_t g0 = range.g0;
     const int64_t g1 = range.g1;
@@ -561,15 +578,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     Join rest{};
     while (g0 < g1) {
         const Seq sq = seq_of<SH>(a, s);
-        const int units = few_units(a, sq);
+        const int units = few_units<UNIT, LEAD>(a, sq);
         if (g0 >= base + static_cast<int64_t>(units) * a.H) {   // next sequence
             base += static_cast<int64_t>(units) * a.H;
             ++s;
             continue;
         }
         const int h = direct ? blockIdx.x % a.H : quotient(g0 - base, units);
-        const int u0 = static_cast<int>(g0 - base - static_cast<int64_t>(h) * units);
-        const int u1 = static_cast<int>(min(static_cast<int64_t>(units), u0 + g1 - g0));
+        const int at = static_cast<int>(g0 - base - static_cast<int64_t>(h) * units);
+        const int end = static_cast<int>(min(static_cast<int64_t>(units), at + g1 - g0));
+        const int u0 = max(at - LEAD, 0), u1 = end - LEAD;   // of the units that hold rows
+        if (LEAD > 0 && u1 <= u0) {
+            g0 += end - at;
+            continue;
+        }
         const int rows = sq.n * a.G;
         const int p0 = sq.p0;
         const Span sp = span_of(a, sq, max(p0, 0), sq.len - 1);
@@ -614,25 +636,32 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
         const uint8_t* const kc = reinterpret_cast<const uint8_t*>(a.k) + static_cast<int64_t>(h) * a.head_s +
                                   lg * (Lo::kPiece * C::kBits / 8);
         const uint8_t* const vc = reinterpret_cast<const uint8_t*>(a.v) + static_cast<int64_t>(h) * a.head_s + 16 * (lane % CH);
-        const uint8_t* const kx = a.ke + static_cast<int64_t>(h) * a.e_head_s;
-        const uint8_t* const vx = a.ve + static_cast<int64_t>(h) * a.e_head_s + Lo::kDims * (lane % CH) / kBlock;
+        const uint8_t* const kx = (TILE == 64 || lane < 32 ? a.ke : a.ve) + static_cast<int64_t>(h) * a.e_head_s;
+        const uint8_t* const vx = a.ve + static_cast<int64_t>(h) * a.e_head_s;
         // lane's rows of a step's tile: of K ln and 16 + ln (the matrix
         // instruction's), of V, which goes through LDS, whole rows of CH lanes
-        auto row_of = [&](int u, int r) { return sp.row(min(u * kUnit + wave * kFewTile + r, vis - 1)); };
+        auto row_of = [&](int u, int r) { return sp.row(min(u * UNIT + wave * TILE + r, vis - 1)); };
         auto k_row = [&](int u, int e) { return row_of(u, 16 * e + ln); };
         auto v_row = [&](int u, int i) { return row_of(u, (64 / CH) * i + lane / CH); };
-        int idk[2] = {s, s}, idv[NV];
+        // (codes: lane r looks row r up and holds its exponents, of K and of V, in
+        // a tile of 32 rows lane 32 + r those of V; lanes get them from there)
+        int idk[2] = {s, s}, idv[NV], id = s;
 #pragma unroll
         for (int i = 0; i < NV; ++i) idv[i] = s;
         auto fetch_ids = [&](int u) {
             if (!a.table) return;
+            if constexpr (kCodes) {
+                id = page_of(a, s, row_of(u, lane % TILE));
+                return;
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) idk[e] = page_of(a, s, k_row(u, e));
 #pragma unroll
             for (int i = 0; i < NV; ++i) idv[i] = page_of(a, s, v_row(u, i));
         };
-        u32x4_t kb[kCodes ? 1 : 2][KK], vb[NF];
-        uint32_t kw[2][Lo::kWords], vw[NV][4], ke[2], ve[NV];   // codes and exponents
+        u32x4_t kb[kCodes ? 1 : 2][KK], vb[kCodes ? 1 : NV];
+        uint32_t kw[KB][Lo::kWords], vw[NV][4], ke = 0, ve = 0;   // codes and exponents
+        auto from = [](int lane, uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * lane, x)); };
         auto fetch = [&](int u) {
             if constexpr (!kCodes) {
 #pragma unroll
@@ -644,12 +673,15 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
                 for (int i = 0; i < NV; ++i) vb[i] = load16(vh + row_offset(a, idv[i], v_row(u, i)));
             } else {
+                const int j = row_of(u, lane % TILE);
+                const uint64_t mine = row_offset(a, id, j);
+                auto offset = [&](int lane) {
+                    return static_cast<uint64_t>(from(lane, mine >> 32)) << 32 | from(lane, mine);
+                };
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int j = k_row(u, e);
-                    const uint8_t* const row = kc + row_offset(a, idk[e], j);
-                    const uint8_t* const x = kx + exp_offset(a, idk[e], j);
-                    if constexpr (Lo::kWords > 4) {   // two pieces, of two blocks
+                for (int e = 0; e < KB; ++e) {
+                    const uint8_t* const row = kc + offset(16 * e + ln);
+                    if constexpr (Lo::kWords > 4) {   // two pieces
 #pragma unroll
                         for (int p = 0; p < 2; ++p) {
                             uint32_t w[4];
@@ -657,26 +689,19 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 #pragma unroll
                             for (int i = 0; i < 4; ++i) kw[e][4 * p + i] = w[i];
                         }
-                        ke[e] = *reinterpret_cast<const uint32_t*>(x);
                     } else {
                         load_words<Lo::kWords>(row, kw[e]);
-                        ke[e] = x[Lo::kPiece * lg / kBlock];
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int j = v_row(u, i);
-                    load_words<4>(vc + row_offset(a, idv[i], j), vw[i]);
-                    ve[i] = vx[exp_offset(a, idv[i], j)];
-                }
-            }
-        };
-        auto key = [&](int e, int c) {
-            if constexpr (!kCodes) {
-                return kb[e][c];
-            } else {
-                const uint32_t x = Lo::kWords > 4 ? (ke[e] >> (8 * (Lo::frag_dim(c, lg) / kBlock))) & 255u : ke[e];
-                return decode8<T, C>(kw[e], c, x);
+                for (int i = 0; i < NV; ++i) load_words<4>(vc + offset((64 / CH) * i + lane / CH), vw[i]);
+                auto load_exps = [&](const uint8_t* p) -> uint32_t {
+                    if constexpr (D == 128) return *reinterpret_cast<const uint32_t*>(p);
+                    else return *reinterpret_cast<const uint16_t*>(p);
+                };
+                const int64_t x = exp_offset(a, id, j);
+                ke = load_exps(kx + x);
+                if constexpr (TILE == 64) ve = load_exps(vx + x);
             }
         };
         // a wave with no row in its share of a unit still runs the step (all
@@ -688,38 +713,68 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             fetch_ids(min(u0 + 1, u1 - 1));
         }
         for (int u = u0; any && u < u1; ++u) {
-            const int v0 = u * kUnit + wave * kFewTile;   // first row of the tile
-            if constexpr (kCodes) {
-#pragma unroll
-                for (int i = 0; i < NF; ++i)
-                    vb[i] = decode8<T, C>(vw[i / (NF / NV)], i % (NF / NV), ve[i / (NF / NV)]);
-            }
-            if (v0 + kFewTile > vis) {   // rows past the end weigh nothing: no NaN may enter through V
-#pragma unroll
-                for (int i = 0; i < NF; ++i)
-                    if (v0 + (64 / CH) * (i / (NF / NV)) + lane / CH >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
-            }
-            const int j_lo = sp.row(v0), j_hi = sp.row(v0 + kFewTile - 1);
-            const bool full = v0 + kFewTile <= vis && j_hi <= p0 &&
+            const int v0 = u * UNIT + wave * TILE;   // first row of the tile
+            const int j_lo = sp.row(v0), j_hi = sp.row(v0 + TILE - 1);
+            const bool full = v0 + TILE <= vis && j_hi <= p0 &&
                               (a.window == 0 || j_lo >= sq.len - a.window || j_hi < a.sinks);
-            if (!full && sq.n > 1) {   // (one token sees every row of its span)
-                if (__builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
-                    keep_finite<T>(vb);
-                    s_odd = 1;
-                }
-            }
+            const bool look = !full && sq.n > 1;   // (one token sees every row of its span)
+            uint16_t* const sv_row = sv + lane / CH * LR + Lo::kDims * (lane % CH);
+            if constexpr (!kCodes) {
+                if (v0 + TILE > vis) {   // rows past the end weigh nothing: no NaN may enter through V
 #pragma unroll
-            for (int i = 0; i < NF; ++i)
-                *reinterpret_cast<u32x4_t*>(sv + ((64 / CH) * (i / (NF / NV)) + lane / CH) * LR + Lo::kDims * (lane % CH) +
-                                            8 * (i % (NF / NV))) = vb[i];
-            f32x4_t sc[NB][2];
+                    for (int i = 0; i < NV; ++i)
+                        if (v0 + (64 / CH) * i + lane / CH >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
+                }
+                if (look) {
+                    if (__builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
+                        keep_finite<T>(vb);
+                        s_odd = 1;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4_t*>(sv_row + (64 / CH) * i * LR) = vb[i];
+            } else {   // the same, piece by piece
+                bool odd = false;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int r = (64 / CH) * i + lane / CH;
+                    const uint32_t x4 = TILE == 64 ? from(r, ve) : from(32 + r, ke);
+                    const uint32_t e = (x4 >> (8 * (Lo::kDims * (lane % CH) / kBlock))) & 255u;
+#pragma unroll
+                    for (int k = 0; k < Lo::kDims / 8; ++k) {
+                        u32x4_t x[1] = {decode8<T, C>(vw[i], k, e)};
+                        if (!full) {
+                            if (v0 + (64 / CH) * i + lane / CH >= vis) x[0] = u32x4_t{0, 0, 0, 0};
+                            if (look) {
+                                odd |= !all_finite<T>(x);
+                                keep_finite<T>(x);
+                            }
+                        }
+                        *reinterpret_cast<u32x4_t*>(sv_row + (64 / CH) * i * LR + 8 * k) = x[0];
+                    }
+                }
+                if (look && __builtin_amdgcn_ballot_w64(odd)) s_odd = 1;
+            }
+            f32x4_t sc[NB][KB];
 #pragma unroll
             for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < KB; ++e) {
                     sc[b][e] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (!kCodes)
 #pragma unroll
-                    for (int c = 0; c < KK; ++c) sc[b][e] = T::mma16(key(e, c), query(b, c), sc[b][e]);
+                        for (int c = 0; c < KK; ++c) sc[b][e] = T::mma16(kb[e][c], query(b, c), sc[b][e]);
+                }
+            if constexpr (kCodes)
+#pragma unroll
+                for (int e = 0; e < KB; ++e) {
+                    const uint32_t x4 = from(16 * e + ln, ke);
+#pragma unroll
+                    for (int c = 0; c < KK; ++c) {
+                        const u32x4_t k8 = decode8<T, C>(kw[e], c, (x4 >> (8 * (Lo::frag_dim(c, lg) / kBlock))) & 255u);
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) sc[b][e] = T::mma16(k8, query(b, c), sc[b][e]);
+                    }
                 }
             if (u + 1 < u1) {
                 fetch(u + 1);
@@ -727,20 +782,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             }
             wave_lds_sync();
             // lane: keys v0 + 16 e + 4 lg + i of row ln
-            u32x4_t pf[NB];
+            u32x4_t pf[NB][KB / 2];
 #pragma unroll
             for (int b = 0; b < NB; ++b) {
                 if (!full) {
                     const Sees sees(a, pos[b], sp.lo - sp.sink, sp.sink, vis);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e)
+                    for (int e = 0; e < KB; ++e)
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             sc[b][e][i] = sees.row(16 * e + i, v0 + 4 * lg) ? sc[b][e][i] : -INFINITY;
                 }
                 float mx = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < KB; ++e)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[b][e][i]);
                 mx = fmaxf(mx, xor16(mx));
@@ -758,22 +813,28 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                     const float off = fabsf(mc) > kFar ? m[b] : 0.0f;
                     mc = fabsf(mc) > kFar ? 0.0f : mc;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) sc[b][i >> 2][i & 3] -= off;
+                    for (int i = 0; i < 4 * KB; ++i) sc[b][i >> 2][i & 3] -= off;
                 }
                 mc -= T::kShift;
-                float p[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][i >> 2][i & 3], a.c, -mc));
-                l[b] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                pf[b] = u32x4_t{T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                for (int x = 0; x < KB / 2; ++x) {
+                    float p[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][2 * x + (i >> 2)][i & 3], a.c, -mc));
+                    l[b] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    pf[b][x] = u32x4_t{T::pack(p[0], p[1]), T::pack(p[2], p[3]), T::pack(p[4], p[5]), T::pack(p[6], p[7])};
+                }
             }
 #pragma unroll
             for (int d = 0; d < DB; ++d) {
-                const uint16_t* vp = sv + (4 * lg + (ln >> 2)) * LR + 16 * d + 4 * (ln & 3);
-                const u32x4_t vt = join(read_tr(vp), read_tr(vp + 16 * LR));
 #pragma unroll
-                for (int b = 0; b < NB; ++b) acc[b][d] = T::mma16(vt, pf[b], acc[b][d]);
+                for (int x = 0; x < KB / 2; ++x) {
+                    const uint16_t* vp = sv + (32 * x + 4 * lg + (ln >> 2)) * LR + 16 * d + 4 * (ln & 3);
+                    const u32x4_t vt = join(read_tr(vp), read_tr(vp + 16 * LR));
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[b][d] = T::mma16(vt, pf[b][x], acc[b][d]);
+                }
             }
             wave_lds_sync();
         }
@@ -787,7 +848,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                 s_ml[wave][16 * b + ln][1] = l[b];
             }
         }
-        const bool whole = u0 == 0 && u1 == units;
+        const bool whole = u0 == 0 && u1 == units - LEAD;
         bool odd = false;
         const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
         float* const so = reinterpret_cast<float*>(sv);   // [16 rows][D]
@@ -842,14 +903,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
         if (odd) {
             __threadfence();
             __syncthreads();
-            patch_rows<T, D, C, SH>(a, sq, s, h, sp, 0, rows, u0 * kUnit, min(u1 * kUnit, vis), whole ? -1 : slot);
+            patch_rows<T, D, C, SH>(a, sq, s, h, sp, 0, rows, u0 * UNIT, min(u1 * UNIT, vis), whole ? -1 : slot);
             __syncthreads();
             if (tid == 0) s_odd = 0;
             __syncthreads();
         }
-        if (u0 == 0 && u1 < units)
-            rest = Join{range.total, g0, g0 + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G, sq.lo};
-        g0 += u1 - u0;
+        if (u0 == 0 && u1 < units - LEAD)
+            rest = Join{range.total, g0 - at, g0 - at + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G, sq.lo};
+        g0 += end - at;
         first = false;
     }
     if (!direct && tid == 0) a.joins[blockIdx.x] = rest;
@@ -860,7 +921,7 @@ struct Parts {
     const Join* joins;
     const float* rows;   // [2 W][cap][D]
     const float* ml;     // [2 W][cap][2]
-    int cap;
+    int cap, lead;       // lead: units without rows before those of a (sequence, head)
 };
 struct MergeParams {
     Parts few, tiles;
@@ -899,7 +960,7 @@ struct Partial {
             for (int i = 0; i < N; ++i) {
                 const int wi = min(w + i * step, w1);
                 const int64_t b = cut(j.total, wi, log);
-                use[i] = w + i * step <= w1 && b != cut(j.total, wi + 1, log);
+                use[i] = w + i * step <= w1 && max(b, j.lo + p.lead) < cut(j.total, wi + 1, log);
                 const int64_t e = (2 * static_cast<int64_t>(wi) + (b < j.lo ? 1 : 0)) * p.cap + r;
                 m[i] = p.ml[2 * e];
                 l[i] = p.ml[2 * e + 1];
@@ -1373,32 +1434,38 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         const uint8_t* const kc = reinterpret_cast<const uint8_t*>(a.k) + static_cast<int64_t>(h) * a.head_s;
         const uint8_t* const vc = reinterpret_cast<const uint8_t*>(a.v) + static_cast<int64_t>(h) * a.head_s +
                                   4 * C::kWords * st.l_ch;
-        const uint8_t* const kx = a.ke + static_cast<int64_t>(h) * a.e_head_s;
-        const uint8_t* const vx = a.ve + static_cast<int64_t>(h) * a.e_head_s + 8 * st.l_ch / kBlock;
+        // and the exponents of a wave's 16 rows of K are in lanes 0 .. 15 (and
+        // 32 ..), of V in 16 .. 31
+        const uint8_t* const ex = (lane & 16 ? a.ve : a.ke) + static_cast<int64_t>(h) * a.e_head_s;
+        const int ex_row = 16 * wave + (lane & 15);
         // an easy step: one page lookup, one step ahead of its use, and one
         // address per thread
-        int id = s;
+        int id = s, ex_id = s;
         auto fetch_id = [&](int u) {
             if (a.table) id = page_of(a, s, sp.row(min(u * kStep + st.l_row, vis - 1)));
+            if constexpr (kCodes)
+                if (a.table) ex_id = page_of(a, s, sp.row(min(u * kStep + ex_row, vis - 1)));
         };
         u32x4_t vb[NR];
-        uint32_t kw[NR][C::kWords], vw[NR][C::kWords], ke[NR], ve[NR];   // codes and exponents
-        auto fetch_row = [&](int i, int64_t o, int64_t x) {
-            const int piece = st.k_piece ^ i;
-            load_words<C::kWords>(kc + o + 4 * C::kWords * piece, kw[i]);
-            ke[i] = kx[x + 8 * piece / kBlock];
+        uint32_t kw[NR][C::kWords], vw[NR][C::kWords], exps = 0;   // codes and exponents
+        auto fetch_row = [&](int i, int64_t o) {
+            load_words<C::kWords>(kc + o + 4 * C::kWords * (st.k_piece ^ i), kw[i]);
             load_words<C::kWords>(vc + o, vw[i]);
-            ve[i] = vx[x];
+        };
+        auto fetch_exps = [&](int u) {
+            const uint8_t* const p = ex + exp_offset(a, ex_id, sp.row(min(u * kStep + ex_row, vis - 1)));
+            if constexpr (D == 128) exps = *reinterpret_cast<const uint32_t*>(p);
+            else exps = *reinterpret_cast<const uint16_t*>(p);
         };
         auto fetch = [&](int u) {
             char* const sk = s_k + (u & 1) * 2 * SB;
+            if constexpr (kCodes) fetch_exps(u);
             if (u >= easy_lo && u < easy_hi) {
                 const int j = u * kStep + st.l_row + sp.shift;
                 const int64_t o = row_offset(a, id, j);
                 if constexpr (kCodes) {
-                    const int64_t x = exp_offset(a, id, j);
 #pragma unroll
-                    for (int i = 0; i < NR; ++i) fetch_row(i, o + i * a.tok_s, x + i * a.e_tok_s);
+                    for (int i = 0; i < NR; ++i) fetch_row(i, o + i * a.tok_s);
                 } else {
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
@@ -1413,7 +1480,7 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                     const int page = page_of(a, s, j);
                     const int64_t o = row_offset(a, page, j);
                     if constexpr (kCodes) {
-                        fetch_row(i, o, exp_offset(a, page, j));
+                        fetch_row(i, o);
                     } else {
                         st.load_k(kh + o, i, sk);
                         vb[i] = load16(vh + o);
@@ -1426,8 +1493,15 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                 char* const sk = s_k + (u & 1) * 2 * SB;
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
-                    st.store_k(decode8<T, C>(kw[i], 0, ke[i]), i, sk);
-                    vb[i] = decode8<T, C>(vw[i], 0, ve[i]);
+                    const int from = 4 * (NR * (lane / Stage<D>::CH) + i);
+                    const uint32_t e = __builtin_amdgcn_ds_bpermute(from, exps);
+                    st.store_k(decode8<T, C>(kw[i], 0, (e >> (8 * ((st.k_piece ^ i) / 4))) & 255u), i, sk);
+                }
+#pragma unroll
+                for (int i = 0; i < NR; ++i) {
+                    const int from = 4 * (16 + NR * (lane / Stage<D>::CH) + i);
+                    const uint32_t e = __builtin_amdgcn_ds_bpermute(from, exps);
+                    vb[i] = decode8<T, C>(vw[i], 0, (e >> (8 * (st.l_ch / 4))) & 255u);
                 }
             }
             if (u < plain_lo || u >= plain_hi) {   // no NaN may enter through a row that is not seen
@@ -1658,14 +1732,14 @@ struct Shape {
     bool tiles = false;
     int tile_most = 0;      // rows of a tile that can be in use
     int slots = 0;
-    size_t few_part = 0, tile_part = 0, plan = 0, joins = 0;   // workspace bytes
+    size_t few_part = 0, tile_part = 0, plan = 0;   // workspace bytes
 };
 
-// A workgroup per (sequence, head) up to this many units.  One sequence of 519
+// A workgroup per (sequence, head) up to this many rows.  One sequence of 519
 // rows of 128 dims called in a loop takes 13.3 us so, 15.4-15.9 with a join, whose
 // workspace and second launch cost the host more than the GPU gains (replayed
 // in a graph: 512, 768, 1024 rows 11.3, 14.1, 16.8 us without, 11.4 each with).
-constexpr int kDirectUnits = 3;
+constexpr int kDirectRows = 768;
 constexpr int kDirectGrid = 1 << 22;   // workgroups of 512 threads in a launch of at most 2^32 - 1
 
 inline Shape shape_of(const imi_paged_attention_args* a) {
@@ -1676,7 +1750,6 @@ inline Shape shape_of(const imi_paged_attention_args* a) {
     p.max_rows = static_cast<int>(most);
     // a workgroup of eight waves per CU: its registers and LDS fill one
     while ((2 << p.w_log) <= std::min(device_cus(), kMaxRanges)) ++p.w_log;
-    p.joins = sizeof(Join) << p.w_log;
     if (most <= 32) {
         p.few_rows = most <= 16 ? 16 : 32;
     } else {
@@ -1698,7 +1771,7 @@ inline Shape shape_of(const imi_paged_attention_args* a) {
         int64_t longest = cap;   // visible rows of the longest sequence
         if (a->window > 0)
             longest = std::min<int64_t>(cap, static_cast<int64_t>(a->window) + a->sinks + p.few_rows / a->groups);
-        p.direct = (longest + kUnit - 1) / kUnit <= kDirectUnits &&
+        p.direct = longest <= kDirectRows &&
                    static_cast<int64_t>(b.n_seqs) * a->kv_heads <= kDirectGrid;
         if (!p.direct) p.few_part = (size_t(2) << p.w_log) * p.most * (a->dim + 2) * sizeof(float);
     }
@@ -1719,7 +1792,6 @@ inline Shape common_shape_of(const imi_paged_attention_args* a) {
     const int64_t most = static_cast<int64_t>(b.n_tokens) * a->groups;
     p.max_rows = static_cast<int>(most);
     while ((2 << p.w_log) <= std::min(device_cus(), kMaxRanges)) ++p.w_log;
-    p.joins = sizeof(Join) << p.w_log;
     p.tiles = true;
     p.slots = static_cast<int>(most / kTileRows + b.n_seqs);
     p.tile_most = static_cast<int>(std::min<int64_t>(most, kTileRows));
@@ -1735,7 +1807,7 @@ struct Rooms {
 };
 inline size_t carve(const Shape& p, void* base, Rooms& r) {
     Carver c(base);
-    r.joins = c.take<Join>(2 * (p.joins / sizeof(Join)));   // of the few-row launch, of the tile launch
+    r.joins = c.take<Join>(size_t(2) << p.w_log);   // of the few-row launch, of the tile launch
     r.few = c.take<float>(p.few_part / sizeof(float));
     r.tile = c.take<float>(p.tile_part / sizeof(float));
     r.plan = c.take<int32_t>(p.plan / sizeof(int32_t));
@@ -1816,8 +1888,10 @@ int launch(const Shape& p, PagedParams P, const Rooms& room, hipStream_t stream)
     }
     const int few_blocks = p.few_rows && !p.direct ? W * p.most : 0;
     if (few_blocks || p.tiles) {
-        const MergeParams M{{F.joins, F.part, F.part_ml, F.cap}, {Q.joins, Q.part, Q.part_ml, Q.cap}, P.out, P.lse,
-                            P.o_ts, P.o_hs, P.l_ts, few_blocks, P.H, P.G, P.w_log, P.c, P.px, P.px_ml, P.common};
+        const MergeParams M{{F.joins, F.part, F.part_ml, F.cap, FewLoads<C, D>::kLead},
+                            {Q.joins, Q.part, Q.part_ml, Q.cap, 0}, P.out, P.lse,
+                            P.o_ts, P.o_hs, P.l_ts, few_blocks, P.H, P.G, p.w_log, P.c, P.px,
+                            P.px_ml, P.common};
         // for the tiles: the pairs there can be, as far as workgroups are worth it
         const int64_t pairs = std::min<int64_t>(W, int64_t(p.slots) * P.H) * p.tile_most;
         const int more = p.tiles ? static_cast<int>(std::min<int64_t>(8 * W, pairs)) : 0;
