@@ -154,9 +154,10 @@ struct PagedParams {
     // shared first rows (see Seq)
     const int32_t* shared;     // [S] rows, or null
     const int32_t* members;    // [S] sequences of the run that s leads, or 0
-    bool common;               // this launch attends the shared rows, not the others
-    float* px;                 // [N][H G][D] what the shared rows gave each query row,
-    float* px_ml;              // [N][H G][2] its maximum and sum
+    bool common;               // the shared rows are attended, not the others
+    float* keep;               // [N][H G][D] rows that one range attended whole, before the division,
+    float* keep_ml;            // [N][H G][2] their maxima and sums
+    int32_t* place;            // [keys][H] where a tile's rows are: see place_key
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -164,12 +165,11 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x,
 // New tokens [t0, t0 + n), length, position of the first new token and first
 // row to attend of sequence s, forced into the tensors.
 //
-// With shared first rows (SH) a call attends twice.  First, of each run of
-// sequences that begin with the same pages, the rows that all of them share, by
-// the tokens of all: one problem, led by the run's first sequence, whose rows
-// all tokens see (p0 at its end).  Its results stay as they are before the
-// division (px), and what then writes the rows of a sequence from `lo` on adds
-// them.
+// With shared first rows (SH) a call attends two kinds of problem: of each run
+// of sequences that begin with the same pages, the rows that all of them share,
+// by the tokens of all (common: led by the run's first sequence, and all tokens
+// see all rows, p0 being their end); and of each sequence its rows from `lo` on.
+// What either gives a query row is joined afterwards (join_kernel).
 struct Seq {
     int t0, n, len, p0, lo;
 };
@@ -339,10 +339,10 @@ __device__ __forceinline__ void patch_rows(const PagedParams& a, const Seq& sq, 
             if (!(m >> 16)) add[1] += T::wide(w >> 16);
         }
         if (add[0] == 0.0f && add[1] == 0.0f) continue;
-        if (slot >= 0 || (SH && a.common)) {
+        if (slot >= 0 || (SH && (a.common || sq.lo > 0))) {
             float* const o =
                 slot >= 0 ? a.part + (slot * a.cap + r - first) * D + d
-                          : a.px + (static_cast<int64_t>(sq.t0 + r / a.G) * (a.H * a.G) + h * a.G + r % a.G) * D + d;
+                          : a.keep + (static_cast<int64_t>(sq.t0 + r / a.G) * (a.H * a.G) + h * a.G + r % a.G) * D + d;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 o[i] = __hip_atomic_load(o + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + add[i];
@@ -359,34 +359,12 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
 }
 
-// Four dims of a row's sums: what the shared rows gave is kept (true), or added.
-template <int D>
-__device__ __forceinline__ bool shared_rows(float* px, float* px_ml, bool common, int lo, int heads, int64_t t, int head,
-                                            int d4, float c, float& M, float& L, f32x4_t& A) {
-    const int64_t e = t * heads + head;
-    f32x4_t* const x = reinterpret_cast<f32x4_t*>(px + e * D + 4 * d4);
-    if (common) {
-        *x = A;
-        if (d4 == 0) {
-            px_ml[2 * e] = M;
-            px_ml[2 * e + 1] = L;
-        }
-        return true;
-    }
-    if (lo > 0) {
-        const float m = px_ml[2 * e], l = px_ml[2 * e + 1];
-        const float Mn = fmaxf(M, m);
-        const float f0 = exp2_weight(M, Mn, c), f1 = exp2_weight(m, Mn, c);
-        L = L * f0 + l * f1;
-        A = A * f0 + *x * f1;
-        M = Mn;
-    }
-    return false;
-}
-template <int D>
-__device__ __forceinline__ bool shared_rows(const PagedParams& a, const Seq& q, int64_t t, int head, int d4, float& M,
-                                            float& L, f32x4_t& A) {
-    return shared_rows<D>(a.px, a.px_ml, a.common, q.lo, a.H * a.G, t, head, d4, a.c, M, L, A);
+// Where the rows of a problem (r0 ..: its first row, or of a tile) are with
+// shared rows, for each head: -1, in `keep`, or the range that holds its first
+// unit, in that range's partials and those after it.  Problems begin at query
+// rows t0 G in the order of s, so no two tiles have the same key.
+__device__ __forceinline__ int place_key(const PagedParams& a, int t0, int s, int r0) {
+    return static_cast<int>((static_cast<int64_t>(t0) * a.G + r0) / 256) + s;
 }
 
 // What a row's sum L of weights divides by: nothing for a row that sees nothing
@@ -451,7 +429,6 @@ struct Join {
     int first, end;     // rows (token, head of the group) [first, end)
     int h;
     int blind;          // the sequence's rows before this one see nothing (more new tokens than rows)
-    int from;           // Seq::lo
 };
 __device__ __forceinline__ int ranges_log(int w_log, int64_t total) {
     return total <= 1 ? 0 : min(w_log, 64 - __builtin_clzll(static_cast<uint64_t>(total - 1)));
@@ -479,7 +456,7 @@ struct FewRange {
     int s;
 };
 template <bool SH, int UNIT, int LEAD>
-__device__ __forceinline__ FewRange few_range(const PagedParams& a) {
+__device__ __forceinline__ FewRange few_range(const PagedParams& a, int block) {
     FewRange r{0, 0, 0, 0, 0};
     int u = 0, incl = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
@@ -490,9 +467,9 @@ __device__ __forceinline__ FewRange few_range(const PagedParams& a) {
     }
     r.total *= a.H;
     const int log = ranges_log(a.w_log, r.total);
-    if (blockIdx.x >> log) return r;
-    r.g0 = cut(r.total, blockIdx.x, log);
-    r.g1 = cut(r.total, blockIdx.x + 1, log);
+    if (block >> log) return r;
+    r.g0 = cut(r.total, block, log);
+    r.g1 = cut(r.total, block + 1, log);
     if (r.g0 >= r.g1) return r;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
         if (a.S > 64) {   // else the only 64 are still at hand
@@ -532,8 +509,22 @@ struct FewLoads {
     }
 };
 
+// The kernel's LDS: tiles of V (partials afterwards), maxima and sums, and the
+// queries where they are not in registers, as two blocks of 128 dims (32 registers
+// more than there are).
+template <typename C, int D, int NB>
+struct FewLds {
+    static constexpr bool kQuery = NB * D > 128;
+    static constexpr int kRows = FewLoads<C, D>::kTile * kRow<D>;
+    static constexpr int kWave = kRows > 16 * D * 2 ? kRows : 16 * D * 2;   // u16
+    uint16_t buf[kFewWaves * kWave];
+    uint16_t q[kQuery ? 16 * NB * kRow<D> : 8];
+    float ml[kFewWaves][16 * NB][2];
+    int odd;   // a masked tile held infinities or NaN
+};
+
 template <typename T, int D, int NB, typename C, bool SH>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, int direct) {
+__device__ __forceinline__ void few_body(const PagedParams& a, int direct, int block, FewLds<C, D, NB>& lds) {
     constexpr int KK = D / 32;     // matrix instructions over the head dim
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
@@ -542,16 +533,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
     constexpr bool kCodes = C::kBits != 16;
     constexpr int CH = Lo::CH, NV = Lo::NV;          // 16-byte pieces of a row, loads of a tile of V
     constexpr int TILE = Lo::kTile, UNIT = TILE * kFewWaves, KB = TILE / 16;   // KB: blocks of 16 rows
-    constexpr int kWaveLds = TILE * LR > 16 * D * 2 ? TILE * LR : 16 * D * 2;   // u16
-    __shared__ __align__(16) uint16_t s_buf[kFewWaves * kWaveLds];
-    static_assert(__alignof__(s_buf) >= 16 && kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0,
-                  "rows and partials are read and written 16 bytes at a time");
-    __shared__ float s_ml[kFewWaves][16 * NB][2];
-    __shared__ int s_odd;   // a masked tile held infinities or NaN
-    // Queries: in registers, but for two blocks of 128 dims (32 registers more
-    // than there are) in LDS.
-    constexpr bool kQueryLds = NB * D > 128;
-    __shared__ __align__(16) uint16_t s_q[kQueryLds ? 16 * NB * LR : 8];
+    constexpr int kWaveLds = FewLds<C, D, NB>::kWave;
+    constexpr bool kQueryLds = FewLds<C, D, NB>::kQuery;
+    static_assert(kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0, "rows and partials are read and written 16 bytes at a time");
+    uint16_t* const s_buf = lds.buf;
+    uint16_t* const s_q = lds.q;
+    auto& s_ml = lds.ml;
+    int& s_odd = lds.odd;
     const int tid = threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 15, lg = lane >> 4;
@@ -561,14 +549,14 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
 
     FewRange range;
     if (direct) {     // a workgroup per (sequence, head): nothing to join
-        range.s = blockIdx.x / a.H;
+        range.s = block / a.H;
         range.before = 0;
         const int u = few_units<UNIT, LEAD>(a, seq_of<SH>(a, range.s));
         if (u == 0) return;
-        range.g0 = static_cast<int64_t>(blockIdx.x % a.H) * u;
+        range.g0 = static_cast<int64_t>(block % a.H) * u;
         range.g1 = range.g0 + u;
     } else {
-        range = few_range<SH, UNIT, LEAD>(a);
+        range = few_range<SH, UNIT, LEAD>(a, block);
     }
     int64_t g0 = range.g0;
     const int64_t g1 = range.g1;
@@ -584,7 +572,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             ++s;
             continue;
         }
-        const int h = direct ? blockIdx.x % a.H : quotient(g0 - base, units);
+        const int h = direct ? block % a.H : quotient(g0 - base, units);
         const int at = static_cast<int>(g0 - base - static_cast<int64_t>(h) * units);
         const int end = static_cast<int>(min(static_cast<int64_t>(units), at + g1 - g0));
         const int u0 = max(at - LEAD, 0), u1 = end - LEAD;   // of the units that hold rows
@@ -850,7 +838,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
         }
         const bool whole = u0 == 0 && u1 == units - LEAD;
         bool odd = false;
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
+        const int64_t slot = 2 * static_cast<int64_t>(block) + (first ? 0 : 1);
         float* const so = reinterpret_cast<float*>(sv);   // [16 rows][D]
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
@@ -881,8 +869,17 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
                 if (whole) {
                     const int64_t t = sq.t0 + r / a.G;
                     const int x_head = h * a.G + r % a.G;
-                    if constexpr (SH)
-                        if (shared_rows<D>(a, sq, t, x_head, d4, M, L, A)) continue;
+                    if constexpr (SH) {
+                        if (a.common || sq.lo > 0) {
+                            const int64_t e = t * (a.H * a.G) + x_head;
+                            *reinterpret_cast<f32x4_t*>(a.keep + e * D + 4 * d4) = A;
+                            if (d4 == 0) {
+                                a.keep_ml[2 * e] = M;
+                                a.keep_ml[2 * e + 1] = L;
+                            }
+                            continue;
+                        }
+                    }
                     const float inv = inverse(L, p0 + r / a.G < 0);
                     uint2 o;
                     o.x = T::pack(A[0] * inv, A[1] * inv);
@@ -908,12 +905,20 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, i
             if (tid == 0) s_odd = 0;
             __syncthreads();
         }
+        if constexpr (SH)
+            if (u0 == 0 && tid == 0) a.place[static_cast<int64_t>(place_key(a, sq.t0, s, 0)) * a.H + h] = whole ? -1 : block;
         if (u0 == 0 && u1 < units - LEAD)
-            rest = Join{range.total, g0 - at, g0 - at + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G, sq.lo};
+            rest = Join{range.total, g0 - at, g0 - at + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G};
         g0 += end - at;
         first = false;
     }
-    if (!direct && tid == 0) a.joins[blockIdx.x] = rest;
+    if (!direct && tid == 0) a.joins[block] = rest;
+}
+
+template <typename T, int D, int NB, typename C, bool SH>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, int direct) {
+    __shared__ __align__(16) FewLds<C, D, NB> s_lds;
+    few_body<T, D, NB, C, SH>(a, direct, blockIdx.x, s_lds);
 }
 
 // What merge_kernel needs: the partials of the few-row launch and of the tiles.
@@ -921,7 +926,7 @@ struct Parts {
     const Join* joins;
     const float* rows;   // [2 W][cap][D]
     const float* ml;     // [2 W][cap][2]
-    int cap, lead;       // lead: units without rows before those of a (sequence, head)
+    int cap;
 };
 struct MergeParams {
     Parts few, tiles;
@@ -929,10 +934,8 @@ struct MergeParams {
     float* lse;
     int64_t o_ts, o_hs, l_ts;
     int few_blocks;      // workgroups for the few-row launch: W cap, or none
-    int H, G, w_log;
+    int G, w_log;
     float c;
-    float *px, *px_ml;   // as in PagedParams
-    bool common;
 };
 
 template <int D>
@@ -950,7 +953,7 @@ struct Partial {
     // loads under way at a time (behind a branch each they would be one); an
     // empty range, whose slot holds anything, and one past w1 are left out
     __device__ __forceinline__ void gather(const Parts& p, const Join& j, int log, int w0, int w1, int r, int d4,
-                                           int first, int step, float c) {
+                                           int first, int step, float c, int lead) {
         constexpr int N = 4;
         for (int w = w0 + first; w <= w1; w += N * step) {
             float m[N], l[N];
@@ -960,7 +963,7 @@ struct Partial {
             for (int i = 0; i < N; ++i) {
                 const int wi = min(w + i * step, w1);
                 const int64_t b = cut(j.total, wi, log);
-                use[i] = w + i * step <= w1 && max(b, j.lo + p.lead) < cut(j.total, wi + 1, log);
+                use[i] = w + i * step <= w1 && (lead > 0 ? max(b, j.lo + lead) : b) < cut(j.total, wi + 1, log);
                 const int64_t e = (2 * static_cast<int64_t>(wi) + (b < j.lo ? 1 : 0)) * p.cap + r;
                 m[i] = p.ml[2 * e];
                 l[i] = p.ml[2 * e + 1];
@@ -971,12 +974,10 @@ struct Partial {
                 if (use[i]) add(m[i], l[i], x[i], c);
         }
     }
-    template <typename T, bool SH>
-    __device__ __forceinline__ void write(const MergeParams& a, const Join& j, int row, int d4) {
+    template <typename T>
+    __device__ __forceinline__ void write(const MergeParams& a, const Join& j, int row, int d4) const {
         const int64_t tok = j.t0 + row / a.G;
         const int head = j.h * a.G + row % a.G;
-        if constexpr (SH)
-            if (shared_rows<D>(a.px, a.px_ml, a.common, j.from, a.H * a.G, tok, head, d4, a.c, M, L, A)) return;
         const float inv = inverse(L, row < j.blind);
         uint2 o;
         o.x = T::pack(A[0] * inv, A[1] * inv);
@@ -985,6 +986,20 @@ struct Partial {
         if (a.lse && d4 == 0) a.lse[tok * a.l_ts + head] = log_sum<T>(M, L, a.c);
     }
 };
+
+// the last range that holds some of a join: about hi W / total, then exactly
+__device__ __forceinline__ int last_of(const Join& j, int w0, int log) {
+    int w1 = max(w0, static_cast<int>(static_cast<float>(j.hi - 1) / static_cast<float>(j.total) * (1 << log)) - 1);
+    while (cut(j.total, w1 + 1, log) < j.hi) ++w1;
+    return w1;
+}
+
+// groups of D / 4 threads to a row of so many partials, of P
+__device__ __forceinline__ int groups_of(int parts, int P) {
+    int K = 1;
+    while (K < P && 4 * K < parts) K *= 2;
+    return K;
+}
 
 // Joins what the ranges left.  D / 4 threads hold a row's partial, so a
 // workgroup holds P of them: P / K rows with K groups each, K about a quarter
@@ -999,7 +1014,7 @@ struct Partial {
 constexpr int kMergeThreads = 256;
 constexpr int kMaxRanges = kMergeThreads;   // (a thread looks at one)
 
-template <typename T, int D, bool SH>
+template <typename T, int D, int LEAD>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
     constexpr int Q = D / 4, P = kMergeThreads / Q;
     __shared__ float s_ml[P][2];
@@ -1010,11 +1025,11 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
     const int tid = threadIdx.x, W = 1 << a.w_log;
     const int d4 = tid % Q, g = tid / Q;
     // rows r0 .. of a join that range w0 left, K groups to a row
-    auto merge = [&](const Parts& from, const Join& j, int w0, int w1, int log, int r0, int K) {
+    auto merge = [&](const Parts& from, const Join& j, int w0, int w1, int log, int r0, int K, int lead) {
         const int r = r0 + g / K, k = g % K;
         const bool live = r < j.end - j.first;
         Partial<D> p;
-        if (live) p.gather(from, j, log, w0, w1, r, d4, k, K, a.c);
+        if (live) p.gather(from, j, log, w0, w1, r, d4, k, K, a.c, lead);
         if (K > 1) {
             __syncthreads();
             if (d4 == 0) {
@@ -1027,26 +1042,15 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
                 for (int x = g + 1; x < g + K; ++x)
                     p.add(s_ml[x][0], s_ml[x][1], *reinterpret_cast<const f32x4_t*>(&s_acc[x][4 * d4]), a.c);
         }
-        if (live && k == 0) p.template write<T, SH>(a, j, j.first + r, d4);
-    };
-    // the last range that holds some of a join: about hi W / total, then exactly
-    auto last_of = [&](const Join& j, int w0, int log) {
-        int w1 = max(w0, static_cast<int>(static_cast<float>(j.hi - 1) / static_cast<float>(j.total) * (1 << log)) - 1);
-        while (cut(j.total, w1 + 1, log) < j.hi) ++w1;
-        return w1;
-    };
-    auto groups = [&](int parts) {
-        int K = 1;
-        while (K < P && 4 * K < parts) K *= 2;
-        return K;
+        if (live && k == 0) p.template write<T>(a, j, j.first + r, d4);
     };
     if (static_cast<int>(blockIdx.x) < a.few_blocks) {
         const int w0 = blockIdx.x % W, y = blockIdx.x / W;
         const Join j = a.few.joins[w0];
         if (j.lo == j.hi) return;
         const int log = ranges_log(a.w_log, j.total), w1 = last_of(j, w0, log);
-        const int K = groups(w1 - w0 + 1), r0 = y * (P / K);
-        if (r0 < j.end - j.first) merge(a.few, j, w0, w1, log, r0, K);
+        const int K = groups_of(w1 - w0 + 1, P), r0 = y * (P / K);
+        if (r0 < j.end - j.first) merge(a.few, j, w0, w1, log, r0, K, LEAD);
         return;
     }
     // the ranges that hold a join
@@ -1064,13 +1068,13 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
     if (has) s_range[before + __builtin_popcountll(mask & ((1ull << lane_id()) - 1))] = tid;
     __syncthreads();
     const int log = ranges_log(a.w_log, a.tiles.joins[s_range[0]].total);
-    const int K = groups(((1 << log) + n - 1) / n);
+    const int K = groups_of(((1 << log) + n - 1) / n, P);
     const int blocks = (a.tiles.cap * K + P - 1) / P;
     for (int item = blockIdx.x - a.few_blocks; item < n * blocks; item += gridDim.x - a.few_blocks) {
         const int w0 = __builtin_amdgcn_readfirstlane(s_range[item / blocks]);
         const Join j = a.tiles.joins[w0];
         const int r0 = item % blocks * (P / K);
-        if (r0 < j.end - j.first) merge(a.tiles, j, w0, last_of(j, w0, log), log, r0, K);
+        if (r0 < j.end - j.first) merge(a.tiles, j, w0, last_of(j, w0, log), log, r0, K, 0);
     }
 }
 
@@ -1320,22 +1324,24 @@ __device__ __forceinline__ int find_tile(const int64_t* steps, int n, int64_t x)
     return lo;
 }
 
+// LDS of the tile kernel, one array: with two, the compiler makes every read of
+// K wait for the loads into LDS that are under way for the next step
+template <int D, bool OWN>
+constexpr int kTileLds = 8 * Stage<D>::kBytes + 16 + (OWN ? kOwnPlan * 20 + 128 : 0);
+
 template <typename T, int D, bool OWN, typename C, bool SH>
-__global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
+__device__ __forceinline__ void tile_body(const PagedParams& a, int block, char* const s_stage) {
     constexpr int KK = D / 16;
     constexpr int DB = D / 32;
     constexpr int NF = 4;                   // operand blocks read ahead of their use (2, 6, 8 cost 2, 0, 4 percent)
     constexpr int NR = Stage<D>::NR;
     constexpr int SB = Stage<D>::kBytes;
     constexpr bool kCodes = C::kBits != 16;
-    // one array: with two, the compiler makes every read of K wait for the
-    // loads into LDS that are under way for the next step
-    __shared__ __align__(1024) char s_stage[8 * SB + 16 + (OWN ? kOwnPlan * 20 + 128 : 0)];
     char* const s_k = s_stage;
     char* const s_v = s_stage + 4 * SB;
     // a masked step held infinities or NaN: this tile's word and the next one's
     int* const s_odd = reinterpret_cast<int*>(s_stage + 8 * SB);
-    static_assert(__alignof__(s_stage) >= 16 && SB % 16 == 0, "read and written 16 bytes at a time");
+    static_assert(SB % 16 == 0, "read and written 16 bytes at a time");
     int turn = 0;
     if (threadIdx.x == 0) s_odd[0] = 0;
     Stage<D> st;
@@ -1362,8 +1368,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
     // workgroups go round robin over the 8 dies: die x takes the x-th eighth
     // of the steps, so that its workgroups read the same head's K and V
     const int log = ranges_log(a.w_log, total), W = 1 << log;
-    const bool used = static_cast<int>(blockIdx.x) < W;
-    const int wg = W >= 8 && used ? (blockIdx.x % 8) * (W / 8) + blockIdx.x / 8 : blockIdx.x;
+    const bool used = block < W;
+    const int wg = W >= 8 && used ? (block % 8) * (W / 8) + block / 8 : block;
     int64_t g0 = used ? cut(total, wg, log) : 0;
     const int64_t g1 = used ? cut(total, wg + 1, log) : 0;
     bool first = true;
@@ -1634,41 +1640,8 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         }
         l += xor32(l);
         if (live) {
-            bool kept = false;
-            if constexpr (SH) {   // (shared_rows for this lane's dims)
-                if (u0 == 0 && u1 == units) {
-                    const int64_t e = q_tok * (a.H * a.G) + x_head;
-                    float* const x = a.px + e * D + 4 * hi;
-                    if (a.common) {
-                        kept = true;
-#pragma unroll
-                        for (int d = 0; d < DB; ++d)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                *reinterpret_cast<f32x4_t*>(x + 32 * d + 8 * i) =
-                                    f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
-                        if (hi == 0) {
-                            a.px_ml[2 * e] = m;
-                            a.px_ml[2 * e + 1] = l;
-                        }
-                    } else if (sq.lo > 0) {
-                        const float m1 = a.px_ml[2 * e], Mn = fmaxf(m, m1);
-                        const float f0 = exp2_weight(m, Mn, a.c), f1 = exp2_weight(m1, Mn, a.c);
-                        l = l * f0 + a.px_ml[2 * e + 1] * f1;
-                        m = Mn;
-#pragma unroll
-                        for (int d = 0; d < DB; ++d)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const f32x4_t y = *reinterpret_cast<const f32x4_t*>(x + 32 * d + 8 * i);
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) acc[d][4 * i + k] = acc[d][4 * i + k] * f0 + y[k] * f1;
-                            }
-                    }
-                }
-            }
-            if (kept) {
-            } else if (u0 == 0 && u1 == units) {
+            const bool keep = SH && u0 == 0 && u1 == units && (a.common || sq.lo > 0);
+            if (u0 == 0 && u1 == units && !keep) {
                 const float inv = inverse(l, pos < 0);
                 uint16_t* const op = a.out + q_tok * a.o_ts + x_head * a.o_hs + 4 * hi;
 #pragma unroll
@@ -1683,8 +1656,9 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                 if (a.lse && hi == 0)
                     a.lse[q_tok * a.l_ts + x_head] = log_sum<T>(m, l, a.c);
             } else {
-                const int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
-                float* const op = a.part + e * D + 4 * hi;
+                const int64_t e = keep ? q_tok * (a.H * a.G) + x_head
+                                       : (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
+                float* const op = (keep ? a.keep : a.part) + e * D + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1692,8 +1666,9 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                         *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * i) =
                             f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
                 if (hi == 0) {
-                    a.part_ml[2 * e] = m;
-                    a.part_ml[2 * e + 1] = l;
+                    float* const ml = keep ? a.keep_ml : a.part_ml;
+                    ml[2 * e] = m;
+                    ml[2 * e + 1] = l;
                 }
             }
         }
@@ -1707,8 +1682,11 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
                                      u0 == 0 && u1 == units ? -1 : 2 * static_cast<int64_t>(wg) + (first ? 0 : 1));
         }
         turn ^= 1;
+        if constexpr (SH)
+            if (u0 == 0 && tid == 0)
+                a.place[static_cast<int64_t>(place_key(a, sq.t0, s, tile.y)) * a.H + h] = u1 == units ? -1 : wg;
         if (u0 == 0 && u1 < units)
-            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, t_end, h, max(-p0, 0) * a.G, sq.lo};
+            rest = Join{total, t_lo, t_lo + units, sq.t0, tile.y, t_end, h, max(-p0, 0) * a.G};
         g0 += u1 - u0;
         first = false;
         if (++t == n_tiles) {
@@ -1717,6 +1695,105 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
         }
     }
     if (tid == 0) a.joins[wg] = rest;
+}
+
+template <typename T, int D, bool OWN, typename C, bool SH>
+__global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
+    __shared__ __align__(1024) char s_stage[kTileLds<D, OWN>];
+    tile_body<T, D, OWN, C, SH>(a, blockIdx.x, s_stage);
+}
+
+// ------------------------------------------------------------ shared rows --
+// A launch for the shared rows (the first 2^w_log workgroups, tiles: a run of 64
+// sequences of 4 heads has 256 rows, and reads K and V once for all) and for the
+// rows of the sequences' own (few rows each), so that neither waits for the other.
+template <typename T, int D, int NB, typename C>
+__global__ __launch_bounds__(512, 2) void both_kernel(PagedParams common, PagedParams own) {
+    static_assert(64 * kFewWaves == 512, "both kinds have eight waves");
+    constexpr int kLds = std::max(kTileLds<D, true>, static_cast<int>(sizeof(FewLds<C, D, NB>)));
+    __shared__ __align__(1024) char s_lds[kLds];
+    const int W = 1 << common.w_log;
+    if (static_cast<int>(blockIdx.x) < W)
+        tile_body<T, D, true, C, true>(common, blockIdx.x, s_lds);
+    else
+        few_body<T, D, NB, C, true>(own, 0, blockIdx.x - W, *reinterpret_cast<FewLds<C, D, NB>*>(s_lds));
+}
+
+struct JoinParams {
+    PagedParams own;             // sequences, and where their own rows' results are
+    int few_rows;                // up to so many rows they are in few, above in tiles
+    Parts few, tiles, common;
+    const float *keep, *keep_ml;         // of the shared rows
+    const int32_t *place, *leaders;
+};
+
+// Joins what the shared rows and its own rows gave each query row: a workgroup
+// per (sequence, head) and some rows, D / 4 threads to a partial as in
+// merge_kernel, all of a workgroup's for a row after the other.
+template <typename T, int D, int LEAD>
+__global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
+    constexpr int Q = D / 4, K = kMergeThreads / Q;
+    __shared__ float s_ml[K][2];
+    __shared__ __align__(16) float s_acc[K][D];
+    const PagedParams& a = p.own;
+    const int s = blockIdx.x / a.H, h = blockIdx.x % a.H;
+    const int d4 = threadIdx.x % Q, k = threadIdx.x / Q;
+    const Seq sq = seq_of<true>(a, s);
+    const int64_t rows = static_cast<int64_t>(sq.n) * a.G;
+    if (rows == 0 || rows > a.max_rows) return;
+    const int heads = a.H * a.G;
+    const int lead = sq.lo > 0 ? clampi(p.leaders[s], 0, s) : s;
+    const int lead_t0 = clampi(a.start[lead], 0, sq.t0);
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        const int i = static_cast<int>(r / a.G), g = static_cast<int>(r % a.G);
+        const int64_t t = sq.t0 + i;
+        const int head = h * a.G + g;
+        const int64_t e = t * heads + head;
+        Partial<D> x;
+        int used = K;   // groups that hold something
+        auto add = [&](int place, const Parts& from, const float* keep, const float* keep_ml, int row, int lead) {
+            if (place < 0) {
+                if (k == 0)
+                    x.add(keep_ml[2 * e], keep_ml[2 * e + 1], *reinterpret_cast<const f32x4_t*>(keep + e * D + 4 * d4),
+                          a.c);
+                return;
+            }
+            const int w0 = place & ((1 << a.w_log) - 1);
+            const Join j = from.joins[w0];
+            if (j.lo >= j.hi) return;
+            const int log = ranges_log(a.w_log, j.total), w1 = last_of(j, w0, log);
+            if (sq.lo == 0) used = groups_of(w1 - w0 + 1, K);   // the order of merge_kernel
+            if (k < used) x.gather(from, j, log, w0, w1, row, d4, k, used, a.c, lead);
+        };
+        const int tile = static_cast<int>(r) & ~(kTileRows - 1);
+        const int mine = a.place[static_cast<int64_t>(place_key(a, sq.t0, s, tile)) * a.H + h];
+        if (sq.lo == 0 && mine < 0) continue;   // written by its range
+        const bool in_few = rows <= p.few_rows;
+        add(mine, in_few ? p.few : p.tiles, a.keep, a.keep_ml, static_cast<int>(r) - tile, in_few ? LEAD : 0);
+        if (sq.lo > 0) {
+            const int64_t rc = (t - lead_t0) * a.G + g;
+            const int first = static_cast<int>(rc) & ~(kTileRows - 1);
+            add(p.place[static_cast<int64_t>(place_key(a, lead_t0, lead, first)) * a.H + h], p.common, p.keep,
+                p.keep_ml, static_cast<int>(rc) - first, 0);
+        }
+        __syncthreads();
+        if (d4 == 0) {
+            s_ml[k][0] = x.M;
+            s_ml[k][1] = x.L;
+        }
+        *reinterpret_cast<f32x4_t*>(&s_acc[k][4 * d4]) = x.A;
+        __syncthreads();
+        if (k == 0) {
+            for (int y = 1; y < used; ++y)
+                x.add(s_ml[y][0], s_ml[y][1], *reinterpret_cast<const f32x4_t*>(&s_acc[y][4 * d4]), a.c);
+            const float inv = inverse(x.L, sq.p0 + i < 0);
+            uint2 o;
+            o.x = T::pack(x.A[0] * inv, x.A[1] * inv);
+            o.y = T::pack(x.A[2] * inv, x.A[3] * inv);
+            *reinterpret_cast<uint2*>(a.out + t * a.o_ts + head * a.o_hs + 4 * d4) = o;
+            if (a.lse && d4 == 0) a.lse[t * a.l_ts + head] = log_sum<T>(x.M, x.L, a.c);
+        }
+    }
 }
 
 // ------------------------------------------------------------- host -------
@@ -1821,12 +1898,14 @@ inline bool shares(const imi_paged_attention_args* a) {
            (a->window == 0 || a->window >= batch_capacity(&b));
 }
 
-// The workspace: what the shared rows gave (if any are looked for), then the
-// partials of the launches, which come one after the other.
+// The workspace: what whole ranges gave the rows, and where the rows are, of the
+// shared rows and of the sequences' own (if any are looked for), then the
+// partials of the launches.
 struct Work {
     Shape own, common;
     bool shared;
-    float *px, *px_ml;
+    float *keep[2], *keep_ml[2];
+    int32_t* place[2];
     Rooms of_own, of_common;
     size_t bytes;
 };
@@ -1834,70 +1913,142 @@ inline Work work_of(const imi_paged_attention_args* a, void* base) {
     Work w{};
     w.own = shape_of(a);
     w.shared = shares(a);
-    size_t before = 0, common = 0;
-    if (w.shared) {
-        w.common = common_shape_of(a);
-        const size_t rows = static_cast<size_t>(a->batch.n_tokens) * a->kv_heads * a->groups;
-        Carver c(base);
-        w.px = c.take<float>(rows * a->dim);
-        w.px_ml = c.take<float>(rows * 2);
-        before = c.used();
+    if (!w.shared) {
+        w.bytes = carve(w.own, base, w.of_own);
+        return w;
     }
-    void* const rest = base ? static_cast<char*>(base) + before : nullptr;
-    if (w.shared) common = carve(w.common, rest, w.of_common);
-    w.bytes = before + std::max(common, carve(w.own, rest, w.of_own));
+    w.common = common_shape_of(a);
+    if (w.own.direct) {
+        w.own.direct = false;
+        w.own.few_part = (size_t(2) << w.own.w_log) * w.own.most * (a->dim + 2) * sizeof(float);
+    }
+    const size_t rows = static_cast<size_t>(a->batch.n_tokens) * a->kv_heads * a->groups;
+    Carver c(base);
+    for (int i = 0; i < 2; ++i) {
+        w.keep[i] = c.take<float>(rows * a->dim);
+        w.keep_ml[i] = c.take<float>(rows * 2);
+        w.place[i] = c.take<int32_t>(static_cast<size_t>(w.common.slots + 1) * a->kv_heads);
+    }
+    const size_t before = c.used();
+    auto at = [&](size_t off) { return base ? static_cast<char*>(base) + off : nullptr; };
+    const size_t common = carve(w.common, at(before), w.of_common);
+    w.bytes = before + common + carve(w.own, at(before + common), w.of_own);
     return w;
 }
 
-template <typename T, int D, typename C, bool SH>
-int launch(const Shape& p, PagedParams P, const Rooms& room, hipStream_t stream) {
-    const int W = 1 << p.w_log;
+inline PagedParams few_params(const Shape& p, PagedParams P, const Rooms& room, int D) {
     P.w_log = p.w_log;
+    P.min_rows = 1;
+    P.max_rows = p.most;
+    P.cap = p.most;
+    P.joins = room.joins;
+    P.part = room.few;
+    P.part_ml = room.few + (size_t(2) << p.w_log) * p.most * D;
+    return P;
+}
+inline PagedParams tile_params(const Shape& p, PagedParams P, const Rooms& room, int D) {
+    P.w_log = p.w_log;
+    P.min_rows = p.few_rows + 1;
+    P.max_rows = p.max_rows;
+    P.cap = p.tile_most;
+    P.joins = room.joins + (1 << p.w_log);
+    P.part = room.tile;
+    P.part_ml = room.tile + (size_t(2) << p.w_log) * p.tile_most * D;
+    P.plan = room.plan;
+    P.slots = p.slots;
+    return P;
+}
+
+template <typename T, int D, typename C, bool SH>
+int launch_tiles(const Shape& p, const PagedParams& Q, hipStream_t stream) {
+    const int W = 1 << p.w_log;
+    if (p.slots <= kOwnPlan) {
+        tile_kernel<T, D, true, C, SH><<<W, 512, 0, stream>>>(Q);
+    } else {
+        plan_kernel<SH><<<1, 1024, 0, stream>>>(Q);
+        IMI_LAUNCH_CHECK("plan_kernel");
+        tile_kernel<T, D, false, C, SH><<<W, 512, 0, stream>>>(Q);
+    }
+    IMI_LAUNCH_CHECK("tile_kernel");
+    return IMI_OK;
+}
+template <typename T, int D, typename C, bool SH>
+int launch_few(const Shape& p, const PagedParams& F, hipStream_t stream) {
+    const int grid = p.direct ? F.S * F.H : 1 << p.w_log;
+    if (p.few_rows == 16)
+        few_kernel<T, D, 1, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
+    else
+        few_kernel<T, D, 2, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
+    IMI_LAUNCH_CHECK("few_kernel");
+    return IMI_OK;
+}
+
+inline Parts parts_of(const PagedParams& P) { return Parts{P.joins, P.part, P.part_ml, P.cap}; }
+
+template <typename T, int D, typename C>
+int launch(const Shape& p, const PagedParams& P, const Rooms& room, hipStream_t stream) {
+    const int W = 1 << p.w_log;
     PagedParams F = P, Q = P;
     if (p.tiles) {
-        Q.min_rows = p.few_rows + 1;
-        Q.max_rows = p.max_rows;
-        Q.cap = p.tile_most;
-        Q.joins = room.joins + W;
-        Q.part = room.tile;
-        Q.part_ml = room.tile + size_t(2) * W * p.tile_most * D;
-        Q.plan = room.plan;
-        Q.slots = p.slots;
-        if (p.slots <= kOwnPlan) {
-            tile_kernel<T, D, true, C, SH><<<W, 512, 0, stream>>>(Q);
-        } else {
-            plan_kernel<SH><<<1, 1024, 0, stream>>>(Q);
-            IMI_LAUNCH_CHECK("plan_kernel");
-            tile_kernel<T, D, false, C, SH><<<W, 512, 0, stream>>>(Q);
-        }
-        IMI_LAUNCH_CHECK("tile_kernel");
+        Q = tile_params(p, P, room, D);
+        if (const int rc = launch_tiles<T, D, C, false>(p, Q, stream)) return rc;
     }
     if (p.few_rows) {
-        F.min_rows = 1;
-        F.max_rows = p.most;
-        F.cap = p.most;
-        F.joins = room.joins;
-        F.part = room.few;
-        F.part_ml = room.few + size_t(2) * W * p.most * D;
-        const int grid = p.direct ? P.S * P.H : W;
-        if (p.few_rows == 16)
-            few_kernel<T, D, 1, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
-        else
-            few_kernel<T, D, 2, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
-        IMI_LAUNCH_CHECK("few_kernel");
+        F = few_params(p, P, room, D);
+        if (const int rc = launch_few<T, D, C, false>(p, F, stream)) return rc;
     }
     const int few_blocks = p.few_rows && !p.direct ? W * p.most : 0;
     if (few_blocks || p.tiles) {
-        const MergeParams M{{F.joins, F.part, F.part_ml, F.cap, FewLoads<C, D>::kLead},
-                            {Q.joins, Q.part, Q.part_ml, Q.cap, 0}, P.out, P.lse,
-                            P.o_ts, P.o_hs, P.l_ts, few_blocks, P.H, P.G, p.w_log, P.c, P.px,
-                            P.px_ml, P.common};
+        const MergeParams M{parts_of(F), parts_of(Q), P.out, P.lse, P.o_ts, P.o_hs, P.l_ts,
+                            few_blocks, P.G, p.w_log, P.c};
         // for the tiles: the pairs there can be, as far as workgroups are worth it
         const int64_t pairs = std::min<int64_t>(W, int64_t(p.slots) * P.H) * p.tile_most;
         const int more = p.tiles ? static_cast<int>(std::min<int64_t>(8 * W, pairs)) : 0;
-        merge_kernel<T, D, SH><<<few_blocks + more, kMergeThreads, 0, stream>>>(M);
+        merge_kernel<T, D, FewLoads<C, D>::kLead><<<few_blocks + more, kMergeThreads, 0, stream>>>(M);
         IMI_LAUNCH_CHECK("merge_kernel");
     }
+    return IMI_OK;
+}
+
+// Shared and own rows: a launch, where the workgroups can plan for themselves,
+// one for sequences of many new tokens, and the join.
+constexpr int kJoinRows = 64;   // workgroups to a (sequence, head), at most
+template <typename T, int D, typename C>
+int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, hipStream_t stream) {
+    P.shared = b.shared;
+    P.members = b.members;
+    P.keep = w.keep[0];
+    P.keep_ml = w.keep_ml[0];
+    P.place = w.place[0];
+    PagedParams common = tile_params(w.common, P, w.of_common, D);
+    common.common = true;
+    P.keep = w.keep[1];
+    P.keep_ml = w.keep_ml[1];
+    P.place = w.place[1];
+    PagedParams few = P, tiles = P;
+    if (w.own.few_rows) few = few_params(w.own, P, w.of_own, D);
+    if (w.own.few_rows && w.common.slots <= kOwnPlan) {
+        const int grid = 2 << w.own.w_log;
+        if (w.own.few_rows == 16) both_kernel<T, D, 1, C><<<grid, 512, 0, stream>>>(common, few);
+        else both_kernel<T, D, 2, C><<<grid, 512, 0, stream>>>(common, few);
+        IMI_LAUNCH_CHECK("both_kernel");
+    } else {
+        if (const int rc = launch_tiles<T, D, C, true>(w.common, common, stream)) return rc;
+        if (w.own.few_rows)
+            if (const int rc = launch_few<T, D, C, true>(w.own, few, stream)) return rc;
+    }
+    if (w.own.tiles) {
+        tiles = tile_params(w.own, P, w.of_own, D);
+        if (const int rc = launch_tiles<T, D, C, true>(w.own, tiles, stream)) return rc;
+    }
+    JoinParams J{P, w.own.few_rows, parts_of(few), parts_of(tiles), parts_of(common), w.keep[0], w.keep_ml[0], w.place[0], b.leaders};
+    J.own.w_log = w.own.w_log;
+    J.own.max_rows = w.own.max_rows;
+    const int64_t pairs = static_cast<int64_t>(P.S) * P.H;
+    const unsigned rows = static_cast<unsigned>(std::min(w.own.max_rows, kJoinRows));
+    IMI_REQUIRE(pairs <= (1 << 24) / kJoinRows * 16, IMI_ERR_UNSUPPORTED, "too many sequences to share rows (%d)", P.S);
+    join_kernel<T, D, FewLoads<C, D>::kLead><<<dim3(static_cast<unsigned>(pairs), rows), kMergeThreads, 0, stream>>>(J);
+    IMI_LAUNCH_CHECK("join_kernel");
     return IMI_OK;
 }
 
@@ -1938,15 +2089,7 @@ int run_on(const imi_paged_attention_args* a, hipStream_t stream) {
     P.e_head_s = a->exponent_head_stride;
     P.e_page_s = static_cast<uint32_t>(a->exponent_page_stride);
     P.e_tok_s = static_cast<uint32_t>(a->exponent_row_stride);
-    if (!w.shared) return launch<T, D, C, false>(w.own, P, w.of_own, stream);
-    P.shared = b.shared;
-    P.members = b.members;
-    P.px = w.px;
-    P.px_ml = w.px_ml;
-    P.common = true;
-    if (const int rc = launch<T, D, C, true>(w.common, P, w.of_common, stream)) return rc;
-    P.common = false;
-    return launch<T, D, C, true>(w.own, P, w.of_own, stream);
+    return w.shared ? launch_shared<T, D, C>(w, b, P, stream) : launch<T, D, C>(w.own, P, w.of_own, stream);
 }
 
 template <typename C>

@@ -20,7 +20,7 @@ struct ShareParams {
     const int32_t *table, *lens, *start, *labels;
     int64_t table_s;
     int S, page_size, capacity;
-    int32_t *shared, *members, *pairs;
+    int32_t *shared, *members, *leaders, *pairs;
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -83,6 +83,7 @@ __global__ __launch_bounds__(64) void runs_kernel(ShareParams a) {
     for (int t = s + lane; t < end; t += 64) {
         a.shared[t] = rows;
         a.members[t] = t == s && rows > 0 ? end - s : 0;
+        a.leaders[t] = rows > 0 ? s : t;
     }
 }
 
@@ -107,18 +108,18 @@ extern "C" int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_
 }
 
 extern "C" int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
-                                  void* workspace, size_t workspace_bytes, imi_stream_t stream) {
+                                  int32_t* leaders, void* workspace, size_t workspace_bytes, imi_stream_t stream) {
     using namespace imi;
     clear_error();
     IMI_REQUIRE(b, IMI_ERR_INVALID, "null argument");
     if (const int rc = validate(b)) return rc;
     if (b->n_seqs == 0) return IMI_OK;
-    IMI_REQUIRE(shared && members, IMI_ERR_INVALID, "null shared or members");
+    IMI_REQUIRE(shared && members && leaders, IMI_ERR_INVALID, "null shared, members or leaders");
     const size_t need = static_cast<size_t>(b->n_seqs) * sizeof(int32_t);
     IMI_REQUIRE(workspace && workspace_bytes >= need, IMI_ERR_WORKSPACE, "workspace of %zu bytes, need %zu",
                 workspace_bytes, need);
     const ShareParams P{b->page_table, b->lens, b->query_start, labels, b->table_stride, b->n_seqs,
-                        b->page_size, static_cast<int>(batch_capacity(b)), shared, members,
+                        b->page_size, static_cast<int>(batch_capacity(b)), shared, members, leaders,
                         static_cast<int32_t*>(workspace)};
     hipStream_t st = static_cast<hipStream_t>(stream);
     pairs_kernel<<<P.S, kPairThreads, 0, st>>>(P);

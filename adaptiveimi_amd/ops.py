@@ -1024,10 +1024,11 @@ class PagedBatch:
     longest sequence (default: what the table holds); only the split of short
     batches depends on it.
 
-    ``shared`` and ``members`` are None but in a batch of share_prefixes."""
+    ``shared``, ``members`` and ``leaders`` are None but in a batch of
+    share_prefixes."""
 
     __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device", "pool_pages",
-                 "page_size", "shared", "members")
+                 "page_size", "shared", "members", "leaders")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
@@ -1049,7 +1050,7 @@ class PagedBatch:
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.pool_pages, self.page_size = 0, None   # what a PageTable knows of the pools
-        self.shared = self.members = None
+        self.shared = self.members = self.leaders = None
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
                                    _c_int(self.max_query), _c_int(max_len or 0))
 
@@ -1379,7 +1380,8 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
     (all sequences begin with one system prompt, and the beams of a prompt share
     more).  In the result ``shared`` int32 [S] are the rows that each sequence
     shares (multiples of 8; 0 for those on their own, or with fewer than 64) and
-    ``members`` the sequences of the run that each leads.  ``page_size``: the
+    ``members`` the sequences of the run that each leads, ``leaders`` the first of
+    each one's run (itself, on its own).  ``page_size``: the
     pools', where the batch was not made by a PageTable.
 
     Found on the device, without a synchronisation; the result holds for the
@@ -1409,13 +1411,13 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
         L = _lib.lib()
         ref = ctypes.byref(a)
         need = ctypes.c_size_t()
-        new.shared, new.members = torch.empty((2, S), dtype=torch.int32, device=dev)
+        new.shared, new.members, new.leaders = torch.empty((3, S), dtype=torch.int32, device=dev)
         with _on(dev):
             check(L.imi_share_prefixes_workspace_size(ref, ctypes.byref(need)), "imi_share_prefixes")
             ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            check(L.imi_share_prefixes(ref, f, new.shared.data_ptr(), new.members.data_ptr(), ws.data_ptr(),
-                                       need.value, _raw_stream(dev.index)), "imi_share_prefixes")
-        a.shared, a.members = new.shared.data_ptr(), new.members.data_ptr()
+            check(L.imi_share_prefixes(ref, f, new.shared.data_ptr(), new.members.data_ptr(), new.leaders.data_ptr(),
+                                       ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_share_prefixes")
+        a.shared, a.members, a.leaders = (t.data_ptr() for t in (new.shared, new.members, new.leaders))
     return new
 
 

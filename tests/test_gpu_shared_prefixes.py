@@ -29,10 +29,10 @@ def i32(x):
 # ---------------------------------------------------------------- the runs --
 
 def runs(table, lens, start, page, labels=None):
-    """(shared, members) by the definition."""
+    """(shared, members, leaders) by the definition."""
     S, cap = len(lens), table.shape[1] * page
     old = [max(min(max(n, 0), cap) - max(start[s + 1] - start[s], 0), 0) // page for s, n in enumerate(lens)]
-    shared, members = [0] * S, [0] * S
+    shared, members, leaders = [0] * S, [0] * S, list(range(S))
     s = 0
     while s < S:
         def joins(t):
@@ -48,8 +48,9 @@ def runs(table, lens, start, page, labels=None):
         if end - s > 1 and rows >= LEAST:
             shared[s:end] = [rows] * (end - s)
             members[s] = end - s
+            leaders[s:end] = [s] * (end - s)
         s = end
-    return shared, members
+    return shared, members, leaders
 
 
 def families(sizes, commons, page, width, seed=0, loners=1):
@@ -84,6 +85,7 @@ def test_runs(ops, page, width):
         got = ops.share_prefixes(batch, page, labels=None if lab is None else i32(lab))
         want = runs(table, lens, start, page, lab)
         assert got.shared.tolist() == want[0] and got.members.tolist() == want[1]
+        assert got.leaders.tolist() == want[2]
         assert batch.shared is None and got.lens is batch.lens
 
 
