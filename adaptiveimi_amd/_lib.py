@@ -102,7 +102,8 @@ class HostcacheGatherArgs(ctypes.Structure):
 class PagedBatchArgs(ctypes.Structure):
     _fields_ = [("page_table", _vp), ("table_stride", _i64), ("max_pages", _i32), ("n_pages", _i32),
                 ("page_size", _i32), ("lens", _vp), ("query_start", _vp), ("n_seqs", _i32), ("n_tokens", _i32),
-                ("max_query", _i32), ("max_len", _i32), ("shared", _vp), ("members", _vp), ("leaders", _vp)]
+                ("max_query", _i32), ("max_len", _i32), ("shared", _vp), ("members", _vp), ("leaders", _vp),
+                ("saved", _vp), ("share_bytes", _i64)]
 
 
 class PagedAttentionArgs(ctypes.Structure):
@@ -189,7 +190,7 @@ EXPORTS = {
     "imi_read_pages": (ctypes.c_int, [ctypes.POINTER(ReadPagesArgs), _vp]),
     "imi_share_prefixes_workspace_size": (ctypes.c_int, [ctypes.POINTER(PagedBatchArgs),
                                                          ctypes.POINTER(ctypes.c_size_t)]),
-    "imi_share_prefixes": (ctypes.c_int, [ctypes.POINTER(PagedBatchArgs)] + [_vp] * 5 + [ctypes.c_size_t, _vp]),
+    "imi_share_prefixes": (ctypes.c_int, [ctypes.POINTER(PagedBatchArgs)] + [_vp] * 6 + [ctypes.c_size_t, _vp]),
     "imi_fork_pages": (ctypes.c_int, [ctypes.POINTER(PageTableArgs), _vp, ctypes.POINTER(PageTableArgs), _vp]),
     "imi_extend_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(PageTableArgs),
                                                        ctypes.POINTER(ctypes.c_size_t)]),

@@ -62,8 +62,10 @@ namespace {
 int validate(const imi_paged_attention_args* a) {
     const imi_paged_batch* const b = &a->batch;
     if (const int rc = validate_batch(b)) return rc;
-    IMI_REQUIRE(!b->shared == !b->members && !b->shared == !b->leaders, IMI_ERR_INVALID,
-                "shared, members and leaders go together");
+    IMI_REQUIRE(!b->shared == !b->members && !b->shared == !b->leaders && !b->shared == !b->saved, IMI_ERR_INVALID,
+                "shared, members, leaders and saved go together");
+    IMI_REQUIRE(b->share_bytes >= 0, IMI_ERR_INVALID, "share_bytes=%lld must be >= 0",
+                static_cast<long long>(b->share_bytes));
     IMI_REQUIRE(a->dtype == IMI_BF16 || a->dtype == IMI_FP16, IMI_ERR_UNSUPPORTED, "dtype=%d is not bf16 or fp16",
                 a->dtype);
     IMI_REQUIRE(a->dim == 64 || a->dim == 128, IMI_ERR_UNSUPPORTED, "dim=%d is not 64 or 128", a->dim);

@@ -154,6 +154,8 @@ struct PagedParams {
     // shared first rows (see Seq)
     const int32_t* shared;     // [S] rows, or null
     const int32_t* members;    // [S] sequences of the run that s leads, or 0
+    const int64_t* saved;      // rows that sharing saves, and how many it has to
+    int64_t least_saved;
     bool common;               // the shared rows are attended, not the others
     float* keep;               // [N][H G][D] rows that one range attended whole, before the division,
     float* keep_ml;            // [N][H G][2] their maxima and sums
@@ -177,7 +179,7 @@ template <bool SH>
 __device__ __forceinline__ Seq seq_of(const PagedParams& a, int s) {
     const int b = clampi(a.start[s], 0, a.N);
     if constexpr (SH) {
-        const int rows = clampi(a.shared[s], 0, a.capacity);
+        const int rows = *a.saved >= a.least_saved ? clampi(a.shared[s], 0, a.capacity) : 0;
         if (a.common) {
             const int m = clampi(a.members[s], 0, a.S - s);
             const int e = m > 1 && rows > 0 ? clampi(a.start[s + m], 0, a.N) : b;
@@ -1891,11 +1893,33 @@ inline size_t carve(const Shape& p, void* base, Rooms& r) {
     return p.few_part || p.tile_part ? c.used() : 0;
 }
 
-// Shared rows are attended together where no window hides some of them.
+// Shared rows are attended together where no window hides some of them and that
+// saves kShareBytes of keys and values.  A cache behind the dies' L2 holds as much,
+// so that rows which many sequences read are soon read from there, and sharing
+// costs a longer chain (the tiles and the join).  One token each, 20 .. 200 own
+// rows, 4 query heads per KV head of 128 dims, us without and with sharing:
+//   8 heads, bf16:  32 sequences behind 1024 rows (130 MB saved) 24.7, 32.9
+//                   32 behind 2048 (260 MB)                      35.9, 34.5
+//                   32 behind 16384 (2.1 GB)                    172.7, 47.1
+//                   4 behind 16384 (201 MB)                      36.1, 42.5
+//                   8 behind 16384 (470 MB)                      57.0, 39.0
+//   8 heads, fp8:   32 behind 2048 (134 MB)                      27.4, 33.4
+//                   8 behind 16384 (242 MB)                      41.6, 38.7
+//   1 head, bf16:   32 behind 16384 (260 MB)                     36.0, 27.7
+// What is saved is known on the device alone; the host knows a bound.
+constexpr int64_t kShareBytes = int64_t(230) << 20;
+inline int64_t least_saved(const imi_paged_attention_args* a) {
+    static constexpr int kBits[] = {16, 8, 8, 4};
+    const int64_t row = 2 * a->kv_heads * (a->dim * kBits[a->format] / 8 + (a->format == IMI_ROWS ? 0 : a->dim / kBlock));
+    return std::max<int64_t>((a->batch.share_bytes ? a->batch.share_bytes : kShareBytes) / row, 1);
+}
 inline bool shares(const imi_paged_attention_args* a) {
     const imi_paged_batch& b = a->batch;
-    return b.shared && b.page_table && b.n_seqs > 1 && b.n_tokens > 0 &&
-           (a->window == 0 || a->window >= batch_capacity(&b));
+    if (!b.shared || !b.page_table || b.n_seqs < 2 || b.n_tokens == 0) return false;
+    const int64_t capacity = batch_capacity(&b);
+    if (a->window > 0 && a->window < capacity) return false;
+    const int64_t longest = b.max_len > 0 ? std::min<int64_t>(capacity, b.max_len) : capacity;
+    return (b.n_seqs - 1) * longest >= least_saved(a);
 }
 
 // The workspace: what whole ranges gave the rows, and where the rows are, of the
@@ -2014,9 +2038,11 @@ int launch(const Shape& p, const PagedParams& P, const Rooms& room, hipStream_t 
 // one for sequences of many new tokens, and the join.
 constexpr int kJoinRows = 64;   // workgroups to a (sequence, head), at most
 template <typename T, int D, typename C>
-int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, hipStream_t stream) {
+int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, int64_t least, hipStream_t stream) {
     P.shared = b.shared;
     P.members = b.members;
+    P.saved = b.saved;
+    P.least_saved = least;
     P.keep = w.keep[0];
     P.keep_ml = w.keep_ml[0];
     P.place = w.place[0];
@@ -2089,7 +2115,7 @@ int run_on(const imi_paged_attention_args* a, hipStream_t stream) {
     P.e_head_s = a->exponent_head_stride;
     P.e_page_s = static_cast<uint32_t>(a->exponent_page_stride);
     P.e_tok_s = static_cast<uint32_t>(a->exponent_row_stride);
-    return w.shared ? launch_shared<T, D, C>(w, b, P, stream) : launch<T, D, C>(w.own, P, w.of_own, stream);
+    return w.shared ? launch_shared<T, D, C>(w, b, P, least_saved(a), stream) : launch<T, D, C>(w.own, P, w.of_own, stream);
 }
 
 template <typename C>

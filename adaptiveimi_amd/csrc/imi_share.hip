@@ -12,15 +12,14 @@ namespace imi {
 namespace {
 
 constexpr int kPairThreads = 256;
-// Fewer common rows are left to each sequence: see the reasons at the rule in
-// the attention's host code.
-constexpr int kMinShared = 64;
+constexpr int kMinShared = 64;   // fewer common rows are left to each sequence
 
 struct ShareParams {
     const int32_t *table, *lens, *start, *labels;
     int64_t table_s;
     int S, page_size, capacity;
     int32_t *shared, *members, *leaders, *pairs;
+    int64_t* saved;
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -35,6 +34,7 @@ __device__ __forceinline__ int old_pages(const ShareParams& a, int s) {
 __global__ __launch_bounds__(kPairThreads) void pairs_kernel(ShareParams a) {
     __shared__ int s_first;
     const int s = blockIdx.x;
+    if (s == 0 && threadIdx.x == 0) *a.saved = 0;   // for runs_kernel
     int most = s > 0 ? min(old_pages(a, s), old_pages(a, s - 1)) : 0;
     if (s > 0 && a.labels && a.labels[s] != a.labels[s - 1]) most = 0;
     if (threadIdx.x == 0) s_first = most;
@@ -80,6 +80,9 @@ __global__ __launch_bounds__(64) void runs_kernel(ShareParams a) {
     end = min(end, a.S);
     int rows = end - s > 1 ? (least * a.page_size) & ~7 : 0;   // (least pages lie within the table)
     if (rows < kMinShared) rows = 0;
+    if (lane == 0 && rows > 0)   // (whole numbers: in any order)
+        atomicAdd(reinterpret_cast<unsigned long long*>(a.saved),
+                  static_cast<unsigned long long>(end - s - 1) * static_cast<unsigned long long>(rows));
     for (int t = s + lane; t < end; t += 64) {
         a.shared[t] = rows;
         a.members[t] = t == s && rows > 0 ? end - s : 0;
@@ -108,19 +111,19 @@ extern "C" int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_
 }
 
 extern "C" int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
-                                  int32_t* leaders, void* workspace, size_t workspace_bytes, imi_stream_t stream) {
+                                  int32_t* leaders, int64_t* saved, void* workspace, size_t workspace_bytes, imi_stream_t stream) {
     using namespace imi;
     clear_error();
     IMI_REQUIRE(b, IMI_ERR_INVALID, "null argument");
     if (const int rc = validate(b)) return rc;
     if (b->n_seqs == 0) return IMI_OK;
-    IMI_REQUIRE(shared && members && leaders, IMI_ERR_INVALID, "null shared, members or leaders");
+    IMI_REQUIRE(shared && members && leaders && saved, IMI_ERR_INVALID, "null shared, members, leaders or saved");
     const size_t need = static_cast<size_t>(b->n_seqs) * sizeof(int32_t);
     IMI_REQUIRE(workspace && workspace_bytes >= need, IMI_ERR_WORKSPACE, "workspace of %zu bytes, need %zu",
                 workspace_bytes, need);
     const ShareParams P{b->page_table, b->lens, b->query_start, labels, b->table_stride, b->n_seqs,
                         b->page_size, static_cast<int>(batch_capacity(b)), shared, members, leaders,
-                        static_cast<int32_t*>(workspace)};
+                        static_cast<int32_t*>(workspace), saved};
     hipStream_t st = static_cast<hipStream_t>(stream);
     pairs_kernel<<<P.S, kPairThreads, 0, st>>>(P);
     IMI_LAUNCH_CHECK("pairs_kernel");

@@ -1024,11 +1024,11 @@ class PagedBatch:
     longest sequence (default: what the table holds); only the split of short
     batches depends on it.
 
-    ``shared``, ``members`` and ``leaders`` are None but in a batch of
+    ``shared``, ``members``, ``leaders`` and ``saved`` are None but in a batch of
     share_prefixes."""
 
     __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device", "pool_pages",
-                 "page_size", "shared", "members", "leaders")
+                 "page_size", "shared", "members", "leaders", "saved")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
@@ -1050,7 +1050,7 @@ class PagedBatch:
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.pool_pages, self.page_size = 0, None   # what a PageTable knows of the pools
-        self.shared = self.members = self.leaders = None
+        self.shared = self.members = self.leaders = self.saved = None
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
                                    _c_int(self.max_query), _c_int(max_len or 0))
 
@@ -1368,8 +1368,8 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
     return keys, values
 
 
-def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
-                   labels: Optional[torch.Tensor] = None) -> PagedBatch:
+def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None, labels: Optional[torch.Tensor] = None,
+                   least_bytes: Optional[int] = None) -> PagedBatch:
     """The batch, with what its sequences have in common: paged_attention then
     attends common rows once for all sequences of a run, in every layer.
 
@@ -1381,7 +1381,11 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
     more).  In the result ``shared`` int32 [S] are the rows that each sequence
     shares (multiples of 8; 0 for those on their own, or with fewer than 64) and
     ``members`` the sequences of the run that each leads, ``leaders`` the first of
-    each one's run (itself, on its own).  ``page_size``: the
+    each one's run (itself, on its own) and ``saved`` int64 [1] the rows that need
+    not be read again.  paged_attention makes use of it where that saves
+    ``least_bytes`` of a layer's keys and values (by default about 240 MB: fewer
+    are sooner read from the caches); only speed and rounding depend on
+    that.  ``page_size``: the
     pools', where the batch was not made by a PageTable.
 
     Found on the device, without a synchronisation; the result holds for the
@@ -1395,6 +1399,8 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
             raise ValueError("give the page_size of the pools")
     elif batch.page_size not in (None, page_size):
         raise ValueError(f"page_size={page_size} under a table of {batch.page_size} rows per page")
+    if least_bytes is not None and least_bytes < 1:
+        raise ValueError(f"least_bytes={least_bytes} must be positive")
     dev, S = batch.device, batch.args.n_seqs
     f = 0
     if labels is not None:
@@ -1411,13 +1417,18 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None,
         L = _lib.lib()
         ref = ctypes.byref(a)
         need = ctypes.c_size_t()
-        new.shared, new.members, new.leaders = torch.empty((3, S), dtype=torch.int32, device=dev)
+        found = torch.empty((3 * S + 3,), dtype=torch.int32, device=dev)
+        at = 3 * S + S % 2   # the next multiple of 8 bytes
+        new.shared, new.members, new.leaders = (found[i * S:(i + 1) * S] for i in range(3))
+        new.saved = found[at:at + 2].view(torch.int64)
         with _on(dev):
             check(L.imi_share_prefixes_workspace_size(ref, ctypes.byref(need)), "imi_share_prefixes")
             ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
             check(L.imi_share_prefixes(ref, f, new.shared.data_ptr(), new.members.data_ptr(), new.leaders.data_ptr(),
-                                       ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_share_prefixes")
-        a.shared, a.members, a.leaders = (t.data_ptr() for t in (new.shared, new.members, new.leaders))
+                                       new.saved.data_ptr(), ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_share_prefixes")
+        a.shared, a.members, a.leaders, a.saved = (t.data_ptr()
+                                                   for t in (new.shared, new.members, new.leaders, new.saved))
+        a.share_bytes = min(least_bytes or 0, 2 ** 62)
     return new
 
 

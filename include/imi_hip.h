@@ -504,9 +504,11 @@ typedef struct {
     int32_t n_seqs, n_tokens;    /* n_tokens: rows of the query tensor */
     int32_t max_query;           /* at least every sequence's new tokens */
     int32_t max_len;             /* hint: about the longest sequence; 0 = what the table holds */
-    const int32_t* shared;       /* device [n_seqs], what imi_share_prefixes found, or NULL (all three); */
+    const int32_t* shared;       /* device [n_seqs], what imi_share_prefixes found, or NULL (all four); */
     const int32_t* members;      /*   read by imi_paged_attention alone */
     const int32_t* leaders;
+    const int64_t* saved;        /* device [1] */
+    int64_t share_bytes;         /* bytes of a call's keys and values that sharing has to save; 0: as measured */
 } imi_paged_batch;
 
 /* How a pool holds its rows: IMI_ROWS as bf16 or fp16 (the call's dtype), the
@@ -624,13 +626,15 @@ int imi_read_pages(const imi_read_pages_args* a, imi_stream_t stream);
  * them have in common, as far as they lie before the new tokens of each.
  * shared[s] = rows that sequence s shares with its run, a multiple of 8, or 0
  * where it is alone or they are fewer than 64; members[s] = sequences of the run
- * that s is the first of, or 0; leaders[s] = the first of its run, or s itself.  Given a batch with the three, imi_paged_attention
- * attends those rows once for all sequences of a run (without a window): the
- * results differ in their rounding alone.  They hold for the tables, lens and
- * query_start that they were made of. */
+ * that s is the first of, or 0; leaders[s] = the first of its run, or s itself;
+ * saved[0] = the sum over the runs of (members - 1) * shared.  Given a batch with
+ * the four, imi_paged_attention attends those rows once for all sequences of a
+ * run, where there is no window and that saves share_bytes: the results differ in
+ * their rounding alone.  They hold for the tables, lens and query_start that they
+ * were made of. */
 int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_t* bytes);
 int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
-                       int32_t* leaders, void* workspace, size_t workspace_bytes, imi_stream_t stream);
+                       int32_t* leaders, int64_t* saved, void* workspace, size_t workspace_bytes, imi_stream_t stream);
 
 /* The page tables.  Sequence s holds the first ceil(lens[s] / page_size)
  * entries of its row; refs[p] counts the sequences that hold page p, 0 =

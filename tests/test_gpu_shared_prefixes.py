@@ -86,6 +86,7 @@ def test_runs(ops, page, width):
         want = runs(table, lens, start, page, lab)
         assert got.shared.tolist() == want[0] and got.members.tolist() == want[1]
         assert got.leaders.tolist() == want[2]
+        assert got.saved.tolist() == [sum(max(m - 1, 0) * r for r, m in zip(*want[:2]))]
         assert batch.shared is None and got.lens is batch.lens
 
 
@@ -146,7 +147,7 @@ def forked(groups, H, G, D, page, dtype, layout="heads", seed=0, pad=0):
 
 def attend(ops, x, labels=None, max_query=None, max_len=None, **kw):
     batch = ops.PagedBatch(x["table"], x["lens"], x["start"], max_query or x["most"], max_len)
-    batch = ops.share_prefixes(batch, x["page"], labels)
+    batch = ops.share_prefixes(batch, x["page"], labels, least_bytes=1)
     return batch, ops.paged_attention(x["q"], x["k"], x["v"], batch, return_lse=True, **kw)
 
 
@@ -196,6 +197,21 @@ def test_windows_see_their_rows(ops):
     for window, sinks in ((64, 5), (290, 0), (10 ** 6, 3)):
         _, (out, lse) = attend(ops, x, window=window, sinks=sinks)
         check(x, out, lse, window, sinks)
+
+
+def test_little_to_save(ops):
+    """Below what sharing has to save, on the device's and on the host's count: the
+    bits of the call without."""
+    x = forked([(640, ones(30, 5, 90)), (640, ones(400))], 2, 4, 128, 16, BF)
+    plain = ops.PagedBatch(x["table"], x["lens"], x["start"], 1)
+    want = ops.paged_attention(x["q"], x["k"], x["v"], plain, return_lse=True)
+    row = 2 * 2 * 128 * 2
+    for least, same in ((2 * 640 * row, False), (2 * 640 * row + row, True), (10 ** 18, True), (None, True)):
+        batch = ops.share_prefixes(plain, 16, least_bytes=least)
+        assert batch.saved.tolist() == [2 * 640]
+        out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch, return_lse=True)
+        assert torch.equal(lse, want[1]) == same and (torch.equal(out, want[0]) or not same)
+        check(x, out, lse)
 
 
 def test_nothing_shared_changes_nothing(ops):
@@ -257,7 +273,7 @@ def test_captured_steps(ops):
     y = forked([(128, ones(5, 6))], 2, 4, 128, 16, BF, seed=9)
 
     def step(x, out):
-        batch = ops.share_prefixes(ops.PagedBatch(x["table"], x["lens"], x["start"], 1), x["page"])
+        batch = ops.share_prefixes(ops.PagedBatch(x["table"], x["lens"], x["start"], 1), x["page"], least_bytes=1)
         ops.paged_attention(x["q"], x["k"], x["v"], batch, out=out[0])
         ops.paged_attention(out[0], x["k"], x["v"], batch, out=out[1])
 
@@ -306,7 +322,7 @@ def test_a_server_with_beams(ops):
         for c in counts:
             start.append(start[-1] + c)
         q, k, v = (torch.randn((start[-1], h, D), generator=g).to(BF).to(DEV) for h in (H * G, H, H))
-        batch = ops.share_prefixes(table.batch(i32(start), max(counts)))
+        batch = ops.share_prefixes(table.batch(i32(start), max(counts)), least_bytes=1)
         q, _ = ops.qk_norm_rope(q, k, inv_freq=inv_freq, value=v, batch=batch, key_pages=pools[0], value_pages=pools[1])
         out, lse = ops.paged_attention(q, *pools, batch, return_lse=True)
         keys, values = ops.read_pages(*pools, batch)

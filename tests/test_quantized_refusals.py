@@ -107,24 +107,29 @@ def test_share_prefixes_refuses(L):
                              (dict(table_stride=3), 1, "table_stride"), (dict(lens=None), 1, "null"),
                              (dict(query_start=None), 1, "null")):
         assert size(batch(**over)) == code, over
-        assert share(batch(**over), 256, 256, 256, 256, 8) == code
+        assert share(batch(**over), 256, 256, 256, 256, 256, 8) == code
     assert size(batch(n_tokens=0, n_pages=0, max_query=0)) == 0 and need.value == 8
-    for i in range(3):
-        assert share(batch(), *[None if k == i else 256 for k in range(3)], 256, 8) == 1
-    assert share(batch(), 256, 256, 256, 256, 7) == 4 and share(batch(), 256, 256, 256, None, 8) == 4
-    assert share(batch(n_seqs=0), None, None, None, None, 0) == 0
+    for i in range(4):
+        assert share(batch(), *[None if k == i else 256 for k in range(4)], 256, 8) == 1
+    assert share(batch(), 256, 256, 256, 256, 256, 7) == 4 and share(batch(), 256, 256, 256, 256, None, 8) == 4
+    assert share(batch(n_seqs=0), None, None, None, None, None, 0) == 0
 
 
 def test_shared_goes_with_members(L):
     need = ctypes.c_size_t()
     size = lambda **b: L.imi_paged_attention_workspace_size(ctypes.byref(attention(batch(**b))), ctypes.byref(need))
-    assert size(shared=256) == 1 and size(members=256) == 1 and size(shared=256, members=256) == 1
+    assert size(shared=256) == 1 and size(members=256) == 1 and size(shared=256, members=256, leaders=256) == 1
+    assert size(shared=256, members=256, leaders=256, saved=256, share_bytes=-1) == 1
     assert size() == 0
     plain = need.value
-    assert size(shared=256, members=256, leaders=256) == 0 and need.value > plain
+    found = dict(shared=256, members=256, leaders=256, saved=256)
+    assert size(**found, share_bytes=1) == 0 and need.value > plain
+    # 100 pages cannot save what sharing costs
+    assert size(**found) == 0 and need.value == plain
+    assert size(**found, share_bytes=1 << 62) == 0 and need.value == plain
     # a window hides some of the common rows: nothing is attended together
     sizes = []
-    for b in (batch(shared=256, members=256, leaders=256), batch()):
+    for b in (batch(**found, share_bytes=1), batch()):
         a = attention(b, window=64)
         assert L.imi_paged_attention_workspace_size(ctypes.byref(a), ctypes.byref(need)) == 0
         sizes.append(need.value)
