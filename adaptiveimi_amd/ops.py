@@ -1028,7 +1028,7 @@ class PagedBatch:
     share_prefixes."""
 
     __slots__ = ("page_table", "lens", "query_start", "max_query", "max_len", "args", "device", "pool_pages",
-                 "page_size", "shared", "members", "leaders", "saved")
+                 "page_size", "found")
 
     def __init__(self, page_table: Optional[torch.Tensor], lens: torch.Tensor, query_start: torch.Tensor,
                  max_query: int, max_len: Optional[int] = None):
@@ -1050,9 +1050,18 @@ class PagedBatch:
         self.page_table, self.lens, self.query_start = page_table, lens, query_start
         self.max_query, self.max_len, self.device = int(max_query), max_len, dev
         self.pool_pages, self.page_size = 0, None   # what a PageTable knows of the pools
-        self.shared = self.members = self.leaders = self.saved = None
+        self.found = None   # by share_prefixes: shared, members, leaders [S] each, S ints of room, saved
         self.args = PagedBatchArgs(table, stride, cols, 0, 0, lens.data_ptr(), query_start.data_ptr(), S, 0,
                                    _c_int(self.max_query), _c_int(max_len or 0))
+
+    def _part(self, i: int) -> Optional[torch.Tensor]:
+        S = self.lens.shape[0]
+        return None if self.found is None else self.found[i * S:(i + 1) * S]
+
+    shared = property(lambda self: self._part(0))
+    members = property(lambda self: self._part(1))
+    leaders = property(lambda self: self._part(2))
+    saved = property(lambda self: None if self.found is None else self.found[-2:].view(torch.int64))
 
     def bind(self, n_pages: int, page_size: int, n_tokens: int) -> PagedBatchArgs:
         """The C struct for pools of n_pages pages and n_tokens query rows: a
@@ -1409,25 +1418,17 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None, labels: O
             raise ValueError(f"labels has {labels.shape[0]} entries for {S} sequences")
         f = labels.data_ptr()
     new = PagedBatch.__new__(PagedBatch)
-    for name in PagedBatch.__slots__:
-        setattr(new, name, getattr(batch, name))
-    new.page_size = page_size
+    new.page_table, new.lens, new.query_start = batch.page_table, batch.lens, batch.query_start
+    new.max_query, new.max_len, new.device = batch.max_query, batch.max_len, dev
+    new.pool_pages, new.page_size, new.found = batch.pool_pages, page_size, None
     a = new.args = batch.bind(1, _c_int(page_size), 1)
     if S:
-        L = _lib.lib()
-        ref = ctypes.byref(a)
-        need = ctypes.c_size_t()
-        found = torch.empty((3 * S + 3,), dtype=torch.int32, device=dev)
-        at = 3 * S + S % 2   # the next multiple of 8 bytes
-        new.shared, new.members, new.leaders = (found[i * S:(i + 1) * S] for i in range(3))
-        new.saved = found[at:at + 2].view(torch.int64)
+        new.found = torch.empty((4 * S + 2,), dtype=torch.int32, device=dev)   # (4 S ints: a multiple of 16 bytes)
+        at = new.found.data_ptr()
         with _on(dev):
-            check(L.imi_share_prefixes_workspace_size(ref, ctypes.byref(need)), "imi_share_prefixes")
-            ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-            check(L.imi_share_prefixes(ref, f, new.shared.data_ptr(), new.members.data_ptr(), new.leaders.data_ptr(),
-                                       new.saved.data_ptr(), ws.data_ptr(), need.value, _raw_stream(dev.index)), "imi_share_prefixes")
-        a.shared, a.members, a.leaders, a.saved = (t.data_ptr()
-                                                   for t in (new.shared, new.members, new.leaders, new.saved))
+            check(_lib.lib().imi_share_prefixes(ctypes.byref(a), f, at, at + 4 * S, at + 8 * S, at + 16 * S, at + 12 * S,
+                                                4 * S, _raw_stream(dev.index)), "imi_share_prefixes")
+        a.shared, a.members, a.leaders, a.saved = at, at + 4 * S, at + 8 * S, at + 16 * S
         a.share_bytes = min(least_bytes or 0, 2 ** 62)
     return new
 

@@ -631,7 +631,7 @@ int imi_read_pages(const imi_read_pages_args* a, imi_stream_t stream);
  * the four, imi_paged_attention attends those rows once for all sequences of a
  * run, where there is no window and that saves share_bytes: the results differ in
  * their rounding alone.  They hold for the tables, lens and query_start that they
- * were made of. */
+ * were made of.  The workspace: 4 bytes for each sequence. */
 int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_t* bytes);
 int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
                        int32_t* leaders, int64_t* saved, void* workspace, size_t workspace_bytes, imi_stream_t stream);
