@@ -9,7 +9,9 @@
 namespace imi {
 namespace {
 
-constexpr int kRows = 4;        // rows of a thread
+// Rows of a thread.  32768 rows of 8 heads of 128 dims, fp8: 45.2 us with 2 (4.5 TB/s,
+// a large copy runs at 4.98), 48 with 4, 51 with 8.
+constexpr int kRows = 2;
 constexpr int kThreads = 256;
 
 struct ReadParams {
