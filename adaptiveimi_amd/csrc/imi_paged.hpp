@@ -34,6 +34,12 @@
 // it, and 131072 rows of such weights, which one row outweighs, by 2^-19 in all
 // (unshifted they would be lost: 2^-25 of it each, 2^-8 in all).  Either way 8192
 // fp16 tokens over 32768 rows take 3.91-4.0 ms.
+//
+// Rows may be held as codes of 8 or 4 bits (C, imi_blocks.hpp).  They become bf16
+// or fp16 in registers, which rounds nothing in bf16, on the way to the matrix
+// instruction (K of the few-row kernel) or to LDS (all others), and from there on
+// both kernels are the same: the masks, the statistics and the look for infinities
+// and NaN see values, and no scale enters a score or a weight.
 #pragma once
 
 #include <algorithm>
@@ -118,7 +124,11 @@ constexpr int kRow = D == 128 ? 144 : 72;
 
 struct Join;
 
-struct PagedParams {
+// Threads of the kernels that attend (a constant, as all sizes of launches: a kernel
+// that asks for them has 256 bytes of arguments more).
+constexpr int kThreads = 512;
+
+struct BaseParams {
     const uint16_t* q;
     const uint16_t* k;
     const uint16_t* v;
@@ -147,12 +157,14 @@ struct PagedParams {
     int cap;                   // rows of a partial
     int32_t* plan;             // tile kernel: see plan_kernel
     int slots;                 // tile kernel: tiles that the plan can hold
-    // codes (strides above in bytes then): exponents of their blocks
+};
+struct ExpParams {   // codes (strides above in bytes then): exponents of their blocks
     const uint8_t *ke, *ve;
     int64_t e_head_s;
     uint32_t e_page_s, e_tok_s;
-    // shared first rows (see Seq)
-    const int32_t* shared;     // [S] rows, or null
+};
+struct SharedParams {   // shared first rows (see Seq)
+    const int32_t* shared;     // [S] rows
     const int32_t* members;    // [S] sequences of the run that s leads, or 0
     const int64_t* saved;      // rows that sharing saves, and how many it has to
     int64_t least_saved;
@@ -161,6 +173,13 @@ struct PagedParams {
     float* keep_ml;            // [N][H G][2] their maxima and sums
     int32_t* place;            // [keys][H] where a tile's rows are: see place_key
 };
+// A kernel's arguments are those that it reads.
+template <int>
+struct NoParams {};
+template <typename C, bool SH>
+struct PagedParams : BaseParams,
+                     std::conditional_t<C::kBits != 16, ExpParams, NoParams<0>>,
+                     std::conditional_t<SH, SharedParams, NoParams<1>> {};
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
@@ -175,8 +194,8 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x,
 struct Seq {
     int t0, n, len, p0, lo;
 };
-template <bool SH>
-__device__ __forceinline__ Seq seq_of(const PagedParams& a, int s) {
+template <bool SH, typename P>
+__device__ __forceinline__ Seq seq_of(const P& a, int s) {
     const int b = clampi(a.start[s], 0, a.N);
     if constexpr (SH) {
         const int rows = *a.saved >= a.least_saved ? clampi(a.shared[s], 0, a.capacity) : 0;
@@ -199,7 +218,7 @@ struct Span {
     __device__ __forceinline__ int count() const { return sink + hi - lo; }
     __device__ __forceinline__ int row(int v) const { return v < sink ? v : v - sink + lo; }
 };
-__device__ __forceinline__ Span span_of(const PagedParams& a, const Seq& q, int p0, int p1) {
+__device__ __forceinline__ Span span_of(const BaseParams& a, const Seq& q, int p0, int p1) {
     Span r;
     r.hi = clampi(p1 + 1, 0, q.len);
     r.lo = a.window > 0 ? clampi(p0 - a.window + 1, 0, r.hi) : q.lo;   // (not both)
@@ -212,7 +231,7 @@ __device__ __forceinline__ Span span_of(const PagedParams& a, const Seq& q, int 
 // `from` on or under `sinks`.
 struct Sees {
     int last, from, sinks;
-    __device__ __forceinline__ Sees(const PagedParams& a, int pos, int shift, int sink, int vis)
+    __device__ __forceinline__ Sees(const BaseParams& a, int pos, int shift, int sink, int vis)
         : last(min(pos - shift, vis - 1)),
           from(a.window > 0 ? pos - a.window + 1 - shift : 0),
           sinks(shift ? sink : a.sinks) {}
@@ -221,18 +240,26 @@ struct Sees {
     }
 };
 
+// Whether the rows of a problem are kept for the join, where a range holds them whole.
+template <bool SH, typename P>
+__device__ __forceinline__ bool keeps(const P& a, const Seq& q) {
+    if constexpr (SH) return a.common || q.lo > 0;
+    else return false;
+}
+
 // Element offset of cached row j of sequence s (head offset not included).
 // A page id outside the pool is forced into it.
-__device__ __forceinline__ int page_of(const PagedParams& a, int s, int j) {
+__device__ __forceinline__ int page_of(const BaseParams& a, int s, int j) {
     return a.table ? a.table[static_cast<int64_t>(s) * a.table_s + (j >> a.page_shift)] : s;
 }
-__device__ __forceinline__ int64_t row_offset(const PagedParams& a, int page, int j) {
+__device__ __forceinline__ int64_t row_offset(const BaseParams& a, int page, int j) {
     const uint32_t slot = static_cast<uint32_t>(j) & ((1u << a.page_shift) - 1u);
     return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(clampi(page, 0, a.n_pages - 1))) * a.page_s +
                                 slot * a.tok_s);
 }
 // Of the exponents of cached row j.
-__device__ __forceinline__ int64_t exp_offset(const PagedParams& a, int page, int j) {
+template <typename P>
+__device__ __forceinline__ int64_t exp_offset(const P& a, int page, int j) {
     const uint32_t slot = static_cast<uint32_t>(j) & ((1u << a.page_shift) - 1u);
     return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(clampi(page, 0, a.n_pages - 1))) * a.e_page_s +
                                 slot * a.e_tok_s);
@@ -314,9 +341,9 @@ __device__ __forceinline__ void keep_finite(u32x4_t (&x)[N]) {
 // of the span's rows [v0, v1) that each sees, to the output (slot < 0) or to
 // the partial.  The workgroup's own writes of these rows are done.
 template <typename T, int D, typename C, bool SH, typename SpanT>
-__device__ __forceinline__ void patch_rows(const PagedParams& a, const Seq& sq, int s, int h, const SpanT& sp, int first,
+__device__ __forceinline__ void patch_rows(const PagedParams<C, SH>& a, const Seq& sq, int s, int h, const SpanT& sp, int first,
                                            int end, int v0, int v1, int64_t slot) {
-    for (int x = threadIdx.x; x < (end - first) * (D / 2); x += blockDim.x) {
+    for (int x = threadIdx.x; x < (end - first) * (D / 2); x += kThreads) {
         const int r = first + x / (D / 2), d = 2 * (x % (D / 2));
         const int p = sq.p0 + r / a.G;
         float add[2] = {0.0f, 0.0f};
@@ -341,10 +368,11 @@ __device__ __forceinline__ void patch_rows(const PagedParams& a, const Seq& sq, 
             if (!(m >> 16)) add[1] += T::wide(w >> 16);
         }
         if (add[0] == 0.0f && add[1] == 0.0f) continue;
-        if (slot >= 0 || (SH && (a.common || sq.lo > 0))) {
-            float* const o =
-                slot >= 0 ? a.part + (slot * a.cap + r - first) * D + d
-                          : a.keep + (static_cast<int64_t>(sq.t0 + r / a.G) * (a.H * a.G) + h * a.G + r % a.G) * D + d;
+        if (slot >= 0 || keeps<SH>(a, sq)) {
+            float* o = a.part + (slot * a.cap + r - first) * D + d;
+            if constexpr (SH)
+                if (slot < 0)
+                    o = a.keep + (static_cast<int64_t>(sq.t0 + r / a.G) * (a.H * a.G) + h * a.G + r % a.G) * D + d;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 o[i] = __hip_atomic_load(o + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + add[i];
@@ -365,7 +393,7 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
 // shared rows, for each head: -1, in `keep`, or the range that holds its first
 // unit, in that range's partials and those after it.  Problems begin at query
 // rows t0 G in the order of s, so no two tiles have the same key.
-__device__ __forceinline__ int place_key(const PagedParams& a, int t0, int s, int r0) {
+__device__ __forceinline__ int place_key(const BaseParams& a, int t0, int s, int r0) {
     return static_cast<int>((static_cast<int64_t>(t0) * a.G + r0) / 256) + s;
 }
 
@@ -399,7 +427,7 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 94 us,
 // 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
 // join.
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = kThreads / 64;
 // Rows of K / V per wave and step: 32, or 64 of 64 dims in 4 bits, which then
 // have as many bytes under way as others (3 tokens each of 12 sequences over 4000 ..
 // 60000 rows, 8 heads: 46 us instead of 54, one over 131072 28.6 instead of 29.9).
@@ -438,7 +466,7 @@ __device__ __forceinline__ int ranges_log(int w_log, int64_t total) {
 __device__ __forceinline__ int64_t cut(int64_t total, int64_t w, int log) { return (total * w) >> log; }
 
 template <int UNIT, int LEAD>
-__device__ __forceinline__ int few_units(const PagedParams& a, const Seq& q) {
+__device__ __forceinline__ int few_units(const BaseParams& a, const Seq& q) {
     const int rows = q.n * a.G;
     if (q.n <= 0 || rows < a.min_rows || rows > a.max_rows) return 0;
     const Span sp = span_of(a, q, max(q.p0, 0), q.len - 1);
@@ -457,8 +485,8 @@ struct FewRange {
     int64_t total, g0, g1, before;
     int s;
 };
-template <bool SH, int UNIT, int LEAD>
-__device__ __forceinline__ FewRange few_range(const PagedParams& a, int block) {
+template <bool SH, int UNIT, int LEAD, typename P>
+__device__ __forceinline__ FewRange few_range(const P& a, int block) {
     FewRange r{0, 0, 0, 0, 0};
     int u = 0, incl = 0;
     for (int s0 = 0; s0 < a.S; s0 += 64) {
@@ -519,14 +547,17 @@ struct FewLds {
     static constexpr bool kQuery = NB * D > 128;
     static constexpr int kRows = FewLoads<C, D>::kTile * kRow<D>;
     static constexpr int kWave = kRows > 16 * D * 2 ? kRows : 16 * D * 2;   // u16
-    uint16_t buf[kFewWaves * kWave];
-    uint16_t q[kQuery ? 16 * NB * kRow<D> : 8];
-    float ml[kFewWaves][16 * NB][2];
-    int odd;   // a masked tile held infinities or NaN
+    static constexpr int kBuf = kFewWaves * kWave, kQ = kQuery ? 16 * NB * kRow<D> : 8;
+    static constexpr int kBytes = 2 * (kBuf + kQ) + kFewWaves * 16 * NB * 8 + 4;
+    typedef float Ml[16 * NB][2];
+    uint16_t* buf;
+    uint16_t* q;
+    Ml* ml;     // [kFewWaves]
+    int* odd;   // a masked tile held infinities or NaN
 };
 
 template <typename T, int D, int NB, typename C, bool SH>
-__device__ __forceinline__ void few_body(const PagedParams& a, int direct, int block, FewLds<C, D, NB>& lds) {
+__device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct, int block, const FewLds<C, D, NB>& lds) {
     constexpr int KK = D / 32;     // matrix instructions over the head dim
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
@@ -540,8 +571,8 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
     static_assert(kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0, "rows and partials are read and written 16 bytes at a time");
     uint16_t* const s_buf = lds.buf;
     uint16_t* const s_q = lds.q;
-    auto& s_ml = lds.ml;
-    int& s_odd = lds.odd;
+    auto* const s_ml = lds.ml;
+    int& s_odd = *lds.odd;
     const int tid = threadIdx.x, lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int ln = lane & 15, lg = lane >> 4;
@@ -626,8 +657,11 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
         const uint8_t* const kc = reinterpret_cast<const uint8_t*>(a.k) + static_cast<int64_t>(h) * a.head_s +
                                   lg * (Lo::kPiece * C::kBits / 8);
         const uint8_t* const vc = reinterpret_cast<const uint8_t*>(a.v) + static_cast<int64_t>(h) * a.head_s + 16 * (lane % CH);
-        const uint8_t* const kx = (TILE == 64 || lane < 32 ? a.ke : a.ve) + static_cast<int64_t>(h) * a.e_head_s;
-        const uint8_t* const vx = a.ve + static_cast<int64_t>(h) * a.e_head_s;
+        const uint8_t *kx = nullptr, *vx = nullptr;
+        if constexpr (kCodes) {
+            kx = (TILE == 64 || lane < 32 ? a.ke : a.ve) + static_cast<int64_t>(h) * a.e_head_s;
+            vx = a.ve + static_cast<int64_t>(h) * a.e_head_s;
+        }
         // lane's rows of a step's tile: of K ln and 16 + ln (the matrix
         // instruction's), of V, which goes through LDS, whole rows of CH lanes
         auto row_of = [&](int u, int r) { return sp.row(min(u * UNIT + wave * TILE + r, vis - 1)); };
@@ -704,18 +738,17 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
         }
         for (int u = u0; any && u < u1; ++u) {
             const int v0 = u * UNIT + wave * TILE;   // first row of the tile
+            if (!kCodes && v0 + TILE > vis) {   // rows past the end weigh nothing: no NaN may enter through V
+#pragma unroll
+                for (int i = 0; i < (kCodes ? 0 : NV); ++i)
+                    if (v0 + (64 / CH) * i + lane / CH >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
+            }
             const int j_lo = sp.row(v0), j_hi = sp.row(v0 + TILE - 1);
             const bool full = v0 + TILE <= vis && j_hi <= p0 &&
                               (a.window == 0 || j_lo >= sq.len - a.window || j_hi < a.sinks);
-            const bool look = !full && sq.n > 1;   // (one token sees every row of its span)
             uint16_t* const sv_row = sv + lane / CH * LR + Lo::kDims * (lane % CH);
             if constexpr (!kCodes) {
-                if (v0 + TILE > vis) {   // rows past the end weigh nothing: no NaN may enter through V
-#pragma unroll
-                    for (int i = 0; i < NV; ++i)
-                        if (v0 + (64 / CH) * i + lane / CH >= vis) vb[i] = u32x4_t{0, 0, 0, 0};
-                }
-                if (look) {
+                if (!full && sq.n > 1) {   // (one token sees every row of its span)
                     if (__builtin_amdgcn_ballot_w64(!all_finite<T>(vb))) {
                         keep_finite<T>(vb);
                         s_odd = 1;
@@ -724,6 +757,7 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
 #pragma unroll
                 for (int i = 0; i < NV; ++i) *reinterpret_cast<u32x4_t*>(sv_row + (64 / CH) * i * LR) = vb[i];
             } else {   // the same, piece by piece
+                const bool look = !full && sq.n > 1;
                 bool odd = false;
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
@@ -817,14 +851,15 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
                 }
             }
 #pragma unroll
-            for (int d = 0; d < DB; ++d) {
+            for (int x = 0; x < KB / 2; ++x) {
+                const uint16_t* const vp = sv + (32 * x + 4 * lg + (ln >> 2)) * LR + 4 * (ln & 3);
+                u32x4_t vt[DB];   // all reads under way before the first is waited for
 #pragma unroll
-                for (int x = 0; x < KB / 2; ++x) {
-                    const uint16_t* vp = sv + (32 * x + 4 * lg + (ln >> 2)) * LR + 16 * d + 4 * (ln & 3);
-                    const u32x4_t vt = join(read_tr(vp), read_tr(vp + 16 * LR));
+                for (int d = 0; d < DB; ++d) vt[d] = join(read_tr(vp + 16 * d), read_tr(vp + 16 * d + 16 * LR));
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) acc[b][d] = T::mma16(vt, pf[b][x], acc[b][d]);
-                }
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) acc[b][d] = T::mma16(vt[d], pf[b][x], acc[b][d]);
             }
             wave_lds_sync();
         }
@@ -872,7 +907,7 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
                     const int64_t t = sq.t0 + r / a.G;
                     const int x_head = h * a.G + r % a.G;
                     if constexpr (SH) {
-                        if (a.common || sq.lo > 0) {
+                        if (keeps<SH>(a, sq)) {
                             const int64_t e = t * (a.H * a.G) + x_head;
                             *reinterpret_cast<f32x4_t*>(a.keep + e * D + 4 * d4) = A;
                             if (d4 == 0) {
@@ -918,9 +953,13 @@ __device__ __forceinline__ void few_body(const PagedParams& a, int direct, int b
 }
 
 template <typename T, int D, int NB, typename C, bool SH>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void few_kernel(PagedParams a, int direct) {
-    __shared__ __align__(16) FewLds<C, D, NB> s_lds;
-    few_body<T, D, NB, C, SH>(a, direct, blockIdx.x, s_lds);
+__global__ __launch_bounds__(kThreads, 2) void few_kernel(PagedParams<C, SH> a, int direct) {
+    typedef FewLds<C, D, NB> Lds;   // arrays of their own: in one, the writes of V hold up the reads of others
+    __shared__ __align__(16) uint16_t s_buf[Lds::kBuf];
+    __shared__ typename Lds::Ml s_ml[kFewWaves];
+    __shared__ int s_odd;
+    __shared__ __align__(16) uint16_t s_q[Lds::kQ];
+    few_body<T, D, NB, C, SH>(a, direct, blockIdx.x, Lds{s_buf, s_q, s_ml, &s_odd});
 }
 
 // What merge_kernel needs: the partials of the few-row launch and of the tiles.
@@ -936,6 +975,7 @@ struct MergeParams {
     float* lse;
     int64_t o_ts, o_hs, l_ts;
     int few_blocks;      // workgroups for the few-row launch: W cap, or none
+    int tile_blocks;     // and for the tiles
     int G, w_log;
     float c;
 };
@@ -1072,7 +1112,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
     const int log = ranges_log(a.w_log, a.tiles.joins[s_range[0]].total);
     const int K = groups_of(((1 << log) + n - 1) / n, P);
     const int blocks = (a.tiles.cap * K + P - 1) / P;
-    for (int item = blockIdx.x - a.few_blocks; item < n * blocks; item += gridDim.x - a.few_blocks) {
+    for (int item = blockIdx.x - a.few_blocks; item < n * blocks; item += a.tile_blocks) {
         const int w0 = __builtin_amdgcn_readfirstlane(s_range[item / blocks]);
         const Join j = a.tiles.joins[w0];
         const int r0 = item % blocks * (P / K);
@@ -1184,7 +1224,7 @@ struct Stage {
     }
 };
 
-__device__ __forceinline__ int seq_tiles(const PagedParams& a, const Seq& q) {
+__device__ __forceinline__ int seq_tiles(const BaseParams& a, const Seq& q) {
     const int64_t rows = static_cast<int64_t>(q.n) * a.G;
     if (q.n <= 0 || rows < a.min_rows || rows > a.max_rows) return 0;
     return static_cast<int>((rows + kTileRows - 1) / kTileRows);
@@ -1204,7 +1244,7 @@ struct TileSpan {
         return v >= vis || (j >= sink && j < lo);
     }
 };
-__device__ __forceinline__ TileSpan tile_span(const PagedParams& a, const Seq& q, int first) {
+__device__ __forceinline__ TileSpan tile_span(const BaseParams& a, const Seq& q, int first) {
     const int p0 = q.p0;
     const int i0 = first / a.G;
     const int i1 = min((first + kTileRows - 1) / a.G, q.n - 1);
@@ -1236,7 +1276,7 @@ struct Plan {
     int32_t* seqs;     // [S]
 };
 __host__ __device__ inline size_t plan_bytes(int slots, int S) { return 16 + size_t(slots) * 16 + size_t(S) * 4; }
-__device__ __forceinline__ Plan plan_of(const PagedParams& a) {
+__device__ __forceinline__ Plan plan_of(const BaseParams& a) {
     Plan p;
     p.n = a.plan;
     p.tiles = reinterpret_cast<int2*>(a.plan + 4);
@@ -1245,7 +1285,7 @@ __device__ __forceinline__ Plan plan_of(const PagedParams& a) {
     return p;
 }
 
-template <typename V>
+template <int THREADS, typename V>
 __device__ __forceinline__ V block_incl_scan(V x, V* s_wave, V& total) {
     const int lane = lane_id(), wave = threadIdx.x >> 6;
 #pragma unroll
@@ -1258,7 +1298,7 @@ __device__ __forceinline__ V block_incl_scan(V x, V* s_wave, V& total) {
     __syncthreads();
     V before = 0;
     total = 0;
-    for (int w = 0; w < static_cast<int>(blockDim.x >> 6); ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
         if (w < wave) before += s_wave[w];
         total += s_wave[w];
     }
@@ -1267,21 +1307,20 @@ __device__ __forceinline__ V block_incl_scan(V x, V* s_wave, V& total) {
 
 // Fills the plan (all of the workgroup's threads; what it wrote is there after
 // the next barrier) and returns the number of tiles.
-template <bool SH>
-__device__ __forceinline__ int make_plan(const PagedParams& a, const Plan& p, int64_t* s_wave) {
-    const int threads = blockDim.x;
+template <bool SH, int THREADS, typename P>
+__device__ __forceinline__ int make_plan(const P& a, const Plan& p, int64_t* s_wave) {
     int64_t n = 0;
-    for (int s0 = 0; s0 < a.S; s0 += threads) {
+    for (int s0 = 0; s0 < a.S; s0 += THREADS) {
         const int s = s0 + threadIdx.x;
         int64_t total;
-        const int64_t incl = block_incl_scan<int64_t>(s < a.S ? seq_tiles(a, seq_of<SH>(a, s)) : 0, s_wave, total);
+        const int64_t incl = block_incl_scan<THREADS, int64_t>(s < a.S ? seq_tiles(a, seq_of<SH>(a, s)) : 0, s_wave, total);
         if (s < a.S) p.seqs[s] = static_cast<int32_t>(min(n + incl, static_cast<int64_t>(a.slots)));
         n += total;
     }
     const int n_tiles = static_cast<int>(min(n, static_cast<int64_t>(a.slots)));
     __syncthreads();   // the prefix is read by other threads of this workgroup
     int64_t before = 0;
-    for (int t0 = 0; t0 < n_tiles; t0 += threads) {
+    for (int t0 = 0; t0 < n_tiles; t0 += THREADS) {
         const int t = t0 + threadIdx.x;
         int64_t u = 0;
         if (t < n_tiles) {
@@ -1296,18 +1335,18 @@ __device__ __forceinline__ int make_plan(const PagedParams& a, const Plan& p, in
             u = max((tile_span(a, seq_of<SH>(a, lo), row).vis + kStep - 1) / kStep, 1);
         }
         int64_t total;
-        const int64_t incl = block_incl_scan<int64_t>(u, s_wave, total);
+        const int64_t incl = block_incl_scan<THREADS, int64_t>(u, s_wave, total);
         if (t < n_tiles) p.steps[t] = before + incl;
         before += total;
     }
     return n_tiles;
 }
 
-template <bool SH>
-__global__ __launch_bounds__(1024) void plan_kernel(PagedParams a) {
+template <bool SH, typename P>
+__global__ __launch_bounds__(1024) void plan_kernel(P a) {
     __shared__ int64_t s_wave[16];
     const Plan p = plan_of(a);
-    const int n_tiles = make_plan<SH>(a, p, s_wave);
+    const int n_tiles = make_plan<SH, 1024>(a, p, s_wave);
     if (threadIdx.x == 0) *p.n = n_tiles;
 }
 
@@ -1332,7 +1371,7 @@ template <int D, bool OWN>
 constexpr int kTileLds = 8 * Stage<D>::kBytes + 16 + (OWN ? kOwnPlan * 20 + 128 : 0);
 
 template <typename T, int D, bool OWN, typename C, bool SH>
-__device__ __forceinline__ void tile_body(const PagedParams& a, int block, char* const s_stage) {
+__device__ __forceinline__ void tile_body(const PagedParams<C, SH>& a, int block, char* const s_stage) {
     constexpr int KK = D / 16;
     constexpr int DB = D / 32;
     constexpr int NF = 4;                   // operand blocks read ahead of their use (2, 6, 8 cost 2, 0, 4 percent)
@@ -1358,7 +1397,7 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
         plan.steps = reinterpret_cast<int64_t*>(s_stage + 8 * SB + 16);
         plan.tiles = reinterpret_cast<int2*>(plan.steps + kOwnPlan);
         plan.seqs = reinterpret_cast<int32_t*>(plan.tiles + kOwnPlan);
-        n_tiles = make_plan<SH>(a, plan, reinterpret_cast<int64_t*>(plan.seqs + kOwnPlan));
+        n_tiles = make_plan<SH, kThreads>(a, plan, reinterpret_cast<int64_t*>(plan.seqs + kOwnPlan));
         __syncthreads();
     } else {
         plan = plan_of(a);
@@ -1444,7 +1483,8 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
                                   4 * C::kWords * st.l_ch;
         // and the exponents of a wave's 16 rows of K are in lanes 0 .. 15 (and
         // 32 ..), of V in 16 .. 31
-        const uint8_t* const ex = (lane & 16 ? a.ve : a.ke) + static_cast<int64_t>(h) * a.e_head_s;
+        const uint8_t* ex = nullptr;
+        if constexpr (kCodes) ex = (lane & 16 ? a.ve : a.ke) + static_cast<int64_t>(h) * a.e_head_s;
         const int ex_row = 16 * wave + (lane & 15);
         // an easy step: one page lookup, one step ahead of its use, and one
         // address per thread
@@ -1461,13 +1501,15 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
             load_words<C::kWords>(vc + o, vw[i]);
         };
         auto fetch_exps = [&](int u) {
-            const uint8_t* const p = ex + exp_offset(a, ex_id, sp.row(min(u * kStep + ex_row, vis - 1)));
-            if constexpr (D == 128) exps = *reinterpret_cast<const uint32_t*>(p);
-            else exps = *reinterpret_cast<const uint16_t*>(p);
+            if constexpr (kCodes) {
+                const uint8_t* const p = ex + exp_offset(a, ex_id, sp.row(min(u * kStep + ex_row, vis - 1)));
+                if constexpr (D == 128) exps = *reinterpret_cast<const uint32_t*>(p);
+                else exps = *reinterpret_cast<const uint16_t*>(p);
+            }
         };
         auto fetch = [&](int u) {
             char* const sk = s_k + (u & 1) * 2 * SB;
-            if constexpr (kCodes) fetch_exps(u);
+            fetch_exps(u);
             if (u >= easy_lo && u < easy_hi) {
                 const int j = u * kStep + st.l_row + sp.shift;
                 const int64_t o = row_offset(a, id, j);
@@ -1642,7 +1684,7 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
         }
         l += xor32(l);
         if (live) {
-            const bool keep = SH && u0 == 0 && u1 == units && (a.common || sq.lo > 0);
+            const bool keep = u0 == 0 && u1 == units && keeps<SH>(a, sq);
             if (u0 == 0 && u1 == units && !keep) {
                 const float inv = inverse(l, pos < 0);
                 uint16_t* const op = a.out + q_tok * a.o_ts + x_head * a.o_hs + 4 * hi;
@@ -1658,9 +1700,11 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
                 if (a.lse && hi == 0)
                     a.lse[q_tok * a.l_ts + x_head] = log_sum<T>(m, l, a.c);
             } else {
-                const int64_t e = keep ? q_tok * (a.H * a.G) + x_head
-                                       : (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
-                float* const op = (keep ? a.keep : a.part) + e * D + 4 * hi;
+                int64_t e = (2 * static_cast<int64_t>(wg) + (first ? 0 : 1)) * a.cap + wave * 32 + q32;
+                float *rows_at = a.part, *ml = a.part_ml;
+                if constexpr (SH)
+                    if (keep) e = q_tok * (a.H * a.G) + x_head, rows_at = a.keep, ml = a.keep_ml;
+                float* const op = rows_at + e * D + 4 * hi;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -1668,7 +1712,6 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
                         *reinterpret_cast<f32x4_t*>(op + 32 * d + 8 * i) =
                             f32x4_t{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
                 if (hi == 0) {
-                    float* const ml = keep ? a.keep_ml : a.part_ml;
                     ml[2 * e] = m;
                     ml[2 * e + 1] = l;
                 }
@@ -1700,7 +1743,7 @@ __device__ __forceinline__ void tile_body(const PagedParams& a, int block, char*
 }
 
 template <typename T, int D, bool OWN, typename C, bool SH>
-__global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
+__global__ __launch_bounds__(kThreads, 2) void tile_kernel(PagedParams<C, SH> a) {
     __shared__ __align__(1024) char s_stage[kTileLds<D, OWN>];
     tile_body<T, D, OWN, C, SH>(a, blockIdx.x, s_stage);
 }
@@ -1709,21 +1752,46 @@ __global__ __launch_bounds__(512, 2) void tile_kernel(PagedParams a) {
 // A launch for the shared rows (the first 2^w_log workgroups, tiles: a run of 64
 // sequences of 4 heads has 256 rows, and reads K and V once for all) and for the
 // rows of the sequences' own (few rows each), so that neither waits for the other.
+// (Twice the whole arguments, 912 bytes instead of 392, cost 1.5 us a launch.)
+struct Common {   // what differs in the launch's arguments for the shared rows
+    Join* joins;
+    float *part, *part_ml, *keep, *keep_ml;
+    int32_t* place;
+    int min_rows, max_rows, cap, slots;
+};
 template <typename T, int D, int NB, typename C>
-__global__ __launch_bounds__(512, 2) void both_kernel(PagedParams common, PagedParams own) {
-    static_assert(64 * kFewWaves == 512, "both kinds have eight waves");
-    constexpr int kLds = std::max(kTileLds<D, true>, static_cast<int>(sizeof(FewLds<C, D, NB>)));
+__global__ __launch_bounds__(kThreads, 2) void both_kernel(PagedParams<C, true> own, Common c) {
+    typedef FewLds<C, D, NB> Lds;
+    constexpr int kLds = std::max(kTileLds<D, true>, Lds::kBytes);
     __shared__ __align__(1024) char s_lds[kLds];
-    const int W = 1 << common.w_log;
-    if (static_cast<int>(blockIdx.x) < W)
-        tile_body<T, D, true, C, true>(common, blockIdx.x, s_lds);
-    else
-        few_body<T, D, NB, C, true>(own, 0, blockIdx.x - W, *reinterpret_cast<FewLds<C, D, NB>*>(s_lds));
+    const int W = 1 << own.w_log;
+    if (static_cast<int>(blockIdx.x) < W) {
+        own.common = true;
+        own.joins = c.joins;
+        own.part = c.part;
+        own.part_ml = c.part_ml;
+        own.keep = c.keep;
+        own.keep_ml = c.keep_ml;
+        own.place = c.place;
+        own.min_rows = c.min_rows;
+        own.max_rows = c.max_rows;
+        own.cap = c.cap;
+        own.slots = c.slots;
+        tile_body<T, D, true, C, true>(own, blockIdx.x, s_lds);
+    } else {
+        char* const q = s_lds + 2 * Lds::kBuf;
+        char* const ml = q + 2 * Lds::kQ;
+        few_body<T, D, NB, C, true>(own, 0, blockIdx.x - W,
+                                    Lds{reinterpret_cast<uint16_t*>(s_lds), reinterpret_cast<uint16_t*>(q),
+                                        reinterpret_cast<typename Lds::Ml*>(ml),
+                                        reinterpret_cast<int*>(ml + kFewWaves * sizeof(typename Lds::Ml))});
+    }
 }
 
 struct JoinParams {
-    PagedParams own;             // sequences, and where their own rows' results are
+    PagedParams<Raw16, true> own;        // sequences, and where their own rows' results are
     int few_rows;                // up to so many rows they are in few, above in tiles
+    int blocks;                  // to a (sequence, head)
     Parts few, tiles, common;
     const float *keep, *keep_ml;         // of the shared rows
     const int32_t *place, *leaders;
@@ -1737,7 +1805,7 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
     constexpr int Q = D / 4, K = kMergeThreads / Q;
     __shared__ float s_ml[K][2];
     __shared__ __align__(16) float s_acc[K][D];
-    const PagedParams& a = p.own;
+    const auto& a = p.own;
     const int s = blockIdx.x / a.H, h = blockIdx.x % a.H;
     const int d4 = threadIdx.x % Q, k = threadIdx.x / Q;
     const Seq sq = seq_of<true>(a, s);
@@ -1746,7 +1814,7 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
     const int heads = a.H * a.G;
     const int lead = sq.lo > 0 ? clampi(p.leaders[s], 0, s) : s;
     const int lead_t0 = clampi(a.start[lead], 0, sq.t0);
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+    for (int64_t r = blockIdx.y; r < rows; r += p.blocks) {
         const int i = static_cast<int>(r / a.G), g = static_cast<int>(r % a.G);
         const int64_t t = sq.t0 + i;
         const int head = h * a.G + g;
@@ -1960,59 +2028,61 @@ inline Work work_of(const imi_paged_attention_args* a, void* base) {
     return w;
 }
 
-inline PagedParams few_params(const Shape& p, PagedParams P, const Rooms& room, int D) {
-    P.w_log = p.w_log;
-    P.min_rows = 1;
-    P.max_rows = p.most;
-    P.cap = p.most;
-    P.joins = room.joins;
-    P.part = room.few;
-    P.part_ml = room.few + (size_t(2) << p.w_log) * p.most * D;
-    return P;
+template <typename P>
+P few_params(const Shape& p, P a, const Rooms& room, int D) {
+    a.w_log = p.w_log;
+    a.min_rows = 1;
+    a.max_rows = p.most;
+    a.cap = p.most;
+    a.joins = room.joins;
+    a.part = room.few;
+    a.part_ml = room.few + (size_t(2) << p.w_log) * p.most * D;
+    return a;
 }
-inline PagedParams tile_params(const Shape& p, PagedParams P, const Rooms& room, int D) {
-    P.w_log = p.w_log;
-    P.min_rows = p.few_rows + 1;
-    P.max_rows = p.max_rows;
-    P.cap = p.tile_most;
-    P.joins = room.joins + (1 << p.w_log);
-    P.part = room.tile;
-    P.part_ml = room.tile + (size_t(2) << p.w_log) * p.tile_most * D;
-    P.plan = room.plan;
-    P.slots = p.slots;
-    return P;
+template <typename P>
+P tile_params(const Shape& p, P a, const Rooms& room, int D) {
+    a.w_log = p.w_log;
+    a.min_rows = p.few_rows + 1;
+    a.max_rows = p.max_rows;
+    a.cap = p.tile_most;
+    a.joins = room.joins + (1 << p.w_log);
+    a.part = room.tile;
+    a.part_ml = room.tile + (size_t(2) << p.w_log) * p.tile_most * D;
+    a.plan = room.plan;
+    a.slots = p.slots;
+    return a;
 }
 
 template <typename T, int D, typename C, bool SH>
-int launch_tiles(const Shape& p, const PagedParams& Q, hipStream_t stream) {
+int launch_tiles(const Shape& p, const PagedParams<C, SH>& Q, hipStream_t stream) {
     const int W = 1 << p.w_log;
     if (p.slots <= kOwnPlan) {
-        tile_kernel<T, D, true, C, SH><<<W, 512, 0, stream>>>(Q);
+        tile_kernel<T, D, true, C, SH><<<W, kThreads, 0, stream>>>(Q);
     } else {
-        plan_kernel<SH><<<1, 1024, 0, stream>>>(Q);
+        plan_kernel<SH, PagedParams<C, SH>><<<1, 1024, 0, stream>>>(Q);
         IMI_LAUNCH_CHECK("plan_kernel");
-        tile_kernel<T, D, false, C, SH><<<W, 512, 0, stream>>>(Q);
+        tile_kernel<T, D, false, C, SH><<<W, kThreads, 0, stream>>>(Q);
     }
     IMI_LAUNCH_CHECK("tile_kernel");
     return IMI_OK;
 }
 template <typename T, int D, typename C, bool SH>
-int launch_few(const Shape& p, const PagedParams& F, hipStream_t stream) {
+int launch_few(const Shape& p, const PagedParams<C, SH>& F, hipStream_t stream) {
     const int grid = p.direct ? F.S * F.H : 1 << p.w_log;
     if (p.few_rows == 16)
-        few_kernel<T, D, 1, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
+        few_kernel<T, D, 1, C, SH><<<grid, kThreads, 0, stream>>>(F, p.direct ? 1 : 0);
     else
-        few_kernel<T, D, 2, C, SH><<<grid, 64 * kFewWaves, 0, stream>>>(F, p.direct ? 1 : 0);
+        few_kernel<T, D, 2, C, SH><<<grid, kThreads, 0, stream>>>(F, p.direct ? 1 : 0);
     IMI_LAUNCH_CHECK("few_kernel");
     return IMI_OK;
 }
 
-inline Parts parts_of(const PagedParams& P) { return Parts{P.joins, P.part, P.part_ml, P.cap}; }
+inline Parts parts_of(const BaseParams& P) { return Parts{P.joins, P.part, P.part_ml, P.cap}; }
 
 template <typename T, int D, typename C>
-int launch(const Shape& p, const PagedParams& P, const Rooms& room, hipStream_t stream) {
+int launch(const Shape& p, const PagedParams<C, false>& P, const Rooms& room, hipStream_t stream) {
     const int W = 1 << p.w_log;
-    PagedParams F = P, Q = P;
+    PagedParams<C, false> F = P, Q = P;
     if (p.tiles) {
         Q = tile_params(p, P, room, D);
         if (const int rc = launch_tiles<T, D, C, false>(p, Q, stream)) return rc;
@@ -2023,11 +2093,11 @@ int launch(const Shape& p, const PagedParams& P, const Rooms& room, hipStream_t 
     }
     const int few_blocks = p.few_rows && !p.direct ? W * p.most : 0;
     if (few_blocks || p.tiles) {
-        const MergeParams M{parts_of(F), parts_of(Q), P.out, P.lse, P.o_ts, P.o_hs, P.l_ts,
-                            few_blocks, P.G, p.w_log, P.c};
         // for the tiles: the pairs there can be, as far as workgroups are worth it
         const int64_t pairs = std::min<int64_t>(W, int64_t(p.slots) * P.H) * p.tile_most;
         const int more = p.tiles ? static_cast<int>(std::min<int64_t>(8 * W, pairs)) : 0;
+        const MergeParams M{parts_of(F), parts_of(Q), P.out, P.lse, P.o_ts, P.o_hs, P.l_ts,
+                            few_blocks, more, P.G, p.w_log, P.c};
         merge_kernel<T, D, FewLoads<C, D>::kLead><<<few_blocks + more, kMergeThreads, 0, stream>>>(M);
         IMI_LAUNCH_CHECK("merge_kernel");
     }
@@ -2038,7 +2108,7 @@ int launch(const Shape& p, const PagedParams& P, const Rooms& room, hipStream_t 
 // one for sequences of many new tokens, and the join.
 constexpr int kJoinRows = 64;   // workgroups to a (sequence, head), at most
 template <typename T, int D, typename C>
-int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, int64_t least, hipStream_t stream) {
+int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> P, int64_t least, hipStream_t stream) {
     P.shared = b.shared;
     P.members = b.members;
     P.saved = b.saved;
@@ -2046,17 +2116,19 @@ int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, int64_
     P.keep = w.keep[0];
     P.keep_ml = w.keep_ml[0];
     P.place = w.place[0];
-    PagedParams common = tile_params(w.common, P, w.of_common, D);
+    PagedParams<C, true> common = tile_params(w.common, P, w.of_common, D);
     common.common = true;
     P.keep = w.keep[1];
     P.keep_ml = w.keep_ml[1];
     P.place = w.place[1];
-    PagedParams few = P, tiles = P;
+    PagedParams<C, true> few = P, tiles = P;
     if (w.own.few_rows) few = few_params(w.own, P, w.of_own, D);
     if (w.own.few_rows && w.common.slots <= kOwnPlan) {
         const int grid = 2 << w.own.w_log;
-        if (w.own.few_rows == 16) both_kernel<T, D, 1, C><<<grid, 512, 0, stream>>>(common, few);
-        else both_kernel<T, D, 2, C><<<grid, 512, 0, stream>>>(common, few);
+        const Common c{common.joins, common.part,     common.part_ml,  common.keep, common.keep_ml,
+                       common.place, common.min_rows, common.max_rows, common.cap,  common.slots};
+        if (w.own.few_rows == 16) both_kernel<T, D, 1, C><<<grid, kThreads, 0, stream>>>(few, c);
+        else both_kernel<T, D, 2, C><<<grid, kThreads, 0, stream>>>(few, c);
         IMI_LAUNCH_CHECK("both_kernel");
     } else {
         if (const int rc = launch_tiles<T, D, C, true>(w.common, common, stream)) return rc;
@@ -2067,22 +2139,23 @@ int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams P, int64_
         tiles = tile_params(w.own, P, w.of_own, D);
         if (const int rc = launch_tiles<T, D, C, true>(w.own, tiles, stream)) return rc;
     }
-    JoinParams J{P, w.own.few_rows, parts_of(few), parts_of(tiles), parts_of(common), w.keep[0], w.keep_ml[0], w.place[0], b.leaders};
+    const int blocks = std::min(w.own.max_rows, kJoinRows);
+    JoinParams J{{}, w.own.few_rows, blocks, parts_of(few), parts_of(tiles), parts_of(common), w.keep[0], w.keep_ml[0], w.place[0], b.leaders};
+    static_cast<BaseParams&>(J.own) = P;
+    static_cast<SharedParams&>(J.own) = P;
     J.own.w_log = w.own.w_log;
     J.own.max_rows = w.own.max_rows;
     const int64_t pairs = static_cast<int64_t>(P.S) * P.H;
-    const unsigned rows = static_cast<unsigned>(std::min(w.own.max_rows, kJoinRows));
     IMI_REQUIRE(pairs <= (1 << 24) / kJoinRows * 16, IMI_ERR_UNSUPPORTED, "too many sequences to share rows (%d)", P.S);
-    join_kernel<T, D, FewLoads<C, D>::kLead><<<dim3(static_cast<unsigned>(pairs), rows), kMergeThreads, 0, stream>>>(J);
+    join_kernel<T, D, FewLoads<C, D>::kLead><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>(blocks)), kMergeThreads, 0, stream>>>(J);
     IMI_LAUNCH_CHECK("join_kernel");
     return IMI_OK;
 }
 
-template <typename T, int D, typename C>
-int run_on(const imi_paged_attention_args* a, hipStream_t stream) {
+template <typename C, bool SH>
+PagedParams<C, SH> params_of(const imi_paged_attention_args* a) {
     const imi_paged_batch& b = a->batch;
-    const Work w = work_of(a, a->workspace);
-    PagedParams P{};
+    PagedParams<C, SH> P{};
     P.q = a->query;
     P.k = static_cast<const uint16_t*>(a->keys);
     P.v = static_cast<const uint16_t*>(a->values);
@@ -2110,12 +2183,21 @@ int run_on(const imi_paged_attention_args* a, hipStream_t stream) {
     P.window = a->window < P.capacity ? a->window : 0;   // (a window of all rows is none)
     P.sinks = P.window > 0 ? a->sinks : 0;
     P.c = a->scale * kLog2e;
-    P.ke = a->key_exponents;
-    P.ve = a->value_exponents;
-    P.e_head_s = a->exponent_head_stride;
-    P.e_page_s = static_cast<uint32_t>(a->exponent_page_stride);
-    P.e_tok_s = static_cast<uint32_t>(a->exponent_row_stride);
-    return w.shared ? launch_shared<T, D, C>(w, b, P, least_saved(a), stream) : launch<T, D, C>(w.own, P, w.of_own, stream);
+    if constexpr (C::kBits != 16) {
+        P.ke = a->key_exponents;
+        P.ve = a->value_exponents;
+        P.e_head_s = a->exponent_head_stride;
+        P.e_page_s = static_cast<uint32_t>(a->exponent_page_stride);
+        P.e_tok_s = static_cast<uint32_t>(a->exponent_row_stride);
+    }
+    return P;
+}
+
+template <typename T, int D, typename C>
+int run_on(const imi_paged_attention_args* a, hipStream_t stream) {
+    const Work w = work_of(a, a->workspace);
+    return w.shared ? launch_shared<T, D, C>(w, a->batch, params_of<C, true>(a), least_saved(a), stream)
+                    : launch<T, D, C>(w.own, params_of<C, false>(a), w.of_own, stream);
 }
 
 template <typename C>

@@ -1135,15 +1135,12 @@ def _same_rows(name: str, a: torch.Tensor, b: torch.Tensor, dev: torch.device) -
     return steps[:3]
 
 
-_NO_CODES = (0, 0, 0, 0, 0, 0)
-
-
 def _pools(key_pages, value_pages, batch: PagedBatch, dim: int, dtype: torch.dtype):
     """Checks a key and a value pool [pages, kv_heads, page_size, D] of any
     memory order with the head dim adjacent.  Returns (pages, heads, rows), the
     addresses and the page, head and row strides, and (format, addresses and
-    strides of the exponents)."""
-    codes = _NO_CODES
+    strides of the exponents) or nothing."""
+    codes = ()
     if type(key_pages) is QuantizedPages or type(value_pages) is QuantizedPages:
         if type(key_pages) is not type(value_pages) or key_pages.format != value_pages.format:
             raise TypeError("key_pages and value_pages must have the same format")
@@ -1214,7 +1211,7 @@ def paged_attention(query: torch.Tensor, key_pages, value_pages, batch: PagedBat
         l = lse.data_ptr()
     a = PagedAttentionArgs(batch.bind(P, page, N), code, H, Hq // H, D, q, q_ts, q_hs, *pools,
                            D ** -0.5 if scale is None else scale, _c_int(window), _c_int(sinks),
-                           o, o_ts, o_hs, l, l_ts, 0, 0, *codes)
+                           o, o_ts, o_hs, l, l_ts, *((0, 0) + codes if codes else ()))
     L = _lib.lib()
     ref = ctypes.byref(a)
     need = ctypes.c_size_t()
@@ -1293,7 +1290,7 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
         (P, H, page), pools, codes = _pools(key_pages, value_pages, batch, D, dtype)
         if H != Hk:
             raise ValueError(f"pages hold {H} KV heads, key has {Hk}")
-        for sp, sh, sr in (pools[2:], codes[3:]) if codes[0] else (pools[2:],):
+        for sp, sh, sr in (pools[2:], codes[3:]) if codes else (pools[2:],):
             if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1):
                 raise ValueError("pages are written, so no two of their elements may share memory")
         a = QkNormRopeArgs(batch.bind(P, page, N), code, Hq, Hk, D, *_rows("query", query, shape, dtype, dev),
@@ -1370,7 +1367,7 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
         if first.shape[0] != S:
             raise ValueError(f"first has {first.shape[0]} entries for {S} sequences")
         f = first.data_ptr()
-    a = ReadPagesArgs(batch.bind(P, page, 0), code, H, dim, *pools, *codes, f, rows, keys.data_ptr(),
+    a = ReadPagesArgs(batch.bind(P, page, 0), code, H, dim, *pools, *(codes or (0,) * 6), f, rows, keys.data_ptr(),
                       values.data_ptr(), *steps)
     with _on(dev):
         check(_lib.lib().imi_read_pages(ctypes.byref(a), _raw_stream(dev.index)), "imi_read_pages")
