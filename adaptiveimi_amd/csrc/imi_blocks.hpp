@@ -93,13 +93,15 @@ struct Int8 {
         return r;
     }
     static __device__ __forceinline__ void encode(const float (&y)[8], uint32_t (&w)[2]) {
+        // next to 1.5 * 2^23 fp32 has steps of 1: the sum is rounded as wanted and
+        // its low byte is the code
+        uint32_t b[8];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            w[i] = 0;
+        for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(y[i] + 12582912.0f);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                w[i] |= (static_cast<uint32_t>(static_cast<int>(rintf(y[4 * i + k]))) & 255u) << (8 * k);
-        }
+        for (int i = 0; i < 2; ++i)
+            w[i] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x0C0C0400u),
+                                         __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0C0C0400u), 0x05040100u);
     }
 };
 struct Fp4 {   // e2m1, two in a byte, the lower half first
@@ -152,12 +154,14 @@ __device__ __forceinline__ uint32_t block_exponent(uint32_t top) {
 template <typename C, bool HALF>
 __device__ __forceinline__ void block_encode(const float (&y)[8], uint32_t e, uint32_t (&w)[C::kWords]) {
     float x[8];
-    const float s = e == 255 ? 0.0f : __uint_as_float((254 - e) << 23);   // 2^-k
-    const float lim = e == 127 + kTopPower<C, HALF> ? C::kSafe : 1024.0f;
+    const float s = __uint_as_float((254 - e) << 23);   // 2^-k (255: left out below)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = e == 255 ? 0.0f : y[i] * s;
-        x[i] = fminf(fmaxf(x[i], -lim), lim);
+    for (int i = 0; i < 8; ++i) x[i] = y[i] * s;
+    const bool top = e >= 127 + kTopPower<C, HALF>;   // rare, 255 among them
+    if (__ballot(top)) {
+        const float lim = top ? C::kSafe : 1024.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = e == 255 ? 0.0f : __builtin_amdgcn_fmed3f(x[i], -lim, lim);
     }
     C::encode(x, w);
 }

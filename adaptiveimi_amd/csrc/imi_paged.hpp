@@ -427,6 +427,13 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 94 us,
 // 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
 // join.
+//
+// Of codes there are half or a quarter of the bytes under way, and the same number
+// of rows, so the work on a row tells: over 131072 rows of 8 heads of 128 fp8 takes
+// 54 us (5.1 TB/s), int8, whose codes take five instructions a pair where the others
+// take one, 58, fp4 36 (4.0 TB/s).  In a ragged int8 batch vector instructions hold
+// half of the issue slots.  Two workgroups per CU (128 registers, spilled) took 88
+// us for the 61 with its join in fp8; with 64 dims, where they fit, 41 for 37.
 constexpr int kFewWaves = kThreads / 64;
 // Rows of K / V per wave and step: 32, or 64 of 64 dims in 4 bits, which then
 // have as many bytes under way as others (3 tokens each of 12 sequences over 4000 ..
@@ -522,7 +529,9 @@ __device__ __forceinline__ FewRange few_range(const P& a, int block) {
 // Codes (C): a lane loads D / 4 of a K row's dims for the matrix instruction,
 // in pieces of up to 16 bytes; which of them an instruction takes is free, as
 // long as the queries come in the same order (frag_dim).  They become bf16 or
-// fp16 in registers, those of V on the way to LDS.
+// fp16 in registers, those of V on the way to LDS.  A row's place and exponents
+// are looked up by one lane and go to the others by lane exchange: a load for each
+// piece (a byte) and 64-bit addresses in every lane cost 45 registers more.
 template <typename C, int D>
 struct FewLoads {
     static constexpr int kWords = C::kBits == 16 ? 4 : D * C::kBits / 128;       // a lane's words of a K row
@@ -1134,6 +1143,12 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
 // the staging the same loop runs at 1190, without the softmax at 1100.  Tiles
 // of 128 rows read K and V twice as often and were slower, 64 rows per wave
 // (half as many reads of LDS) no faster.
+//
+// Codes are loaded a step ahead into registers (as many as V's rows take in 16
+// bits) and become bf16 or fp16 on their way to LDS, once for all waves; the
+// exponents of a wave's 16 rows are one load of a lane each.  A byte for each piece
+// spilled 74 registers, in every step: 2.21 ms for 4096 fp8 tokens over 16384 rows
+// (32 heads), now 0.96, 1000 TFLOP/s; int8 1.05, fp4 0.93, in 16 bits 0.98.
 constexpr int kTileRows = 256;
 constexpr int kStage = 64;            // cached rows of a stage in LDS
 constexpr int kStep = 2 * kStage;     // and of a step

