@@ -389,12 +389,14 @@ __device__ __forceinline__ float exp2_weight(float m, float M, float c) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - M) * c);
 }
 
+constexpr int kTileRows = 256;   // rows of a tile of the tile kernel
+
 // Where the rows of a problem (r0 ..: its first row, or of a tile) are with
 // shared rows, for each head: -1, in `keep`, or the range that holds its first
 // unit, in that range's partials and those after it.  Problems begin at query
 // rows t0 G in the order of s, so no two tiles have the same key.
 __device__ __forceinline__ int place_key(const BaseParams& a, int t0, int s, int r0) {
-    return static_cast<int>((static_cast<int64_t>(t0) * a.G + r0) / 256) + s;
+    return static_cast<int>((static_cast<int64_t>(t0) * a.G + r0) / kTileRows) + s;
 }
 
 // What a row's sum L of weights divides by: nothing for a row that sees nothing
@@ -424,7 +426,7 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // the matrix instruction wants it, 64 bytes of 16 rows at a time; V goes through
 // LDS and is loaded in whole rows, which the cache serves faster (768 rows in a
 // workgroup 16.0 -> 14.1 us; K in the same way 12.0, but then the long streams
-// lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 94 us,
+// lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 95 us,
 // 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
 // join.
 //
@@ -1148,8 +1150,8 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(MergeParams a) {
 // bits) and become bf16 or fp16 on their way to LDS, once for all waves; the
 // exponents of a wave's 16 rows are one load of a lane each.  A byte for each piece
 // spilled 74 registers, in every step: 2.21 ms for 4096 fp8 tokens over 16384 rows
-// (32 heads), now 0.96, 1000 TFLOP/s; int8 1.05, fp4 0.93, in 16 bits 0.98.
-constexpr int kTileRows = 256;
+// (32 heads), now 0.96-1.02, 950-1000 TFLOP/s (of one card: fp8 1.016, int8 1.105,
+// fp4 0.974, in 16 bits 1.035).
 constexpr int kStage = 64;            // cached rows of a stage in LDS
 constexpr int kStep = 2 * kStage;     // and of a step
 

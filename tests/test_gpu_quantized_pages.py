@@ -413,3 +413,48 @@ def test_captured_steps_and_streams(ops):
             step(eager, e_out, e_back)
         side.synchronize()
         assert torch.equal(out, e_out) and torch.equal(back[0], e_back[0]) and torch.equal(back[1], e_back[1])
+
+
+def test_layer_of_arguments_refuses(ops):
+    """The Python layer's checks of pools, outputs and rows."""
+    P, H, page, D = 6, 2, 8, 64
+    pool = ops.QuantizedPages.zeros(P, H, page, D, "fp8", DEV)
+    batch = ops.PagedBatch(i32([[0, 1, 2]]), i32([20]), i32([0, 1]), 1)
+    q = torch.zeros((1, 4, D), dtype=BF, device=DEV)
+    key = torch.zeros((1, H, D), dtype=BF, device=DEV)
+    plain = torch.zeros((P, H, page, D), dtype=BF, device=DEV)
+    wide = ops.QuantizedPages.zeros(P, H, page, 128, "fp8", DEV)
+    whole = ops.QuantizedPages.zeros(P, H, page, D, "int8", DEV)
+    flat = ops.QuantizedPages(pool.codes, pool.exponents[:1].expand(P, H, page, 2))
+    for k, v in ((pool, plain), (plain, pool), (pool, whole), (wide, wide)):
+        with pytest.raises((TypeError, ValueError)):
+            ops.paged_attention(q, k, v, batch)
+        with pytest.raises((TypeError, ValueError)):
+            ops.qk_norm_rope(q, key, value=key, batch=batch, key_pages=k, value_pages=v)
+    assert ops.paged_attention(q, flat, flat, batch).shape == q.shape      # read, not written
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope(q, key, value=key, batch=batch, key_pages=flat, value_pages=flat)
+    with pytest.raises((TypeError, ValueError)):
+        ops.read_pages(pool, plain, batch)
+    out = [torch.zeros((1, H, 20, D), dtype=BF, device=DEV) for _ in range(2)]
+    assert ops.read_pages(pool, pool, batch, out=tuple(out))[0] is out[0]
+    for kw in (dict(rows=-1), dict(dtype=torch.float32), dict(out=tuple(out), rows=19), dict(first=i32([0, 0])),
+               dict(first=torch.zeros(1, dtype=torch.int64, device=DEV)), dict(out=(out[0], out[1].half())),
+               dict(out=(out[0], out[1].transpose(2, 3).contiguous().transpose(2, 3))),
+               dict(out=(out[0][:, :1].expand(1, H, 20, D), out[1][:, :1].expand(1, H, 20, D)))):
+        with pytest.raises((TypeError, ValueError)):
+            ops.read_pages(pool, pool, batch, **kw)
+    with pytest.raises(TypeError):
+        ops.read_pages(plain, plain, batch, dtype=HF)       # 16-bit rows are read as they are
+
+
+def test_sixteen_bit_type_of_the_rows_read(ops):
+    """One pool read as bf16 and as fp16."""
+    codes, exps, c, e = fill("fp8", 4, 1, 16, 128, "heads", 3)
+    pool = ops.QuantizedPages(c, e)
+    batch = ops.PagedBatch(i32([[2, 0]]), i32([32]), i32([0, 0]), 1)
+    want = blocks.decode(codes, exps, "fp8")
+    for dtype in (BF, HF):
+        keys, _ = ops.read_pages(pool, pool, batch, rows=32, dtype=dtype)
+        assert keys.dtype is dtype
+        assert torch.equal(keys[0, 0].cpu(), torch.cat([blocks.rounded(want[i, 0], dtype) for i in (2, 0)]))

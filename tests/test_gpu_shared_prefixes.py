@@ -345,3 +345,51 @@ def test_a_server_with_beams(ops):
     batch = step(other, [1, 0, 3, 1])
     assert batch.members.tolist() == [0, 0, 2, 0]
     assert math.isfinite(float(batch.shared.sum()))
+
+
+@pytest.mark.parametrize("chunk", [1, 60])
+def test_many_sequences(ops, chunk):
+    """More tiles than a workgroup plans for itself, of common and of own rows."""
+    groups = [(72, ones(*[1 + i % 9 for i in range(259)])), (64, ones(*[1 + i % 5 for i in range(258)]) + [(60, chunk)])]
+    x = forked(groups, 1, 2, 64, 8, BF)
+    batch, (out, lse) = attend(ops, x)
+    assert sorted(batch.members.tolist())[-2:] == [259, 259]
+    check(x, out, lse)
+
+
+def test_a_batch_is_shared_again(ops):
+    """The result of share_prefixes is a batch like others; the given one stays."""
+    x = forked([(200, ones(5, 60, 9))], 2, 4, 128, 8, BF)
+    plain = ops.PagedBatch(x["table"], x["lens"], x["start"], 1)
+    once = ops.share_prefixes(plain, 8, least_bytes=1)
+    twice = ops.share_prefixes(once, labels=i32([0, 0, 1]), least_bytes=1)
+    assert plain.shared is None and once.members.tolist() == [3, 0, 0] and twice.members.tolist() == [2, 0, 0]
+    for batch in (plain, once, twice):
+        out, lse = ops.paged_attention(x["q"], x["k"], x["v"], batch, return_lse=True)
+        check(x, out, lse)
+    with pytest.raises(ValueError):
+        ops.paged_attention(x["q"], x["k"][:, :, :4], x["v"][:, :, :4], once)   # pages of another size
+    for kw in (dict(page_size=None), dict(page_size=8, labels=i32([0])), dict(page_size=8, least_bytes=0)):
+        with pytest.raises(ValueError):
+            ops.share_prefixes(plain, **kw)
+    with pytest.raises(ValueError):
+        ops.share_prefixes(once, 16)
+    with pytest.raises(ValueError):
+        ops.share_prefixes(ops.PagedBatch(None, x["lens"], x["start"], 1), 8)
+
+
+def test_a_sequence_handed_to_retrieval(ops):
+    """Rows of an 8-bit paged cache, read back, build the same index as the same rows
+    in a tensor of their own."""
+    H, D, page, n = 2, 128, 16, 700
+    x = forked([(0, ones(n))], H, 4, D, page, BF, seed=5)
+    x = quantize(ops, x, "int8")
+    batch = ops.PagedBatch(x["table"], x["lens"], x["start"], 1)
+    keys, values = ops.read_pages(x["k"], x["v"], batch, rows=n)
+    own_k, own_v = (t.to(DEV).contiguous() for t in x["rows"][0])
+    assert torch.equal(keys[0], own_k) and torch.equal(values[0], own_v)
+    got = []
+    for k, v in ((keys[0], values[0]), (own_k, own_v)):
+        cent, labels, _ = ops.kmeans(k, (8, 8), 5)
+        got.append(ops.build_index(k, v, cent, labels, (8, 8)))
+    assert all(torch.equal(got[0][name], got[1][name]) for name in ("cell_count", "perm", "list_keys", "list_values"))
