@@ -261,8 +261,8 @@ __device__ __forceinline__ int64_t row_offset(const BaseParams& a, int page, int
 template <typename P>
 __device__ __forceinline__ int64_t exp_offset(const P& a, int page, int j) {
     const uint32_t slot = static_cast<uint32_t>(j) & ((1u << a.page_shift) - 1u);
-    return static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(clampi(page, 0, a.n_pages - 1))) * a.e_page_s +
-                                slot * a.e_tok_s);
+    const uint64_t id = static_cast<uint32_t>(clampi(page, 0, a.n_pages - 1));
+    return static_cast<int64_t>(id * a.e_page_s + slot * a.e_tok_s);
 }
 
 __device__ __forceinline__ void wave_lds_sync() {
@@ -341,8 +341,8 @@ __device__ __forceinline__ void keep_finite(u32x4_t (&x)[N]) {
 // of the span's rows [v0, v1) that each sees, to the output (slot < 0) or to
 // the partial.  The workgroup's own writes of these rows are done.
 template <typename T, int D, typename C, bool SH, typename SpanT>
-__device__ __forceinline__ void patch_rows(const PagedParams<C, SH>& a, const Seq& sq, int s, int h, const SpanT& sp, int first,
-                                           int end, int v0, int v1, int64_t slot) {
+__device__ __forceinline__ void patch_rows(const PagedParams<C, SH>& a, const Seq& sq, int s, int h, const SpanT& sp,
+                                           int first, int end, int v0, int v1, int64_t slot) {
     for (int x = threadIdx.x; x < (end - first) * (D / 2); x += kThreads) {
         const int r = first + x / (D / 2), d = 2 * (x % (D / 2));
         const int p = sq.p0 + r / a.G;
@@ -353,15 +353,15 @@ __device__ __forceinline__ void patch_rows(const PagedParams<C, SH>& a, const Se
             const int page = page_of(a, s, j);
             uint32_t w;
             if constexpr (C::kBits == 16) {
-                w = *reinterpret_cast<const uint32_t*>(a.v + row_offset(a, page, j) + static_cast<int64_t>(h) * a.head_s +
-                                                       d);
+                w = *reinterpret_cast<const uint32_t*>(a.v + row_offset(a, page, j) +
+                                                       static_cast<int64_t>(h) * a.head_s + d);
             } else {
                 const uint8_t* const row =
                     reinterpret_cast<const uint8_t*>(a.v) + row_offset(a, page, j) + static_cast<int64_t>(h) * a.head_s;
-                uint32_t x[C::kWords] = {};
-                x[0] = C::kBits == 8 ? *reinterpret_cast<const uint16_t*>(row + d) : row[d / 2];
+                uint32_t codes[C::kWords] = {};   // the two that count, first
+                codes[0] = C::kBits == 8 ? *reinterpret_cast<const uint16_t*>(row + d) : row[d / 2];
                 w = C::template decode<T::kHalf>(
-                    x, a.ve[exp_offset(a, page, j) + static_cast<int64_t>(h) * a.e_head_s + d / kBlock])[0];
+                    codes, a.ve[exp_offset(a, page, j) + static_cast<int64_t>(h) * a.e_head_s + d / kBlock])[0];
             }
             const uint32_t m = finite_halves<T>(w);
             if (!(m & 0xFFFFu)) add[0] += T::wide(w & 0xFFFFu);
@@ -568,7 +568,8 @@ struct FewLds {
 };
 
 template <typename T, int D, int NB, typename C, bool SH>
-__device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct, int block, const FewLds<C, D, NB>& lds) {
+__device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct, int block,
+                                         const FewLds<C, D, NB>& lds) {
     constexpr int KK = D / 32;     // matrix instructions over the head dim
     constexpr int DB = D / 16;     // output blocks of 16 dims
     constexpr int LR = kRow<D>;
@@ -579,7 +580,8 @@ __device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct
     constexpr int TILE = Lo::kTile, UNIT = TILE * kFewWaves, KB = TILE / 16;   // KB: blocks of 16 rows
     constexpr int kWaveLds = FewLds<C, D, NB>::kWave;
     constexpr bool kQueryLds = FewLds<C, D, NB>::kQuery;
-    static_assert(kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0, "rows and partials are read and written 16 bytes at a time");
+    static_assert(kWaveLds * 2 % 16 == 0 && LR * 2 % 16 == 0,
+                  "rows and partials are read and written 16 bytes at a time");
     uint16_t* const s_buf = lds.buf;
     uint16_t* const s_q = lds.q;
     auto* const s_ml = lds.ml;
@@ -667,7 +669,8 @@ __device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct
         // (codes)
         const uint8_t* const kc = reinterpret_cast<const uint8_t*>(a.k) + static_cast<int64_t>(h) * a.head_s +
                                   lg * (Lo::kPiece * C::kBits / 8);
-        const uint8_t* const vc = reinterpret_cast<const uint8_t*>(a.v) + static_cast<int64_t>(h) * a.head_s + 16 * (lane % CH);
+        const uint8_t* const vc = reinterpret_cast<const uint8_t*>(a.v) + static_cast<int64_t>(h) * a.head_s +
+                                  16 * (lane % CH);
         const uint8_t *kx = nullptr, *vx = nullptr;
         if constexpr (kCodes) {
             kx = (TILE == 64 || lane < 32 ? a.ke : a.ve) + static_cast<int64_t>(h) * a.e_head_s;
@@ -696,7 +699,9 @@ __device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct
         };
         u32x4_t kb[kCodes ? 1 : 2][KK], vb[kCodes ? 1 : NV];
         uint32_t kw[KB][Lo::kWords], vw[NV][4], ke = 0, ve = 0;   // codes and exponents
-        auto from = [](int lane, uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * lane, x)); };
+        auto from = [](int lane, uint32_t x) {
+            return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(4 * lane, x));
+        };
         auto fetch = [&](int u) {
             if constexpr (!kCodes) {
 #pragma unroll
@@ -954,7 +959,8 @@ __device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct
             __syncthreads();
         }
         if constexpr (SH)
-            if (u0 == 0 && tid == 0) a.place[static_cast<int64_t>(place_key(a, sq.t0, s, 0)) * a.H + h] = whole ? -1 : block;
+            if (u0 == 0 && tid == 0)
+                a.place[static_cast<int64_t>(place_key(a, sq.t0, s, 0)) * a.H + h] = whole ? -1 : block;
         if (u0 == 0 && u1 < units - LEAD)
             rest = Join{range.total, g0 - at, g0 - at + units, sq.t0, 0, rows, h, max(-p0, 0) * a.G};
         g0 += end - at;
@@ -1330,7 +1336,8 @@ __device__ __forceinline__ int make_plan(const P& a, const Plan& p, int64_t* s_w
     for (int s0 = 0; s0 < a.S; s0 += THREADS) {
         const int s = s0 + threadIdx.x;
         int64_t total;
-        const int64_t incl = block_incl_scan<THREADS, int64_t>(s < a.S ? seq_tiles(a, seq_of<SH>(a, s)) : 0, s_wave, total);
+        const int64_t tiles = s < a.S ? seq_tiles(a, seq_of<SH>(a, s)) : 0;
+        const int64_t incl = block_incl_scan<THREADS>(tiles, s_wave, total);
         if (s < a.S) p.seqs[s] = static_cast<int32_t>(min(n + incl, static_cast<int64_t>(a.slots)));
         n += total;
     }
@@ -1352,7 +1359,7 @@ __device__ __forceinline__ int make_plan(const P& a, const Plan& p, int64_t* s_w
             u = max((tile_span(a, seq_of<SH>(a, lo), row).vis + kStep - 1) / kStep, 1);
         }
         int64_t total;
-        const int64_t incl = block_incl_scan<THREADS, int64_t>(u, s_wave, total);
+        const int64_t incl = block_incl_scan<THREADS>(u, s_wave, total);
         if (t < n_tiles) p.steps[t] = before + incl;
         before += total;
     }
@@ -1995,7 +2002,8 @@ inline size_t carve(const Shape& p, void* base, Rooms& r) {
 constexpr int64_t kShareBytes = int64_t(230) << 20;
 inline int64_t least_saved(const imi_paged_attention_args* a) {
     static constexpr int kBits[] = {16, 8, 8, 4};
-    const int64_t row = 2 * a->kv_heads * (a->dim * kBits[a->format] / 8 + (a->format == IMI_ROWS ? 0 : a->dim / kBlock));
+    const int row_bytes = a->dim * kBits[a->format] / 8 + (a->format == IMI_ROWS ? 0 : a->dim / kBlock);
+    const int64_t row = int64_t(2) * a->kv_heads * row_bytes;
     return std::max<int64_t>((a->batch.share_bytes ? a->batch.share_bytes : kShareBytes) / row, 1);
 }
 inline bool shares(const imi_paged_attention_args* a) {
@@ -2157,14 +2165,16 @@ int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> 
         if (const int rc = launch_tiles<T, D, C, true>(w.own, tiles, stream)) return rc;
     }
     const int blocks = std::min(w.own.max_rows, kJoinRows);
-    JoinParams J{{}, w.own.few_rows, blocks, parts_of(few), parts_of(tiles), parts_of(common), w.keep[0], w.keep_ml[0], w.place[0], b.leaders};
+    JoinParams J{{},           w.own.few_rows, blocks,     parts_of(few), parts_of(tiles), parts_of(common),
+                 w.keep[0],    w.keep_ml[0],   w.place[0], b.leaders};
     static_cast<BaseParams&>(J.own) = P;
     static_cast<SharedParams&>(J.own) = P;
     J.own.w_log = w.own.w_log;
     J.own.max_rows = w.own.max_rows;
     const int64_t pairs = static_cast<int64_t>(P.S) * P.H;
     IMI_REQUIRE(pairs <= (1 << 24) / kJoinRows * 16, IMI_ERR_UNSUPPORTED, "too many sequences to share rows (%d)", P.S);
-    join_kernel<T, D, FewLoads<C, D>::kLead><<<dim3(static_cast<unsigned>(pairs), static_cast<unsigned>(blocks)), kMergeThreads, 0, stream>>>(J);
+    const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(blocks));
+    join_kernel<T, D, FewLoads<C, D>::kLead><<<grid, kMergeThreads, 0, stream>>>(J);
     IMI_LAUNCH_CHECK("join_kernel");
     return IMI_OK;
 }

@@ -407,8 +407,13 @@ extern "C" int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t str
     const int grid = (P.N + P.tokens - 1) / P.tokens;
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int format = paged ? a->format : IMI_ROWS;
-    if (a->dtype == IMI_BF16) a->dim == 128 ? launch<BF16, 128>(P, format, grid, st) : launch<BF16, 64>(P, format, grid, st);
-    else a->dim == 128 ? launch<FP16, 128>(P, format, grid, st) : launch<FP16, 64>(P, format, grid, st);
+    if (a->dtype == IMI_BF16) {
+        if (a->dim == 128) launch<BF16, 128>(P, format, grid, st);
+        else launch<BF16, 64>(P, format, grid, st);
+    } else {
+        if (a->dim == 128) launch<FP16, 128>(P, format, grid, st);
+        else launch<FP16, 64>(P, format, grid, st);
+    }
     IMI_LAUNCH_CHECK("qk_norm_rope_kernel");
     return IMI_OK;
 }

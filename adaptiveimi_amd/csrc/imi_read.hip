@@ -136,8 +136,13 @@ extern "C" int imi_read_pages(const imi_read_pages_args* a, imi_stream_t stream)
                        static_cast<int>(batch_capacity(&b)), a->rows, static_cast<int>(chunks)};
     const unsigned grid = static_cast<unsigned>(chunks * a->kv_heads * b.n_seqs);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (a->dtype == IMI_BF16) a->dim == 128 ? launch<false, 128>(P, a->format, grid, st) : launch<false, 64>(P, a->format, grid, st);
-    else a->dim == 128 ? launch<true, 128>(P, a->format, grid, st) : launch<true, 64>(P, a->format, grid, st);
+    if (a->dtype == IMI_BF16) {
+        if (a->dim == 128) launch<false, 128>(P, a->format, grid, st);
+        else launch<false, 64>(P, a->format, grid, st);
+    } else {
+        if (a->dim == 128) launch<true, 128>(P, a->format, grid, st);
+        else launch<true, 64>(P, a->format, grid, st);
+    }
     IMI_LAUNCH_CHECK("read_kernel");
     return IMI_OK;
 }

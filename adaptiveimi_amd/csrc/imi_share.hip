@@ -112,7 +112,8 @@ extern "C" int imi_share_prefixes_workspace_size(const imi_paged_batch* b, size_
 }
 
 extern "C" int imi_share_prefixes(const imi_paged_batch* b, const int32_t* labels, int32_t* shared, int32_t* members,
-                                  int32_t* leaders, int64_t* saved, void* workspace, size_t workspace_bytes, imi_stream_t stream) {
+                                  int32_t* leaders, int64_t* saved, void* workspace, size_t workspace_bytes,
+                                  imi_stream_t stream) {
     using namespace imi;
     clear_error();
     IMI_REQUIRE(b, IMI_ERR_INVALID, "null argument");

@@ -1423,8 +1423,8 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None, labels: O
         new.found = torch.empty((4 * S + 2,), dtype=torch.int32, device=dev)   # (4 S ints: a multiple of 16 bytes)
         at = new.found.data_ptr()
         with _on(dev):
-            check(_lib.lib().imi_share_prefixes(ctypes.byref(a), f, at, at + 4 * S, at + 8 * S, at + 16 * S, at + 12 * S,
-                                                4 * S, _raw_stream(dev.index)), "imi_share_prefixes")
+            check(_lib.lib().imi_share_prefixes(ctypes.byref(a), f, at, at + 4 * S, at + 8 * S, at + 16 * S,
+                                                at + 12 * S, 4 * S, _raw_stream(dev.index)), "imi_share_prefixes")
         a.shared, a.members, a.leaders, a.saved = at, at + 4 * S, at + 8 * S, at + 16 * S
         a.share_bytes = min(least_bytes or 0, 2 ** 62)
     return new
