@@ -426,7 +426,7 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 // the matrix instruction wants it, 64 bytes of 16 rows at a time; V goes through
 // LDS and is loaded in whole rows, which the cache serves faster (768 rows in a
 // workgroup 16.0 -> 14.1 us; K in the same way 12.0, but then the long streams
-// lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 95 us,
+// lose 3 percent to LDS).  One token over 131072 rows of 8 heads of 128: 94 us,
 // 5.7 TB/s (a large copy runs at 4.84); 64 dims, 4 x 30000 rows: 44 us with its
 // join.
 //
@@ -817,7 +817,11 @@ __device__ __forceinline__ void few_body(const PagedParams<C, SH>& a, int direct
                     }
                 }
             if (u + 1 < u1) {
+                // a wave that gets here issues its loads ahead of the other's work
+                // (131072 bf16 rows: 99.8 us, 102 without; codes as fast either way)
+                __builtin_amdgcn_s_setprio(3);
                 fetch(u + 1);
+                __builtin_amdgcn_s_setprio(0);
                 fetch_ids(min(u + 2, u1 - 1));
             }
             wave_lds_sync();

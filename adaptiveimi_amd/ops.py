@@ -1131,7 +1131,7 @@ def _same_rows(name: str, a: torch.Tensor, b: torch.Tensor, dev: torch.device) -
     if b.shape != a.shape or (b.stride() != a.stride() and _steps(b) != steps):
         raise ValueError(f"{name} must share shape and strides")
     if a.device != dev or b.device != dev:
-        raise ValueError(f"pages are on {a.device} and {b.device}, expected {dev}")
+        raise ValueError(f"{name} are on {a.device} and {b.device}, expected {dev}")
     return steps[:3]
 
 
@@ -1290,9 +1290,10 @@ def qk_norm_rope(query: torch.Tensor, key: torch.Tensor, positions: Optional[tor
         (P, H, page), pools, codes = _pools(key_pages, value_pages, batch, D, dtype)
         if H != Hk:
             raise ValueError(f"pages hold {H} KV heads, key has {Hk}")
-        for sp, sh, sr in (pools[2:], codes[3:]) if codes else (pools[2:],):
-            if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1):
-                raise ValueError("pages are written, so no two of their elements may share memory")
+        _, _, sp, sh, sr = pools
+        if (sp == 0 and P > 1) or (sh == 0 and H > 1) or (sr == 0 and page > 1) or (
+                codes and any(step == 0 and n > 1 for step, n in zip(codes[3:], (P, H, page)))):
+            raise ValueError("pages are written, so no two of their elements may share memory")
         a = QkNormRopeArgs(batch.bind(P, page, N), code, Hq, Hk, D, *_rows("query", query, shape, dtype, dev),
                            *_rows("key", key, k_shape, dtype, dev), *_rows("value", value, k_shape, dtype, dev), 0, 0,
                            f, rotary, int(interleaved), qw, kw, w32, eps,
