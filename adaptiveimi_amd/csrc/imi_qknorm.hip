@@ -20,8 +20,9 @@
 // magnitude two lane exchanges find; the codes are made of the fp32 results, so
 // a key is rounded once there too.  10529 tokens of 48 heads into fp8: 60 us, bound
 // by vector instructions (0.77 of the issue slots; 237 MB, 3.9 TB/s).  A row's four
-// exponents gathered for one store were slower (7 us) than a byte by each block's
-// first lane, one path for keys and values 2 us.
+// exponents gathered for one store were no faster than a byte by each block's first
+// lane.  Keys and values take one path: with one each, 4 bits spill two registers,
+// which costs 6 us (8 bits gain 1).
 #include <algorithm>
 
 #include "imi_blocks.hpp"
@@ -224,24 +225,15 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
             const int ti = token_of(p), h = p - ti * HT;
             const int64_t t = t0 + ti;
             if (!s_own[ti]) continue;
-            if (h >= a.Hq + a.Hk) {   // a value head: copied
-                if (s_slot[ti] >= 0) {
-                    const int kv = h - a.Hq - a.Hk;
-                    if constexpr (kCodes) {
-                        float y[8];
-                        unpack8<T>(x[i], y);
-                        store_codes<T, C>(y, reinterpret_cast<uint8_t*>(a.vo) + s_slot[ti] + kv * a.ko_hs,
-                                          a.ve + s_exp[ti] + kv * a.e_hs, c);
-                    } else {
-                        *reinterpret_cast<u32x4_t*>(a.vo + s_slot[ti] + kv * a.ko_hs + 8 * c) = x[i];
-                    }
-                }
+            const bool is_v = h >= a.Hq + a.Hk, is_q = h < a.Hq;
+            if (!kCodes && is_v) {   // copied
+                if (s_slot[ti] >= 0)
+                    *reinterpret_cast<u32x4_t*>(a.vo + s_slot[ti] + (h - a.Hq - a.Hk) * a.ko_hs + 8 * c) = x[i];
                 continue;
             }
-            const bool is_q = h < a.Hq;
             float y[8];
             unpack8<T>(x[i], y);
-            if (is_q ? a.qw != nullptr : a.kw != nullptr) {
+            if (!(kCodes && is_v) && (is_q ? a.qw != nullptr : a.kw != nullptr)) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ss += y[j] * y[j];
@@ -253,7 +245,7 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) y[j] = y[j] * inv * s_w[is_q ? 0 : 1][8 * c + j];
             }
-            if (a.half) {
+            if (!(kCodes && is_v) && a.half) {
                 if (a.interleaved) {
                     if (8 * c < 2 * a.half) {
 #pragma unroll
@@ -280,9 +272,10 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
             }
             if constexpr (kCodes) {
                 if (!is_q) {
+                    const int kv = h - a.Hq - (is_v ? a.Hk : 0);
                     if (s_slot[ti] >= 0)
-                        store_codes<T, C>(y, reinterpret_cast<uint8_t*>(a.ko) + s_slot[ti] + (h - a.Hq) * a.ko_hs,
-                                          a.ke + s_exp[ti] + (h - a.Hq) * a.e_hs, c);
+                        store_codes<T, C>(y, reinterpret_cast<uint8_t*>(is_v ? a.vo : a.ko) + s_slot[ti] + kv * a.ko_hs,
+                                          (is_v ? a.ve : a.ke) + s_exp[ti] + kv * a.e_hs, c);
                     continue;
                 }
             }
