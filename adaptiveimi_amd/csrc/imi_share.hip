@@ -2,9 +2,10 @@
 //
 // Pairs first: a workgroup per sequence compares its table with its neighbour's
 // (a(s) = equal leading pages of s - 1 and s, at most those before the new
-// tokens of either).  Pages are equal for all of a run where they are for each
-// pair, so a run is a stretch of a(s) >= 1 behind its first sequence and shares
-// the smallest of them: a wave per run.  Reads each table twice at most; one
+// tokens of either; none where another page follows before kMinShared rows).
+// Pages are equal for all of a run where they are for each pair, so a run is a
+// stretch of a(s) >= 1 behind its first sequence and shares the smallest of them:
+// a wave per run.  Reads each table twice at most; one
 // call serves every layer of a step.  64 sequences of 512 common pages: 4.8 us and
 // 4.8 us, most of it the chain of loads; the host's call takes 8.6.
 #include "imi_common.hpp"
@@ -56,7 +57,9 @@ __global__ __launch_bounds__(kPairThreads) void pairs_kernel(ShareParams a) {
         __syncthreads();
         if (found) break;
     }
-    if (threadIdx.x == 0) a.pairs[s] = s_first;
+    // tables that part within kMinShared rows part the runs: chained, the pair would
+    // leave those on either side of it nothing to share
+    if (threadIdx.x == 0) a.pairs[s] = s_first < most && s_first * a.page_size < kMinShared ? 0 : s_first;
 }
 
 __global__ __launch_bounds__(64) void runs_kernel(ShareParams a) {

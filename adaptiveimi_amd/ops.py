@@ -1383,7 +1383,8 @@ def share_prefixes(batch: PagedBatch, page_size: Optional[int] = None, labels: O
     A run is a row of neighbouring sequences whose tables begin with the same
     page (forked prompts, beams: fork_pages keeps them so); it shares the
     leading pages that all of them have in common before their new tokens.
-    ``labels`` int32 [S]: neighbours of different labels are not put together
+    Neighbours whose tables part within the first 64 rows (a short header of
+    all prompts) are in different runs.  ``labels`` int32 [S]: neighbours of different labels are not put together
     (all sequences begin with one system prompt, and the beams of a prompt share
     more).  In the result ``shared`` int32 [S] are the rows that each sequence
     shares (multiples of 8; 0 for those on their own, or with fewer than 64) and

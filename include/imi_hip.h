@@ -624,6 +624,7 @@ int imi_read_pages(const imi_read_pages_args* a, imi_stream_t stream);
  * sequences of the batch whose tables begin with the same page (and, with
  * labels, that have the same label); it shares the leading pages that all of
  * them have in common, as far as they lie before the new tokens of each.
+ * Neighbours whose tables part within the first 64 rows are in different runs.
  * shared[s] = rows that sequence s shares with its run, a multiple of 8, or 0
  * where it is alone or they are fewer than 64; members[s] = sequences of the run
  * that s is the first of, or 0; leaders[s] = the first of its run, or s itself;
