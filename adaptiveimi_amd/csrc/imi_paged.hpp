@@ -2010,9 +2010,12 @@ inline int64_t least_saved(const imi_paged_attention_args* a) {
     const int64_t row = int64_t(2) * a->kv_heads * row_bytes;
     return std::max<int64_t>((a->batch.share_bytes ? a->batch.share_bytes : kShareBytes) / row, 1);
 }
+constexpr int kJoinRows = 64;          // workgroups of join_kernel to a (sequence, head), at most
+constexpr int kJoinPairs = 1 << 22;    // (sequence, head) pairs, at most: 2^30 threads along x
 inline bool shares(const imi_paged_attention_args* a) {
     const imi_paged_batch& b = a->batch;
     if (!b.shared || !b.page_table || b.n_seqs < 2 || b.n_tokens == 0) return false;
+    if (static_cast<int64_t>(b.n_seqs) * a->kv_heads > kJoinPairs) return false;
     const int64_t capacity = batch_capacity(&b);
     if (a->window > 0 && a->window < capacity) return false;
     const int64_t longest = b.max_len > 0 ? std::min<int64_t>(capacity, b.max_len) : capacity;
@@ -2135,7 +2138,6 @@ int launch(const Shape& p, const PagedParams<C, false>& P, const Rooms& room, hi
 
 // Shared and own rows: a launch, where the workgroups can plan for themselves,
 // one for sequences of many new tokens, and the join.
-constexpr int kJoinRows = 64;   // workgroups to a (sequence, head), at most
 template <typename T, int D, typename C>
 int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> P, int64_t least, hipStream_t stream) {
     P.shared = b.shared;
@@ -2175,9 +2177,7 @@ int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> 
     static_cast<SharedParams&>(J.own) = P;
     J.own.w_log = w.own.w_log;
     J.own.max_rows = w.own.max_rows;
-    const int64_t pairs = static_cast<int64_t>(P.S) * P.H;
-    IMI_REQUIRE(pairs <= (1 << 24) / kJoinRows * 16, IMI_ERR_UNSUPPORTED, "too many sequences to share rows (%d)", P.S);
-    const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(blocks));
+    const dim3 grid(static_cast<unsigned>(P.S) * P.H, static_cast<unsigned>(blocks));
     join_kernel<T, D, FewLoads<C, D>::kLead><<<grid, kMergeThreads, 0, stream>>>(J);
     IMI_LAUNCH_CHECK("join_kernel");
     return IMI_OK;
