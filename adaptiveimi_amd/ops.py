@@ -1020,9 +1020,11 @@ class PagedBatch:
     query_start: int32 [S + 1], sequence s's new tokens are the query rows
     query_start[s] .. query_start[s + 1] - 1; query rows behind the last
     sequence belong to none.  max_query: at least every sequence's new tokens
-    (the rows of one with more may be left as they are).  max_len: a hint, about the
-    longest sequence (default: what the table holds); only the split of short
-    batches depends on it.
+    (the rows of one with more may be left as they are).  max_len: at least the
+    rows of every sequence (default: what the table holds).  paged_attention sees
+    the rows of a longer one too, and only goes by max_len where it splits short
+    batches and looks for rows to share; read_pages gives so many rows, no more,
+    where it is not told how many.
 
     ``shared``, ``members``, ``leaders`` and ``saved`` are None but in a batch of
     share_prefixes."""
@@ -1323,8 +1325,10 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
     e.g. ``keys[s]`` for kmeans and build_index, or for a cache elsewhere.
 
     QuantizedPages are read as their values in ``dtype`` (bf16 unless given or
-    ``out`` says), a tensor's rows as they are.  ``rows``: by default what the
-    batch's max_len, or else the table, says.  ``out``: tensors of any sequence,
+    ``out`` says), a tensor's rows as they are.  ``rows``: by default the batch's
+    max_len, or what the table holds if that is less or there is none; of a sequence
+    that is longer the rest is not read, so give ``rows`` where max_len may be
+    exceeded.  ``out``: tensors of any sequence,
     head and row strides to write to.  Rows that a sequence does not have are
     left as they are (unset in tensors made here)."""
     dev = batch.device
@@ -1347,7 +1351,9 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
     S = batch.args.n_seqs
     if out is None:
         if rows is None:
-            rows = batch.max_len or (page if batch.page_table is None else batch.args.max_pages * page)
+            rows = page if batch.page_table is None else batch.args.max_pages * page
+            if batch.max_len:
+                rows = min(batch.max_len, rows)
         if rows < 0:
             raise ValueError(f"rows={rows}")
         keys, values = (torch.empty((S, H, rows, dim), dtype=dtype, device=dev) for _ in range(2))

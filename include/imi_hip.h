@@ -503,7 +503,7 @@ typedef struct {
     const int32_t* query_start;  /* device [n_seqs + 1], ascending */
     int32_t n_seqs, n_tokens;    /* n_tokens: rows of the query tensor */
     int32_t max_query;           /* at least every sequence's new tokens */
-    int32_t max_len;             /* hint: about the longest sequence; 0 = what the table holds */
+    int32_t max_len;             /* hint: the longest sequence, for splits and shared rows; 0 = what the table holds */
     const int32_t* shared;       /* device [n_seqs], what imi_share_prefixes found, or NULL (all four); */
     const int32_t* members;      /*   read by imi_paged_attention alone */
     const int32_t* leaders;
