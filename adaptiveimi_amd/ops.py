@@ -1366,7 +1366,8 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
         if t.shape != shape or (t.stride(3) != 1 and t.numel()):
             raise ValueError(f"out must be two tensors {list(shape)} with unit stride on dim")
     steps = _same_rows("the two tensors of out", keys, values, dev)
-    if any(step == 0 and n > 1 for step, n in zip(steps, shape)):
+    if any(step == 0 and n > 1 for step, n in zip(steps, shape)) or (
+            keys.numel() and keys.data_ptr() == values.data_ptr()):
         raise ValueError("out is written, so no two of its elements may share memory")
     f = 0
     if first is not None:

@@ -1,4 +1,4 @@
-"""How many rows read_pages gives, and where it and qk_norm_rope may write."""
+"""How many rows read_pages gives, and where it may write them."""
 import pytest
 import torch
 
@@ -43,3 +43,18 @@ def test_rows_by_default(ops):
     q = torch.randn((2, 4, 64), device=DEV).to(BF)
     full = ops.paged_attention(q, *pools, make(None))
     assert torch.equal(ops.paged_attention(q, *pools, make(10)), full)
+
+
+def test_outputs_that_are_one_tensor(ops):
+    """Keys and values read into the same memory: refused; into one buffer side by
+    side: not."""
+    pools = rows_pool(4, 2, 16, 64)
+    batch = ops.PagedBatch(i32([[0, 1, 2, 3]]), i32([20]), i32([0, 1]), 1)
+    out = torch.zeros((1, 2, 64, 64), dtype=BF, device=DEV)
+    with pytest.raises(ValueError):
+        ops.read_pages(*pools, batch, out=(out, out))
+    both = torch.zeros((1, 2, 64, 2, 64), dtype=BF, device=DEV)      # keys and values of a row together
+    got = ops.read_pages(*pools, batch, out=(both[..., 0, :], both[..., 1, :]))
+    want = ops.read_pages(*pools, batch)
+    for a, b in zip(got, want):
+        assert torch.equal(a[:, :, :20], b[:, :, :20])
