@@ -8,7 +8,11 @@
 //
 // The angle: position * f_i in fp64, reduced to a fraction of a turn there
 // (exact to 2^-53 of the turns: an fp32 product at position 2^17 would be off
-// by 2^-8), then sine and cosine of the fraction in fp32.
+// by 2^-8), then sine and cosine of the fraction in fp32.  The fraction's own
+// rounding, up to 2^-26 of a turn, is far under half a step of a 16-bit result
+// next to the largest of its head; a block of small numbers in codes is scaled up
+// (next to a quarter turn it put 1 code in 400 on the other side of a border), so
+// with codes its rest is applied to both.
 //
 // Bound by memory (a 128-wide head is 256 bytes in and out): D / 8 lanes hold
 // a head, 16 bytes each, so the sum of squares is a short lane reduction and
@@ -207,7 +211,15 @@ __global__ __launch_bounds__(256, 6) void qk_norm_rope_kernel(QkParams a) {
         const double turns = static_cast<double>(s_pos[t]) * static_cast<double>(a.inv_freq[f]) *
                              0.15915494309189533577;
         float sn, cs;
-        sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+        const double d = turns - rint(turns);
+        const float near = static_cast<float>(d);
+        sincospif(2.0f * near, &sn, &cs);
+        if constexpr (kCodes) {   // sine and cosine of the rest, r and 1
+            const float r = 6.2831855f * static_cast<float>(d - near);
+            const float sn0 = sn;
+            sn = fmaf(cs, r, sn);
+            cs = fmaf(-sn0, r, cs);
+        }
         s_cs[t][f] = make_float2(cs, sn);
     }
     __syncthreads();
