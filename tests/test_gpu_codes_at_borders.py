@@ -1,4 +1,5 @@
-"""Codes of rotated keys next to their borders, against the definition in 64 bits."""
+"""Codes of rotated keys next to their borders, and of numbers next to the type's
+largest, against the definition in 64 bits."""
 import math
 
 import pytest
@@ -10,7 +11,7 @@ from conftest import gpu_available
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not gpu_available(), reason="needs a HIP device")]
 
 DEV = "cuda:0"
-BF = torch.bfloat16
+BF, HF = torch.bfloat16, torch.float16
 FORMATS = ["fp8", "int8", "fp4"]
 
 
@@ -66,3 +67,37 @@ def test_codes_of_keys_near_a_quarter_turn(ops, fmt, interleaved):
     codes, exps = pools[0].codes.cpu()[at], pools[0].exponents.cpu()[at]
     wrong = (blocks.decode(codes, exps, fmt) != blocks.decode(*want, fmt)) & sure
     assert int(wrong.sum()) == 0, f"{int(wrong.sum())} codes"
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_finite_numbers_read_back_finite(ops, fmt, dtype):
+    """Blocks of numbers up to the type's largest, each with every top from there
+    down through four powers of two, read back in that type."""
+    D, page = 128, 16
+    big = torch.finfo(dtype).max
+    top = torch.tensor([big], dtype=dtype).view(torch.int16).item()
+    near = torch.arange(top, top - 4 * (128 if dtype is BF else 1024), -1 if dtype is BF else -7, dtype=torch.int32)
+    tops = near.to(torch.int16).view(dtype)
+    n = len(tops) // 4 * 4
+    g = torch.Generator().manual_seed(0)
+    x = (torch.rand((n, 32), generator=g) * 2 - 1) * tops[:n, None].float()
+    x[:, 5] = tops[:n].float() * torch.where(torch.arange(n) % 2 == 0, 1.0, -1.0)
+    x = x.to(dtype).view(n // 4, 1, D)
+    N = n // 4
+    P = -(-N // page)
+    table = torch.arange(P, dtype=torch.int32, device=DEV)[None]
+    batch = ops.PagedBatch(table, i32([N]), i32([0, N]), N)
+    pools = [ops.QuantizedPages.zeros(P, 1, page, D, fmt, DEV) for _ in range(2)]
+    ops.qk_norm_rope(x.to(DEV), x.to(DEV), value=(-x).to(DEV), batch=batch, key_pages=pools[0], value_pages=pools[1])
+    keys, values = ops.read_pages(*pools, batch, rows=N, dtype=dtype)
+    assert bool(torch.isfinite(keys).all()) and bool(torch.isfinite(values).all())
+    # and the encoder that the other tests compare with
+    codes, exps = blocks.encode(x.double(), fmt, dtype)
+    assert bool(torch.isfinite(blocks.rounded(blocks.decode(codes, exps, fmt), dtype)).all())
+    # off by half a step of the number at most, or by what the held-back codes leave:
+    # 240, 63 and 3 of 256, 64 and 4
+    left = {"fp8": 240 / 256, "int8": 63 / 64, "fp4": 3 / 4}[fmt]
+    largest = keys[0, 0].view(-1, 32).abs().amax(-1).double().cpu()
+    want = x.view(-1, 32).abs().amax(-1).double()
+    assert bool((largest >= left * want * (1 - 2.0 ** -7)).all())
