@@ -1827,8 +1827,14 @@ struct JoinParams {
 
 // Joins what the shared rows and its own rows gave each query row: a workgroup
 // per (sequence, head) and some rows, D / 4 threads to a partial as in
-// merge_kernel, all of a workgroup's for a row after the other.
-template <typename T, int D, int LEAD>
+// merge_kernel.  All of a workgroup's for a row after the other, or, where there
+// are more than kJoinRows rows (CHUNKS: many rows, of few partials each), a row for
+// each group of D / 4: a chunk of 4096 tokens of 32 heads beside 8 single tokens
+// that share nothing takes 490 us so, 774 with all of the workgroup's for each row
+// (and 470 without looking for shared rows).  Batches that cannot have so many rows
+// have a kernel without that branch, which costs them 1 us (144 -> 146).
+constexpr int kJoinRows = 64;
+template <typename T, int D, int LEAD, bool CHUNKS>
 __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
     constexpr int Q = D / 4, K = kMergeThreads / Q;
     __shared__ float s_ml[K][2];
@@ -1842,13 +1848,12 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
     const int heads = a.H * a.G;
     const int lead = sq.lo > 0 ? clampi(p.leaders[s], 0, s) : s;
     const int lead_t0 = clampi(a.start[lead], 0, sq.t0);
-    for (int64_t r = blockIdx.y; r < rows; r += p.blocks) {
+    // row r's, as far as this one of `groups` groups takes them: returns how many hold
+    // something, none where the row's range has written it
+    auto gather = [&](int64_t r, int k, int groups, Partial<D>& x) {
         const int i = static_cast<int>(r / a.G), g = static_cast<int>(r % a.G);
-        const int64_t t = sq.t0 + i;
-        const int head = h * a.G + g;
-        const int64_t e = t * heads + head;
-        Partial<D> x;
-        int used = K;   // groups that hold something
+        const int64_t t = sq.t0 + i, e = t * heads + h * a.G + g;
+        int used = groups;
         auto add = [&](int place, const Parts& from, const float* keep, const float* keep_ml, int row, int lead) {
             if (place < 0) {
                 if (k == 0)
@@ -1860,12 +1865,12 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
             const Join j = from.joins[w0];
             if (j.lo >= j.hi) return;
             const int log = ranges_log(a.w_log, j.total), w1 = last_of(j, w0, log);
-            if (sq.lo == 0) used = groups_of(w1 - w0 + 1, K);   // the order of merge_kernel
+            if (sq.lo == 0) used = groups_of(w1 - w0 + 1, groups);   // the order of merge_kernel
             if (k < used) x.gather(from, j, log, w0, w1, row, d4, k, used, a.c, lead);
         };
         const int tile = static_cast<int>(r) & ~(kTileRows - 1);
         const int mine = a.place[static_cast<int64_t>(place_key(a, sq.t0, s, tile)) * a.H + h];
-        if (sq.lo == 0 && mine < 0) continue;   // written by its range
+        if (sq.lo == 0 && mine < 0) return 0;
         const bool in_few = rows <= p.few_rows;
         add(mine, in_few ? p.few : p.tiles, a.keep, a.keep_ml, static_cast<int>(r) - tile, in_few ? LEAD : 0);
         if (sq.lo > 0) {
@@ -1874,6 +1879,30 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
             add(p.place[static_cast<int64_t>(place_key(a, lead_t0, lead, first)) * a.H + h], p.common, p.keep,
                 p.keep_ml, static_cast<int>(rc) - first, 0);
         }
+        return used;
+    };
+    auto write = [&](int64_t r, const Partial<D>& x) {
+        const int i = static_cast<int>(r / a.G);
+        const int64_t t = sq.t0 + i;
+        const int head = h * a.G + static_cast<int>(r % a.G);
+        const float inv = inverse(x.L, sq.p0 + i < 0);
+        uint2 o;
+        o.x = T::pack(x.A[0] * inv, x.A[1] * inv);
+        o.y = T::pack(x.A[2] * inv, x.A[3] * inv);
+        *reinterpret_cast<uint2*>(a.out + t * a.o_ts + head * a.o_hs + 4 * d4) = o;
+        if (a.lse && d4 == 0) a.lse[t * a.l_ts + head] = log_sum<T>(x.M, x.L, a.c);
+    };
+    if (CHUNKS && rows > kJoinRows) {
+        for (int64_t r = static_cast<int64_t>(blockIdx.y) * K + k; r < rows; r += static_cast<int64_t>(p.blocks) * K) {
+            Partial<D> x;
+            if (gather(r, 0, 1, x)) write(r, x);
+        }
+        return;
+    }
+    for (int64_t r = blockIdx.y; r < rows; r += p.blocks) {
+        Partial<D> x;
+        const int used = gather(r, k, K, x);
+        if (used == 0) continue;
         __syncthreads();
         if (d4 == 0) {
             s_ml[k][0] = x.M;
@@ -1884,12 +1913,7 @@ __global__ __launch_bounds__(kMergeThreads) void join_kernel(JoinParams p) {
         if (k == 0) {
             for (int y = 1; y < used; ++y)
                 x.add(s_ml[y][0], s_ml[y][1], *reinterpret_cast<const f32x4_t*>(&s_acc[y][4 * d4]), a.c);
-            const float inv = inverse(x.L, sq.p0 + i < 0);
-            uint2 o;
-            o.x = T::pack(x.A[0] * inv, x.A[1] * inv);
-            o.y = T::pack(x.A[2] * inv, x.A[3] * inv);
-            *reinterpret_cast<uint2*>(a.out + t * a.o_ts + head * a.o_hs + 4 * d4) = o;
-            if (a.lse && d4 == 0) a.lse[t * a.l_ts + head] = log_sum<T>(x.M, x.L, a.c);
+            write(r, x);
         }
     }
 }
@@ -2010,7 +2034,6 @@ inline int64_t least_saved(const imi_paged_attention_args* a) {
     const int64_t row = int64_t(2) * a->kv_heads * row_bytes;
     return std::max<int64_t>((a->batch.share_bytes ? a->batch.share_bytes : kShareBytes) / row, 1);
 }
-constexpr int kJoinRows = 64;          // workgroups of join_kernel to a (sequence, head), at most
 constexpr int kJoinPairs = 1 << 22;    // (sequence, head) pairs, at most: 2^30 threads along x
 inline bool shares(const imi_paged_attention_args* a) {
     const imi_paged_batch& b = a->batch;
@@ -2138,6 +2161,11 @@ int launch(const Shape& p, const PagedParams<C, false>& P, const Rooms& room, hi
 
 // Shared and own rows: a launch, where the workgroups can plan for themselves,
 // one for sequences of many new tokens, and the join.
+//
+// Workgroups of a join of long chunks, but at least kJoinRows to a (sequence, head):
+// most find no row.  2^13, 2^15, 2^17: the chunk of 4096 tokens above 491, 490, 545
+// us, one of 8192 beside 32 single tokens 1093, 1084, 1121.
+constexpr int kJoinGrid = 1 << 15;
 template <typename T, int D, typename C>
 int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> P, int64_t least, hipStream_t stream) {
     P.shared = b.shared;
@@ -2170,15 +2198,21 @@ int launch_shared(const Work& w, const imi_paged_batch& b, PagedParams<C, true> 
         tiles = tile_params(w.own, P, w.of_own, D);
         if (const int rc = launch_tiles<T, D, C, true>(w.own, tiles, stream)) return rc;
     }
-    const int blocks = std::min(w.own.max_rows, kJoinRows);
+    // workgroups to a (sequence, head): one for a row, or, where chunks may be long,
+    // as many as kJoinGrid leaves for their groups of rows
+    const int64_t pairs = static_cast<int64_t>(P.S) * P.H;
+    const int64_t most = (w.own.max_rows + kMergeThreads / (D / 4) - 1) / (kMergeThreads / (D / 4));
+    const int blocks = static_cast<int>(std::max<int64_t>(std::min(w.own.max_rows, kJoinRows),
+                                                          std::min<int64_t>(most, kJoinGrid / pairs)));
     JoinParams J{{},           w.own.few_rows, blocks,     parts_of(few), parts_of(tiles), parts_of(common),
                  w.keep[0],    w.keep_ml[0],   w.place[0], b.leaders};
     static_cast<BaseParams&>(J.own) = P;
     static_cast<SharedParams&>(J.own) = P;
     J.own.w_log = w.own.w_log;
     J.own.max_rows = w.own.max_rows;
-    const dim3 grid(static_cast<unsigned>(P.S) * P.H, static_cast<unsigned>(blocks));
-    join_kernel<T, D, FewLoads<C, D>::kLead><<<grid, kMergeThreads, 0, stream>>>(J);
+    const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(blocks));
+    if (w.own.max_rows > kJoinRows) join_kernel<T, D, FewLoads<C, D>::kLead, true><<<grid, kMergeThreads, 0, stream>>>(J);
+    else join_kernel<T, D, FewLoads<C, D>::kLead, false><<<grid, kMergeThreads, 0, stream>>>(J);
     IMI_LAUNCH_CHECK("join_kernel");
     return IMI_OK;
 }

@@ -194,3 +194,17 @@ def test_exponents_of_another_memory_order(ops):
         for a, b in zip(ops.read_pages(y["k"], y["v"], ops.PagedBatch(x["table"], x["lens"], x["start"], 40), rows=230),
                         ops.read_pages(x["k"], x["v"], ops.PagedBatch(x["table"], x["lens"], x["start"], 40), rows=230)):
             assert torch.equal(a[0], b[0]) and torch.equal(a[2], b[2]) and torch.equal(a[1, :, :208], b[1, :, :208])
+
+
+@pytest.mark.parametrize("dtype,D,page", [(BF, 128, 16), (HF, 64, 8)])
+def test_chunks_behind_long_common_rows(ops, dtype, D, page):
+    """Chunks of up to 600 rows (tokens times heads), of runs and on their own, beside
+    single tokens: common and own rows in several ranges each."""
+    groups = [(3008, [(70, 40), (300, 1), (1500, 150), (90, 17)]), (0, ones(500)), (0, [(2700, 100)]),
+              (1504, [(40, 16), (50, 30)])]
+    x = forked(groups, 2, 4, D, page, dtype, seed=11, pad=1)
+    out = torch.full(x["q"].shape, 3.0, dtype=dtype, device=DEV)
+    batch, (_, lse) = attend(ops, x, out=out)
+    assert batch.members.tolist() == [4, 0, 0, 0, 0, 0, 2, 0]
+    check(x, out, lse)
+    assert bool((out[-1] == 3).all())
