@@ -432,8 +432,8 @@ __device__ __forceinline__ float log_sum(float M, float L, float c) {
 //
 // Of codes there are half or a quarter of the bytes under way, and the same number
 // of rows, so the work on a row tells: over 131072 rows of 8 heads of 128 fp8 takes
-// 54 us (5.1 TB/s), int8, whose codes take five instructions a pair where the others
-// take one, 58, fp4 36 (4.0 TB/s).  In a ragged int8 batch vector instructions hold
+// 56 us (5.0 TB/s), int8, whose codes take five instructions a pair where the others
+// take one, 59-67, fp4 36 (4.0 TB/s).  In a ragged int8 batch vector instructions hold
 // half of the issue slots.  Two workgroups per CU (128 registers, spilled) took 88
 // us for the 61 with its join in fp8; with 64 dims, where they fit, 41 for 37.
 constexpr int kFewWaves = kThreads / 64;
@@ -1779,7 +1779,8 @@ __global__ __launch_bounds__(kThreads, 2) void tile_kernel(PagedParams<C, SH> a)
 // ------------------------------------------------------------ shared rows --
 // A launch for the shared rows (the first 2^w_log workgroups, tiles: a run of 64
 // sequences of 4 heads has 256 rows, and reads K and V once for all) and for the
-// rows of the sequences' own (few rows each), so that neither waits for the other.
+// rows of the sequences' own (few rows each).  A CU holds one workgroup (its LDS), so
+// these begin where a CU is done with the former, and not when all are.
 // (Twice the whole arguments, 912 bytes instead of 392, cost 1.5 us a launch.)
 struct Common {   // what differs in the launch's arguments for the shared rows
     Join* joins;

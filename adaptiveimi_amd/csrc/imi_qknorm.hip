@@ -22,8 +22,8 @@
 //
 // Pages in 8 or 4 bits (C): a block of 32 dims is four lanes, whose largest
 // magnitude two lane exchanges find; the codes are made of the fp32 results, so
-// a key is rounded once there too.  10529 tokens of 48 heads into fp8: 60 us, bound
-// by vector instructions (0.77 of the issue slots; 237 MB, 3.9 TB/s).  A row's four
+// a key is rounded once there too.  10529 tokens of 48 heads into fp8, int8 or fp4: 63
+// us, bound by vector instructions (0.77 of the issue slots; in fp8 237 MB, 3.8 TB/s).  A row's four
 // exponents gathered for one store were no faster than a byte by each block's first
 // lane.  Keys and values take one path: with one each, 4 bits spill two registers,
 // which costs 6 us (8 bits gain 1).

@@ -1330,7 +1330,9 @@ def read_pages(key_pages, value_pages, batch: PagedBatch, rows: Optional[int] = 
     that is longer the rest is not read, so give ``rows`` where max_len may be
     exceeded.  ``out``: tensors of any sequence,
     head and row strides to write to.  Rows that a sequence does not have are
-    left as they are (unset in tensors made here)."""
+    left as they are (unset in tensors made here).  As in paged_attention, a page
+    id outside the pool below lens counts as the nearest one, and lens past the
+    table as what it holds."""
     dev = batch.device
     quantized = type(key_pages) is QuantizedPages
     if out is not None:

@@ -598,7 +598,7 @@ int imi_qk_norm_rope(const imi_qk_norm_rope_args* a, imi_stream_t stream);
 /* Cached rows read back: keys[s][h][i] and values[s][h][i], i < rows, are row
  * first[s] + i of sequence s (first NULL: 0) in the call's dtype, codes as their
  * values rounded to it.  Rows outside 0 .. lens[s] - 1 are left as they are in
- * the outputs.  Of the batch, tables, lens and sizes are read, not the new
+ * the outputs; a page id outside the pool counts as the nearest.  Of the batch, tables, lens and sizes are read, not the new
  * tokens. */
 typedef struct {
     imi_paged_batch batch;
